@@ -451,6 +451,158 @@ int sah_mlp_residual_norm(
  * solution/kernels/boundary/triton_ffn_residual_norm.py:30-38). */
 int sah_mlp_residual_norm_launch_supported(int64_t width, int block_rows, int num_warps);
 
+/*
+ * The operators of a decoding step.  No counterpart in the reference, whose
+ * forward takes whole sequences: with these a program answers token by token, or
+ * takes a prompt in chunks, behind a key/value cache.
+ *
+ * starts[b] (int32, device) is the number of tokens that sequence b holds before
+ * the step; counts[b] (int32, device; NULL for seq_len of every sequence) the
+ * number of its new tokens, at most seq_len of the padded tensors (more counts
+ * as seq_len, fewer than one as none).  New token i stands at position starts[b] + i.
+ */
+
+/*
+ * Norm of every query and key head and the position rotation, one pass:
+ *   y   = norm(x) * weight + bias     over head_dim, statistics in fp32
+ *   out = round_to(dtype, rotated y)
+ * The first rotary_dim features are rotated, (a, b) -> (a cos - b sin, b cos +
+ * a sin), where the pair is y[i] and y[i + rotary_dim / 2], or with interleaved
+ * y[2 i] and y[2 i + 1].  table row p holds the rotary_dim / 2 cosines of position
+ * p, then the sines, in fp32: [table_rows, rotary_dim].  A position outside the
+ * table gives NaN in the rotated features.  starts may be NULL (positions from 0).
+ *
+ * query [batch, heads, seq_len, head_dim] and key [batch, kv_heads, seq_len,
+ * head_dim] by strides, head_dim contiguous (views of a packed projection);
+ * query_out and key_out contiguous, overlapping no input.  weight and bias
+ * [head_dim] of either, in param_dtype (f32 or dtype), may be NULL (1, 0).  dtype
+ * f32, f16 or bf16; head_dim 64, 128 or 256; rotary_dim 0 (no rotation, table may
+ * be NULL) or a multiple of 16 (interleaved: 8) up to head_dim; batch * seq_len
+ * below 2^31; strides multiples of 16 bytes, tensors 16-byte aligned.
+ */
+int sah_qk_norm_rotary(
+    const void* query, const void* key,
+    const void* query_weight, const void* query_bias,
+    const void* key_weight, const void* key_bias,
+    const float* table, const int32_t* starts,
+    void* query_out, void* key_out,
+    int64_t batch, int64_t seq_len, int64_t heads, int64_t kv_heads, int64_t head_dim,
+    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+    int64_t rotary_dim, int64_t table_rows, int interleaved,
+    int norm_kind, float eps, int dtype, int param_dtype,
+    sah_stream_t stream);
+
+/*
+ * The 8-bit block cache of keys and values.
+ *
+ * A sequence's tokens stand in blocks of 64; block_table [batch, max_blocks]
+ * (int32) names the place of each, in [0, num_blocks).  A complete block holds
+ *   key_codes   [num_blocks, kv_heads, 64, head_dim]   e4m3
+ *   value_codes [num_blocks, kv_heads, head_dim, 64]   e4m3, feature by feature
+ *   key_scales, value_scales [num_blocks, kv_heads]    fp32
+ * and stands for code * scale.  The scale is the smallest power of two s, at least
+ * 2^-100, with max|x| / s <= 448 over the block's tokens of the head (1 for zeros),
+ * and codes are x / s rounded to nearest, ties to even.  A sequence's incomplete
+ * block stands in dtype in key_tail [batch, kv_heads, 64, head_dim] and value_tail
+ * [batch, kv_heads, head_dim, 64] until its last token comes, so the cache's
+ * contents do not depend on the steps in which the tokens came, and a complete
+ * block is never written again (sequences may share it).  A token with a
+ * non-finite key or value is held as a key of NaN and a value of zeros: queries
+ * that attend to it answer NaN, others are not touched by it.
+ *
+ * head_dim 64 or 128; dtype f16 or bf16; codes and tails contiguous and 16-byte
+ * aligned, the rest 4-byte.
+ */
+
+/*
+ * Appends counts[b] tokens to each sequence: key and value [batch, kv_heads,
+ * seq_len, head_dim] by strides (multiples of 8 elements, head_dim contiguous,
+ * 16-byte aligned).  A block whose table entry is outside [0, num_blocks), or
+ * behind max_blocks, is not stored; a sequence with a negative start takes nothing.
+ * Blocks that one call completes must be different places of the cache.
+ */
+int sah_block_cache_append(
+    const void* key, const void* value,
+    void* key_codes, void* value_codes, float* key_scales, float* value_scales,
+    void* key_tail, void* value_tail, const int32_t* block_table,
+    const int32_t* starts, const int32_t* counts,
+    int64_t batch, int64_t kv_heads, int64_t seq_len, int64_t head_dim,
+    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+    int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
+    int64_t num_blocks, int64_t max_blocks, int dtype,
+    sah_stream_t stream);
+
+/*
+ * Reads what the cache holds back in dtype: key and value [batch, kv_heads, tokens,
+ * head_dim] contiguous, row i the token at position firsts[b] + i, zeros where that
+ * is negative or lengths[b] (the tokens that sequence b holds) or more, NaN where
+ * its block has no place in the cache.  A code times its scale that left dtype's
+ * range takes the largest value of dtype.
+ */
+int sah_block_cache_read(
+    const void* key_codes, const void* value_codes,
+    const float* key_scales, const float* value_scales,
+    const void* key_tail, const void* value_tail, const int32_t* block_table,
+    const int32_t* firsts, const int32_t* lengths, void* key, void* value,
+    int64_t batch, int64_t kv_heads, int64_t tokens, int64_t head_dim,
+    int64_t num_blocks, int64_t max_blocks, int dtype,
+    sah_stream_t stream);
+
+/*
+ * Causal attention of the new tokens over the cache, which holds them already
+ * (starts and counts are those of the append): row i of sequence b attends to
+ * positions 0 .. starts[b] + i.
+ *   output = round_to(dtype, softmax(scale q K^T) V), fp32 softmax and accumulation
+ * query [batch, heads, seq_len, head_dim] by strides (multiples of 8 elements,
+ * head_dim contiguous); query head j reads key head j / (heads / kv_heads); output
+ * [batch, seq_len, heads * head_dim] by strides, overlapping no input.  Rows from
+ * counts[b] on, and all rows of a sequence with a negative start, are zeros; rows
+ * that see a block without a place in the cache are NaN.
+ * max_length bounds starts + counts; it lays out the
+ * launch and sizes the workspace.  Longer sequences are still computed whole.
+ * workspace: device memory of sah_block_cache_attention_workspace_bytes(), 16-byte
+ * aligned, NULL when that is 0; calls that share one must not overlap.
+ */
+int sah_block_cache_attention(
+    const void* query,
+    const void* key_codes, const void* value_codes,
+    const float* key_scales, const float* value_scales,
+    const void* key_tail, const void* value_tail, const int32_t* block_table,
+    const int32_t* starts, const int32_t* counts, void* output,
+    int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t head_dim,
+    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+    int64_t o_stride_b, int64_t o_stride_s,
+    int64_t num_blocks, int64_t max_blocks, int64_t max_length,
+    float scale, int dtype, void* workspace, size_t workspace_bytes,
+    sah_stream_t stream);
+
+/* Bytes of the merged parts' outputs and statistics, where the launch splits the
+ * history; 0 where it does not. */
+size_t sah_block_cache_attention_workspace_bytes(
+    int64_t batch, int64_t seq_len, int64_t heads, int64_t kv_heads, int64_t head_dim,
+    int64_t max_length);
+
+/*
+ * Linear layer with 4-bit weights for few rows (the projections of a decoding step):
+ *   y = round_to(dtype, act(x W^T + bias)),  W[n][k] = scale[k / group_size][n] * code[n][k]
+ * fp32 accumulation; activation as in sah_linear.  codes: 32-bit words [out_features
+ * / 16, in_features / 128, 64, 4]; word [N, K, lane, step] holds the codes, -7 .. 7,
+ * of output 16 N + lane % 16 and inputs 128 K + 32 step + 8 (lane / 16) + e, e = 0
+ * .. 7.  Code e < 4 has its magnitude at bits 8 e .. 8 e + 2 and its sign at bit 8 e
+ * + 7; code e >= 4 stands as code e - 4, turned left by 4 bits.  scales
+ * [in_features / group_size, out_features] and bias [out_features] (or NULL) in
+ * dtype; x [rows, in_features] and y [rows, out_features] by row strides (multiples
+ * of 8 elements), y overlapping no input.  dtype f16 or bf16; group_size 32, 64 or
+ * 128; in_features a multiple of 128, out_features of 16; tensors 16-byte aligned,
+ * bias 8-byte.
+ */
+int sah_linear_w4(
+    const void* x, const void* codes, const void* scales, const void* bias, void* y,
+    int64_t rows, int64_t in_features, int64_t out_features, int64_t group_size,
+    int64_t x_row_stride, int64_t y_row_stride, int dtype, int activation,
+    sah_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

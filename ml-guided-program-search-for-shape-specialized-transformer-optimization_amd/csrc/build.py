@@ -36,6 +36,10 @@ SOURCES = (
     "gelu.hip",
     "linear_norm.hip",
     "mlp_norm.hip",
+    "qk_rotary.hip",
+    "block_cache.hip",
+    "cached_attention.hip",
+    "linear_w4.hip",
 )
 OFFLOAD_ARCH = "gfx950"
 

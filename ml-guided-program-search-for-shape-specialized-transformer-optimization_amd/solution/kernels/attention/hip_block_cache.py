@@ -1,0 +1,422 @@
+"""Key/value cache in 8 bits and the attention that reads it, on gfx950.
+
+No counterpart in the reference, whose forward takes whole sequences.  These
+are the operators of a decoding step beside the causal attention of whole
+sequences (solution/shape14/hip_streaming_dh64.py), in the manner of its
+modules: ``can_use_*``, strict calls that return ``(..., marker)``, RuntimeError
+"... ineligible ..." for inputs that the kernels do not take.
+
+A step of one layer, for ``batch`` sequences of which ``starts`` tokens are held::
+
+    query, key, _ = hip_qk_norm_rotary(query, key, wq, wk, table, starts)
+    hip_block_cache_append(cache, key, value, starts)
+    context, _ = hip_block_cache_attention(query, cache, starts)
+
+and after the step's last layer ``starts += 1`` (or ``+= counts``).
+
+:class:`BlockCache` describes the format; include/shape_aware_hip.h defines it.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from ..hip._library import (
+    HipLibraryError,
+    check_status,
+    dtype_code,
+    is_gfx950,
+    launch_device,
+    library_available,
+    load_library,
+    stream_handle,
+)
+
+HIP_BLOCK_CACHE_APPEND_BACKEND = "hip_block_cache_append"
+HIP_BLOCK_CACHE_READ_BACKEND = "hip_block_cache_read"
+HIP_BLOCK_CACHE_ATTENTION_BACKEND = "hip_block_cache_attention"
+
+BLOCK_TOKENS = 64
+SUPPORTED_HEAD_DIMS = frozenset({64, 128})
+SUPPORTED_DTYPES = frozenset({torch.bfloat16, torch.float16})
+_MAX_LENGTH = 2**31 - 1
+
+
+@dataclass(frozen=True, eq=False)
+class BlockCache:
+    """One layer's keys and values, in blocks of 64 tokens.
+
+    ``block_table`` [batch, max_blocks] (int32) names the place of each block of
+    a sequence among ``num_blocks``; layers that share their sequences' layout may
+    share it.  A complete block holds e4m3 codes (bytes) and one power-of-two scale
+    a head: ``key_codes`` [num_blocks, kv_heads, 64, head_dim] and ``key_scales``
+    [num_blocks, kv_heads]; values feature by feature, ``value_codes`` [num_blocks,
+    kv_heads, head_dim, 64].  The block that a sequence has not filled stands in 16
+    bits in ``key_tail`` [batch, kv_heads, 64, head_dim] and ``value_tail`` [batch,
+    kv_heads, head_dim, 64].
+    """
+
+    key_codes: torch.Tensor
+    value_codes: torch.Tensor
+    key_scales: torch.Tensor
+    value_scales: torch.Tensor
+    key_tail: torch.Tensor
+    value_tail: torch.Tensor
+    block_table: torch.Tensor
+
+    def __post_init__(self) -> None:
+        tail = self.key_tail
+        if tail.ndim != 4 or tail.shape[2] != BLOCK_TOKENS or tail.shape[3] not in SUPPORTED_HEAD_DIMS:
+            raise ValueError("key_tail must be [batch, kv_heads, 64, head_dim] with head_dim 64 or 128")
+        if tail.dtype not in SUPPORTED_DTYPES:
+            raise ValueError("the cache's tails must be bfloat16 or float16")
+        batch, heads, _, dim = tail.shape
+        if self.key_codes.ndim != 4 or self.block_table.ndim != 2 or heads < 1:
+            raise ValueError("the cache's tensors do not belong together")
+        blocks = self.key_codes.shape[0]
+        expected = (
+            (self.key_codes, (blocks, heads, BLOCK_TOKENS, dim), torch.uint8),
+            (self.value_codes, (blocks, heads, dim, BLOCK_TOKENS), torch.uint8),
+            (self.key_scales, (blocks, heads), torch.float32),
+            (self.value_scales, (blocks, heads), torch.float32),
+            (self.key_tail, (batch, heads, BLOCK_TOKENS, dim), tail.dtype),
+            (self.value_tail, (batch, heads, dim, BLOCK_TOKENS), tail.dtype),
+            (self.block_table, (batch, self.block_table.shape[1]), torch.int32),
+        )
+        for tensor, shape, dtype in expected:
+            if tuple(tensor.shape) != shape or tensor.dtype != dtype:
+                raise ValueError(f"the cache's tensors do not belong together: expected {dtype} {shape}")
+            if not tensor.is_contiguous() or tensor.device != tail.device or tensor.requires_grad:
+                raise ValueError("the cache's tensors must be contiguous, on one device and need no gradient")
+        for tensor in (self.key_codes, self.value_codes, self.key_tail, self.value_tail):
+            if tensor.data_ptr() % 16:
+                raise ValueError("the cache's codes and tails must be 16-byte aligned")
+
+    @classmethod
+    def allocate(
+        cls,
+        batch: int,
+        kv_heads: int,
+        head_dim: int,
+        *,
+        max_tokens: int,
+        num_blocks: int | None = None,
+        dtype: torch.dtype = torch.bfloat16,
+        device: torch.device | str = "cuda",
+        block_table: torch.Tensor | None = None,
+    ) -> "BlockCache":
+        """An empty cache for sequences of up to ``max_tokens``.  By default every
+        sequence has places of its own for all of them; with ``num_blocks`` given
+        and no ``block_table``, no place is named yet (-1)."""
+
+        width = max_tokens // BLOCK_TOKENS
+        if block_table is not None:
+            width = block_table.shape[1]
+        if num_blocks is None:
+            num_blocks = batch * width
+            if block_table is None:
+                block_table = torch.arange(num_blocks, dtype=torch.int32, device=device).reshape(batch, width)
+        elif block_table is None:
+            block_table = torch.full((batch, width), -1, dtype=torch.int32, device=device)
+        codes = (num_blocks, kv_heads, BLOCK_TOKENS * head_dim)
+        return cls(
+            torch.zeros(codes, dtype=torch.uint8, device=device).view(num_blocks, kv_heads, BLOCK_TOKENS, head_dim),
+            torch.zeros(codes, dtype=torch.uint8, device=device).view(num_blocks, kv_heads, head_dim, BLOCK_TOKENS),
+            torch.ones((num_blocks, kv_heads), device=device),
+            torch.ones((num_blocks, kv_heads), device=device),
+            torch.zeros((batch, kv_heads, BLOCK_TOKENS, head_dim), dtype=dtype, device=device),
+            torch.zeros((batch, kv_heads, head_dim, BLOCK_TOKENS), dtype=dtype, device=device),
+            block_table,
+        )
+
+    @property
+    def batch(self) -> int:
+        return self.key_tail.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.key_tail.shape[1]
+
+    @property
+    def head_dim(self) -> int:
+        return self.key_tail.shape[3]
+
+    @property
+    def max_tokens(self) -> int:
+        """The most tokens that a sequence can hold: its table's blocks and a tail."""
+
+        return min(self.block_table.shape[1] * BLOCK_TOKENS + BLOCK_TOKENS - 1, _MAX_LENGTH)
+
+    def _pointers(self) -> tuple[int, ...]:
+        return (
+            self.key_codes.data_ptr(),
+            self.value_codes.data_ptr(),
+            self.key_scales.data_ptr(),
+            self.value_scales.data_ptr(),
+            self.key_tail.data_ptr(),
+            self.value_tail.data_ptr(),
+            self.block_table.data_ptr(),
+        )
+
+
+def hip_block_cache_available() -> bool:
+    """Whether the gfx950 library loads in this process."""
+
+    return library_available()
+
+
+def _lengths_ok(lengths: torch.Tensor | None, cache: BlockCache) -> bool:
+    return lengths is None or (
+        lengths.dtype is torch.int32
+        and lengths.shape == (cache.key_tail.shape[0],)
+        and lengths.is_contiguous()
+        and lengths.device == cache.key_tail.device
+    )
+
+
+def _rows_ok(value: torch.Tensor, cache: BlockCache) -> bool:
+    """A [batch, heads, seq_len, head_dim] view of the cache's type that the kernels read in place."""
+
+    tail = cache.key_tail
+    if value.ndim != 4 or value.dtype is not tail.dtype or value.device != tail.device:
+        return False
+    shape, strides = value.shape, value.stride()
+    if shape[0] != tail.shape[0] or shape[3] != tail.shape[3]:
+        return False
+    if strides[3] != 1 or value.data_ptr() % 16 or (value.requires_grad and torch.is_grad_enabled()):
+        return False
+    return not any(stride % 8 and size != 1 for size, stride in zip(shape[:3], strides))
+
+
+def _strides(value: torch.Tensor) -> tuple[int, ...]:
+    """Strides of the first three axes, 0 for an axis of size 1 (never stepped)."""
+
+    return tuple(0 if size == 1 else stride for size, stride in zip(value.shape[:3], value.stride()))
+
+
+def can_use_hip_block_cache_append(
+    cache: BlockCache,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    starts: torch.Tensor,
+    counts: torch.Tensor | None = None,
+) -> bool:
+    """Whether the append kernel takes these tensors."""
+
+    return (
+        _rows_ok(key, cache)
+        and key.shape[1] == cache.key_tail.shape[1]
+        and value.shape == key.shape
+        and _rows_ok(value, cache)
+        and starts is not None
+        and _lengths_ok(starts, cache)
+        and _lengths_ok(counts, cache)
+        and is_gfx950(key.device)
+        and library_available()
+    )
+
+
+def hip_block_cache_append(
+    cache: BlockCache,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    starts: torch.Tensor,
+    counts: torch.Tensor | None = None,
+) -> str:
+    """Append each sequence's new tokens to the cache, in place.
+
+    ``key`` and ``value`` are [batch, kv_heads, seq_len, head_dim] (any strides,
+    head_dim contiguous); sequence b holds ``starts[b]`` tokens and takes the first
+    ``counts[b]`` rows, or all ``seq_len`` without ``counts``.  A block is coded when
+    its 64th token comes.  Blocks without a place in the cache are dropped, and the
+    attention that would read them answers NaN.  A token with a non-finite key or
+    value makes NaN of every query that attends to it, and of no other.
+    """
+
+    if not can_use_hip_block_cache_append(cache, key, value, starts, counts):
+        raise RuntimeError("HIP block cache append is ineligible for the requested inputs")
+    batch, heads, seq_len, dim = key.shape
+    try:
+        with launch_device(key.device):
+            status = load_library().sah_block_cache_append(
+                key.data_ptr(),
+                value.data_ptr(),
+                *cache._pointers(),
+                starts.data_ptr(),
+                None if counts is None else counts.data_ptr(),
+                batch,
+                heads,
+                seq_len,
+                dim,
+                *_strides(key),
+                *_strides(value),
+                cache.key_codes.shape[0],
+                cache.block_table.shape[1],
+                dtype_code(key.dtype),
+                stream_handle(key.device),
+            )
+            check_status(status, "sah_block_cache_append")
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block cache append execution failed") from exc
+    return HIP_BLOCK_CACHE_APPEND_BACKEND
+
+
+def can_use_hip_block_cache_read(
+    cache: BlockCache, firsts: torch.Tensor, lengths: torch.Tensor, tokens: int
+) -> bool:
+    """Whether the read kernel takes these tensors."""
+
+    return (
+        isinstance(tokens, int)
+        and not isinstance(tokens, bool)
+        and tokens >= 0
+        and firsts is not None
+        and lengths is not None
+        and _lengths_ok(firsts, cache)
+        and _lengths_ok(lengths, cache)
+        and is_gfx950(cache.key_tail.device)
+        and library_available()
+    )
+
+
+def hip_block_cache_read(
+    cache: BlockCache, firsts: torch.Tensor, lengths: torch.Tensor, tokens: int
+) -> tuple[torch.Tensor, torch.Tensor, str]:
+    """What the cache holds, in its 16-bit type: keys and values [batch, kv_heads,
+    tokens, head_dim] of positions ``firsts[b] ..``, zeros before position 0 and from
+    ``lengths[b]`` (the tokens that sequence b holds) on."""
+
+    if not can_use_hip_block_cache_read(cache, firsts, lengths, tokens):
+        raise RuntimeError("HIP block cache read is ineligible for the requested inputs")
+    tail = cache.key_tail
+    batch, heads, _, dim = tail.shape
+    key = torch.empty((batch, heads, tokens, dim), dtype=tail.dtype, device=tail.device)
+    value = torch.empty_like(key)
+    try:
+        with launch_device(tail.device):
+            status = load_library().sah_block_cache_read(
+                *cache._pointers(),
+                firsts.data_ptr(),
+                lengths.data_ptr(),
+                key.data_ptr(),
+                value.data_ptr(),
+                batch,
+                heads,
+                tokens,
+                dim,
+                cache.key_codes.shape[0],
+                cache.block_table.shape[1],
+                dtype_code(tail.dtype),
+                stream_handle(tail.device),
+            )
+            check_status(status, "sah_block_cache_read")
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block cache read execution failed") from exc
+    return key, value, HIP_BLOCK_CACHE_READ_BACKEND
+
+
+def can_use_hip_block_cache_attention(
+    query: torch.Tensor,
+    cache: BlockCache,
+    starts: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    *,
+    scale: float | None = None,
+    max_length: int | None = None,
+) -> bool:
+    """Whether the attention kernel takes these tensors."""
+
+    return (
+        _rows_ok(query, cache)
+        and query.shape[1] > 0
+        and query.shape[1] % cache.key_tail.shape[1] == 0
+        and starts is not None
+        and _lengths_ok(starts, cache)
+        and _lengths_ok(counts, cache)
+        and (scale is None or math.isfinite(scale))
+        and (max_length is None or 0 <= max_length <= _MAX_LENGTH)
+        and is_gfx950(query.device)
+        and library_available()
+    )
+
+
+def hip_block_cache_attention(
+    query: torch.Tensor,
+    cache: BlockCache,
+    starts: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    *,
+    scale: float | None = None,
+    max_length: int | None = None,
+) -> tuple[torch.Tensor, str]:
+    """Causal attention of the new tokens over the cache that holds them already.
+
+    ``query`` is [batch, heads, seq_len, head_dim] (any strides, head_dim
+    contiguous), heads a multiple of the cache's: row i of sequence b stands at
+    position ``starts[b] + i`` and attends to all positions up to its own, with
+    ``starts`` and ``counts`` those of the append.  Returns [batch, seq_len, heads *
+    head_dim]; rows from ``counts[b]`` on are zeros.  ``scale`` defaults to
+    head_dim ** -0.5.  ``max_length``, where the program knows one, bounds the
+    sequences' lengths below what the table has room for: it spares launching the
+    parts of histories that no sequence has.  Longer ones are still computed whole.
+    """
+
+    if not can_use_hip_block_cache_attention(query, cache, starts, counts, scale=scale, max_length=max_length):
+        raise RuntimeError("HIP block cache attention is ineligible for the requested inputs")
+    batch, heads, seq_len, dim = query.shape
+    kv_heads = cache.key_tail.shape[1]
+    most = cache.max_tokens if max_length is None else min(max_length, cache.max_tokens)
+    output = torch.empty((batch, seq_len, heads * dim), dtype=query.dtype, device=query.device)
+    try:
+        library = load_library()
+        size = library.sah_block_cache_attention_workspace_bytes(batch, seq_len, heads, kv_heads, dim, most)
+        workspace = torch.empty(size, dtype=torch.uint8, device=query.device) if size else None
+        with launch_device(query.device):
+            status = library.sah_block_cache_attention(
+                query.data_ptr(),
+                *cache._pointers(),
+                starts.data_ptr(),
+                None if counts is None else counts.data_ptr(),
+                output.data_ptr(),
+                batch,
+                heads,
+                kv_heads,
+                seq_len,
+                dim,
+                *_strides(query),
+                seq_len * heads * dim,
+                heads * dim,
+                cache.key_codes.shape[0],
+                cache.block_table.shape[1],
+                most,
+                dim**-0.5 if scale is None else float(scale),
+                dtype_code(query.dtype),
+                None if workspace is None else workspace.data_ptr(),
+                size,
+                stream_handle(query.device),
+            )
+            check_status(status, "sah_block_cache_attention")
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block cache attention execution failed") from exc
+    return output, HIP_BLOCK_CACHE_ATTENTION_BACKEND
+
+
+__all__ = [
+    "BLOCK_TOKENS",
+    "BlockCache",
+    "HIP_BLOCK_CACHE_APPEND_BACKEND",
+    "HIP_BLOCK_CACHE_ATTENTION_BACKEND",
+    "HIP_BLOCK_CACHE_READ_BACKEND",
+    "SUPPORTED_DTYPES",
+    "SUPPORTED_HEAD_DIMS",
+    "can_use_hip_block_cache_append",
+    "can_use_hip_block_cache_attention",
+    "can_use_hip_block_cache_read",
+    "hip_block_cache_append",
+    "hip_block_cache_attention",
+    "hip_block_cache_available",
+    "hip_block_cache_read",
+]

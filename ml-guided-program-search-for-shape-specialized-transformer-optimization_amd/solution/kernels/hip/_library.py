@@ -106,6 +106,19 @@ _SIGNATURES: dict[str, tuple[list[object], object]] = {
         _int,
     ),
     "sah_mlp_residual_norm_launch_supported": ([_i64, _int, _int], _int),
+    "sah_qk_norm_rotary": (
+        [_ptr] * 10 + [_i64] * 5 + [_i64] * 6 + [_i64] * 2 + [_int] * 2 + [ctypes.c_float] + [_int] * 2 + [_ptr],
+        _int,
+    ),
+    "sah_block_cache_append": ([_ptr] * 11 + [_i64] * 4 + [_i64] * 6 + [_i64] * 2 + [_int, _ptr], _int),
+    "sah_block_cache_read": ([_ptr] * 11 + [_i64] * 4 + [_i64] * 2 + [_int, _ptr], _int),
+    "sah_block_cache_attention": (
+        [_ptr] * 11 + [_i64] * 5 + [_i64] * 5 + [_i64] * 3
+        + [ctypes.c_float, _int, _ptr, ctypes.c_size_t, _ptr],
+        _int,
+    ),
+    "sah_block_cache_attention_workspace_bytes": ([_i64] * 6, ctypes.c_size_t),
+    "sah_linear_w4": ([_ptr] * 5 + [_i64] * 6 + [_int] * 2 + [_ptr], _int),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 # SAH_ATTENTION_STATIC_WORKSPACE_BYTES of the header: the device array behind
@@ -196,6 +209,28 @@ def stream_handle(device: torch.device) -> int:
     return int(torch._C._cuda_getCurrentRawStream(_device_index(device)))
 
 
+class _SameDevice:
+    """The launch is on the current device: nothing to switch."""
+
+    def __enter__(self) -> None:
+        return None
+
+    def __exit__(self, *exc: object) -> None:
+        return None
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def launch_device(device: torch.device) -> _SameDevice | torch.cuda.device:
+    """Context in which ``device`` is the current one, which a HIP launch on one of
+    its streams needs; free where it is already."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
 # gfx950 or not, per device index: device properties do not change within a
 # process, and every operator's eligibility check asks.
 _GFX950_BY_INDEX: dict[int, bool] = {}
@@ -234,6 +269,7 @@ __all__ = [
     "check_status",
     "dtype_code",
     "is_gfx950",
+    "launch_device",
     "library_available",
     "load_library",
     "stream_handle",

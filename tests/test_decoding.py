@@ -1,0 +1,331 @@
+"""The decoding operators without a GPU: refusals of the C entries before any
+launch, eligibility in Python, the cache's and the packed weight's own checks, and
+the 4-bit format against a plain decoder."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from solution.kernels.attention import BlockCache, hip_block_cache_append, hip_block_cache_attention, hip_block_cache_read
+from solution.kernels.hip import _library
+from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
+from solution.kernels.projection import PackedLinearW4, hip_linear_w4, pack_linear_w4_codes, quantize_linear_w4
+
+# An address that the host checks may look at and no kernel reads: every call below
+# is refused, or has nothing to do, before a launch.
+P = 0x10000
+BF16, F16, F32 = 2, 1, 0
+OK, INVALID, UNSUPPORTED, WORKSPACE = 0, 1, 2, 4
+
+
+def _call(name, defaults, **changes):
+    unknown = set(changes) - set(defaults)
+    assert not unknown, unknown
+    return getattr(_library.load_library(), name)(*{**defaults, **changes}.values())
+
+
+ROTARY = dict(
+    query=P, key=P, query_weight=P, query_bias=None, key_weight=P, key_bias=None, table=P, starts=P, query_out=P,
+    key_out=P, batch=1, seq_len=4, heads=8, kv_heads=2, head_dim=64, q_sb=0, q_sh=64, q_ss=640, k_sb=0, k_sh=64,
+    k_ss=640, rotary_dim=64, table_rows=10, interleaved=0, norm_kind=1, eps=1e-6, dtype=BF16, param_dtype=F32,
+    stream=None,
+)
+
+
+@pytest.mark.parametrize(
+    "changes,status",
+    [
+        ({"batch": 0}, OK),
+        ({"seq_len": 0}, OK),
+        ({"head_dim": 96}, UNSUPPORTED),
+        ({"dtype": 7}, INVALID),
+        ({"param_dtype": F16}, UNSUPPORTED),
+        ({"norm_kind": 2}, INVALID),
+        ({"eps": -1.0}, INVALID),
+        ({"eps": float("nan")}, INVALID),
+        ({"heads": 0}, INVALID),
+        ({"kv_heads": -1}, INVALID),
+        ({"batch": -1}, INVALID),
+        ({"batch": 1 << 16, "seq_len": 1 << 15}, UNSUPPORTED),
+        ({"rotary_dim": 128}, UNSUPPORTED),
+        ({"rotary_dim": 24}, UNSUPPORTED),
+        ({"rotary_dim": 12, "interleaved": 1}, UNSUPPORTED),
+        ({"rotary_dim": -16}, UNSUPPORTED),
+        ({"query": None}, INVALID),
+        ({"key_out": None}, INVALID),
+        ({"table": None}, INVALID),
+        ({"table_rows": -1}, INVALID),
+        ({"key": P + 8}, INVALID),
+        ({"query_weight": P + 4}, INVALID),
+        ({"starts": P + 2}, INVALID),
+        ({"q_ss": 641}, INVALID),
+        ({"k_sh": 4}, INVALID),
+    ],
+)
+def test_rotary_entry_refuses_before_launch(changes, status):
+    assert _call("sah_qk_norm_rotary", ROTARY, **changes) == status
+
+
+CACHE = dict(key_codes=P, value_codes=P, key_scales=P, value_scales=P, key_tail=P, value_tail=P, table=P)
+APPEND = dict(
+    key=P, value=P, **CACHE, starts=P, counts=None, batch=2, kv_heads=2, seq_len=3, head_dim=64, k_sb=0, k_sh=64,
+    k_ss=256, v_sb=0, v_sh=64, v_ss=256, num_blocks=4, max_blocks=2, dtype=BF16, stream=None,
+)
+READ = dict(
+    **CACHE, firsts=P, lengths=P, key=P, value=P, batch=2, kv_heads=2, tokens=3, head_dim=64, num_blocks=4,
+    max_blocks=2, dtype=BF16, stream=None,
+)
+ATTENTION = dict(
+    query=P, **CACHE, starts=P, counts=None, output=P, batch=2, heads=4, kv_heads=2, seq_len=1, head_dim=64,
+    q_sb=0, q_sh=64, q_ss=256, o_sb=256, o_ss=256, num_blocks=4, max_blocks=2, max_length=128, scale=0.125,
+    dtype=BF16, workspace=None, workspace_bytes=0, stream=None,
+)
+OF_CACHE = [
+    ({"batch": 0}, OK),
+    ({"head_dim": 96}, UNSUPPORTED),
+    ({"dtype": F32}, UNSUPPORTED),
+    ({"batch": -1}, INVALID),
+    ({"kv_heads": 0}, INVALID),
+    ({"num_blocks": -1}, INVALID),
+    ({"max_blocks": -1}, INVALID),
+    ({"max_blocks": 1 << 30}, INVALID),
+    ({"key_codes": None}, INVALID),
+    ({"value_scales": None}, INVALID),
+    ({"table": None}, INVALID),
+    ({"value_tail": None}, INVALID),
+    ({"key_tail": P + 8}, INVALID),
+    ({"value_codes": P + 1}, INVALID),
+    ({"key_scales": P + 2}, INVALID),
+]
+
+
+@pytest.mark.parametrize(
+    "changes,status",
+    OF_CACHE
+    + [
+        ({"seq_len": 0}, OK),
+        ({"seq_len": -1}, INVALID),
+        ({"key": None}, INVALID),
+        ({"starts": None}, INVALID),
+        ({"value": P + 8}, INVALID),
+        ({"counts": P + 1}, INVALID),
+        ({"v_ss": 100}, INVALID),
+        ({"batch": 1 << 20, "seq_len": 1 << 20}, UNSUPPORTED),
+    ],
+)
+def test_append_entry_refuses_before_launch(changes, status):
+    assert _call("sah_block_cache_append", APPEND, **changes) == status
+
+
+@pytest.mark.parametrize(
+    "changes,status",
+    OF_CACHE
+    + [
+        ({"tokens": 0}, OK),
+        ({"tokens": -1}, INVALID),
+        ({"lengths": None}, INVALID),
+        ({"value": None}, INVALID),
+        ({"key": P + 2}, INVALID),
+        ({"firsts": P + 2}, INVALID),
+        ({"batch": 1 << 20, "tokens": 1 << 20}, UNSUPPORTED),
+    ],
+)
+def test_read_entry_refuses_before_launch(changes, status):
+    assert _call("sah_block_cache_read", READ, **changes) == status
+
+
+@pytest.mark.parametrize(
+    "changes,status",
+    OF_CACHE
+    + [
+        ({"seq_len": 0}, OK),
+        ({"seq_len": -1}, INVALID),
+        ({"heads": 5}, INVALID),
+        ({"heads": 0}, INVALID),
+        ({"scale": float("nan")}, INVALID),
+        ({"scale": float("inf")}, INVALID),
+        ({"scale": 3e38}, INVALID),
+        ({"max_length": -1}, INVALID),
+        ({"output": None}, INVALID),
+        ({"query": P + 8}, INVALID),
+        ({"q_ss": 4}, INVALID),
+        ({"o_sb": 4}, INVALID),
+        ({"starts": P + 1}, INVALID),
+        # a history long enough to be split, with no or too little workspace
+        ({"max_length": 100000}, WORKSPACE),
+        ({"max_length": 100000, "workspace": P, "workspace_bytes": 64}, WORKSPACE),
+        ({"max_length": 100000, "workspace": P + 4, "workspace_bytes": 1 << 30}, INVALID),
+    ],
+)
+def test_attention_entry_refuses_before_launch(changes, status):
+    assert _call("sah_block_cache_attention", ATTENTION, **changes) == status
+
+
+def test_attention_workspace_sizes():
+    size = _library.load_library().sah_block_cache_attention_workspace_bytes
+    assert size(1, 1, 16, 16, 64, 64) == 0
+    assert size(1, 0, 16, 16, 64, 100000) == 0
+    assert size(0, 1, 16, 16, 64, 100000) == 0
+    assert size(1, 1, 16, 3, 64, 100000) == 0  # not a size that runs
+    split = size(1, 1, 16, 16, 64, 100000)
+    assert split > 0 and split % (16 * (64 + 2) * 4) == 0
+
+
+LINEAR = dict(
+    x=P, codes=P, scales=P, bias=None, y=P, rows=4, in_features=256, out_features=32, group_size=64, x_stride=256,
+    y_stride=32, dtype=BF16, activation=0, stream=None,
+)
+
+
+@pytest.mark.parametrize(
+    "changes,status",
+    [
+        ({"rows": 0}, OK),
+        ({"rows": -1}, INVALID),
+        ({"dtype": F32}, UNSUPPORTED),
+        ({"activation": 2}, UNSUPPORTED),
+        ({"group_size": 16}, UNSUPPORTED),
+        ({"in_features": 192}, UNSUPPORTED),
+        ({"out_features": 24}, UNSUPPORTED),
+        ({"in_features": 0}, INVALID),
+        ({"codes": None}, INVALID),
+        ({"x": P + 8}, INVALID),
+        ({"bias": P + 4}, INVALID),
+        ({"x_stride": 257}, INVALID),
+        ({"y_stride": 36}, INVALID),
+        ({"rows": 1 << 39}, UNSUPPORTED),
+    ],
+)
+def test_linear_w4_entry_refuses_before_launch(changes, status):
+    assert _call("sah_linear_w4", LINEAR, **changes) == status
+
+
+def _cpu_cache(**changes):
+    sizes = dict(dtype=torch.bfloat16, device="cpu", max_tokens=200)
+    return BlockCache.allocate(2, 3, 64, **{**sizes, **changes})
+
+
+def test_cache_allocation():
+    cache = _cpu_cache()
+    assert cache.batch == 2 and cache.kv_heads == 3 and cache.head_dim == 64
+    assert cache.block_table.tolist() == [[0, 1, 2], [3, 4, 5]] and cache.max_tokens == 255
+    shared = _cpu_cache(num_blocks=10, block_table=cache.block_table)
+    assert shared.key_codes.shape == (10, 3, 64, 64) and shared.block_table is cache.block_table
+    assert _cpu_cache(num_blocks=4).block_table.eq(-1).all()
+    short = _cpu_cache(max_tokens=63)
+    assert short.block_table.shape == (2, 0) and short.key_codes.shape[0] == 0 and short.max_tokens == 63
+
+
+@pytest.mark.parametrize(
+    "name,make",
+    [
+        ("key_codes", lambda t: t.to(torch.int8)),
+        ("value_codes", lambda t: t[:, :, :, :32]),
+        ("key_scales", lambda t: t.double()),
+        ("value_scales", lambda t: t[:-1]),
+        ("key_tail", lambda t: t.float()),
+        ("value_tail", lambda t: t.half()),
+        ("value_tail", lambda t: t.transpose(-2, -1)),
+        ("block_table", lambda t: t.long()),
+        ("block_table", lambda t: t[0]),
+        ("key_tail", lambda t: t[..., :32]),
+    ],
+)
+def test_cache_of_tensors_that_do_not_belong_together(name, make):
+    cache = _cpu_cache()
+    parts = {field: getattr(cache, field) for field in cache.__dataclass_fields__}
+    BlockCache(**parts)
+    parts[name] = make(parts[name])
+    with pytest.raises(ValueError):
+        BlockCache(**parts)
+
+
+def test_operators_refuse_cpu_tensors():
+    cache = _cpu_cache()
+    starts = torch.zeros(2, dtype=torch.int32)
+    kv = torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="ineligible"):
+        hip_block_cache_append(cache, kv, kv, starts)
+    with pytest.raises(RuntimeError, match="ineligible"):
+        hip_block_cache_read(cache, starts, starts, 4)
+    with pytest.raises(RuntimeError, match="ineligible"):
+        hip_block_cache_attention(kv, cache, starts)
+    with pytest.raises(RuntimeError, match="ineligible"):
+        hip_qk_norm_rotary(kv, kv, None, None, rotary_table(4, 64, device="cpu"), starts)
+    packed = quantize_linear_w4(torch.ones(16, 128, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="ineligible"):
+        hip_linear_w4(torch.zeros(1, 128, dtype=torch.bfloat16), packed)
+
+
+def test_rotary_table():
+    table = rotary_table(1001, 16, base=500.0, device="cpu")
+    assert table.shape == (1001, 16) and table.dtype == torch.float32
+    angle = 1000 * 500.0 ** (-torch.arange(8, dtype=torch.float64) / 8)
+    assert torch.equal(table[1000], torch.cat([angle.cos(), angle.sin()]).float())
+    for bad in ((-1, 16), (4, 7), (4, 0)):
+        with pytest.raises(ValueError):
+            rotary_table(*bad, device="cpu")
+
+
+def _decoded(word):
+    """The eight codes of a word, bit by bit."""
+
+    word &= 0xFFFFFFFF
+    codes = []
+    for e in range(8):
+        turned = word if e < 4 else ((word >> 4) | (word << 28)) & 0xFFFFFFFF
+        byte = (turned >> (8 * (e % 4))) & 0xFF
+        codes.append((byte & 7) * (-1 if byte & 0x80 else 1))
+    return codes
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_packed_words_hold_the_codes(group):
+    generator = torch.Generator().manual_seed(group)
+    out_features, in_features = 48, 384
+    codes = torch.randint(-7, 8, (out_features, in_features), generator=generator)
+    scales = torch.rand(out_features, in_features // group, generator=generator).to(torch.float16)
+    packed = pack_linear_w4_codes(codes, scales)
+    assert packed.group_size == group and packed.out_features == out_features and packed.in_features == in_features
+    for n, k, lane, step in ((0, 0, 0, 0), (2, 1, 37, 3), (1, 2, 63, 1), (0, 2, 16, 2)):
+        first = 128 * k + 32 * step + 8 * (lane // 16)
+        want = codes[16 * n + lane % 16, first : first + 8].tolist()
+        assert _decoded(int(packed.codes[n, k, lane, step])) == want
+    want = codes.float() * scales.float().repeat_interleave(group, dim=1)
+    assert torch.equal(packed.dequantize(), want)
+
+
+def test_quantized_weights_are_within_half_a_step():
+    generator = torch.Generator().manual_seed(3)
+    weight = torch.randn(32, 256, generator=generator).to(torch.bfloat16)
+    weight[5, 64:128] = 0.0
+    packed = quantize_linear_w4(weight, 64)
+    scales = packed.scales.t().float().repeat_interleave(64, dim=1)
+    # half a step, and what the scale's rounding (2^-8 of seven steps) takes off the largest codes
+    bound = scales * (0.5 + 7 * 2.0**-8)
+    assert bool(((packed.dequantize() - weight.float()).abs() <= bound).all())
+    assert bool((packed.dequantize()[5, 64:128] == 0).all())
+
+
+@pytest.mark.parametrize(
+    "make",
+    [
+        lambda: pack_linear_w4_codes(torch.full((16, 128), 8), torch.ones(16, 1).half()),
+        lambda: pack_linear_w4_codes(torch.full((16, 128), -8), torch.ones(16, 1).half()),
+        lambda: pack_linear_w4_codes(torch.zeros(16, 128), torch.ones(16, 1).half()),
+        lambda: pack_linear_w4_codes(torch.zeros(8, 128, dtype=torch.int8), torch.ones(8, 1).half()),
+        lambda: pack_linear_w4_codes(torch.zeros(16, 96, dtype=torch.int8), torch.ones(16, 3).half()),
+        lambda: pack_linear_w4_codes(torch.zeros(16, 128, dtype=torch.int8), torch.ones(32, 1).half()),
+        lambda: pack_linear_w4_codes(torch.zeros(16, 128, dtype=torch.int8), torch.ones(16, 8).half()),
+        lambda: pack_linear_w4_codes(torch.zeros(16, 128, dtype=torch.int8), torch.ones(16, 1)),
+        lambda: quantize_linear_w4(torch.ones(16, 128)),
+        lambda: quantize_linear_w4(torch.ones(16, 128).half(), 16),
+        lambda: quantize_linear_w4(torch.full((16, 128), float("inf")).half()),
+        lambda: PackedLinearW4(torch.zeros(1, 1, 64, 4), torch.ones(1, 16).half()),
+        lambda: PackedLinearW4(torch.zeros(1, 0, 64, 4, dtype=torch.int32), torch.ones(1, 16).half()),
+    ],
+)
+def test_weights_that_cannot_be_packed(make):
+    with pytest.raises(ValueError):
+        make()

@@ -1,0 +1,729 @@
+"""GPU parity of the decoding operators against their plain 64-bit forms
+(tests/decoding_reference.py), one by one and as a decoding step runs them."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import decoding_reference as plain
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _rand(shape, seed, dtype, spread=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * spread).to(dtype)
+
+
+def _near(got, want, bound, what):
+    """|got - want| <= bound elementwise; NaN exactly where ``want`` has it."""
+
+    got = got.double().cpu()
+    assert got.shape == want.shape, what
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in other places"
+    off = torch.where(torch.isnan(want), torch.zeros_like(want), (got - want).abs() - bound)
+    assert float(off.max()) <= 0 if off.numel() else True, f"{what}: {float(off.max()):.3g} above the bound"
+
+
+# ---------------------------------------------------------------------------
+# norm and rotation
+
+
+def _rotary_case(device, *, batch, seq, heads, kv_heads, dim, rotary, dtype, norm="rms", interleaved=False,
+                 params=F32, bias=False, starts=None, rows=None, weights=True, seed=0):
+    from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
+
+    # views of a packed projection's output, as a program has them
+    packed = _rand((batch, seq, heads + 2 * kv_heads, dim), seed, dtype)
+    wq, wk, bq, bk = (_rand((dim,), seed + i, params) if on else None
+                      for i, on in ((1, weights), (2, weights), (3, bias), (4, bias)))
+    most = max([0] if starts is None else starts) + seq
+    table = rotary_table(most if rows is None else rows, rotary, device="cpu") if rotary else None
+    starts_t = None if starts is None else torch.tensor(starts, dtype=torch.int32)
+    to = lambda t: None if t is None else t.to(device)  # noqa: E731
+    on_gpu = packed.to(device)
+    with torch.inference_mode():
+        got = hip_qk_norm_rotary(
+            on_gpu[:, :, :heads].transpose(1, 2), on_gpu[:, :, heads : heads + kv_heads].transpose(1, 2),
+            to(wq), to(wk), to(table), to(starts_t), query_bias=to(bq), key_bias=to(bk), norm=norm,
+            interleaved=interleaved,
+        )
+    assert got[2] == "hip_qk_norm_rotary"
+    for out, view, w, b in ((got[0], packed[:, :, :heads], wq, bq), (got[1], packed[:, :, heads : heads + kv_heads], wk, bk)):
+        want = plain.norm_rotary(view.transpose(1, 2).double(), w, b, table, starts_t, norm=norm, eps=1e-6,
+                                 interleaved=interleaved)
+        # one rounding, and fp32 arithmetic on values of up to a row's largest: a sum of
+        # `dim` squares, a square root and two products of two terms, (dim / 2 + 16) 2^-24
+        size = want.nan_to_num().abs().amax(-1, keepdim=True) * 2 + 1
+        bound = plain.half_step(dtype) * want.nan_to_num().abs() + (dim / 2 + 16) * 2.0**-24 * size
+        assert out.is_contiguous() and out.dtype == dtype
+        _near(out, want, bound, f"rotary batch={batch} seq={seq} dim={dim} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_types_and_head_dims(gpu_device, dtype, dim, interleaved):
+    _rotary_case(gpu_device, batch=2, seq=5, heads=6, kv_heads=2, dim=dim, rotary=dim, dtype=dtype,
+                 interleaved=interleaved, starts=[0, 999], seed=dim)
+
+
+@pytest.mark.parametrize(
+    "changes",
+    [
+        dict(heads=1, kv_heads=1, seq=1),
+        dict(heads=16, kv_heads=16, seq=1),
+        dict(heads=5, kv_heads=3, seq=67),
+        dict(heads=40, kv_heads=5, seq=3),
+        dict(batch=1, heads=12, kv_heads=4, seq=333, starts=[7]),
+        dict(starts=None),
+        dict(rotary=0),
+        dict(rotary=0, norm="layer", bias=True),
+        dict(rotary=32),
+        dict(rotary=16, dim=128),
+        dict(rotary=48),
+        dict(rotary=24, interleaved=True),
+        dict(norm="layer"),
+        dict(norm="layer", bias=True, interleaved=True),
+        dict(bias=True, params=BF16),
+        dict(weights=False),
+        # positions before and behind the table
+        dict(starts=[-2, 20], rows=22, seq=4),
+        dict(starts=[0, 5], rows=8, rotary=32, interleaved=True),
+    ],
+)
+def test_rotary_layouts(gpu_device, changes):
+    sizes = dict(batch=2, seq=4, heads=4, kv_heads=2, dim=64, rotary=64, dtype=BF16, starts=[0, 50], seed=9)
+    _rotary_case(gpu_device, **{**sizes, **changes})
+
+
+def test_rotary_of_zeros_and_broadcast_heads(gpu_device):
+    from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
+
+    table = rotary_table(8, 64, device=gpu_device)
+    one = _rand((1, 1, 4, 64), 3, BF16).to(gpu_device)
+    zeros = torch.zeros(3, 2, 4, 64, dtype=BF16, device=gpu_device)
+    with torch.inference_mode():
+        query, key, _ = hip_qk_norm_rotary(one.expand(3, 6, 4, 64), zeros, None, None, table)
+    want = plain.norm_rotary(one.double().cpu(), None, None, table.cpu(), None, norm="rms", eps=1e-6, interleaved=False)
+    _near(query, want.expand(3, 6, 4, 64), 2.0**-8 * want.abs() + 2.0**-17, "broadcast heads")
+    assert bool((key == 0).all())
+
+
+def test_rotary_refusals(gpu_device):
+    from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
+
+    q, k = (torch.zeros(2, h, 4, 64, dtype=BF16, device=gpu_device) for h in (4, 2))
+    w = torch.ones(64, device=gpu_device)
+    table = rotary_table(8, 64, device=gpu_device)
+    starts = torch.zeros(2, dtype=torch.int32, device=gpu_device)
+    good = dict(query=q, key=k, query_weight=w, key_weight=w, table=table, starts=starts)
+    hip_qk_norm_rotary(**good)
+    for changes in (
+        dict(query=q.double()), dict(key=k.half()), dict(key=k[:1]), dict(query=q[..., :32], key=k[..., :32]),
+        dict(query=q.transpose(2, 3)), dict(query_weight=w[:32]), dict(key_weight=w.half()), dict(starts=starts.long()),
+        dict(starts=starts[:1]), dict(table=table.half()), dict(table=table[:, :40].contiguous()), dict(table=table.t()),
+        dict(table=table.cpu()), dict(norm="batch"), dict(eps=-1.0), dict(query=q[0]),
+        dict(query=q.clone().requires_grad_()), dict(query_weight=w.clone().requires_grad_()),
+    ):
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_qk_norm_rotary(**{**good, **changes})
+
+
+# ---------------------------------------------------------------------------
+# the cache
+
+
+class _Tokens:
+    """Sequences' keys and values as the program appends them, and the cache beside."""
+
+    def __init__(self, device, lengths, kv_heads, dim, dtype, *, room=None, seed=0, spread=1.0, spare=3):
+        from solution.kernels.attention import BlockCache
+
+        self.device, self.dtype, self.lengths = device, dtype, list(lengths)
+        batch, most = len(lengths), max(list(lengths) + [1])
+        room = most if room is None else room
+        width = room // 64 + 1
+        order = torch.randperm(batch * width + spare, generator=torch.Generator().manual_seed(seed + 5))
+        table = order[: batch * width].to(torch.int32).reshape(batch, width)
+        self.key = _rand((batch, kv_heads, most, dim), seed, dtype, spread)
+        self.value = _rand((batch, kv_heads, most, dim), seed + 1, dtype, spread)
+        self.cache = BlockCache.allocate(batch, kv_heads, dim, max_tokens=room, num_blocks=batch * width + spare,
+                                         dtype=dtype, device=device, block_table=table.to(device))
+
+    def append(self, starts, counts, padded=None):
+        """Append tokens starts[b] .. starts[b] + counts[b] - 1 of each sequence."""
+
+        from solution.kernels.attention import hip_block_cache_append
+
+        seq = padded or max(max(counts), 1)
+        batch, heads, _, dim = self.key.shape
+        # rows of a packed projection; what stands behind the counts is not to be read
+        packed = torch.full((batch, seq, 2 * heads, dim), math.nan, dtype=self.dtype)
+        for b, (start, count) in enumerate(zip(starts, counts)):
+            packed[b, :count, :heads] = self.key[b, :, start : start + count].transpose(0, 1)
+            packed[b, :count, heads:] = self.value[b, :, start : start + count].transpose(0, 1)
+        packed = packed.to(self.device)
+        to = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)  # noqa: E731
+        with torch.inference_mode():
+            marker = hip_block_cache_append(
+                self.cache, packed[:, :, :heads].transpose(1, 2), packed[:, :, heads:].transpose(1, 2), to(starts),
+                None if counts == [seq] * batch else to(counts),
+            )
+        assert marker == "hip_block_cache_append"
+
+    def fill(self):
+        self.append([0] * len(self.lengths), self.lengths)
+        return self
+
+    def stored(self, b, h, length=None):
+        length = self.lengths[b] if length is None else length
+        return plain.stored_tokens(self.key[b, h, :length].double(), self.value[b, h, :length].double())
+
+    def read(self, firsts, lengths, tokens):
+        from solution.kernels.attention import hip_block_cache_read
+
+        to = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)  # noqa: E731
+        with torch.inference_mode():
+            key, value, marker = hip_block_cache_read(self.cache, to(firsts), to(lengths), tokens)
+        assert marker == "hip_block_cache_read"
+        return key.double().cpu(), value.double().cpu()
+
+    def check(self, lengths=None):
+        """Everything that the cache holds is what the plain form stores."""
+
+        lengths = self.lengths if lengths is None else lengths
+        batch, heads, _, dim = self.key.shape
+        key, value = self.read([0] * batch, lengths, max(lengths) + 3)
+        for b in range(batch):
+            for h in range(heads):
+                want_key, want_value = self.stored(b, h, lengths[b])
+                n = lengths[b]
+                assert torch.equal(value[b, h, :n], want_value), (b, h)
+                assert torch.equal(key[b, h, :n].nan_to_num(7e4), want_key.nan_to_num(7e4)), (b, h)
+                assert not bool(key[b, h, n:].any()) and not bool(value[b, h, n:].any())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths", [[1], [63], [64], [65], [1, 0, 64, 129, 300, 127]])
+def test_append_stores_what_the_plain_form_stores(gpu_device, lengths, dtype, dim):
+    _Tokens(gpu_device, lengths, 3, dim, dtype, seed=len(lengths)).fill().check()
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 128)])
+def test_cache_does_not_depend_on_the_steps(gpu_device, dtype, dim):
+    whole = _Tokens(gpu_device, [300, 193, 70], 2, dim, dtype, seed=4).fill()
+    steps = _Tokens(gpu_device, [300, 193, 70], 2, dim, dtype, seed=4)
+    held = [0, 0, 0]
+    for chunk in ([1, 1, 1], [62, 0, 64], [1, 130, 0], [1, 1, 5], [64, 1, 0], [150, 0, 0], [1, 60, 0], [20, 0, 0]):
+        steps.append(held, chunk, padded=max(chunk) + 2)
+        held = [a + b for a, b in zip(held, chunk)]
+        steps.check(held)
+    assert held == [300, 193, 70]
+    for name in ("key_codes", "value_codes", "key_scales", "value_scales"):
+        assert torch.equal(getattr(whole.cache, name), getattr(steps.cache, name)), name
+    for b, length in enumerate(held):  # tails up to the last token
+        n = length % 64
+        assert torch.equal(whole.cache.key_tail[b, :, :n], steps.cache.key_tail[b, :, :n])
+        assert torch.equal(whole.cache.value_tail[b, ..., :n], steps.cache.value_tail[b, ..., :n])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scales_of_extreme_blocks(gpu_device, dtype):
+    t = _Tokens(gpu_device, [64 * 6 + 1], 1, 64, dtype, seed=11)
+    most = torch.finfo(dtype).max
+    t.key[0, 0, :64] = 0.0  # a block of zeros
+    t.key[0, 0, 64:128] *= 1e-4
+    t.key[0, 0, 130, 3] = 448.0  # on the border of a scale, and just above it
+    t.key[0, 0, 128:192] = t.key[0, 0, 128:192].clamp(-448, 448)
+    t.key[0, 0, 195, 7] = 450.0 if dtype is BF16 else 448.25
+    t.value[0, 0, :64] = torch.finfo(dtype).smallest_normal
+    t.value[0, 0, 64:128, 5] = most / 2
+    t.value[0, 0, 256:320] = 2.0**-24 if dtype is F16 else 2.0**-133
+    t.fill()
+    scales = t.cache.key_scales.cpu()[t.cache.block_table.cpu()[0, :6].long(), 0]
+    assert scales[0] == 1.0 and scales[2] == 1.0 and scales[3] == 2.0
+    t.check()
+    # the largest value of the type: its code times the scale leaves the type's range, and is read as the largest
+    t = _Tokens(gpu_device, [64], 1, 64, dtype, seed=12)
+    t.value[0, 0, 9, 9] = most
+    t.fill()
+    _, value = t.read([0], [64], 64)
+    assert value[0, 0, 9, 9] == most
+
+
+def test_non_finite_tokens_are_kept_apart(gpu_device):
+    t = _Tokens(gpu_device, [200, 130], 2, 64, BF16, seed=21)
+    t.key[0, 1, 5, 3] = math.nan
+    t.key[0, 0, 70, 0] = math.inf
+    t.value[0, 0, 71, 63] = -math.inf
+    t.value[1, 1, 129, 1] = math.nan  # in the tail
+    t.key[1, 0, 128] = math.nan
+    t.fill().check()
+    # the same token by token around the border of a block: a tail's NaN is coded later
+    t2 = _Tokens(gpu_device, [200, 130], 2, 64, BF16, seed=21)
+    t2.key, t2.value = t.key, t.value
+    t2.append([0, 0], [63, 127])
+    t2.append([63, 127], [10, 2])
+    t2.append([73, 129], [127, 1])
+    t2.check()
+
+
+def test_read_of_any_span(gpu_device):
+    t = _Tokens(gpu_device, [200, 130, 0], 2, 64, F16, seed=31).fill()
+    whole = [torch.stack([t.stored(b, h)[i].nan_to_num() if t.lengths[b] else torch.zeros(0, 64).double()
+                          for b in range(1) for h in range(2)]) for i in range(2)]
+    for firsts, tokens in (([0, 0, 0], 0), ([63, 1, 0], 1), ([70, 129, 5], 90), ([-5, -70, -1], 100), ([199, 500, 64], 70)):
+        got = t.read(firsts, t.lengths, tokens)
+        for i in range(2):
+            assert got[i].shape == (3, 2, tokens, 64)
+            for row in range(tokens):
+                p = firsts[0] + row
+                want = whole[i][:, p] if 0 <= p < 200 else torch.zeros(2, 64).double()
+                assert torch.equal(got[i][0, :, row], want), (firsts, row)
+            assert not bool(got[i][2].any())
+
+
+def test_pages_outside_the_cache(gpu_device):
+    from solution.kernels.attention import hip_block_cache_attention
+
+    t = _Tokens(gpu_device, [300, 300, 300], 2, 64, BF16, seed=41)
+    codes = t.cache.key_codes.clone()
+    t.cache.block_table[0, 1] = t.cache.key_codes.shape[0]
+    t.cache.block_table[1, 3] = -1
+    t.fill()
+    key, value = t.read([0] * 3, [300] * 3, 300)
+    lost = torch.zeros(3, 300, dtype=torch.bool)
+    lost[0, 64:128] = lost[1, 192:256] = True
+    assert bool((key.isnan().all(-1) == lost[:, None]).all()) and bool((value.isnan().all(-1) == lost[:, None]).all())
+    named = t.cache.block_table[t.cache.block_table.ge(0) & t.cache.block_table.lt(codes.shape[0])].long()
+    others = torch.ones(codes.shape[0], dtype=torch.bool, device=gpu_device)
+    others[named] = False
+    assert torch.equal(t.cache.key_codes[others], codes[others])
+    # rows before the lost page answer, rows that see it are NaN
+    query = _rand((3, 4, 130, 64), 42, BF16).to(gpu_device)
+    starts = torch.tensor([0, 150, 170], dtype=torch.int32, device=gpu_device)
+    with torch.inference_mode():
+        out = hip_block_cache_attention(query, t.cache, starts)[0].cpu()
+    bad = out.isnan().all(-1)
+    assert bool(out.isnan().any(-1).eq(bad).all())
+    position = starts.cpu()[:, None] + torch.arange(130)
+    first_lost = torch.tensor([64, 192, 10**6])[:, None]
+    assert torch.equal(bad, position >= first_lost)
+
+
+def test_lengths_beyond_the_table_and_sequences_without_tokens(gpu_device):
+    from solution.kernels.attention import hip_block_cache_append, hip_block_cache_attention
+
+    t = _Tokens(gpu_device, [100, 100, 100], 2, 64, BF16, room=127, seed=51).fill()
+    assert t.cache.block_table.shape[1] == 2
+    before = {n: getattr(t.cache, n).clone() for n in ("key_codes", "value_codes", "key_tail", "value_tail", "key_scales")}
+    kv = _rand((3, 2, 2, 64), 52, BF16).to(gpu_device)
+    starts = torch.tensor([-1, 100, 2**31 - 1], dtype=torch.int32, device=gpu_device)
+    counts = torch.tensor([2, -3, 0], dtype=torch.int32, device=gpu_device)
+    with torch.inference_mode():
+        hip_block_cache_append(t.cache, kv, kv, starts, counts)
+        for name, want in before.items():
+            assert torch.equal(getattr(t.cache, name), want), name
+        query = _rand((3, 4, 2, 64), 53, BF16).to(gpu_device)
+        out = hip_block_cache_attention(query, t.cache, starts, counts)[0]
+        assert not bool(out.any())
+        # more tokens than the table has room for: NaN, and an end
+        far = torch.tensor([192, 2**31 - 64, 98], dtype=torch.int32, device=gpu_device)
+        out = hip_block_cache_attention(query, t.cache, far)[0].cpu()
+    assert bool(out[:2].isnan().all()) and bool(out[2].isfinite().all())
+
+
+# ---------------------------------------------------------------------------
+# attention over the cache
+
+
+def _attend(t, query, starts, counts=None, **options):
+    from solution.kernels.attention import hip_block_cache_attention
+
+    to = lambda v: None if v is None else torch.tensor(v, dtype=torch.int32, device=t.device)  # noqa: E731
+    with torch.inference_mode():
+        out, marker = hip_block_cache_attention(query.to(t.device), t.cache, to(starts), to(counts), **options)
+    assert marker == "hip_block_cache_attention"
+    return out.cpu()
+
+
+def _check_attention(t, query, starts, counts=None, *, scale=None, rows=None, **options):
+    """Every row (or the rows named) against the plain form over what the cache stands for."""
+
+    batch, heads, seq, dim = query.shape
+    group = heads // t.key.shape[1]
+    out = _attend(t, query, starts, counts, scale=scale, **options)
+    assert out.shape == (batch, seq, heads * dim) and out.dtype == t.dtype
+    out = out.reshape(batch, seq, heads, dim)
+    scale = dim**-0.5 if scale is None else scale
+    for b in range(batch):
+        count = seq if counts is None else counts[b]
+        assert not bool(out[b, count:].any())
+        for h in range(heads):
+            keys, values = t.stored(b, h // group, starts[b] + count)
+            for i in range(count) if rows is None else [r for r in rows if r < count]:
+                q = query[b, h, i].double()
+                want, size = plain.attention(q, keys, values, starts[b] + i, scale)
+                bound = plain.attention_bound(want, size, q, keys, starts[b] + i, scale, t.dtype)
+                _near(out[b, i, h], want, bound, f"attention sequence {b} head {h} row {i} of {starts[b]}+{count}")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 2), (12, 1), (20, 1), (6, 2)])
+def test_one_token_over_ragged_histories(gpu_device, heads, kv_heads, dtype, dim):
+    lengths = [1, 2, 63, 64, 65, 128, 129, 500, 1100]
+    t = _Tokens(gpu_device, lengths, kv_heads, dim, dtype, seed=heads + dim).fill()
+    query = _rand((len(lengths), heads, 1, dim), 61, dtype)
+    _check_attention(t, query, [n - 1 for n in lengths])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 4, 64, BF16), (8, 2, 64, F16), (4, 1, 128, BF16), (3, 3, 128, F16)])
+@pytest.mark.parametrize("seq", [2, 5, 17, 33, 70, 150])
+def test_chunks_over_ragged_histories(gpu_device, seq, heads, kv_heads, dim, dtype):
+    counts = [seq, 1, max(1, seq // 2), 0, seq]
+    starts = [0, 130, 61, 40, 700]
+    t = _Tokens(gpu_device, [a + b for a, b in zip(starts, counts)], kv_heads, dim, dtype, seed=seq).fill()
+    query = _rand((5, heads, seq, dim), 71, dtype)
+    rows = None if seq <= 17 else [0, 1, 2, 3, 15, 16, 31, 32, 47, 63, 64, 69, 100, seq - 1]
+    _check_attention(t, query, starts, counts, rows=rows)
+
+
+@pytest.mark.parametrize("max_length", [None, 1, 500, 5000])
+@pytest.mark.parametrize("seq", [1, 20, 80])
+def test_long_histories_in_parts(gpu_device, seq, max_length):
+    starts = [4990 - seq, 63, 2500, 0]
+    t = _Tokens(gpu_device, [s + seq for s in starts], 1, 64, BF16, room=6000, seed=81).fill()
+    query = _rand((4, 2, seq, 64), 82, BF16)
+    _check_attention(t, query, starts, rows=[0, 7, seq - 1], max_length=max_length)
+
+
+@pytest.mark.parametrize("scale", [0.5, -0.125, 0.0, 1e-30, 3.0])
+@pytest.mark.parametrize("seq", [1, 40])
+def test_scales_of_the_scores(gpu_device, scale, seq):
+    t = _Tokens(gpu_device, [seq + 100, seq + 3], 2, 64, BF16, seed=91).fill()
+    _check_attention(t, _rand((2, 4, seq, 64), 92, BF16), [100, 3], scale=scale)
+
+
+def test_blocks_of_very_different_sizes(gpu_device):
+    t = _Tokens(gpu_device, [64 * 5 + 10], 1, 64, BF16, seed=95)
+    for block, size in enumerate((1e-30, 1e20, 1e-6, 0.0, 1e30)):
+        t.value[0, 0, 64 * block : 64 * block + 64] *= size
+    t.key[0, 0, 64:128] *= 30.0
+    t.key[0, 0, 256:320] = 0.0
+    t.fill()
+    _check_attention(t, _rand((1, 8, 1, 64), 96, BF16), [t.lengths[0] - 1])
+    _check_attention(t, _rand((1, 3, 329, 64), 97, BF16), [0], [329], rows=[0, 63, 64, 127, 200, 255, 256, 328])
+
+
+def test_strided_queries_and_broadcast_heads(gpu_device):
+    from solution.kernels.attention import hip_block_cache_attention
+
+    t = _Tokens(gpu_device, [150, 90], 2, 64, BF16, seed=101).fill()
+    packed = _rand((2, 3, 10, 64), 102, BF16)
+    _check_attention(t, packed[:, :, 1:7].transpose(1, 2), [147, 87])
+    wide = packed.to(gpu_device)[:, :, 1:7].transpose(1, 2)
+    assert not wide.is_contiguous()
+    starts = torch.tensor([147, 87], dtype=torch.int32, device=gpu_device)
+    with torch.inference_mode():
+        assert torch.equal(hip_block_cache_attention(wide, t.cache, starts)[0],
+                           hip_block_cache_attention(wide.contiguous(), t.cache, starts)[0])
+        one = wide[:, :1].expand(2, 6, 3, 64)
+        assert torch.equal(hip_block_cache_attention(one, t.cache, starts)[0],
+                           hip_block_cache_attention(one.contiguous(), t.cache, starts)[0])
+
+
+@pytest.mark.parametrize("seq", [1, 30])
+def test_non_finite_tokens_touch_only_the_rows_that_see_them(gpu_device, seq):
+    length = 200
+    for place in (length - 1, length - 20, 70):
+        clean = _Tokens(gpu_device, [length], 2, 64, BF16, seed=111)
+        bad = _Tokens(gpu_device, [length], 2, 64, BF16, seed=111)
+        for t in (clean, bad):  # the same coded blocks: the token takes no part in a scale
+            t.key[0, 0, place] = t.value[0, 0, place] = 0.0
+        bad.value[0, 0, place, 3] = math.nan
+        query = _rand((1, 4, seq, 64), 112, BF16)
+        start = length - seq
+        want, got = (_attend(t.fill(), query, [start]).reshape(seq, 4, 64) for t in (clean, bad))
+        sees = torch.arange(start, length) >= place
+        assert bool(got[sees][:, :2].isnan().all())
+        assert torch.equal(got[~sees], want[~sees]) and torch.equal(got[:, 2:], want[:, 2:])
+
+
+def test_what_stands_behind_the_last_token_is_not_read(gpu_device):
+    t = _Tokens(gpu_device, [70, 64], 2, 64, BF16, seed=121).fill()
+    query = _rand((2, 4, 1, 64), 122, BF16)
+    want = _attend(t, query, [69, 63])
+    t.cache.key_tail[0, :, 6:] = math.nan
+    t.cache.value_tail[0, ..., 6:] = math.nan
+    t.cache.key_tail[1] = math.nan
+    t.cache.value_tail[1] = math.nan
+    spare = torch.ones(t.cache.key_codes.shape[0], dtype=torch.bool, device=gpu_device)
+    spare[t.cache.block_table[:, 0].long()] = False
+    t.cache.key_codes[spare] = 0x7F
+    t.cache.value_codes[spare] = 0x7F
+    t.cache.block_table[:, 1:] = -1
+    assert torch.equal(_attend(t, query, [69, 63]), want)
+
+
+def test_blocks_shared_by_sequences(gpu_device):
+    """A common beginning is held once: the second sequence's table names the first's blocks."""
+
+    t = _Tokens(gpu_device, [200, 192], 2, 64, F16, seed=131)
+    t.key[1, :, :192], t.value[1, :, :192] = t.key[0, :, :192], t.value[0, :, :192]
+    t.append([0, 0], [200, 0])
+    t.cache.block_table[1, :3] = t.cache.block_table[0, :3]
+    query = _rand((1, 4, 1, 64), 132, F16).expand(2, 4, 1, 64)
+    # the second holds the 192 tokens of the blocks, and asks from the last of them
+    _check_attention(t, query.contiguous(), [199, 191])
+
+
+def test_cache_of_more_than_four_gigabytes(gpu_device):
+    from solution.kernels.attention import BlockCache
+
+    t = _Tokens(gpu_device, [130, 70], 16, 64, BF16, seed=141)
+    blocks = 70_001  # 64 KiB of codes each, for keys and for values
+    table = torch.tensor([[70_000, 65_537, 3], [66_000, 0, 32_768]], dtype=torch.int32, device=gpu_device)
+    t.cache = BlockCache.allocate(2, 16, 64, max_tokens=200, num_blocks=blocks, dtype=BF16, device=gpu_device, block_table=table)
+    t.fill().check()
+    _check_attention(t, _rand((2, 16, 1, 64), 142, BF16), [129, 69])
+
+
+def test_attention_refusals(gpu_device):
+    from solution.kernels.attention import hip_block_cache_append, hip_block_cache_attention, hip_block_cache_read
+
+    t = _Tokens(gpu_device, [70, 64], 2, 64, BF16, seed=151).fill()
+    q = torch.zeros(2, 4, 1, 64, dtype=BF16, device=gpu_device)
+    starts = torch.tensor([69, 63], dtype=torch.int32, device=gpu_device)
+    good = dict(query=q, cache=t.cache, starts=starts)
+    hip_block_cache_attention(**good)
+    for changes in (
+        dict(query=q.half()), dict(query=q[:, :3]), dict(query=q[:1]), dict(query=q[..., :32]), dict(query=q.cpu()),
+        dict(query=q[:, :0]), dict(query=torch.zeros(2, 4, 3, 68, dtype=BF16, device=gpu_device)[..., :64]),
+        dict(starts=starts.long()), dict(starts=starts[:1]), dict(starts=None), dict(starts=starts.cpu()),
+        dict(counts=starts.long()), dict(scale=math.inf), dict(max_length=-1), dict(query=q.clone().requires_grad_()),
+    ):
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_block_cache_attention(**{**good, **changes})
+    kv = torch.zeros(2, 2, 1, 64, dtype=BF16, device=gpu_device)
+    for key, value in ((kv[:, :1], kv[:, :1]), (kv, kv[:, :, :0]), (kv.half(), kv.half()), (kv, kv.float())):
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_block_cache_append(t.cache, key, value, starts)
+    for tokens in (-1, 2.0, True):
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_block_cache_read(t.cache, starts, starts, tokens)
+
+
+# ---------------------------------------------------------------------------
+# the 4-bit linear layer
+
+
+def _linear_case(device, rows, k, n, group, dtype, *, bias=True, gelu=False, seed=0):
+    from solution.kernels.projection import hip_linear_w4, pack_linear_w4_codes
+
+    generator = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-7, 8, (n, k), generator=generator)
+    scales = (torch.rand(n, k // group, generator=generator) * 0.02 + 0.001).to(dtype)
+    packed = pack_linear_w4_codes(codes.to(device), scales.to(device))
+    x = _rand((rows, k), seed + 1, dtype)
+    b = _rand((n,), seed + 2, dtype) if bias else None
+    with torch.inference_mode():
+        got, marker = hip_linear_w4(x.to(device), packed, None if b is None else b.to(device),
+                                    activation="gelu" if gelu else "none")
+    assert marker == "hip_linear_w4" and got.dtype == dtype
+    weight = codes.double() * scales.double().repeat_interleave(group, dim=1)
+    want, size = plain.linear(x.double(), weight, None if b is None else b.double(), gelu)
+    _near(got, want, plain.linear_bound(want, size, k, gelu, dtype), f"linear {rows}x{k}x{n} group {group} {dtype}")
+
+
+@pytest.mark.parametrize("rows", [1, 2, 13, 16, 17, 32, 33, 64, 65, 130])
+@pytest.mark.parametrize("dtype,group", [(BF16, 32), (BF16, 128), (F16, 64)])
+def test_linear_w4_rows(gpu_device, rows, dtype, group):
+    _linear_case(gpu_device, rows, 640, 80, group, dtype, seed=rows)
+
+
+@pytest.mark.parametrize("k,n", [(128, 16), (128, 4096), (1024, 48), (2176, 1024), (4096, 272), (16384, 32)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("gelu", [False, True])
+def test_linear_w4_sizes(gpu_device, k, n, group, gelu):
+    _linear_case(gpu_device, 3, k, n, group, BF16 if group != 64 else F16, bias=n != 48, gelu=gelu, seed=k + n)
+
+
+def test_linear_w4_layouts_and_extremes(gpu_device):
+    from solution.kernels.projection import hip_linear_w4, quantize_linear_w4
+
+    weight = _rand((64, 256), 161, BF16).to(gpu_device)
+    weight[3] = 0.0
+    packed = quantize_linear_w4(weight, 32)
+    wide = _rand((2, 3, 512), 162, BF16).to(gpu_device)
+    with torch.inference_mode():
+        x = wide[:, :, 128:384]
+        assert torch.equal(hip_linear_w4(x, packed)[0], hip_linear_w4(x.contiguous(), packed)[0])
+        one = wide[0, 0, :256]
+        assert torch.equal(hip_linear_w4(one, packed)[0], hip_linear_w4(one[None], packed)[0][0])
+        same = one.expand(5, 256)
+        assert torch.equal(hip_linear_w4(same, packed)[0], hip_linear_w4(same.contiguous(), packed)[0])
+        assert hip_linear_w4(wide[:0, :, :256], packed)[0].shape == (0, 3, 64)
+        # a row's infinities and NaN stay in the row; large inputs lose nothing
+        x = _rand((20, 256), 163, BF16).to(gpu_device)
+        want = hip_linear_w4(x, packed)[0]
+        x2 = x.clone()
+        x2[4, 7], x2[18, 200] = math.nan, math.inf
+        got = hip_linear_w4(x2, packed)[0]
+        keep = [i for i in range(20) if i not in (4, 18)]
+        assert torch.equal(got[keep], want[keep]) and bool(got[4].isnan().all())
+        big = hip_linear_w4((x * 2.0**100).to(BF16), packed)[0]
+        assert torch.equal(big, (want.float() * 2.0**100).to(BF16))
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_linear_w4(wide.transpose(0, 1)[:, :, :256], packed)  # rows at two strides
+    for x in (wide[..., :128], wide[..., :256].half(), wide[..., 4:260], wide[..., :256].cpu(),
+              torch.zeros(2, 256, dtype=BF16, device=gpu_device).requires_grad_()):
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_linear_w4(x, packed)
+    for bias in (torch.zeros(32, dtype=BF16, device=gpu_device), torch.zeros(64, device=gpu_device)):
+        with pytest.raises(RuntimeError, match="ineligible"):
+            hip_linear_w4(one, packed, bias)
+    with pytest.raises(RuntimeError, match="ineligible"):
+        hip_linear_w4(one, packed, activation="relu")
+
+
+# ---------------------------------------------------------------------------
+# a decoding step
+
+
+class _Layer:
+    """One layer's attention branch with all four operators: 4-bit projections, the
+    norm and rotation of heads, the cache and the attention over it."""
+
+    def __init__(self, device, batch, heads, kv_heads, dim, dtype, max_tokens, seed=0):
+        from solution.kernels.attention import BlockCache
+        from solution.kernels.norm import rotary_table
+        from solution.kernels.projection import quantize_linear_w4
+
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, dim
+        width = heads * dim
+        self.width = width
+        self.qkv = quantize_linear_w4(_rand(((heads + 2 * kv_heads) * dim, width), seed, dtype, width**-0.5).to(device), 64)
+        self.out = quantize_linear_w4(_rand((width, width), seed + 1, dtype, width**-0.5).to(device), 64)
+        self.bias = _rand(((heads + 2 * kv_heads) * dim,), seed + 2, dtype).to(device)
+        self.wq, self.wk = (1 + _rand((dim,), seed + i, F32, 0.2).to(device) for i in (3, 4))
+        self.table = rotary_table(max_tokens, dim, device=device)
+        self.cache = BlockCache.allocate(batch, kv_heads, dim, max_tokens=max_tokens, dtype=dtype, device=device)
+
+    def __call__(self, x, starts, counts=None):
+        from solution.kernels.attention import hip_block_cache_append, hip_block_cache_attention
+        from solution.kernels.norm import hip_qk_norm_rotary
+        from solution.kernels.projection import hip_linear_w4
+
+        batch, seq, _ = x.shape
+        packed = hip_linear_w4(x, self.qkv, self.bias)[0].view(batch, seq, -1, self.dim)
+        ends = self.heads, self.heads + self.kv_heads
+        query, key, value = (t.transpose(1, 2) for t in packed.tensor_split(ends, dim=2))
+        query, key, _ = hip_qk_norm_rotary(query, key, self.wq, self.wk, self.table, starts)
+        hip_block_cache_append(self.cache, key, value, starts, counts)
+        context, _ = hip_block_cache_attention(query, self.cache, starts, counts)
+        return hip_linear_w4(context, self.out)[0], (packed, query, key, value, context)
+
+
+def test_a_prompt_and_tokens_through_all_operators(gpu_device):
+    """A ragged prompt, then token by token, every operator's answer against the
+    plain form of what it was given."""
+
+    batch, heads, kv_heads, dim = 3, 6, 2, 64
+    layer = _Layer(gpu_device, batch, heads, kv_heads, dim, BF16, 400, seed=171)
+    qkv, out_weight = (w.dequantize().double().cpu() for w in (layer.qkv, layer.out))
+    starts = torch.zeros(batch, dtype=torch.int32, device=gpu_device)
+    held = [[], [], []]  # (key, value) of each sequence so far
+    for step, counts in enumerate([[130, 61, 1], None, None, None, [5, 1, 70], None]):
+        seq = 1 if counts is None else max(counts)
+        x = _rand((batch, seq, layer.width), 180 + step, BF16)
+        counts_t = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=gpu_device)
+        with torch.inference_mode():
+            y, parts = layer(x.to(gpu_device), starts, counts_t)
+        packed, query, key, value, context = (p.cpu() for p in parts)
+        want, size = plain.linear(x.double().reshape(-1, layer.width), qkv, layer.bias.double().cpu(), False)
+        _near(packed.reshape(want.shape), want, plain.linear_bound(want, size, layer.width, False, BF16), "projection")
+        first = starts.cpu()
+        for got, view, weight in ((query, packed[:, :, :heads], layer.wq), (key, packed[:, :, heads : heads + kv_heads], layer.wk)):
+            want = plain.norm_rotary(view.transpose(1, 2).double(), weight.cpu(), None, layer.table.cpu(), first,
+                                     norm="rms", eps=1e-6, interleaved=False)
+            size = want.abs().amax(-1, keepdim=True) * 2 + 1
+            _near(got, want, 2.0**-8 * want.abs() + 48 * 2.0**-24 * size, "norm and rotation")
+        context = context.reshape(batch, seq, heads, dim)
+        for b in range(batch):
+            count = 1 if counts is None else counts[b]
+            held[b].append((key[b, :, :count], value[b, :, :count]))
+            all_key, all_value = (torch.cat([t[i] for t in held[b]], dim=1).double() for i in range(2))
+            for h in (0, 2, 3, 5):
+                keys, values = plain.stored_tokens(all_key[h // 3], all_value[h // 3])
+                for i in {0, count // 2, count - 1}:
+                    q, position = query[b, h, i].double(), int(first[b]) + i
+                    want, size = plain.attention(q, keys, values, position, dim**-0.5)
+                    bound = plain.attention_bound(want, size, q, keys, position, dim**-0.5, BF16)
+                    _near(context[b, i, h], want, bound, f"step {step} sequence {b} head {h} row {i}")
+        want, size = plain.linear(context.double().reshape(-1, layer.width), out_weight, None, False)
+        _near(y.reshape(want.shape), want, plain.linear_bound(want, size, layer.width, False, BF16), "output projection")
+        starts += torch.tensor(counts, dtype=torch.int32, device=gpu_device) if counts else 1
+
+
+def test_captured_steps_replay_as_eager_ones(gpu_device):
+    """Token after token from one captured graph, beside eager work: across the
+    border of a block, against the same steps run eagerly."""
+
+    batch = 4
+    layers = [_Layer(gpu_device, batch, 8, 2, 64, BF16, 3000, seed=191) for _ in range(2)]
+    prompt = _rand((batch, 123, 512), 192, BF16).to(gpu_device)
+    tokens = [_rand((batch, 1, 512), 193 + i, BF16).to(gpu_device) for i in range(8)]
+    with torch.inference_mode():
+        zeros = torch.zeros(batch, dtype=torch.int32, device=gpu_device)
+        for layer in layers:
+            layer(prompt, zeros)
+        starts = torch.full((batch,), 123, dtype=torch.int32, device=gpu_device)
+        x = tokens[0].clone()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+            y = layers[0](x, starts)[0]
+            starts += 1
+        torch.cuda.current_stream().wait_stream(stream)
+        eager_starts = torch.full((batch,), 123, dtype=torch.int32, device=gpu_device)
+        for i, token in enumerate(tokens):
+            want = layers[1](token, eager_starts)[0]
+            eager_starts += 1
+            x.copy_(token)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), f"step {i}"
+        assert torch.equal(starts, eager_starts)
+    for name in ("key_codes", "value_codes", "key_scales", "key_tail", "value_tail"):
+        assert torch.equal(getattr(layers[0].cache, name), getattr(layers[1].cache, name)), name
+
+
+def test_two_streams_at_once(gpu_device):
+    """Calls that overlap on two streams have workspaces of their own."""
+
+    layers = [_Layer(gpu_device, 2, 8, 8, 64, BF16, 5000, seed=201 + i) for i in range(2)]
+    x = _rand((2, 4000, 512), 203, BF16).to(gpu_device)
+    token = _rand((2, 1, 512), 204, BF16).to(gpu_device)
+    starts = torch.full((2,), 4000, dtype=torch.int32, device=gpu_device)
+    with torch.inference_mode():
+        for layer in layers:
+            layer(x, torch.zeros_like(starts))
+        want = [layer(token, starts)[0] for layer in layers]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in layers]
+        got = [[], []]
+        for _ in range(5):
+            for layer, stream, out in zip(layers, streams, got):
+                with torch.cuda.stream(stream):
+                    out.append(layer(token, starts)[0])
+        torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, y) for y in g)
