@@ -62,13 +62,35 @@ struct AttentionArgs {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The maximum over the four lanes l % 16 + {0, 16, 32, 48}.
+__device__ __forceinline__ float quarters_max(float x) {
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+  const uint32_t a = __float_as_uint(x);
+  const u32x2_t h = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a, a, false, false));
+  const float y = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  const uint32_t c = __float_as_uint(y);
+  const u32x2_t g = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(c, c, false, false));
+  return fmaxf(__uint_as_float(g[0]), __uint_as_float(g[1]));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Powers of two by their fp32 bits: 2^a / 2^b, 2^-126 where it is less.
+__device__ __forceinline__ float power_ratio(int a_bits, int b_bits) {
+  const int bits = 0x3f800000 + (a_bits - b_bits);
+  return __int_as_float(bits < 0x00800000 ? 0x00800000 : bits);
+}
+
 // One block's codes of a wave: 16 bytes of a key row (value feature) a lane and tile.
 template <int D>
-struct BlockCodes {
-  u32x4 k[4][D / 64];
-  u32x4 v[D / 16];
-  float k_scale, v_scale;
-  bool held;
+struct KeyCodes {
+  u32x4 part[4][D / 64];
+};
+template <int D>
+struct ValueCodes {
+  u32x4 part[D / 16];
 };
 
 template <typename T, int D, int TILES, int SPLIT, int ROWS>
@@ -76,6 +98,12 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
   typedef typename Vec8<T>::type V8;
   constexpr int HALVES = D / 64;
   constexpr int FEATURES = D / 16;
+  // One tile of rows waits for memory: keys and values of the next block are loaded
+  // while this one is worked on.  More tiles work: the values come while the scores
+  // are formed and the next keys during the rest, in half the registers.
+  constexpr bool AHEAD = TILES == 1;
+  // With more tiles the matrix cores add up the weights too (a row of ones).
+  constexpr bool ONES = TILES > 1;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15;    // query row of a tile; key row / value feature of an operand
@@ -91,36 +119,39 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
   const int64_t b = at / (uint32_t)a.kv_heads;
 
   const int64_t start = a.starts[b];
-  int64_t count = a.counts != nullptr ? (int64_t)a.counts[b] : (int64_t)a.seq_len;
+  int count = a.counts != nullptr ? a.counts[b] : a.seq_len;
   if (count > a.seq_len) count = a.seq_len;
   if (start < 0 || count < 0) count = 0;
+  // More tokens than the table can name: NaN.  Otherwise positions are below 2^31.
+  const bool beyond = (start + count) / kBlockTokens > a.max_blocks;
+  const int first_position = beyond ? 0 : (int)start;
+  const int tail_block = beyond ? 0 : (int)((start + count) / kBlockTokens);
 
   // This lane's rows: token row / group of the chunk, query head h * group + row % group.
   const uint32_t first_row = row_group * (TILES * 16);  // rows are below 2^31
-  int64_t token[TILES];
-  int head[TILES];
-  int64_t last_position = -1, least_position = INT64_MAX;  // of the wave's rows
+  int token[TILES], head[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     const uint32_t row = first_row + t * 16 + column;
-    const uint32_t i = row / (uint32_t)a.group;
-    token[t] = i;
-    head[t] = h * a.group + (int)(row - i * (uint32_t)a.group);
+    token[t] = (int)(row / (uint32_t)a.group);
+    head[t] = h * a.group + (int)(row - (uint32_t)token[t] * (uint32_t)a.group);
   }
+  int last_position = -1, least_position = INT32_MAX;  // of the wave's rows
   {
-    const int64_t low = first_row / (uint32_t)a.group, high = (first_row + TILES * 16 - 1) / (uint32_t)a.group;
+    const int low = (int)(first_row / (uint32_t)a.group);
+    const int high = (int)((first_row + TILES * 16 - 1) / (uint32_t)a.group);
     if (low < count) {
-      least_position = start + low;
-      last_position = start + (high < count ? high : count - 1);
+      least_position = first_position + low;
+      last_position = first_position + (high < count ? high : count - 1);
     }
   }
   // Positions up to which a row sees; rows without a query see as far as the last.
-  int64_t sees[TILES];
+  int sees[TILES];
   V8 q[TILES][HALVES][2];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     const bool live = token[t] < count;
-    sees[t] = live ? start + token[t] : last_position;
+    sees[t] = live ? first_position + token[t] : last_position;
 #pragma unroll
     for (int hh = 0; hh < HALVES; ++hh)
 #pragma unroll
@@ -136,28 +167,42 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
   }
 
   // Blocks of this wave: the row group's, in chunks, the last chunk with the rest.
-  const int64_t tail_block = (start + count) / kBlockTokens;
-  const bool beyond = tail_block > a.max_blocks;  // more than the table can name
-  const int64_t all_blocks = last_position < 0 || beyond ? 0 : last_position / kBlockTokens + 1;
-  int64_t from = (int64_t)chunk * a.chunk_blocks;
-  const int64_t to = chunk == a.chunks - 1 || from + a.chunk_blocks > all_blocks ? all_blocks : from + a.chunk_blocks;
-  const int64_t coded_to = to < tail_block ? to : tail_block;
+  const int all_blocks = last_position < 0 || beyond ? 0 : last_position / kBlockTokens + 1;
+  const int64_t from64 = (int64_t)chunk * a.chunk_blocks;
+  const int from = from64 < all_blocks ? (int)from64 : all_blocks;
+  const int to = chunk == a.chunks - 1 || all_blocks - from < a.chunk_blocks ? all_blocks : from + a.chunk_blocks;
+  const int coded_to = to < tail_block ? to : tail_block;
 
+  // Outputs are held in units of a power of two, the largest value scale so far.
   f32x4 out[TILES][FEATURES];
+  int unit = 0;  // its bits; 0 before the first block
   float most[TILES], sum[TILES];
+  f32x4 sums[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     most[t] = -INFINITY;
     sum[t] = beyond && last_position >= 0 ? __builtin_nanf("") : 0.0f;
+    sums[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int f = 0; f < FEATURES; ++f) out[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   }
+  auto raise_unit = [&](int bits) {
+    if (bits <= unit) return;
+    if (unit != 0) {
+      const float change = power_ratio(unit, bits);
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) out[t][f] *= change;
+    }
+    unit = bits;
+  };
 
   // The weights of a tile's row for one block, from its scores (16 tokens of the row
   // in this lane): the running maximum, sum and output are brought to it.
-  auto softmax_step = [&](int t, f32x4 (&s)[4], float factor, int64_t block) {
+  auto softmax_step = [&](int t, f32x4 (&s)[4], float factor, int block, bool add) {
     if (block * kBlockTokens + (kBlockTokens - 1) > least_position) {
-      const int64_t open = sees[t] - block * kBlockTokens - quarter * 16;  // last visible of this lane's tokens
+      const int open = sees[t] - block * kBlockTokens - quarter * 16;  // last visible of this lane's tokens
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -166,15 +211,17 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
     }
     float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
-    for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    for (int i = 1; i < 4; ++i) {
+      top = fmaxf(fmaxf(top, s[i][0]), s[i][1]);
+      top = fmaxf(fmaxf(top, s[i][2]), s[i][3]);
+    }
     const float before = most[t];
-    const float now = fmaxf(before, top * factor);
+    const float now = fmaxf(before, quarters_max(top) * factor);
     if (__any(now > before)) {
       // a row that has seen nothing yet has no output to rescale
       const float change = before == -INFINITY ? 0.0f : exp2_fast(before - now);
-      sum[t] = sum[t] * change;
+      sum[t] *= change;
+      if (ONES) sums[t] *= change;
 #pragma unroll
       for (int f = 0; f < FEATURES; ++f) out[t][f] *= change;
       most[t] = now;
@@ -186,87 +233,140 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         s[i][j] = exp2_fast(fmaf(s[i][j], factor, shift));
-        lane_sum += s[i][j];
+        if (add) lane_sum += s[i][j];
       }
-    sum[t] += lane_sum;
+    if (add) sum[t] += lane_sum;
   };
 
-  auto load_block = [&](BlockCodes<D>& c, int64_t block) {
-    const int64_t id = (int64_t)a.table[b * a.max_blocks + block];
-    c.held = id >= 0 && id < a.blocks;  // block < tail_block <= max_blocks
-    const int64_t entry = (c.held ? id : 0) * a.kv_heads + h;
-    if (!c.held) return;
-    const uint8_t* keys = a.key_codes + entry * (kBlockTokens * D) + quarter * 16;
-    const uint8_t* values = a.value_codes + entry * (kBlockTokens * D) + quarter * 16;
+  auto load_keys = [&](KeyCodes<D>& c, int id) {
+    const uint8_t* keys = a.key_codes + ((int64_t)id * a.kv_heads + h) * (kBlockTokens * D) + quarter * 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int hh = 0; hh < HALVES; ++hh)
-        c.k[i][hh] = load16(keys + ((column >> 2) * 16 + i * 4 + (column & 3)) * D + hh * 64);
+        c.part[i][hh] = load16(keys + ((column >> 2) * 16 + i * 4 + (column & 3)) * D + hh * 64);
+  };
+  auto load_values = [&](ValueCodes<D>& c, int id) {
+    const uint8_t* values = a.value_codes + ((int64_t)id * a.kv_heads + h) * (kBlockTokens * D) + quarter * 16;
 #pragma unroll
-    for (int f = 0; f < FEATURES; ++f) c.v[f] = load16(values + (f * 16 + column) * kBlockTokens);
-    c.k_scale = a.key_scales[entry];
-    c.v_scale = a.value_scales[entry];
+    for (int f = 0; f < FEATURES; ++f) c.part[f] = load16(values + (f * 16 + column) * kBlockTokens);
   };
 
-  const int64_t first = from + split;
-  BlockCodes<D> next;
-  if (first < coded_to) load_block(next, first);
-  for (int64_t block = first; block < coded_to; block += SPLIT) {
-    const BlockCodes<D> c = next;
-    if (block + SPLIT < coded_to) load_block(next, block + SPLIT);
-    if (!c.held) {  // a page outside the cache: every row that sees it answers NaN
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        if (sees[t] >= block * kBlockTokens) sum[t] = __builtin_nanf("");
-      continue;
+  // A wave's blocks, 64 at a time: a lane each looks up the page and its scales.
+  for (int base = from + split; base < coded_to; base += 64 * SPLIT) {
+    int pages = -1;
+    float key_scales = 0.0f, value_scales = 0.0f;
+    const int mine = base + lane * SPLIT;
+    if (mine < coded_to) {
+      pages = a.table[b * a.max_blocks + mine];  // mine < tail_block <= max_blocks
+      if (pages < 0 || pages >= a.blocks) pages = -1;
+      if (pages >= 0) {
+        key_scales = a.key_scales[(int64_t)pages * a.kv_heads + h];
+        value_scales = a.value_scales[(int64_t)pages * a.kv_heads + h];
+      }
     }
-    // never 0, which would make NaN of a masked score
-    const float factor = fmaxf(c.k_scale * a.scale_log2, 1.17549435e-38f);
-    f32x4 s[TILES][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int hh = 0; hh < HALVES; ++hh)
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          const V8 k = e4m3_operand<T>(c.k[i][hh][2 * kk], c.k[i][hh][2 * kk + 1], 1.0f);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t)
-            s[t][i] = mfma16(k, q[t][hh][kk], hh + kk == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : s[t][i]);
-        }
+    const int left = (coded_to - base + SPLIT - 1) / SPLIT;
+    const int count_here = left < 64 ? left : 64;
+    KeyCodes<D> next_keys;
+    ValueCodes<D> next_values;
+    int page = __builtin_amdgcn_readlane(pages, 0);
+    if (page >= 0) {
+      load_keys(next_keys, page);
+      if (AHEAD) load_values(next_values, page);
     }
-    f16x8 p[TILES][2];
+    for (int i = 0; i < count_here; ++i) {
+      const int block = base + i * SPLIT;
+      const bool held = page >= 0;
+      const int here = page;
+      KeyCodes<D> keys = next_keys;
+      ValueCodes<D> values;
+      if (AHEAD) values = next_values;
+      page = i + 1 < count_here ? __builtin_amdgcn_readlane(pages, i + 1) : -1;
+      if (AHEAD && page >= 0) {
+        load_keys(next_keys, page);
+        load_values(next_values, page);
+      }
+      f32x4 s[TILES][4];
+      if (held) {
+        if (!AHEAD) load_values(values, here);
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      softmax_step(t, s[t], factor, block);
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+          for (int hh = 0; hh < HALVES; ++hh)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[t][k][e] = (f16)s[t][2 * k + e / 4][e % 4];
-    }
+            for (int kk = 0; kk < 2; ++kk) {
+              const V8 k = e4m3_operand<T>(keys.part[r][hh][2 * kk], keys.part[r][hh][2 * kk + 1], 1.0f);
 #pragma unroll
-    for (int f = 0; f < FEATURES; ++f) {
-      const f16x8 v0 = e4m3_operand<f16>(c.v[f][0], c.v[f][1], 1.0f);
-      const f16x8 v1 = e4m3_operand<f16>(c.v[f][2], c.v[f][3], 1.0f);
+              for (int t = 0; t < TILES; ++t)
+                s[t][r] = mfma16(k, q[t][hh][kk], hh + kk == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : s[t][r]);
+            }
+      }
+      if (!AHEAD && page >= 0) load_keys(next_keys, page);
+      if (!held) {  // a page outside the cache: every row that sees it answers NaN
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+          if (sees[t] >= block * kBlockTokens) sum[t] = __builtin_nanf("");
+        continue;
+      }
+      // never 0, which would make NaN of a masked score
+      const float factor = fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(key_scales), i)) * a.scale_log2,
+                                 1.17549435e-38f);
+      f16x8 p[TILES][2];
+      if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
-        f32x4 sums = mfma16(v0, p[t][0], (f32x4){0.0f, 0.0f, 0.0f, 0.0f});
-        sums = mfma16(v1, p[t][1], sums);
+        softmax_step(t, s[t], factor, block, !ONES);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out[t][f][j] = fmaf(sums[j], c.v_scale, out[t][f][j]);
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[t][k][e] = (f16)s[t][2 * k + e / 4][e % 4];
+          if (ONES) {
+            const f16 one = (f16)1.0f;
+            sums[t] = mfma16((f16x8){one, one, one, one, one, one, one, one}, p[t][k], sums[t]);
+          }
+        }
+      }
+      if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
+      const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
+      raise_unit(scale_bits);
+      const float ratio = power_ratio(scale_bits, unit);
+      if (ratio >= 0x1p-15f) {  // codes times the ratio are exact in fp16
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) {
+          const f16x8 v0 = e4m3_operand<f16>(values.part[f][0], values.part[f][1], ratio);
+          const f16x8 v1 = e4m3_operand<f16>(values.part[f][2], values.part[f][3], ratio);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) out[t][f] = mfma16(v1, p[t][1], mfma16(v0, p[t][0], out[t][f]));
+        }
+      } else {
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) {
+          const f16x8 v0 = e4m3_operand<f16>(values.part[f][0], values.part[f][1], 1.0f);
+          const f16x8 v1 = e4m3_operand<f16>(values.part[f][2], values.part[f][3], 1.0f);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            const f32x4 add = mfma16(v1, p[t][1], mfma16(v0, p[t][0], (f32x4){0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[t][f][j] = fmaf(add[j], ratio, out[t][f][j]);
+          }
+        }
       }
     }
   }
 
-  // The incomplete block, in the tensors' own type.
+  // The incomplete block, in the tensors' own type: weights without the shift, in a
+  // unit of at least 2^12 (the shift), so that large values do not overflow.
   if (tail_block >= from && tail_block < to && (tail_block - from) % SPLIT == split) {
-    const int held = (int)(start + count - tail_block * kBlockTokens);  // tokens in it
+    const int held = first_position + count - tail_block * kBlockTokens;  // tokens in it
     const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
     const T* keys = static_cast<const T*>(a.key_tail) + tail_at + quarter * 16;
     const T* values = static_cast<const T*>(a.value_tail) + tail_at + quarter * 16;
+    constexpr int SHIFT_BITS = (127 + (int)kWeightShift) << 23;
+    raise_unit(SHIFT_BITS);
+    const float ratio = power_ratio(SHIFT_BITS, unit);
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
+      if (t != 0) asm volatile("" ::: "memory");  // each tile loads its operands: kept, they would not fit
       f32x4 s[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -279,39 +379,51 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
                               keys + ((column >> 2) * 16 + i * 4 + (column & 3)) * D + hh * 64 + kk * 8),
                           q[t][hh][kk], s[i]);
       }
-      softmax_step(t, s, fmaxf(a.scale_log2, 1.17549435e-38f), tail_block);
-      // bf16 weights keep 16 bits of precision as a sum of two
+      softmax_step(t, s, fmaxf(a.scale_log2, 1.17549435e-38f), tail_block, true);
+      // bf16 weights keep 16 bits of precision as a sum of two; fp16 ones the shift
+      constexpr bool WIDE = std::is_same<T, bf16>::value;
       V8 p[2], rest[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float w = s[2 * k + e / 4][e % 4];
+          const float w = s[2 * k + e / 4][e % 4] * (WIDE ? 0x1p-12f : 1.0f);
           p[k][e] = (T)w;
           rest[k][e] = (T)(w - (float)p[k][e]);
         }
 #pragma unroll
-      for (int f = 0; f < FEATURES; ++f)
+      for (int f = 0; f < FEATURES; ++f) {
+        f32x4 add = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           V8 v = *reinterpret_cast<const V8*>(values + (f * 16 + column) * kBlockTokens + k * 8);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (quarter * 16 + k * 8 + e >= held) v[e] = (T)0.0f;  // what stands behind the last token
-          out[t][f] = mfma16(v, p[k], out[t][f]);
-          if constexpr (std::is_same<T, bf16>::value) out[t][f] = mfma16(v, rest[k], out[t][f]);
+          add = mfma16(v, p[k], add);
+          if constexpr (WIDE) add = mfma16(v, rest[k], add);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[t][f][j] = fmaf(WIDE ? add[j] : add[j] * 0x1p-12f, ratio, out[t][f][j]);
+      }
     }
   }
 
-  // A row's sum over the four lanes that share it.
+  // A row's sum over the four lanes that share it, and its output over the sum.
+  const float unit_value = __int_as_float(unit);
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
-    sum[t] += __shfl_xor(sum[t], 16);
-    sum[t] += __shfl_xor(sum[t], 32);
+    sum[t] = quarters_sum(sum[t]);
+    if (ONES) sum[t] += sums[t][0];
+    const float inverse = sum[t] != 0.0f ? 1.0f / sum[t] : 0.0f;  // 0: a row that sees nothing here
+#pragma unroll
+    for (int f = 0; f < FEATURES; ++f)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[t][f][j] = out[t][f][j] * inverse * unit_value;
   }
 
-  // Merge of the waves that split the tokens, tile by tile.
+  // Merge of the waves that split the tokens, tile by tile: wave w's output weighs
+  // sum_w 2^(most_w - top).
   if constexpr (SPLIT > 1) {
     constexpr int PITCH = D + 4;
     __shared__ float part[SPLIT * ROWS][16 * PITCH];
@@ -327,23 +439,22 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
       for (int f = 0; f < FEATURES; ++f)
         *reinterpret_cast<f32x4*>(&part[wave][column * PITCH + f * 16 + quarter * 4]) = out[t][f];
       __syncthreads();
-      // Each wave merges the features FEATURES / SPLIT of its rows.
+      // Each wave merges the tiles of features f % SPLIT == split of its rows.
       const int w0 = wave - split;
       float top = -INFINITY, total = 0.0f;
 #pragma unroll
       for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, stats[w0 + w][column][0]);
+      const float base = top == -INFINITY ? 0.0f : top;
       float weight[SPLIT];
 #pragma unroll
       for (int w = 0; w < SPLIT; ++w) {
-        weight[w] = top == -INFINITY ? 0.0f : exp2_fast(stats[w0 + w][column][0] - top);
-        total += stats[w0 + w][column][1] * weight[w];
-      }
-      if (top == -INFINITY) {  // nothing seen, or pages outside the cache alone
-#pragma unroll
-        for (int w = 0; w < SPLIT; ++w) total += stats[w0 + w][column][1];
+        const float part_sum = stats[w0 + w][column][1];
+        weight[w] = part_sum != 0.0f ? part_sum * exp2_fast(stats[w0 + w][column][0] - base) : 0.0f;
+        total += weight[w];
       }
       most[t] = top;
       sum[t] = total;
+      const float inverse = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
       for (int f = 0; f < FEATURES; ++f) {
         if (f % SPLIT != split) continue;
@@ -351,8 +462,9 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
 #pragma unroll
         for (int w = 0; w < SPLIT; ++w) {
           const f32x4 v = *reinterpret_cast<const f32x4*>(&part[w0 + w][column * PITCH + f * 16 + quarter * 4]);
+          const float share = weight[w] * inverse;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) merged[j] = fmaf(v[j], weight[w], merged[j]);
+          for (int j = 0; j < 4; ++j) merged[j] = fmaf(v[j], share, merged[j]);
         }
         out[t][f] = merged;
       }
@@ -362,68 +474,86 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     if (token[t] >= a.seq_len) continue;
-    if (a.chunks == 1) {
-      // rows without a query and rows that see nothing are zeros
-      const float inverse = token[t] < count && sum[t] != 0.0f ? 1.0f / sum[t] : 0.0f;
-      T* o = static_cast<T*>(a.output) + b * a.o_sb + token[t] * a.o_ss + (int64_t)head[t] * D;
+    const int64_t place = (b * a.seq_len + token[t]) * a.heads + head[t];
 #pragma unroll
-      for (int f = 0; f < FEATURES; ++f) {
-        if (SPLIT > 1 && f % SPLIT != split) continue;
+    for (int f = 0; f < FEATURES; ++f) {
+      if (SPLIT > 1 && f % SPLIT != split) continue;
+      if (a.chunks == 1) {
+        T* o = static_cast<T*>(a.output) + b * a.o_sb + token[t] * a.o_ss + (int64_t)head[t] * D;
         typename Vec8<T>::half_type v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = token[t] < count ? (T)(out[t][f][j] * inverse) : (T)0.0f;
+        for (int j = 0; j < 4; ++j) v[j] = token[t] < count ? (T)out[t][f][j] : (T)0.0f;  // rows without a query
         *reinterpret_cast<typename Vec8<T>::half_type*>(o + f * 16 + quarter * 4) = v;
+      } else {
+        *reinterpret_cast<f32x4*>(a.partial + (place * a.chunks + chunk) * D + f * 16 + quarter * 4) = out[t][f];
       }
-    } else {
-      const int64_t row = ((b * a.seq_len + token[t]) * a.heads + head[t]) * a.chunks + chunk;
-#pragma unroll
-      for (int f = 0; f < FEATURES; ++f) {
-        if (SPLIT > 1 && f % SPLIT != split) continue;
-        *reinterpret_cast<f32x4*>(a.partial + row * D + f * 16 + quarter * 4) = out[t][f];
-      }
-      if (split == 0 && quarter == 0) {
-        a.statistics[row * 2] = most[t];
-        a.statistics[row * 2 + 1] = sum[t];
-      }
+    }
+    if (a.chunks > 1 && split == 0 && quarter == 0) {
+      float* statistics = a.statistics + (place * a.chunks + chunk) * 2;
+      statistics[0] = most[t];
+      statistics[1] = sum[t];
     }
   }
 }
 
-// Merge of the chunks: D / 4 lanes a row.
+// Merge of the chunks, a wave a row: chunk c's output weighs sum_c 2^(most_c - top).
+// A lane first looks at one chunk's statistics, then D / 4 lanes take a chunk's
+// output each time, 256 / D chunks at once.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64_t rows) {
   constexpr int LANES = D / 4;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  constexpr int PARTS = 64 / LANES;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  const int feature = (threadIdx.x % LANES) * 4;
+  const int feature = (lane % LANES) * 4;
   const int64_t token_row = row / a.heads;
   const int head = (int)(row - token_row * a.heads);
   const int64_t b = token_row / a.seq_len;
   const int64_t token = token_row - b * a.seq_len;
-  const int64_t start = a.starts[b];
-  const int64_t count = a.counts != nullptr ? (int64_t)a.counts[b] : (int64_t)a.seq_len;
-  const bool live = start >= 0 && token < count;
+  const int count = a.counts != nullptr ? a.counts[b] : a.seq_len;
+  const bool live = a.starts[b] >= 0 && token < count;
 
-  const float* statistics = a.statistics + row * a.chunks * 2;
-  const float* partial = a.partial + row * a.chunks * D + feature;
   f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
   if (live) {
-    float top = -INFINITY, total = 0.0f;
-    for (int c = 0; c < a.chunks; ++c) top = fmaxf(top, statistics[2 * c]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (int c = 0; c < a.chunks; ++c) {
-      const float sum = statistics[2 * c + 1];
-      if (sum == 0.0f) continue;  // a chunk behind this row's last token
-      const float weight = exp2_fast(statistics[2 * c] - base);
-      total += sum * weight;
-      const f32x4 v = *reinterpret_cast<const f32x4*>(partial + (int64_t)c * D);
+    const f32x2* statistics = reinterpret_cast<const f32x2*>(a.statistics) + row * a.chunks;
+    const float* partial = a.partial + row * a.chunks * D + feature;
+    float top = -INFINITY;
+    for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, statistics[c][0]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) out[j] = fmaf(v[j], weight, out[j]);
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f;
+    for (int first = 0; first < a.chunks; first += 64) {
+      float weight = 0.0f;
+      if (first + lane < a.chunks) {
+        const f32x2 s = statistics[first + lane];
+        if (s[1] != 0.0f) weight = s[1] * exp2_fast(s[0] - base);  // 0: a chunk behind the row's last token
+      }
+      total += weight;
+      const int here = a.chunks - first < 64 ? a.chunks - first : 64;
+      for (int c = 0; c < here; c += 4 * PARTS) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int mine = c + u * PARTS + lane / LANES;
+          const float w = __shfl(weight, mine);  // 0 behind the last chunk, whose output is then read again
+          const int read = first + (mine < here ? mine : here - 1);
+          const f32x4 v = *reinterpret_cast<const f32x4*>(partial + (int64_t)read * D);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[j] = fmaf(v[j], w, out[j]);
+        }
+      }
     }
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    total = wave_sum(total);
+    const float inverse = total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+    for (int m = LANES; m < 64; m <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] += __shfl_xor(out[j], m);
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] *= inverse;
   }
+  if (lane >= LANES) return;
   typename Vec8<T>::half_type v;
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = (T)out[j];
@@ -445,16 +575,16 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
                  int64_t max_length) {
   Layout l{};
   const int64_t rows = seq_len * group;
-  const int most_tiles = head_dim == 64 ? 4 : 2;
-  l.tiles = rows <= 16 ? 1 : rows <= 32 || most_tiles == 2 ? 2 : 4;
-  l.split = rows <= 16 * l.tiles ? kWaves : 1;
-  const int64_t rows_a_group = (int64_t)16 * l.tiles * (kWaves / l.split);
-  l.row_groups = ceil_div(rows, rows_a_group);
+  l.tiles = rows <= 16 ? 1 : 2;
+  // waves that the registers leave room for, on all compute units
+  const int64_t room = (int64_t)kUnits * 4 * (head_dim == 128 && l.tiles == 2 ? 1 : head_dim == 64 && l.tiles == 1 ? 3 : 2);
+  const int64_t waves = batch * kv_heads * ceil_div(rows, 16 * l.tiles);
   const int64_t blocks = max_length / kBlockTokens + 1;
-  const int64_t units = batch * kv_heads * l.row_groups;
-  // four workgroups a compute unit, of at least two blocks a wave
-  int64_t chunks = ceil_div(4 * kUnits, units);
-  const int64_t most = ceil_div(blocks, 2 * l.split);
+  l.split = waves >= room ? 1 : l.tiles == 1 && blocks <= 32 ? 8 : 4;
+  if (l.tiles == 1 && l.split == 1) l.split = 4;
+  l.row_groups = ceil_div(rows, (int64_t)16 * l.tiles * (l.split == 1 ? kWaves : 1));
+  int64_t chunks = room / (waves * l.split);
+  const int64_t most = ceil_div(blocks, 4 * l.split);
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
   l.chunk_blocks = (int)ceil_div(blocks, chunks);
@@ -464,23 +594,19 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
 
 template <typename T, int D>
 int launch_attention(AttentionArgs& a, const Layout& l, int64_t batch, unsigned grid, hipStream_t stream) {
-#define SAH_ATTENTION_CASE(TILES, SPLIT)                                                                     \
+#define SAH_ATTENTION_CASE(TILES, SPLIT, ROWS)                                                               \
   if (l.tiles == TILES && l.split == SPLIT)                                                                  \
-    hipLaunchKernelGGL((cached_attention_kernel<T, D, TILES, SPLIT, kWaves / SPLIT>), dim3(grid),            \
-                       dim3(kWaves * 64), 0, stream, a);
-  SAH_ATTENTION_CASE(1, kWaves)
-  SAH_ATTENTION_CASE(2, kWaves)
-  SAH_ATTENTION_CASE(2, 1)
-  if constexpr (D == 64) {
-    SAH_ATTENTION_CASE(4, kWaves)
-    SAH_ATTENTION_CASE(4, 1)
-  }
+    hipLaunchKernelGGL((cached_attention_kernel<T, D, TILES, SPLIT, ROWS>), dim3(grid), dim3(SPLIT * ROWS * 64), 0, \
+                       stream, a);
+  SAH_ATTENTION_CASE(1, 4, 1)
+  SAH_ATTENTION_CASE(1, 8, 1)
+  SAH_ATTENTION_CASE(2, 4, 1)
+  SAH_ATTENTION_CASE(2, 1, 4)
 #undef SAH_ATTENTION_CASE
   int status = check_hip(hipGetLastError(), "cached attention launch");
   if (status != SAH_OK || l.chunks == 1) return status;
   const int64_t rows = batch * a.seq_len * a.heads;
-  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)ceil_div(rows, 256 / (D / 4))), dim3(256), 0, stream, a,
-                     rows);
+  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, a, rows);
   return check_hip(hipGetLastError(), "cached attention merge launch");
 }
 
@@ -549,9 +675,9 @@ extern "C" int sah_block_cache_attention(
   if (need != 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(SAH_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   const int64_t units = batch * kv_heads;
-  const int64_t most = (int64_t)(UINT32_MAX / (kWaves * 64));
+  const int64_t most = (int64_t)(UINT32_MAX / 512);
   if (l.row_groups > most / l.chunks || units > most / (l.row_groups * l.chunks) ||
-      batch * seq_len * heads > most * 8)
+      batch * seq_len * heads > most * 8 - 8)
     return fail(SAH_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
 
   AttentionArgs a{};
