@@ -45,68 +45,149 @@ __device__ __forceinline__ typename Vec8<T>::type code_operand(uint32_t word) {
   return e4m3_operand<T>(low, high, 512.0f);
 }
 
-template <typename T, int GROUP, int TILES, int SPLIT>
+// A workgroup takes OUTS x 16 outputs of TILES x 16 rows; its SPLIT waves share the
+// inputs among them, a tile of 128 at a time, and load the next tile while they work
+// on this one.  Rows of x are read in whole lines and pass through the wave's own
+// part of LDS on their way to the operands (STAGED): a load straight in the operands'
+// order touches a line a lane.  Few rows do without.
+template <typename T, int GROUP, int TILES, int OUTS, int SPLIT, bool STAGED>
 __global__ __launch_bounds__(SPLIT * 64) void linear_w4_kernel(const LinearW4Args a) {
   typedef typename Vec8<T>::type V8;
   typedef typename Vec8<T>::half_type V4;
   constexpr int GROUPS = kUnitK / GROUP;
   constexpr int STEPS = GROUP / 32;  // products of a group
-  __shared__ f32x4 part[SPLIT][TILES][64];
+  constexpr int PARTS = SPLIT < 4 ? SPLIT : 4;
+  constexpr int PITCH = kUnitK + 8;  // values of a row in LDS: operands' rows fall on different banks
+  constexpr int STAGE = STAGED ? TILES * 16 * PITCH : 8;
+  union Shared {
+    f32x4 part[PARTS][TILES * OUTS][64];
+    T stage[SPLIT][STAGE];
+  };
+  __shared__ Shared shared;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15, quarter = lane >> 4;
-  const uint32_t out_tile = blockIdx.x % (uint32_t)a.out_tiles;
-  const int64_t first_row = (int64_t)(blockIdx.x / (uint32_t)a.out_tiles) * (TILES * 16);
+  const uint32_t out_groups = (uint32_t)a.out_tiles / OUTS;
+  const uint32_t out_tile = blockIdx.x % out_groups * OUTS;
+  const int64_t first_row = (int64_t)(blockIdx.x / out_groups) * (TILES * 16);
   const int64_t out_features = (int64_t)a.out_tiles * 16;
 
   const u32x4* codes = reinterpret_cast<const u32x4*>(a.codes) + (int64_t)out_tile * a.in_tiles * 64 + lane;
   const T* scales = static_cast<const T*>(a.scales) + (int64_t)out_tile * 16 + quarter * 4;
-  const T* x[TILES];
+  // Places without a row take the last one's.
+  constexpr int LOADS = STAGED ? TILES * 4 : TILES;
+  const T* x[LOADS];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const int64_t row = first_row + t * 16 + column;  // columns without a row take the last one's
-    x[t] = static_cast<const T*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride + quarter * 8;
+  for (int t = 0; t < LOADS; ++t) {
+    const int64_t row = first_row + (STAGED ? t * 4 + lane / 16 : t * 16 + column);
+    x[t] = static_cast<const T*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride +
+           (STAGED ? lane % 16 : quarter) * 8;
   }
 
-  f32x4 sums[TILES];
+  f32x4 sums[TILES][OUTS];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) sums[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) sums[t][o] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+
+  u32x4 next_codes[OUTS];
+  V4 next_scales[OUTS][GROUPS];
+  V8 next_x[TILES * 4];
+  auto load = [&](int unit) {
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) {
+      next_codes[o] = codes[((int64_t)o * a.in_tiles + unit) * 64];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+        next_scales[o][g] = *reinterpret_cast<const V4*>(scales + ((int64_t)unit * GROUPS + g) * out_features + o * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < TILES * 4; ++i)
+      next_x[i] = *reinterpret_cast<const V8*>(x[STAGED ? i : i / 4] + (int64_t)unit * kUnitK + (STAGED ? 0 : i % 4 * 32));
+  };
+  T* stage = shared.stage[wave];
+  if (wave < a.in_tiles) load(wave);
   for (int unit = wave; unit < a.in_tiles; unit += SPLIT) {
-    const u32x4 words = codes[(int64_t)unit * 64];
+    u32x4 words[OUTS];
+    V4 scale[OUTS][GROUPS];
+    V8 rows[STAGED ? 1 : TILES * 4];
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) {
+      words[o] = next_codes[o];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) scale[o][g] = next_scales[o][g];
+    }
+#pragma unroll
+    for (int i = 0; i < TILES * 4; ++i) {
+      if (STAGED)
+        *reinterpret_cast<V8*>(stage + (i * 4 + lane / 16) * PITCH + lane % 16 * 8) = next_x[i];
+      else
+        rows[i] = next_x[i];
+    }
+    if (unit + SPLIT < a.in_tiles) load(unit + SPLIT);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-      const V4 scale = *reinterpret_cast<const V4*>(scales + ((int64_t)unit * GROUPS + g) * out_features);
-      f32x4 group[TILES];
+      V8 operand[STEPS][TILES];
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const V8 w = code_operand<T>(words[g * STEPS + i]);
+      for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          const V8 v = *reinterpret_cast<const V8*>(x[t] + (int64_t)unit * kUnitK + (g * STEPS + i) * 32);
-          group[t] = mfma16(w, v, i == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : group[t]);
+        for (int t = 0; t < TILES; ++t)
+          operand[i][t] = STAGED ? *reinterpret_cast<const V8*>(stage + (t * 16 + column) * PITCH +
+                                                                (g * STEPS + i) * 32 + quarter * 8)
+                                 : rows[STAGED ? 0 : t * 4 + g * STEPS + i];
+#pragma unroll
+      for (int o = 0; o < OUTS; ++o) {
+        f32x4 group[TILES];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          const V8 w = code_operand<T>(words[o][g * STEPS + i]);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t)
+            group[t] = mfma16(w, operand[i][t], i == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : group[t]);
         }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sums[t][o][j] = fmaf(group[t][j], to_f32(scale[o][g][j]), sums[t][o][j]);
       }
+    }
+  }
+  __syncthreads();  // the sums take the stages' place
+
+  // The waves' sums, in a fixed order: four waves at a time add theirs to those before.
+#pragma unroll
+  for (int turn = 0; turn < SPLIT / PARTS; ++turn) {
+    if (turn != 0) __syncthreads();
+    if (wave / PARTS == turn) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sums[t][j] = fmaf(group[t][j], to_f32(scale[j]), sums[t][j]);
+        for (int o = 0; o < OUTS; ++o) {
+          f32x4& place = shared.part[wave % PARTS][t * OUTS + o][lane];
+          if (turn == 0) {
+            place = sums[t][o];
+          } else {
+            const f32x4 before = place;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[t][o][j] += before[j];
+            place = sums[t][o];
+          }
+        }
     }
   }
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) part[wave][t][lane] = sums[t];
   __syncthreads();
 
-  for (int t = wave; t < TILES; t += SPLIT) {
-    const int64_t row = first_row + t * 16 + column;
+  for (int i = wave; i < TILES * OUTS; i += SPLIT) {
+    const int64_t row = first_row + i / OUTS * 16 + column;
     if (row >= a.rows) continue;
-    f32x4 v = part[0][t][lane];
+    f32x4 v = shared.part[0][i][lane];
 #pragma unroll
-    for (int w = 1; w < SPLIT; ++w) {
-      const f32x4 other = part[w][t][lane];
+    for (int w = 1; w < PARTS; ++w) {
+      const f32x4 other = shared.part[w][i][lane];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += other[j];
     }
-    const int64_t n = (int64_t)out_tile * 16 + quarter * 4;
+    const int64_t n = ((int64_t)out_tile + i % OUTS) * 16 + quarter * 4;
     if (a.bias != nullptr) {
       const V4 bias = *reinterpret_cast<const V4*>(static_cast<const T*>(a.bias) + n);
 #pragma unroll
@@ -119,21 +200,42 @@ __global__ __launch_bounds__(SPLIT * 64) void linear_w4_kernel(const LinearW4Arg
   }
 }
 
-template <typename T, int GROUP>
-int launch_linear_w4(const LinearW4Args& a, hipStream_t stream) {
-  const int tiles = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
-  const int64_t grid = (int64_t)a.out_tiles * ceil_div(a.rows, 16 * tiles);
-  constexpr int SPLIT = 8;
+template <typename T, int GROUP, int TILES, int OUTS, int SPLIT, bool STAGED>
+int launch_tiles(const LinearW4Args& a, hipStream_t stream) {
+  const int64_t grid = (int64_t)(a.out_tiles / OUTS) * ceil_div(a.rows, 16 * TILES);
   if (grid > (int64_t)(UINT32_MAX / (SPLIT * 64)))
     return fail(SAH_ERR_UNSUPPORTED, "sah_linear_w4: too many rows for one launch");
-  const dim3 blocks((unsigned)grid), threads(SPLIT * 64);
-  if (tiles == 1)
-    hipLaunchKernelGGL((linear_w4_kernel<T, GROUP, 1, SPLIT>), blocks, threads, 0, stream, a);
-  else if (tiles == 2)
-    hipLaunchKernelGGL((linear_w4_kernel<T, GROUP, 2, SPLIT>), blocks, threads, 0, stream, a);
-  else
-    hipLaunchKernelGGL((linear_w4_kernel<T, GROUP, 4, SPLIT>), blocks, threads, 0, stream, a);
+  hipLaunchKernelGGL((linear_w4_kernel<T, GROUP, TILES, OUTS, SPLIT, STAGED>), dim3((unsigned)grid), dim3(SPLIT * 64),
+                     0, stream, a);
   return check_hip(hipGetLastError(), "4-bit linear launch");
+}
+
+// Row tiles by the row count; 16-output tiles of a workgroup by how many there are:
+// x is read anew by every workgroup, so as many outputs as still leave the compute
+// units one each.  One row reads x in the operands' order (all its lanes read the
+// same line).  Measured, us, OUTS 1 / 2 / 4 (SPLIT 8 up to 2, then 4):
+//   16 rows  4096 ->  4096   5.5 /  5.9         64 rows  4096 ->  4096  11.5 / 12.9 / 16.1
+//    8 rows  4096 ->  8192   7.8 /  6.5         64 rows  4096 ->  8192  23.0 / 13.0 / 16.5
+//   16 rows  4096 -> 16384  14.7 / 11.3         64 rows  4096 -> 16384  42.7 / 24.1 / 21.0
+//   32 rows  4096 ->  8192  12.4 /  9.1 / 11.0  32 rows  4096 -> 16384  21.6 / 14.4 / 12.5
+// and without / with the stage: 1 row 4096 -> 4096 5.05 / 5.33, 13 rows 6.3 / 5.5.
+template <typename T, int GROUP>
+int launch_linear_w4(const LinearW4Args& a, hipStream_t stream) {
+  const int64_t row_tiles = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
+  const int64_t tiles = a.out_tiles * ceil_div(a.rows, 16 * row_tiles);
+  const bool two = tiles >= 512 && a.out_tiles % 2 == 0;
+  const bool four = tiles >= 1024 && a.out_tiles % 4 == 0;
+  if (a.rows == 1)
+    return two ? launch_tiles<T, GROUP, 1, 2, 8, false>(a, stream) : launch_tiles<T, GROUP, 1, 1, 8, false>(a, stream);
+  if (row_tiles == 1)
+    return two ? launch_tiles<T, GROUP, 1, 2, 8, true>(a, stream) : launch_tiles<T, GROUP, 1, 1, 8, true>(a, stream);
+  if (row_tiles == 2)
+    return four  ? launch_tiles<T, GROUP, 2, 4, 4, true>(a, stream)
+           : two ? launch_tiles<T, GROUP, 2, 2, 8, true>(a, stream)
+                 : launch_tiles<T, GROUP, 2, 1, 8, true>(a, stream);
+  return four  ? launch_tiles<T, GROUP, 4, 4, 4, true>(a, stream)
+         : two ? launch_tiles<T, GROUP, 4, 2, 4, true>(a, stream)
+               : launch_tiles<T, GROUP, 4, 1, 8, true>(a, stream);
 }
 
 template <typename T>

@@ -555,6 +555,14 @@ def test_linear_w4_sizes(gpu_device, k, n, group, gelu):
     _linear_case(gpu_device, 3, k, n, group, BF16 if group != 64 else F16, bias=n != 48, gelu=gelu, seed=k + n)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 25, 50, 100])
+@pytest.mark.parametrize("n", [16 * 512, 16 * 1024, 16 * 1026, 16 * 1027])
+def test_linear_w4_wide(gpu_device, rows, n):
+    """As many outputs as take two and four tiles of them a workgroup, or would."""
+
+    _linear_case(gpu_device, rows, 384, n, 32 if rows == 50 else 128, F16 if rows == 9 else BF16, seed=rows)
+
+
 def test_linear_w4_layouts_and_extremes(gpu_device):
     from solution.kernels.projection import hip_linear_w4, quantize_linear_w4
 
