@@ -26,13 +26,11 @@ import torch
 
 from ..hip._library import (
     HipLibraryError,
-    check_status,
     dtype_code,
     is_gfx950,
-    launch_device,
+    launch,
     library_available,
     load_library,
-    stream_handle,
 )
 
 HIP_BLOCK_CACHE_APPEND_BACKEND = "hip_block_cache_append"
@@ -169,11 +167,12 @@ def hip_block_cache_available() -> bool:
 
 
 def _lengths_ok(lengths: torch.Tensor | None, cache: BlockCache) -> bool:
+    tail = cache.key_tail
     return lengths is None or (
         lengths.dtype is torch.int32
-        and lengths.shape == (cache.key_tail.shape[0],)
+        and lengths.shape == tail.shape[:1]
         and lengths.is_contiguous()
-        and lengths.device == cache.key_tail.device
+        and lengths.device == tail.device
     )
 
 
@@ -181,20 +180,30 @@ def _rows_ok(value: torch.Tensor, cache: BlockCache) -> bool:
     """A [batch, heads, seq_len, head_dim] view of the cache's type that the kernels read in place."""
 
     tail = cache.key_tail
-    if value.ndim != 4 or value.dtype is not tail.dtype or value.device != tail.device:
+    if value.dtype is not tail.dtype or value.device != tail.device:
         return False
-    shape, strides = value.shape, value.stride()
-    if shape[0] != tail.shape[0] or shape[3] != tail.shape[3]:
+    size, stride, of_tail = value.shape, value.stride(), tail.shape
+    if len(size) != 4 or size[0] != of_tail[0] or size[3] != of_tail[3]:
         return False
-    if strides[3] != 1 or value.data_ptr() % 16 or (value.requires_grad and torch.is_grad_enabled()):
-        return False
-    return not any(stride % 8 and size != 1 for size, stride in zip(shape[:3], strides))
+    return not (
+        stride[3] != 1
+        or (stride[0] % 8 and size[0] != 1)
+        or (stride[1] % 8 and size[1] != 1)
+        or (stride[2] % 8 and size[2] != 1)
+        or value.data_ptr() % 16
+        or (value.requires_grad and torch.is_grad_enabled())
+    )
 
 
-def _strides(value: torch.Tensor) -> tuple[int, ...]:
+def _strides(value: torch.Tensor) -> tuple[int, int, int]:
     """Strides of the first three axes, 0 for an axis of size 1 (never stepped)."""
 
-    return tuple(0 if size == 1 else stride for size, stride in zip(value.shape[:3], value.stride()))
+    size, stride = value.shape, value.stride()
+    return (
+        stride[0] if size[0] != 1 else 0,
+        stride[1] if size[1] != 1 else 0,
+        stride[2] if size[2] != 1 else 0,
+    )
 
 
 def can_use_hip_block_cache_append(
@@ -240,25 +249,25 @@ def hip_block_cache_append(
         raise RuntimeError("HIP block cache append is ineligible for the requested inputs")
     batch, heads, seq_len, dim = key.shape
     try:
-        with launch_device(key.device):
-            status = load_library().sah_block_cache_append(
-                key.data_ptr(),
-                value.data_ptr(),
-                *cache._pointers(),
-                starts.data_ptr(),
-                None if counts is None else counts.data_ptr(),
-                batch,
-                heads,
-                seq_len,
-                dim,
-                *_strides(key),
-                *_strides(value),
-                cache.key_codes.shape[0],
-                cache.block_table.shape[1],
-                dtype_code(key.dtype),
-                stream_handle(key.device),
-            )
-            check_status(status, "sah_block_cache_append")
+        launch(
+            key.device,
+            load_library().sah_block_cache_append,
+            "sah_block_cache_append",
+            key.data_ptr(),
+            value.data_ptr(),
+            *cache._pointers(),
+            starts.data_ptr(),
+            None if counts is None else counts.data_ptr(),
+            batch,
+            heads,
+            seq_len,
+            dim,
+            *_strides(key),
+            *_strides(value),
+            cache.key_codes.shape[0],
+            cache.block_table.shape[1],
+            dtype_code(key.dtype),
+        )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block cache append execution failed") from exc
     return HIP_BLOCK_CACHE_APPEND_BACKEND
@@ -296,23 +305,23 @@ def hip_block_cache_read(
     key = torch.empty((batch, heads, tokens, dim), dtype=tail.dtype, device=tail.device)
     value = torch.empty_like(key)
     try:
-        with launch_device(tail.device):
-            status = load_library().sah_block_cache_read(
-                *cache._pointers(),
-                firsts.data_ptr(),
-                lengths.data_ptr(),
-                key.data_ptr(),
-                value.data_ptr(),
-                batch,
-                heads,
-                tokens,
-                dim,
-                cache.key_codes.shape[0],
-                cache.block_table.shape[1],
-                dtype_code(tail.dtype),
-                stream_handle(tail.device),
-            )
-            check_status(status, "sah_block_cache_read")
+        launch(
+            tail.device,
+            load_library().sah_block_cache_read,
+            "sah_block_cache_read",
+            *cache._pointers(),
+            firsts.data_ptr(),
+            lengths.data_ptr(),
+            key.data_ptr(),
+            value.data_ptr(),
+            batch,
+            heads,
+            tokens,
+            dim,
+            cache.key_codes.shape[0],
+            cache.block_table.shape[1],
+            dtype_code(tail.dtype),
+        )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block cache read execution failed") from exc
     return key, value, HIP_BLOCK_CACHE_READ_BACKEND
@@ -368,37 +377,38 @@ def hip_block_cache_attention(
         raise RuntimeError("HIP block cache attention is ineligible for the requested inputs")
     batch, heads, seq_len, dim = query.shape
     kv_heads = cache.key_tail.shape[1]
+    dtype, device = query.dtype, query.device
     most = cache.max_tokens if max_length is None else min(max_length, cache.max_tokens)
-    output = torch.empty((batch, seq_len, heads * dim), dtype=query.dtype, device=query.device)
+    output = torch.empty((batch, seq_len, heads * dim), dtype=dtype, device=device)
     try:
         library = load_library()
         size = library.sah_block_cache_attention_workspace_bytes(batch, seq_len, heads, kv_heads, dim, most)
-        workspace = torch.empty(size, dtype=torch.uint8, device=query.device) if size else None
-        with launch_device(query.device):
-            status = library.sah_block_cache_attention(
-                query.data_ptr(),
-                *cache._pointers(),
-                starts.data_ptr(),
-                None if counts is None else counts.data_ptr(),
-                output.data_ptr(),
-                batch,
-                heads,
-                kv_heads,
-                seq_len,
-                dim,
-                *_strides(query),
-                seq_len * heads * dim,
-                heads * dim,
-                cache.key_codes.shape[0],
-                cache.block_table.shape[1],
-                most,
-                dim**-0.5 if scale is None else float(scale),
-                dtype_code(query.dtype),
-                None if workspace is None else workspace.data_ptr(),
-                size,
-                stream_handle(query.device),
-            )
-            check_status(status, "sah_block_cache_attention")
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        launch(
+            device,
+            library.sah_block_cache_attention,
+            "sah_block_cache_attention",
+            query.data_ptr(),
+            *cache._pointers(),
+            starts.data_ptr(),
+            None if counts is None else counts.data_ptr(),
+            output.data_ptr(),
+            batch,
+            heads,
+            kv_heads,
+            seq_len,
+            dim,
+            *_strides(query),
+            seq_len * heads * dim,
+            heads * dim,
+            cache.key_codes.shape[0],
+            cache.block_table.shape[1],
+            most,
+            dim**-0.5 if scale is None else float(scale),
+            dtype_code(dtype),
+            None if workspace is None else workspace.data_ptr(),
+            size,
+        )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block cache attention execution failed") from exc
     return output, HIP_BLOCK_CACHE_ATTENTION_BACKEND

@@ -209,26 +209,17 @@ def stream_handle(device: torch.device) -> int:
     return int(torch._C._cuda_getCurrentRawStream(_device_index(device)))
 
 
-class _SameDevice:
-    """The launch is on the current device: nothing to switch."""
+def launch(device: torch.device, function, what: str, *args) -> None:
+    """Call a C entry on ``device``'s current stream (its last argument), with that
+    device as the current one, and raise :class:`HipLibraryError` on a status."""
 
-    def __enter__(self) -> None:
-        return None
-
-    def __exit__(self, *exc: object) -> None:
-        return None
-
-
-_SAME_DEVICE = _SameDevice()
-
-
-def launch_device(device: torch.device) -> _SameDevice | torch.cuda.device:
-    """Context in which ``device`` is the current one, which a HIP launch on one of
-    its streams needs; free where it is already."""
-
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _SAME_DEVICE
-    return torch.cuda.device(device)
+    if device.index == torch._C._cuda_getDevice():
+        status = function(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = function(*args, stream_handle(device))
+    if status != SAH_OK:
+        check_status(status, what)
 
 
 # gfx950 or not, per device index: device properties do not change within a
@@ -269,7 +260,7 @@ __all__ = [
     "check_status",
     "dtype_code",
     "is_gfx950",
-    "launch_device",
+    "launch",
     "library_available",
     "load_library",
     "stream_handle",

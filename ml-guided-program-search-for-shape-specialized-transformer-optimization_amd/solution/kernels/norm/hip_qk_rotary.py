@@ -14,13 +14,11 @@ from ..hip._library import (
     SAH_NORM_LAYER,
     SAH_NORM_RMS,
     HipLibraryError,
-    check_status,
     dtype_code,
     is_gfx950,
-    launch_device,
+    launch,
     library_available,
     load_library,
-    stream_handle,
 )
 
 HIP_QK_NORM_ROTARY_BACKEND = "hip_qk_norm_rotary"
@@ -53,12 +51,27 @@ def hip_qk_norm_rotary_available() -> bool:
     return library_available()
 
 
-def _heads_ok(value: torch.Tensor) -> bool:
-    unit = 16 // value.element_size()
-    strides = value.stride()
-    if strides[3] != 1 or value.data_ptr() % 16 or (value.requires_grad and torch.is_grad_enabled()):
-        return False
-    return not any(stride % unit and size != 1 for size, stride in zip(value.shape[:3], strides))
+def _heads_ok(value: torch.Tensor, unit: int) -> bool:
+    size, stride = value.shape, value.stride()
+    return not (
+        stride[3] != 1
+        or (stride[0] % unit and size[0] != 1)
+        or (stride[1] % unit and size[1] != 1)
+        or (stride[2] % unit and size[2] != 1)
+        or value.data_ptr() % 16
+        or (value.requires_grad and torch.is_grad_enabled())
+    )
+
+
+def _strides(value: torch.Tensor) -> tuple[int, int, int]:
+    """Strides of the first three axes, 0 for an axis of size 1 (never stepped)."""
+
+    size, stride = value.shape, value.stride()
+    return (
+        stride[0] if size[0] != 1 else 0,
+        stride[1] if size[1] != 1 else 0,
+        stride[2] if size[2] != 1 else 0,
+    )
 
 
 def _param_dtype(parameters: tuple[torch.Tensor | None, ...], like: torch.Tensor) -> torch.dtype | None:
@@ -66,21 +79,72 @@ def _param_dtype(parameters: tuple[torch.Tensor | None, ...], like: torch.Tensor
     parameter is not one the kernel reads."""
 
     found = None
+    dim, device = like.shape[3], like.device
     for parameter in parameters:
         if parameter is None:
             continue
+        dtype = parameter.dtype
         if (
-            parameter.shape != like.shape[3:]
-            or parameter.device != like.device
+            parameter.shape != (dim,)
+            or parameter.device != device
             or not parameter.is_contiguous()
             or parameter.data_ptr() % 16
             or (parameter.requires_grad and torch.is_grad_enabled())
-            or parameter.dtype not in (torch.float32, like.dtype)
-            or (found is not None and parameter.dtype is not found)
+            or (dtype is not torch.float32 and dtype is not like.dtype)
+            or (found is not None and dtype is not found)
         ):
             return None
-        found = parameter.dtype
+        found = dtype
     return torch.float32 if found is None else found
+
+
+def _request(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    parameters: tuple[torch.Tensor | None, ...],
+    table: torch.Tensor | None,
+    starts: torch.Tensor | None,
+    eps: float,
+    norm: str,
+    interleaved: bool,
+) -> torch.dtype | None:
+    """The parameters' dtype of a request that the kernel takes, else None."""
+
+    dtype, size, device = query.dtype, query.shape, query.device
+    key_size = key.shape
+    if dtype not in SUPPORTED_DTYPES or dtype is not key.dtype or len(size) != 4 or len(key_size) != 4:
+        return None
+    batch, heads, seq_len, dim = size
+    if dim not in SUPPORTED_HEAD_DIMS or key_size[0] != batch or key_size[2] != seq_len or key_size[3] != dim:
+        return None
+    if heads < 1 or key_size[1] < 1 or device != key.device or batch * seq_len >= 2**31:
+        return None
+    unit = 4 if dtype is torch.float32 else 8
+    if not (_heads_ok(query, unit) and _heads_ok(key, unit)) or norm not in NORM_KINDS or not eps >= 0:
+        return None
+    if table is not None:
+        rows = table.shape
+        if (
+            len(rows) != 2
+            or not 0 < rows[1] <= dim
+            or rows[1] % (8 if interleaved else 16)
+            or table.dtype is not torch.float32
+            or table.device != device
+            or not table.is_contiguous()
+            or table.data_ptr() % 16
+            or table.requires_grad
+        ):
+            return None
+    if starts is not None and (
+        starts.dtype is not torch.int32
+        or starts.shape != (batch,)
+        or starts.device != device
+        or not starts.is_contiguous()
+    ):
+        return None
+    if not (is_gfx950(device) and library_available()):
+        return None
+    return _param_dtype(parameters, query)
 
 
 def can_use_hip_qk_norm_rotary(
@@ -99,36 +163,8 @@ def can_use_hip_qk_norm_rotary(
 ) -> bool:
     """Whether the kernel takes this request."""
 
-    if query.ndim != 4 or key.ndim != 4 or query.dtype not in SUPPORTED_DTYPES or query.dtype is not key.dtype:
-        return False
-    batch, heads, seq_len, dim = query.shape
-    if dim not in SUPPORTED_HEAD_DIMS or key.shape[0] != batch or key.shape[2:] != query.shape[2:]:
-        return False
-    if heads < 1 or key.shape[1] < 1 or query.device != key.device or batch * seq_len >= 2**31:
-        return False
-    if not (_heads_ok(query) and _heads_ok(key)) or norm not in NORM_KINDS or not eps >= 0:
-        return False
-    if _param_dtype((query_weight, query_bias, key_weight, key_bias), query) is None:
-        return False
-    if table is not None and (
-        table.ndim != 2
-        or table.dtype is not torch.float32
-        or table.device != query.device
-        or not table.is_contiguous()
-        or table.data_ptr() % 16
-        or not 0 < table.shape[1] <= dim
-        or table.shape[1] % (8 if interleaved else 16)
-        or table.requires_grad
-    ):
-        return False
-    if starts is not None and (
-        starts.dtype is not torch.int32
-        or starts.shape != (batch,)
-        or starts.device != query.device
-        or not starts.is_contiguous()
-    ):
-        return False
-    return is_gfx950(query.device) and library_available()
+    parameters = (query_weight, query_bias, key_weight, key_bias)
+    return _request(query, key, parameters, table, starts, eps, norm, interleaved) is not None
 
 
 def hip_qk_norm_rotary(
@@ -158,41 +194,42 @@ def hip_qk_norm_rotary(
     makes NaN of the rotated features.
     """
 
-    if not can_use_hip_qk_norm_rotary(
-        query, key, query_weight, key_weight, table, starts,
-        query_bias=query_bias, key_bias=key_bias, eps=eps, norm=norm, interleaved=interleaved,
-    ):
+    parameters = (query_weight, query_bias, key_weight, key_bias)
+    param_dtype = _request(query, key, parameters, table, starts, eps, norm, interleaved)
+    if param_dtype is None:
         raise RuntimeError("HIP query/key norm with rotation is ineligible for the requested inputs")
     batch, heads, seq_len, dim = query.shape
     kv_heads = key.shape[1]
-    query_out = torch.empty((batch, heads, seq_len, dim), dtype=query.dtype, device=query.device)
-    key_out = torch.empty((batch, kv_heads, seq_len, dim), dtype=query.dtype, device=query.device)
-    param_dtype = _param_dtype((query_weight, query_bias, key_weight, key_bias), query)
-    pointers = [
-        None if t is None else t.data_ptr()
-        for t in (query, key, query_weight, query_bias, key_weight, key_bias, table, starts, query_out, key_out)
-    ]
+    dtype, device = query.dtype, query.device
+    query_out = torch.empty((batch, heads, seq_len, dim), dtype=dtype, device=device)
+    key_out = torch.empty((batch, kv_heads, seq_len, dim), dtype=dtype, device=device)
     try:
-        with launch_device(query.device):
-            status = load_library().sah_qk_norm_rotary(
-                *pointers,
-                batch,
-                seq_len,
-                heads,
-                kv_heads,
-                dim,
-                *(0 if size == 1 else stride for size, stride in zip(query.shape[:3], query.stride())),
-                *(0 if size == 1 else stride for size, stride in zip(key.shape[:3], key.stride())),
-                0 if table is None else table.shape[1],
-                0 if table is None else table.shape[0],
-                int(interleaved),
-                NORM_KINDS[norm],
-                float(eps),
-                dtype_code(query.dtype),
-                dtype_code(param_dtype),
-                stream_handle(query.device),
-            )
-            check_status(status, "sah_qk_norm_rotary")
+        launch(
+            device,
+            load_library().sah_qk_norm_rotary,
+            "sah_qk_norm_rotary",
+            query.data_ptr(),
+            key.data_ptr(),
+            *[None if parameter is None else parameter.data_ptr() for parameter in parameters],
+            None if table is None else table.data_ptr(),
+            None if starts is None else starts.data_ptr(),
+            query_out.data_ptr(),
+            key_out.data_ptr(),
+            batch,
+            seq_len,
+            heads,
+            kv_heads,
+            dim,
+            *_strides(query),
+            *_strides(key),
+            0 if table is None else table.shape[1],
+            0 if table is None else table.shape[0],
+            1 if interleaved else 0,
+            NORM_KINDS[norm],
+            float(eps),
+            dtype_code(dtype),
+            dtype_code(param_dtype),
+        )
     except HipLibraryError as exc:
         raise RuntimeError("HIP query/key norm with rotation execution failed") from exc
     return query_out, key_out, HIP_QK_NORM_ROTARY_BACKEND

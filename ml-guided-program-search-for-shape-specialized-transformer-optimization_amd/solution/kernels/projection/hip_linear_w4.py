@@ -17,13 +17,11 @@ from ..hip._library import (
     SAH_ACTIVATION_GELU_EXACT,
     SAH_ACTIVATION_NONE,
     HipLibraryError,
-    check_status,
     dtype_code,
     is_gfx950,
-    launch_device,
+    launch,
     library_available,
     load_library,
-    stream_handle,
 )
 
 HIP_LINEAR_W4_BACKEND = "hip_linear_w4"
@@ -173,7 +171,8 @@ def _row_stride(value: torch.Tensor) -> int | None:
     if strides[-1] != 1:
         return None
     stride, span = shape[-1], None
-    for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+    for axis in range(len(shape) - 2, -1, -1):
+        size, step = shape[axis], strides[axis]
         if size == 1:
             continue
         if span is None:
@@ -199,26 +198,27 @@ def hip_linear_w4(
     if not can_use_hip_linear_w4(value, weight, bias, activation=activation):
         raise RuntimeError("HIP 4-bit linear is ineligible for the requested inputs")
     in_features, out_features = weight.in_features, weight.out_features
-    output = torch.empty((*value.shape[:-1], out_features), dtype=value.dtype, device=value.device)
+    dtype, device = value.dtype, value.device
+    output = torch.empty((*value.shape[:-1], out_features), dtype=dtype, device=device)
     try:
-        with launch_device(value.device):
-            status = load_library().sah_linear_w4(
-                value.data_ptr(),
-                weight.codes.data_ptr(),
-                weight.scales.data_ptr(),
-                None if bias is None else bias.data_ptr(),
-                output.data_ptr(),
-                value.numel() // in_features,
-                in_features,
-                out_features,
-                weight.group_size,
-                _row_stride(value),
-                out_features,
-                dtype_code(value.dtype),
-                ACTIVATIONS[activation],
-                stream_handle(value.device),
-            )
-            check_status(status, "sah_linear_w4")
+        launch(
+            device,
+            load_library().sah_linear_w4,
+            "sah_linear_w4",
+            value.data_ptr(),
+            weight.codes.data_ptr(),
+            weight.scales.data_ptr(),
+            None if bias is None else bias.data_ptr(),
+            output.data_ptr(),
+            value.numel() // in_features,
+            in_features,
+            out_features,
+            in_features // weight.scales.shape[0],
+            _row_stride(value),
+            out_features,
+            dtype_code(dtype),
+            ACTIVATIONS[activation],
+        )
     except HipLibraryError as exc:
         raise RuntimeError("HIP 4-bit linear execution failed") from exc
     return output, HIP_LINEAR_W4_BACKEND
