@@ -71,6 +71,14 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
   return (uint32_t)v;
 }
 
+// HBM-bound on prompts: a token is read once, its codes written once, with all of a
+// block's loads in flight before its largest magnitude is known.  Heads are dealt to
+// neighbouring workgroups, so that a token's heads, neighbours in a packed projection,
+// are read at the same time, and past the caches:
+//   4 x 8001 tokens, 8 heads of 128, fp16 (197 MB): 41 us, 4.7 TB/s (48 through the
+//   caches); 8 x 4001 tokens, 16 heads of 64: 43 us (66 block by block of a head)
+//   64 x 1 token, 16 heads of 64: 4.0 us, 6.4 where some blocks are completed
+//
 // One workgroup takes one block of (sequence, head): it codes the block if the
 // append completes it, from the tail's old tokens and the new ones.  The first
 // block's workgroup, the only one that reads the old tail, then also writes the new
@@ -81,14 +89,14 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
   constexpr int LANES = D / 8;                 // of one token
   constexpr int TOKENS = kThreads / LANES;     // of one pass
   constexpr int PASSES = kBlockTokens / TOKENS;
-  constexpr int ROW = kBlockTokens + 16;       // bytes of a feature in LDS
+  constexpr int ROW = kBlockTokens + 4;        // bytes of a feature in LDS: features on different banks
   __shared__ float largest_of[2][kThreads / 64];
-  __shared__ __align__(16) uint8_t turned[D * ROW];
+  __shared__ __align__(4) uint8_t turned[D * ROW];
 
-  const uint32_t index = blockIdx.x % a.span;
-  const uint32_t pair = blockIdx.x / a.span;
-  const int h = (int)(pair % (uint32_t)a.cache.heads);
-  const int64_t b = pair / (uint32_t)a.cache.heads;
+  const uint32_t pair = blockIdx.x / (uint32_t)a.cache.heads;
+  const int h = (int)(blockIdx.x - pair * (uint32_t)a.cache.heads);
+  const uint32_t index = pair % a.span;
+  const int64_t b = pair / a.span;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
 
@@ -102,6 +110,8 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
   const bool complete = (block + 1) * kBlockTokens <= end;
   if (index != 0 && !complete) return;
 
+  const int64_t id = complete && block < a.cache.max_blocks ? (int64_t)a.cache.table[b * a.cache.max_blocks + block] : -1;
+  const bool held = id >= 0 && id < a.cache.blocks;  // a page outside the cache takes nothing
   const int feature = (tid & (LANES - 1)) * 8;
   const int token0 = tid / LANES;
   const T* key = static_cast<const T*>(a.key) + b * a.k_sb + h * a.k_sh + feature;
@@ -125,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
     float k_largest = 0.0f, v_largest = 0.0f;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int slot = p * TOKENS + token0;
+      const int slot = token0 * PASSES + p;
       const int64_t position = block * kBlockTokens + slot;
       if (position < start) {  // index 0 only: an older token of this block
         k[p] = *reinterpret_cast<const V8*>(key_tail + slot * D + feature);
@@ -133,8 +143,8 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
         for (int e = 0; e < 8; ++e) v[p][e] = value_tail[(feature + e) * kBlockTokens + slot];
       } else {
         const int64_t at = position - start;
-        k[p] = *reinterpret_cast<const V8*>(key + at * a.k_ss);
-        v[p] = *reinterpret_cast<const V8*>(value + at * a.v_ss);
+        k[p] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(key + at * a.k_ss));
+        v[p] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(value + at * a.v_ss));
       }
     }
 #pragma unroll
@@ -165,13 +175,13 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
     }
     const int k_power = scale_power(k_largest), v_power = scale_power(v_largest);
     const float k_inverse = power_of_two(-k_power), v_inverse = power_of_two(-v_power);
-    const int64_t id = block < a.cache.max_blocks ? (int64_t)a.cache.table[b * a.cache.max_blocks + block] : -1;
-    const bool held = id >= 0 && id < a.cache.blocks;  // a page outside the cache takes nothing
     const int64_t code_at = (id * a.cache.heads + h) * (int64_t)(kBlockTokens * D);
+    u32x2 value_coded[PASSES];
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int slot = p * TOKENS + token0;
-      u32x2 coded = {0x7f7f7f7fu, 0x7f7f7f7fu}, value_coded = {0u, 0u};
+      const int slot = token0 * PASSES + p;
+      u32x2 coded = {0x7f7f7f7fu, 0x7f7f7f7fu};
+      value_coded[p] = (u32x2){0u, 0u};
       if (!bad[p]) {
         float f[8];
 #pragma unroll
@@ -179,18 +189,28 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
         coded = (u32x2){pack_e4m3(f[0], f[1], f[2], f[3]), pack_e4m3(f[4], f[5], f[6], f[7])};
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = to_f32(v[p][e]) * v_inverse;
-        value_coded = (u32x2){pack_e4m3(f[0], f[1], f[2], f[3]), pack_e4m3(f[4], f[5], f[6], f[7])};
+        value_coded[p] = (u32x2){pack_e4m3(f[0], f[1], f[2], f[3]), pack_e4m3(f[4], f[5], f[6], f[7])};
       }
       if (held) *reinterpret_cast<u32x2*>(a.cache.key_codes + code_at + slot * D + feature) = coded;
+    }
+    // The values turn in LDS: a thread's PASSES neighbouring tokens leave together.
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        turned[(feature + e) * ROW + slot] = (uint8_t)(value_coded[e / 4] >> (8 * (e % 4)));
+    for (int e = 0; e < 8; ++e) {
+      uint32_t codes = 0;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) codes |= (value_coded[p][e / 4] >> (8 * (e % 4)) & 0xffu) << (8 * p);
+      uint8_t* to = turned + (feature + e) * ROW + token0 * PASSES;
+      if constexpr (PASSES == 4)
+        *reinterpret_cast<uint32_t*>(to) = codes;
+      else
+        *reinterpret_cast<uint16_t*>(to) = (uint16_t)codes;
     }
     __syncthreads();
     if (held) {
 #pragma unroll
       for (int i = tid; i < D * 4; i += kThreads) {
-        const u32x4 part = *reinterpret_cast<const u32x4*>(turned + (i / 4) * ROW + (i % 4) * 16);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(turned + (i / 4) * ROW + (i % 4) * 16);
+        const u32x4 part = {from[0], from[1], from[2], from[3]};
         store16(a.cache.value_codes + code_at + i * 16, part);
       }
       if (tid == 0) {
@@ -249,10 +269,10 @@ __global__ __launch_bounds__(kThreads) void block_read_kernel(const ReadArgs a) 
   constexpr int ROW = kBlockTokens + 4;  // values of a feature in LDS
   __shared__ T turned[D * ROW];
 
-  const uint32_t index = blockIdx.x % a.span;
-  const uint32_t pair = blockIdx.x / a.span;
-  const int h = (int)(pair % (uint32_t)a.cache.heads);
-  const int64_t b = pair / (uint32_t)a.cache.heads;
+  const uint32_t pair = blockIdx.x / (uint32_t)a.cache.heads;
+  const int h = (int)(blockIdx.x - pair * (uint32_t)a.cache.heads);
+  const uint32_t index = pair % a.span;
+  const int64_t b = pair / a.span;
   const int tid = threadIdx.x;
   const int64_t first = a.firsts[b], length = a.lengths[b];
   // blocks from the one of `first` on, rounded down (also below zero)

@@ -10,8 +10,11 @@
 // small beside its heads.  D / 8 lanes hold a row of 8 features each, so a
 // wavefront covers 512 / D rows an access; the rows of an access are neighbouring
 // heads of one token (the packed projection's output is read in whole lines), and
-// the wave goes over up to kHeadSteps such groups with one read of the table row.
-// All its loads are issued before the first sum.
+// the wave goes over up to STEPS such groups with one read of the table row.  All its
+// loads are issued before the first sum.
+//   2 x 50001 tokens, 16 + 16 heads of 64, bf16 (846 MB): 208 us, 4.1 TB/s (228 with
+//   cached loads and stores)
+//   1 token of the same: 3.4 us (4.8 with four groups of heads a wave)
 
 #include <type_traits>
 
@@ -22,26 +25,38 @@ namespace {
 
 constexpr int kWave = 64;
 constexpr int kWaves = 4;
-constexpr int kHeadSteps = 4;
 
-template <typename T>
+// 16 bytes, past the caches where STREAM.
+template <bool STREAM>
+__device__ __forceinline__ u32x4 fetch(const void* p) {
+  return STREAM ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)) : load16(p);
+}
+template <bool STREAM>
+__device__ __forceinline__ void put(void* p, u32x4 v) {
+  if (STREAM)
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));
+  else
+    store16(p, v);
+}
+
+template <bool STREAM, typename T>
 __device__ __forceinline__ void load8(const T* p, float* out) {
   if constexpr (sizeof(T) == 4) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    const f32x4 a = __builtin_bit_cast(f32x4, fetch<STREAM>(p)), b = __builtin_bit_cast(f32x4, fetch<STREAM>(p + 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = a[i], out[i + 4] = b[i];
   } else {
-    unpack8<T>(load16(p), out);
+    unpack8<T>(fetch<STREAM>(p), out);
   }
 }
 
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void store8(T* p, const float* in) {
   if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f32x4*>(p) = (f32x4){in[0], in[1], in[2], in[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = (f32x4){in[4], in[5], in[6], in[7]};
+    put<STREAM>(p, __builtin_bit_cast(u32x4, (f32x4){in[0], in[1], in[2], in[3]}));
+    put<STREAM>(p + 4, __builtin_bit_cast(u32x4, (f32x4){in[4], in[5], in[6], in[7]}));
   } else {
-    store16(p, pack8<T>(in));
+    put<STREAM>(p, pack8<T>(in));
   }
 }
 
@@ -65,7 +80,7 @@ struct RotaryArgs {
   float eps;
 };
 
-template <typename T, typename TP, int D>
+template <typename T, typename TP, int D, int STEPS, bool STREAM>
 __global__ __launch_bounds__(kWaves * kWave) void qk_rotary_kernel(const RotaryArgs a) {
   constexpr int LANES = D / 8;            // of one row
   constexpr int ROWS = kWave / LANES;     // of one access
@@ -79,11 +94,11 @@ __global__ __launch_bounds__(kWaves * kWave) void qk_rotary_kernel(const RotaryA
   const uint32_t b = here ? token / (uint32_t)a.seq_len : 0;
   const uint32_t s = here ? token - b * (uint32_t)a.seq_len : 0;
   const int all = a.heads + a.kv_heads;
-  const int first_head = (int)blockIdx.y * a.row_heads * kHeadSteps + (row & (a.row_heads - 1));
+  const int first_head = (int)blockIdx.y * a.row_heads * STEPS + (row & (a.row_heads - 1));
 
-  float x[kHeadSteps][8];
+  float x[STEPS][8];
 #pragma unroll
-  for (int u = 0; u < kHeadSteps; ++u) {
+  for (int u = 0; u < STEPS; ++u) {
     const int h = first_head + u * a.row_heads;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
@@ -91,7 +106,7 @@ __global__ __launch_bounds__(kWaves * kWave) void qk_rotary_kernel(const RotaryA
       const T* p = h < a.heads
                        ? static_cast<const T*>(a.query) + b * a.q_sb + h * a.q_sh + s * a.q_ss
                        : static_cast<const T*>(a.key) + b * a.k_sb + (h - a.heads) * a.k_sh + s * a.k_ss;
-      load8<T>(p + chunk * 8, x[u]);
+      load8<STREAM>(p + chunk * 8, x[u]);
     }
   }
 
@@ -113,8 +128,8 @@ __global__ __launch_bounds__(kWaves * kWave) void qk_rotary_kernel(const RotaryA
         for (int e = 0; e < 8; ++e) cs[e] = c4[e / 2], sn[e] = s4[e / 2];
       } else {
         const int at = chunk * 8 < half ? chunk * 8 : chunk * 8 - half;
-        load8<float>(t + at, cs);
-        load8<float>(t + half + at, sn);
+        load8<false>(t + at, cs);
+        load8<false>(t + half + at, sn);
       }
     } else {
 #pragma unroll
@@ -134,12 +149,12 @@ __global__ __launch_bounds__(kWaves * kWave) void qk_rotary_kernel(const RotaryA
   for (int k = 0; k < 2; ++k) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[k][e] = 1.0f, bias[k][e] = 0.0f;
-    if (a.weight[k] != nullptr) load8<TP>(static_cast<const TP*>(a.weight[k]) + chunk * 8, w[k]);
-    if (a.bias[k] != nullptr) load8<TP>(static_cast<const TP*>(a.bias[k]) + chunk * 8, bias[k]);
+    if (a.weight[k] != nullptr) load8<false>(static_cast<const TP*>(a.weight[k]) + chunk * 8, w[k]);
+    if (a.bias[k] != nullptr) load8<false>(static_cast<const TP*>(a.bias[k]) + chunk * 8, bias[k]);
   }
 
 #pragma unroll
-  for (int u = 0; u < kHeadSteps; ++u) {
+  for (int u = 0; u < STEPS; ++u) {
     const int h = first_head + u * a.row_heads;
     const bool is_key = h >= a.heads;
     float mean = 0.0f;
@@ -182,31 +197,44 @@ __global__ __launch_bounds__(kWaves * kWave) void qk_rotary_kernel(const RotaryA
     if (here && h < all) {
       T* p = is_key ? static_cast<T*>(a.key_out) + ((int64_t)b * a.kv_heads + (h - a.heads)) * a.seq_len * D + (int64_t)s * D
                     : static_cast<T*>(a.query_out) + ((int64_t)b * a.heads + h) * a.seq_len * D + (int64_t)s * D;
-      store8<T>(p + chunk * 8, out);
+      store8<STREAM>(p + chunk * 8, out);
     }
   }
 }
 
-template <typename T, typename TP, int D>
-int launch_rotary(RotaryArgs a, hipStream_t stream) {
-  constexpr int ROWS = 512 / D;
-  const int all = a.heads + a.kv_heads;
-  a.row_heads = 1;
-  while (a.row_heads < ROWS && a.row_heads < all) a.row_heads *= 2;
-  const int64_t tokens_a_block = (int64_t)kWaves * (ROWS / a.row_heads);
-  const unsigned chunks = (unsigned)ceil_div(all, (int64_t)a.row_heads * kHeadSteps);
+template <typename T, typename TP, int D, int STEPS, bool STREAM>
+int launch_steps(RotaryArgs a, int64_t tokens_a_block, hipStream_t stream) {
+  const unsigned chunks = (unsigned)ceil_div(a.heads + a.kv_heads, (int64_t)a.row_heads * STEPS);
   // A grid holds fewer than 2^32 work items a dimension: more tokens go out as several launches.
   const int64_t per_launch = (int64_t)(UINT32_MAX / (kWaves * kWave)) * tokens_a_block;
   for (int64_t first = 0; first < (int64_t)a.tokens; first += per_launch) {
     const int64_t left = (int64_t)a.tokens - first;
     const int64_t count = left < per_launch ? left : per_launch;
     a.first_token = (uint32_t)first;
-    hipLaunchKernelGGL((qk_rotary_kernel<T, TP, D>), dim3((unsigned)ceil_div(count, tokens_a_block), chunks),
-                       dim3(kWaves * kWave), 0, stream, a);
+    hipLaunchKernelGGL((qk_rotary_kernel<T, TP, D, STEPS, STREAM>),
+                       dim3((unsigned)ceil_div(count, tokens_a_block), chunks), dim3(kWaves * kWave), 0, stream, a);
     const int status = check_hip(hipGetLastError(), "query/key rotary kernel launch");
     if (status != SAH_OK) return status;
   }
   return SAH_OK;
+}
+
+// Groups of heads a wave: one where four would leave SIMDs of the 256 compute units
+// without a wave (one read of the table row less against three passes in a row).
+// Past the caches: outputs over half of the 256 MB last-level cache, which the next
+// operator would not find there.
+template <typename T, typename TP, int D>
+int launch_rotary(RotaryArgs a, hipStream_t stream) {
+  constexpr int ROWS = 512 / D;
+  const int64_t all = a.heads + a.kv_heads;
+  a.row_heads = 1;
+  while (a.row_heads < ROWS && a.row_heads < all) a.row_heads *= 2;
+  const int64_t tokens_a_block = (int64_t)kWaves * (ROWS / a.row_heads);
+  const int64_t waves = ceil_div(a.tokens, ROWS / a.row_heads) * ceil_div(all, 4 * a.row_heads);
+  if (waves < 1024) return launch_steps<T, TP, D, 1, false>(a, tokens_a_block, stream);
+  return (int64_t)a.tokens * all * D * (int64_t)sizeof(T) > ((int64_t)128 << 20)
+             ? launch_steps<T, TP, D, 4, true>(a, tokens_a_block, stream)
+             : launch_steps<T, TP, D, 4, false>(a, tokens_a_block, stream);
 }
 
 template <typename T, typename TP>

@@ -101,6 +101,26 @@ def test_rotary_layouts(gpu_device, changes):
     _rotary_case(gpu_device, **{**sizes, **changes})
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rotary_of_many_tokens_is_that_of_few(gpu_device, dtype):
+    """Outputs past the caches, several groups of heads a wave, and few tokens: the same bits."""
+
+    from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
+
+    seq = 34_001 if dtype is BF16 else 17_001
+    packed = torch.randn(2, seq, 20, 64, generator=torch.Generator(device=gpu_device).manual_seed(5), device=gpu_device).to(dtype)
+    table = rotary_table(seq + 9, 64, device=gpu_device)
+    weight = torch.linspace(0.5, 1.5, 64, device=gpu_device)
+    views = lambda t: (t[:, :, :16].transpose(1, 2), t[:, :, 16:].transpose(1, 2))  # noqa: E731
+    starts = lambda at: torch.tensor([at, at + 9], dtype=torch.int32, device=gpu_device)  # noqa: E731
+    with torch.inference_mode():
+        query, key, _ = hip_qk_norm_rotary(*views(packed), weight, weight, table, starts(0))
+        assert query.numel() * query.element_size() > 128 << 20
+        for at, count in ((0, 1), (17_000, 1), (4_999, 3_000), (seq - 77, 77)):
+            part = hip_qk_norm_rotary(*views(packed[:, at : at + count]), weight, weight, table, starts(at))
+            assert torch.equal(query[:, :, at : at + count], part[0]) and torch.equal(key[:, :, at : at + count], part[1])
+
+
 def test_rotary_of_zeros_and_broadcast_heads(gpu_device):
     from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
 
