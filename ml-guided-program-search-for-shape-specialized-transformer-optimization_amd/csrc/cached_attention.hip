@@ -7,7 +7,7 @@
 // block and head, and the incomplete last block in 16 bits.
 //
 // Mapping.  The query heads of one key head and the chunk's tokens are the rows of
-// one matrix; a wave holds TILES x 16 of them and walks over blocks of 64 tokens:
+// one matrix; a wave holds 16 of them and walks over blocks of 64 tokens:
 //   S^T = K Q^T    16 x 16 x 32 instructions with 16 tokens of K as rows
 //   O^T += V^T P^T  the same with 16 features of V as rows
 // In this orientation a lane holds the scores of ONE query row (l % 16) for 16
@@ -16,24 +16,37 @@
 // rescaling is one factor a lane.  K rows are dealt to the instruction's rows so
 // that these 16 tokens are neighbours: the value codes, feature by feature in the
 // cache, are then 16 bytes a lane, as the key codes are.  A wave loads its blocks
-// straight into registers, the next one while it works on this one; nothing but the
-// final merge goes through LDS.
+// straight into registers, the next block's keys and values as soon as this one's are
+// used; nothing but the final merge goes through LDS.  More than 16 rows (a chunk of
+// tokens) go to a kernel of their own further down.
 //
 // Precision.  Codes are exact in both types, so Q K^T takes them in the queries'
-// type; the weights are fp16 (times 2^12, so that none above 2^-26 of the largest is
+// type; the weights are fp16 (times 2^11, so that none above 2^-25 of the largest is
 // subnormal), the scales, maxima, sums and outputs fp32.
 //
 // A long history is split over workgroups (and over the waves of one); a second
 // launch merges their outputs with their maxima and sums.
+//
+// Bounds.  For a single token every feature of a held token is 2 bytes to read for
+// 4 * group operations, so the codes' way from memory bounds it: 4 sequences of 90000
+// to 100000 tokens, 16 heads of 64, 779 MB in 139 us, 5.6 TB/s (a copy moves 4.9), and
+// 4.7 us for the merge of their chunks.  32 ragged sequences of 100 to 4095 tokens,
+// 32 / 8 heads of 128 (138 MB), take 38 us and 4.6, one of 777 tokens 7.5: there the
+// longest wave's chain of loads bounds it.
 
 #include <type_traits>
 
 #include "decode_common.hpp"
+#include "gemm_mainloop.hpp"
 
 namespace sah {
 namespace {
 
-constexpr float kWeightShift = 12.0f;  // log2 of what the weights are scaled by
+// Weights are 2^(score - base + kWeightShift); a row's base is raised to its maximum
+// when that exceeds it by kWeightMargin, so no weight is above 2^15.
+constexpr float kWeightShift = 11.0f;
+constexpr float kWeightMargin = 4.0f;
+constexpr float kUnshift = 0x1p-11f;  // 2^-kWeightShift
 constexpr int kUnits = 256;            // compute units
 
 struct AttentionArgs {
@@ -77,49 +90,48 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// A wave's common value in a scalar register: a branch on it then is one, which the
+// compiler does not see of what it divides or loads in vector registers.
+__device__ __forceinline__ int common(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// The maximum over lanes l and l ^ 32.
+__device__ __forceinline__ float halves_max(float x) {
+  const uint32_t a = __float_as_uint(x);
+  const auto h = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+
 // Powers of two by their fp32 bits: 2^a / 2^b, 2^-126 where it is less.
 __device__ __forceinline__ float power_ratio(int a_bits, int b_bits) {
   const int bits = 0x3f800000 + (a_bits - b_bits);
   return __int_as_float(bits < 0x00800000 ? 0x00800000 : bits);
 }
 
-// One block's codes of a wave: 16 bytes of a key row (value feature) a lane and tile.
-template <int D>
-struct KeyCodes {
-  u32x4 part[4][D / 64];
-};
-template <int D>
-struct ValueCodes {
-  u32x4 part[D / 16];
-};
-
-template <typename T, int D, int TILES, int SPLIT, int ROWS>
-__global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(const AttentionArgs a) {
+template <typename T, int D, int SPLIT>
+__global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const AttentionArgs a) {
   typedef typename Vec8<T>::type V8;
   constexpr int HALVES = D / 64;
   constexpr int FEATURES = D / 16;
-  // One tile of rows waits for memory: keys and values of the next block are loaded
-  // while this one is worked on.  More tiles work: the values come while the scores
-  // are formed and the next keys during the rest, in half the registers.
-  constexpr bool AHEAD = TILES == 1;
-  // With more tiles the matrix cores add up the weights too (a row of ones).
-  constexpr bool ONES = TILES > 1;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int column = lane & 15;    // query row of a tile; key row / value feature of an operand
+  const int split = common(threadIdx.x >> 6);
+  const int column = lane & 15;    // query row; key row / value feature of an operand
   const int quarter = lane >> 4;
-  const int split = wave % SPLIT;
 
   uint32_t at = blockIdx.x;
-  const int chunk = (int)(at % (uint32_t)a.chunks);
+  const int chunk = common((int)(at % (uint32_t)a.chunks));
   at /= (uint32_t)a.chunks;
-  const uint32_t row_group = (at % a.row_groups) * ROWS + wave / SPLIT;
-  at /= a.row_groups;
-  const int h = (int)(at % (uint32_t)a.kv_heads);
-  const int64_t b = at / (uint32_t)a.kv_heads;
+  const int h = common((int)(at % (uint32_t)a.kv_heads));
+  const int64_t b = common((int)(at / (uint32_t)a.kv_heads));
 
-  const int64_t start = a.starts[b];
-  int count = a.counts != nullptr ? a.counts[b] : a.seq_len;
+  // The table entries of this wave's first blocks are asked for before its lengths are
+  // known; those behind the sequence's blocks are not used.
+  const int64_t from64 = (int64_t)chunk * a.chunk_blocks;
+  int first_pages = -1;
+  if (from64 + split + lane * SPLIT < a.max_blocks)
+    first_pages = a.table[b * a.max_blocks + from64 + split + lane * SPLIT];
+
+  const int64_t start = common(a.starts[b]);
+  int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
   if (count > a.seq_len) count = a.seq_len;
   if (start < 0 || count < 0) count = 0;
   // More tokens than the table can name: NaN.  Otherwise positions are below 2^31.
@@ -127,371 +139,710 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void cached_attention_kernel(con
   const int first_position = beyond ? 0 : (int)start;
   const int tail_block = beyond ? 0 : (int)((start + count) / kBlockTokens);
 
-  // This lane's rows: token row / group of the chunk, query head h * group + row % group.
-  const uint32_t first_row = row_group * (TILES * 16);  // rows are below 2^31
-  int token[TILES], head[TILES];
+  // This lane's row: token column / group of the chunk, query head h * group + column % group.
+  const int token = column / a.group;
+  const int head = h * a.group + (column - token * a.group);
+  const bool live = token < count;
+  const int last_position = first_position + count - 1;  // -1 or less: no query
+  // The position up to which the row sees; a row without a query sees as far as the last.
+  const int sees = live ? first_position + token : last_position;
+  V8 q[HALVES][2];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const uint32_t row = first_row + t * 16 + column;
-    token[t] = (int)(row / (uint32_t)a.group);
-    head[t] = h * a.group + (int)(row - (uint32_t)token[t] * (uint32_t)a.group);
-  }
-  int last_position = -1, least_position = INT32_MAX;  // of the wave's rows
-  {
-    const int low = (int)(first_row / (uint32_t)a.group);
-    const int high = (int)((first_row + TILES * 16 - 1) / (uint32_t)a.group);
-    if (low < count) {
-      least_position = first_position + low;
-      last_position = first_position + (high < count ? high : count - 1);
-    }
-  }
-  // Positions up to which a row sees; rows without a query see as far as the last.
-  int sees[TILES];
-  V8 q[TILES][HALVES][2];
+  for (int hh = 0; hh < HALVES; ++hh)
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const bool live = token[t] < count;
-    sees[t] = live ? first_position + token[t] : last_position;
-#pragma unroll
-    for (int hh = 0; hh < HALVES; ++hh)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        u32x4 raw = {0u, 0u, 0u, 0u};
-        if (live) {
-          raw = load16(static_cast<const T*>(a.query) + b * a.q_sb + head[t] * a.q_sh + token[t] * a.q_ss +
-                       hh * 64 + quarter * 16 + kk * 8);
-          raw = (raw ^ a.sign) & a.keep;
-        }
-        q[t][hh][kk] = __builtin_bit_cast(V8, raw);
+    for (int kk = 0; kk < 2; ++kk) {
+      u32x4 raw = {0u, 0u, 0u, 0u};
+      if (live) {
+        raw = load16(static_cast<const T*>(a.query) + b * a.q_sb + head * a.q_sh + token * a.q_ss + hh * 64 +
+                     quarter * 16 + kk * 8);
+        raw = (raw ^ a.sign) & a.keep;
       }
-  }
+      q[hh][kk] = __builtin_bit_cast(V8, raw);
+    }
 
-  // Blocks of this wave: the row group's, in chunks, the last chunk with the rest.
-  const int all_blocks = last_position < 0 || beyond ? 0 : last_position / kBlockTokens + 1;
-  const int64_t from64 = (int64_t)chunk * a.chunk_blocks;
+  // Blocks of this workgroup: the sequence's, in chunks, the last chunk with the rest.
+  const int all_blocks = count == 0 || beyond ? 0 : last_position / kBlockTokens + 1;
   const int from = from64 < all_blocks ? (int)from64 : all_blocks;
   const int to = chunk == a.chunks - 1 || all_blocks - from < a.chunk_blocks ? all_blocks : from + a.chunk_blocks;
   const int coded_to = to < tail_block ? to : tail_block;
 
   // Outputs are held in units of a power of two, the largest value scale so far.
-  f32x4 out[TILES][FEATURES];
+  f32x4 out[FEATURES];
   int unit = 0;  // its bits; 0 before the first block
-  float most[TILES], sum[TILES];
-  f32x4 sums[TILES];
+  float most = -INFINITY;
+  float sum = beyond && count != 0 ? __builtin_nanf("") : 0.0f;
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    most[t] = -INFINITY;
-    sum[t] = beyond && last_position >= 0 ? __builtin_nanf("") : 0.0f;
-    sums[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int f = 0; f < FEATURES; ++f) out[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int f = 0; f < FEATURES; ++f) out[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   auto raise_unit = [&](int bits) {
     if (bits <= unit) return;
     if (unit != 0) {
       const float change = power_ratio(unit, bits);
 #pragma unroll
-      for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int f = 0; f < FEATURES; ++f) out[t][f] *= change;
+      for (int f = 0; f < FEATURES; ++f) out[f] *= change;
     }
     unit = bits;
   };
 
-  // The weights of a tile's row for one block, from its scores (16 tokens of the row
-  // in this lane): the running maximum, sum and output are brought to it.
-  auto softmax_step = [&](int t, f32x4 (&s)[4], float factor, int block, bool add) {
-    if (block * kBlockTokens + (kBlockTokens - 1) > least_position) {
-      const int open = sees[t] - block * kBlockTokens - quarter * 16;  // last visible of this lane's tokens
+  // The weights of the row for one block, from its scores (16 tokens of it in this
+  // lane): the base, the sum and the output are brought to it.
+  auto softmax_step = [&](f32x4 (&s)[4], float factor, int block) {
+    if (block * kBlockTokens + (kBlockTokens - 1) > first_position) {
+      const int open = sees - block * kBlockTokens - quarter * 16;  // last visible of this lane's tokens
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (i * 4 + j > open) s[i][j] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (r > open) s[r / 4][r % 4] = -INFINITY;
     }
-    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    float top = fmaxf(s[0][0], s[0][1]);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      top = fmaxf(fmaxf(top, s[i][0]), s[i][1]);
-      top = fmaxf(fmaxf(top, s[i][2]), s[i][3]);
-    }
-    const float before = most[t];
-    const float now = fmaxf(before, quarters_max(top) * factor);
-    if (__any(now > before)) {
+    for (int r = 2; r < 16; r += 2) top = fmaxf(fmaxf(top, s[r / 4][r % 4]), s[r / 4][r % 4 + 1]);
+    top = quarters_max(top) * factor;
+    if (__any(top > most + kWeightMargin)) {
+      const float now = fmaxf(most, top);
       // a row that has seen nothing yet has no output to rescale
-      const float change = before == -INFINITY ? 0.0f : exp2_fast(before - now);
-      sum[t] *= change;
-      if (ONES) sums[t] *= change;
+      const float change = most == -INFINITY ? 0.0f : exp2_fast(most - now);
+      sum *= change;
 #pragma unroll
-      for (int f = 0; f < FEATURES; ++f) out[t][f] *= change;
-      most[t] = now;
+      for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+      most = now;
     }
-    const float shift = kWeightShift - (now == -INFINITY ? 0.0f : now);
+    const float shift = kWeightShift - (most == -INFINITY ? 0.0f : most);
     float lane_sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = exp2_fast(fmaf(s[i][j], factor, shift));
-        if (add) lane_sum += s[i][j];
-      }
-    if (add) sum[t] += lane_sum;
+    for (int r = 0; r < 16; ++r) {
+      s[r / 4][r % 4] = exp2_fast(fmaf(s[r / 4][r % 4], factor, shift));
+      lane_sum += s[r / 4][r % 4];
+    }
+    sum += lane_sum;
   };
 
-  auto load_keys = [&](KeyCodes<D>& c, int id) {
-    const uint8_t* keys = a.key_codes + ((int64_t)id * a.kv_heads + h) * (kBlockTokens * D) + quarter * 16;
+  // One block's codes: 16 bytes of a key row (value feature) a lane and tile.
+  u32x4 keys[4][HALVES], values[FEATURES];
+  auto load_keys = [&](int page) {
+    const uint8_t* codes = a.key_codes + ((int64_t)page * a.kv_heads + h) * (kBlockTokens * D) + quarter * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int hh = 0; hh < HALVES; ++hh)
-        c.part[i][hh] = load16(keys + ((column >> 2) * 16 + i * 4 + (column & 3)) * D + hh * 64);
+        keys[r][hh] = load16(codes + ((column >> 2) * 16 + r * 4 + (column & 3)) * D + hh * 64);
   };
-  auto load_values = [&](ValueCodes<D>& c, int id) {
-    const uint8_t* values = a.value_codes + ((int64_t)id * a.kv_heads + h) * (kBlockTokens * D) + quarter * 16;
+  auto load_values = [&](int page) {
+    const uint8_t* codes = a.value_codes + ((int64_t)page * a.kv_heads + h) * (kBlockTokens * D) + quarter * 16;
 #pragma unroll
-    for (int f = 0; f < FEATURES; ++f) c.part[f] = load16(values + (f * 16 + column) * kBlockTokens);
+    for (int f = 0; f < FEATURES; ++f) values[f] = load16(codes + (f * 16 + column) * kBlockTokens);
   };
 
   // A wave's blocks, 64 at a time: a lane each looks up the page and its scales.
   for (int base = from + split; base < coded_to; base += 64 * SPLIT) {
-    int pages = -1;
-    float key_scales = 0.0f, value_scales = 0.0f;
     const int mine = base + lane * SPLIT;
-    if (mine < coded_to) {
-      pages = a.table[b * a.max_blocks + mine];  // mine < tail_block <= max_blocks
-      if (pages < 0 || pages >= a.blocks) pages = -1;
-      if (pages >= 0) {
-        key_scales = a.key_scales[(int64_t)pages * a.kv_heads + h];
-        value_scales = a.value_scales[(int64_t)pages * a.kv_heads + h];
-      }
+    int pages = first_pages;
+    if (base != from + split && mine < coded_to) pages = a.table[b * a.max_blocks + mine];
+    if (mine >= coded_to || pages < 0 || pages >= a.blocks) pages = -1;
+    float key_scales = 0.0f, value_scales = 0.0f;
+    if (pages >= 0) {
+      key_scales = a.key_scales[(int64_t)pages * a.kv_heads + h];
+      value_scales = a.value_scales[(int64_t)pages * a.kv_heads + h];
     }
     const int left = (coded_to - base + SPLIT - 1) / SPLIT;
-    const int count_here = left < 64 ? left : 64;
-    KeyCodes<D> next_keys;
-    ValueCodes<D> next_values;
+    const int here = left < 64 ? left : 64;
     int page = __builtin_amdgcn_readlane(pages, 0);
     if (page >= 0) {
-      load_keys(next_keys, page);
-      if (AHEAD) load_values(next_values, page);
+      load_keys(page);
+      load_values(page);
     }
-    for (int i = 0; i < count_here; ++i) {
+    for (int i = 0; i < here; ++i) {
       const int block = base + i * SPLIT;
       const bool held = page >= 0;
-      const int here = page;
-      KeyCodes<D> keys = next_keys;
-      ValueCodes<D> values;
-      if (AHEAD) values = next_values;
-      page = i + 1 < count_here ? __builtin_amdgcn_readlane(pages, i + 1) : -1;
-      if (AHEAD && page >= 0) {
-        load_keys(next_keys, page);
-        load_values(next_values, page);
-      }
-      f32x4 s[TILES][4];
+      page = i + 1 < here ? __builtin_amdgcn_readlane(pages, i + 1) : -1;
+      f32x4 s[4];
       if (held) {
-        if (!AHEAD) load_values(values, here);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int hh = 0; hh < HALVES; ++hh)
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-              const V8 k = e4m3_operand<T>(keys.part[r][hh][2 * kk], keys.part[r][hh][2 * kk + 1], 1.0f);
-#pragma unroll
-              for (int t = 0; t < TILES; ++t)
-                s[t][r] = mfma16(k, q[t][hh][kk], hh + kk == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : s[t][r]);
-            }
+            for (int kk = 0; kk < 2; ++kk)
+              s[r] = mfma16(e4m3_operand<T>(keys[r][hh][2 * kk], keys[r][hh][2 * kk + 1], 1.0f), q[hh][kk],
+                            hh + kk == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : s[r]);
       }
-      if (!AHEAD && page >= 0) load_keys(next_keys, page);
-      if (!held) {  // a page outside the cache: every row that sees it answers NaN
+      if (page >= 0) load_keys(page);
+      if (held) {
+        // never 0, which would make NaN of a masked score
+        const float factor = fmaxf(
+            __int_as_float(__builtin_amdgcn_readlane(__float_as_int(key_scales), i)) * a.scale_log2, 1.17549435e-38f);
+        softmax_step(s, factor, block);
+        f16x8 p[2];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-          if (sees[t] >= block * kBlockTokens) sum[t] = __builtin_nanf("");
-        continue;
-      }
-      // never 0, which would make NaN of a masked score
-      const float factor = fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(key_scales), i)) * a.scale_log2,
-                                 1.17549435e-38f);
-      f16x8 p[TILES][2];
-      if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        softmax_step(t, s[t], factor, block, !ONES);
+          for (int e = 0; e < 8; ++e) p[k][e] = (f16)s[2 * k + e / 4][e % 4];
+        const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
+        raise_unit(scale_bits);
+        const float ratio = power_ratio(scale_bits, unit);
+        if (ratio >= 0x1p-15f) {  // codes times the ratio are exact in fp16
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+          for (int f = 0; f < FEATURES; ++f) {
+            out[f] = mfma16(e4m3_operand<f16>(values[f][0], values[f][1], ratio), p[0], out[f]);
+            out[f] = mfma16(e4m3_operand<f16>(values[f][2], values[f][3], ratio), p[1], out[f]);
+          }
+        } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) p[t][k][e] = (f16)s[t][2 * k + e / 4][e % 4];
-          if (ONES) {
-            const f16 one = (f16)1.0f;
-            sums[t] = mfma16((f16x8){one, one, one, one, one, one, one, one}, p[t][k], sums[t]);
+          for (int f = 0; f < FEATURES; ++f) {
+            f32x4 add = mfma16(e4m3_operand<f16>(values[f][0], values[f][1], 1.0f), p[0], (f32x4){0.0f, 0.0f, 0.0f, 0.0f});
+            add = mfma16(e4m3_operand<f16>(values[f][2], values[f][3], 1.0f), p[1], add);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[f][j] = fmaf(add[j], ratio, out[f][j]);
           }
         }
+      } else if (sees >= block * kBlockTokens) {  // a page outside the cache: NaN of every row that sees it
+        sum = __builtin_nanf("");
       }
-      if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
-      const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
-      raise_unit(scale_bits);
-      const float ratio = power_ratio(scale_bits, unit);
-      if (ratio >= 0x1p-15f) {  // codes times the ratio are exact in fp16
-#pragma unroll
-        for (int f = 0; f < FEATURES; ++f) {
-          const f16x8 v0 = e4m3_operand<f16>(values.part[f][0], values.part[f][1], ratio);
-          const f16x8 v1 = e4m3_operand<f16>(values.part[f][2], values.part[f][3], ratio);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) out[t][f] = mfma16(v1, p[t][1], mfma16(v0, p[t][0], out[t][f]));
-        }
-      } else {
-#pragma unroll
-        for (int f = 0; f < FEATURES; ++f) {
-          const f16x8 v0 = e4m3_operand<f16>(values.part[f][0], values.part[f][1], 1.0f);
-          const f16x8 v1 = e4m3_operand<f16>(values.part[f][2], values.part[f][3], 1.0f);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) {
-            const f32x4 add = mfma16(v1, p[t][1], mfma16(v0, p[t][0], (f32x4){0.0f, 0.0f, 0.0f, 0.0f}));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[t][f][j] = fmaf(add[j], ratio, out[t][f][j]);
-          }
-        }
-      }
+      if (page >= 0) load_values(page);
     }
   }
 
   // The incomplete block, in the tensors' own type: weights without the shift, in a
-  // unit of at least 2^12 (the shift), so that large values do not overflow.
+  // unit of at least 2^11 (the shift), so that large values do not overflow.
   if (tail_block >= from && tail_block < to && (tail_block - from) % SPLIT == split) {
     const int held = first_position + count - tail_block * kBlockTokens;  // tokens in it
     const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
-    const T* keys = static_cast<const T*>(a.key_tail) + tail_at + quarter * 16;
-    const T* values = static_cast<const T*>(a.value_tail) + tail_at + quarter * 16;
+    const T* tail_keys = static_cast<const T*>(a.key_tail) + tail_at + quarter * 16;
+    const T* tail_values = static_cast<const T*>(a.value_tail) + tail_at + quarter * 16;
     constexpr int SHIFT_BITS = (127 + (int)kWeightShift) << 23;
-    raise_unit(SHIFT_BITS);
-    const float ratio = power_ratio(SHIFT_BITS, unit);
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      if (t != 0) asm volatile("" ::: "memory");  // each tile loads its operands: kept, they would not fit
-      f32x4 s[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int hh = 0; hh < HALVES; ++hh)
-#pragma unroll
-          for (int kk = 0; kk < 2; ++kk)
-            s[i] = mfma16(*reinterpret_cast<const V8*>(
-                              keys + ((column >> 2) * 16 + i * 4 + (column & 3)) * D + hh * 64 + kk * 8),
-                          q[t][hh][kk], s[i]);
-      }
-      softmax_step(t, s, fmaxf(a.scale_log2, 1.17549435e-38f), tail_block, true);
-      // bf16 weights keep 16 bits of precision as a sum of two; fp16 ones the shift
-      constexpr bool WIDE = std::is_same<T, bf16>::value;
-      V8 p[2], rest[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float w = s[2 * k + e / 4][e % 4] * (WIDE ? 0x1p-12f : 1.0f);
-          p[k][e] = (T)w;
-          rest[k][e] = (T)(w - (float)p[k][e]);
-        }
-#pragma unroll
-      for (int f = 0; f < FEATURES; ++f) {
-        f32x4 add = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          V8 v = *reinterpret_cast<const V8*>(values + (f * 16 + column) * kBlockTokens + k * 8);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (quarter * 16 + k * 8 + e >= held) v[e] = (T)0.0f;  // what stands behind the last token
-          add = mfma16(v, p[k], add);
-          if constexpr (WIDE) add = mfma16(v, rest[k], add);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out[t][f][j] = fmaf(WIDE ? add[j] : add[j] * 0x1p-12f, ratio, out[t][f][j]);
-      }
-    }
-  }
-
-  // A row's sum over the four lanes that share it, and its output over the sum.
-  const float unit_value = __int_as_float(unit);
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    sum[t] = quarters_sum(sum[t]);
-    if (ONES) sum[t] += sums[t][0];
-    const float inverse = sum[t] != 0.0f ? 1.0f / sum[t] : 0.0f;  // 0: a row that sees nothing here
+    constexpr bool WIDE = std::is_same<T, bf16>::value;
+    V8 v[FEATURES][2];
 #pragma unroll
     for (int f = 0; f < FEATURES; ++f)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) out[t][f][j] = out[t][f][j] * inverse * unit_value;
-  }
-
-  // Merge of the waves that split the tokens, tile by tile: wave w's output weighs
-  // sum_w 2^(most_w - top).
-  if constexpr (SPLIT > 1) {
-    constexpr int PITCH = D + 4;
-    __shared__ float part[SPLIT * ROWS][16 * PITCH];
-    __shared__ float stats[SPLIT * ROWS][16][2];
+      for (int k = 0; k < 2; ++k)
+        v[f][k] = *reinterpret_cast<const V8*>(tail_values + (f * 16 + column) * kBlockTokens + k * 8);
+    f32x4 s[4];
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      if (t != 0) __syncthreads();
-      if (quarter == 0) {
-        stats[wave][column][0] = most[t];
-        stats[wave][column][1] = sum[t];
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int hh = 0; hh < HALVES; ++hh)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+          s[r] = mfma16(*reinterpret_cast<const V8*>(tail_keys + ((column >> 2) * 16 + r * 4 + (column & 3)) * D +
+                                                     hh * 64 + kk * 8),
+                        q[hh][kk], hh + kk == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : s[r]);
+    asm volatile("" ::: "memory");  // the values are under way with the keys
+    raise_unit(SHIFT_BITS);
+    const float ratio = power_ratio(SHIFT_BITS, unit);
+    softmax_step(s, fmaxf(a.scale_log2, 1.17549435e-38f), tail_block);
+    // bf16 weights keep 16 bits of precision as a sum of two; fp16 ones the shift
+    V8 p[2], rest[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = s[2 * k + e / 4][e % 4] * (WIDE ? kUnshift : 1.0f);
+        p[k][e] = (T)w;
+        rest[k][e] = (T)(w - (float)p[k][e]);
       }
-#pragma unroll
-      for (int f = 0; f < FEATURES; ++f)
-        *reinterpret_cast<f32x4*>(&part[wave][column * PITCH + f * 16 + quarter * 4]) = out[t][f];
-      __syncthreads();
-      // Each wave merges the tiles of features f % SPLIT == split of its rows.
-      const int w0 = wave - split;
-      float top = -INFINITY, total = 0.0f;
-#pragma unroll
-      for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, stats[w0 + w][column][0]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      float weight[SPLIT];
-#pragma unroll
-      for (int w = 0; w < SPLIT; ++w) {
-        const float part_sum = stats[w0 + w][column][1];
-        weight[w] = part_sum != 0.0f ? part_sum * exp2_fast(stats[w0 + w][column][0] - base) : 0.0f;
-        total += weight[w];
-      }
-      most[t] = top;
-      sum[t] = total;
-      const float inverse = total != 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll
-      for (int f = 0; f < FEATURES; ++f) {
-        if (f % SPLIT != split) continue;
-        f32x4 merged = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < SPLIT; ++w) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(&part[w0 + w][column * PITCH + f * 16 + quarter * 4]);
-          const float share = weight[w] * inverse;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) merged[j] = fmaf(v[j], share, merged[j]);
-        }
-        out[t][f] = merged;
-      }
-    }
-  }
-
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    if (token[t] >= a.seq_len) continue;
-    const int64_t place = (b * a.seq_len + token[t]) * a.heads + head[t];
 #pragma unroll
     for (int f = 0; f < FEATURES; ++f) {
-      if (SPLIT > 1 && f % SPLIT != split) continue;
-      if (a.chunks == 1) {
-        T* o = static_cast<T*>(a.output) + b * a.o_sb + token[t] * a.o_ss + (int64_t)head[t] * D;
-        typename Vec8<T>::half_type v;
+      f32x4 add = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = token[t] < count ? (T)out[t][f][j] : (T)0.0f;  // rows without a query
-        *reinterpret_cast<typename Vec8<T>::half_type*>(o + f * 16 + quarter * 4) = v;
-      } else {
-        *reinterpret_cast<f32x4*>(a.partial + (place * a.chunks + chunk) * D + f * 16 + quarter * 4) = out[t][f];
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (quarter * 16 + k * 8 + e >= held) v[f][k][e] = (T)0.0f;  // what stands behind the last token
+        add = mfma16(v[f][k], p[k], add);
+        if constexpr (WIDE) add = mfma16(v[f][k], rest[k], add);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[f][j] = fmaf(WIDE ? add[j] : add[j] * kUnshift, ratio, out[f][j]);
+    }
+  }
+
+  // The row's sum over the four lanes that share it, and its output over the sum.
+  sum = quarters_sum(sum);
+  const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;  // 0: a row that sees nothing here
+  const float unit_value = __int_as_float(unit);
+
+  // Merge of the waves: wave w's output weighs sum_w 2^(most_w - top).  Each wave merges
+  // the tiles of 16 features f % SPLIT == split.
+  constexpr int PITCH = D + 4;
+  __shared__ float part[SPLIT][16 * PITCH];
+  __shared__ float stats[SPLIT][16][2];
+  if (quarter == 0) {
+    stats[split][column][0] = most;
+    stats[split][column][1] = sum;
+  }
+#pragma unroll
+  for (int f = 0; f < FEATURES; ++f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[f][j] = out[f][j] * inverse * unit_value;
+    *reinterpret_cast<f32x4*>(&part[split][column * PITCH + f * 16 + quarter * 4]) = out[f];
+  }
+  __syncthreads();
+  if (token >= a.seq_len) return;
+  float top = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, stats[w][column][0]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float weight[SPLIT];
+#pragma unroll
+  for (int w = 0; w < SPLIT; ++w) {
+    const float part_sum = stats[w][column][1];
+    weight[w] = part_sum != 0.0f ? part_sum * exp2_fast(stats[w][column][0] - base) : 0.0f;
+    total += weight[w];
+  }
+  const float share = total != 0.0f ? 1.0f / total : 0.0f;
+  const int64_t place = ((b * a.seq_len + token) * a.heads + head) * a.chunks + chunk;
+  for (int f = split; f < FEATURES; f += SPLIT) {
+    f32x4 merged = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < SPLIT; ++w) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&part[w][column * PITCH + f * 16 + quarter * 4]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) merged[j] = fmaf(v[j], weight[w] * share, merged[j]);
+    }
+    if (!live) merged = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.chunks == 1) {
+      typename Vec8<T>::half_type v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (T)merged[j];
+      *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + token * a.o_ss +
+                                                      (int64_t)head * D + f * 16 + quarter * 4) = v;
+    } else {
+      *reinterpret_cast<f32x4*>(a.partial + place * D + f * 16 + quarter * 4) = merged;
+    }
+  }
+  if (a.chunks > 1 && split == 0 && quarter == 0) {
+    a.statistics[place * 2] = top;
+    a.statistics[place * 2 + 1] = live ? total : 0.0f;
+  }
+}
+
+// Attention of a chunk of new tokens: as above with 32 rows a wave, on 32 x 32 x 16
+// products, which hold the scores of ONE query row (l % 32) for the 32 tokens
+// 32 (l / 32) .. of a block in a lane.
+//
+// Many rows make it matrix work, and then the codes' way matters: read straight into
+// the operands' order, every lane of a load touches another line.  So a block comes
+// by direct-to-LDS loads of whole lines, one block ahead, and ROWS waves of other
+// rows share it; 16-byte parts of a row change places by its number (key_turn,
+// value_turn), so that the operands' reads of 8 and of 16 rows meet no bank twice.
+// SPLIT groups of such waves take blocks in turn and merge in LDS at the end.
+//
+// The vector units bound it (60% busy: 32 weights and 64 conversions a lane and block
+// beside 32 matrix instructions of 16 cycles), so with heads of 64 the products of the
+// next block are issued beside this one's weights.  2 x 512 tokens behind 7680, 16 / 4
+// heads: heads of 64 64 us, 33.3 GFLOP at 520 TFLOP/s; heads of 128 112 us, 595 TFLOP/s.
+template <int D>
+__device__ __forceinline__ int key_turn(int t) {
+  return D == 64 ? (((t >> 1) ^ (t >> 2)) & 1) | (((t >> 5) & 1) << 1)
+                 : ((t ^ (t >> 2)) & 1) | (((t >> 1) & 1) << 1) | (((t >> 5) & 1) << 2);
+}
+__device__ __forceinline__ int value_turn(int d) { return (((d >> 1) ^ (d >> 3)) & 1) | (((d >> 2) & 1) << 1); }
+
+template <typename T, int D, int SPLIT, int ROWS>
+__global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(const AttentionArgs a) {
+  typedef typename Vec8<T>::type V8;
+  constexpr int WAVES = SPLIT * ROWS;
+  constexpr int PAIRS = D / 32;      // 16-byte parts of a key row a lane
+  constexpr int FEATURES = D / 32;   // tiles of 32 features
+  constexpr int BYTES = kBlockTokens * D;  // of a block's keys, and of its values
+  constexpr int LOADS = BYTES / 1024;      // wave loads of them
+  constexpr int PITCH = 36;
+  // Heads of 128 leave no registers for the scores of two blocks.
+  constexpr bool AHEAD = D == 64;
+  static_assert(LOADS % ROWS == 0, "every wave loads the same number of parts");
+  union Shared {
+    uint8_t block[SPLIT][4][BYTES];  // keys and values, twice
+    float part[WAVES][32 * PITCH];
+  };
+  __shared__ __align__(16) Shared shared;
+  __shared__ float stats[WAVES][32][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int column = lane & 31;
+  const int half = lane >> 5;
+  const int split = wave / ROWS, row_wave = wave % ROWS;
+
+  uint32_t at = blockIdx.x;
+  const int chunk = common((int)(at % (uint32_t)a.chunks));
+  at /= (uint32_t)a.chunks;
+  const uint32_t group_row = (uint32_t)common((int)(at % a.row_groups)) * (ROWS * 32);  // rows are below 2^31
+  at /= a.row_groups;
+  const int h = common((int)(at % (uint32_t)a.kv_heads));
+  const int64_t b = common((int)(at / (uint32_t)a.kv_heads));
+
+  const int64_t start = common(a.starts[b]);
+  int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
+  if (count > a.seq_len) count = a.seq_len;
+  if (start < 0 || count < 0) count = 0;
+  const bool beyond = (start + count) / kBlockTokens > a.max_blocks;
+  const int first_position = beyond ? 0 : (int)start;
+  const int tail_block = beyond ? 0 : (int)((start + count) / kBlockTokens);
+
+  // The last position that rows first .. first + rows - 1 see, -1 where none has a query.
+  auto last_of = [&](uint32_t first, int rows) {
+    const int low = common((int)(first / (uint32_t)a.group));
+    const int high = common((int)((first + rows - 1) / (uint32_t)a.group));
+    return low < count ? first_position + (high < count ? high : count - 1) : -1;
+  };
+  const uint32_t first_row = group_row + row_wave * 32;
+  const int last_position = last_of(first_row, 32);
+  const int group_last = last_of(group_row, ROWS * 32);
+  const int least_position = first_position + common((int)(first_row / (uint32_t)a.group));
+  const uint32_t row = first_row + column;
+  const int token = (int)(row / (uint32_t)a.group);
+  const bool live = token < count;
+  const int sees = live ? first_position + token : last_position;
+  V8 q[PAIRS][2];
+#pragma unroll
+  for (int c = 0; c < PAIRS; ++c)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      u32x4 raw = {0u, 0u, 0u, 0u};
+      if (live) {
+        const int head = h * a.group + (int)(row - (uint32_t)token * (uint32_t)a.group);
+        raw = load16(static_cast<const T*>(a.query) + b * a.q_sb + head * a.q_sh + token * a.q_ss + c * 32 + half * 16 + e * 8);
+        raw = (raw ^ a.sign) & a.keep;
+      }
+      q[c][e] = __builtin_bit_cast(V8, raw);
+    }
+
+  // Blocks of the workgroup's rows in this chunk; group `split` takes every SPLIT-th.
+  const int all_blocks = group_last < 0 || beyond ? 0 : group_last / kBlockTokens + 1;
+  const int64_t from64 = (int64_t)chunk * a.chunk_blocks;
+  const int from = from64 < all_blocks ? (int)from64 : all_blocks;
+  const int to = chunk == a.chunks - 1 || all_blocks - from < a.chunk_blocks ? all_blocks : from + a.chunk_blocks;
+  const int coded_to = to < tail_block ? to : tail_block;
+  const int turns = coded_to > from ? (coded_to - from + SPLIT - 1) / SPLIT : 0;
+
+  f32x16 out[FEATURES];
+  int unit = 0;
+  float most = -INFINITY;
+  float sum = beyond && last_position >= 0 ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+  for (int f = 0; f < FEATURES; ++f) out[f] = (f32x16)(0.0f);
+  auto raise_unit = [&](int bits) {
+    if (bits <= unit) return;
+    if (unit != 0) {
+      const float change = power_ratio(unit, bits);
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+    }
+    unit = bits;
+  };
+  // The largest of a row's scores, times the factor (common to the lanes that share it).
+  auto largest = [&](const f32x16 (&s)[2], float factor) {
+    float top[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      top[k] = fmaxf(s[k / 2][k % 2 * 8], s[k / 2][k % 2 * 8 + 1]);
+#pragma unroll
+      for (int r = 2; r < 8; r += 2) top[k] = fmaxf(fmaxf(top[k], s[k / 2][k % 2 * 8 + r]), s[k / 2][k % 2 * 8 + r + 1]);
+    }
+    return halves_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) * factor;
+  };
+  auto hide = [&](f32x16 (&s)[2], int block) {  // what the row does not see
+    const int open = sees - block * kBlockTokens - half * 32;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (r > open) s[r / 16][r % 16] = -INFINITY;
+  };
+  auto raise_base = [&](float top) {
+    const float now = fmaxf(most, top);
+    const float change = most == -INFINITY ? 0.0f : exp2_fast(most - now);
+    sum *= change;
+#pragma unroll
+    for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+    most = now;
+  };
+  auto weigh = [&](f32x16 (&s)[2], float factor) {
+    const float shift = kWeightShift - (most == -INFINITY ? 0.0f : most);
+#pragma unroll
+    for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = exp2_fast(fmaf(s[r / 16][r % 16], factor, shift));
+  };
+
+  // This wave's part of the loads of a block's keys or values: slots of 16 bytes, its
+  // lane's one each.
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&shared.block[split][0][0];
+  auto load_part = [&](int page, int buffer, auto of_values) {
+    constexpr bool VALUES = decltype(of_values)::value;
+    const uint8_t* codes = (VALUES ? a.value_codes : a.key_codes) + ((int64_t)page * a.kv_heads + h) * BYTES;
+#pragma unroll
+    for (int i = 0; i < LOADS / ROWS; ++i) {
+      const int load = i * ROWS + row_wave;
+      const int slot = load * 64 + lane;
+      constexpr int PARTS = VALUES ? 4 : D / 16;  // of a row
+      const int r = slot / PARTS, p = slot % PARTS;
+      const int source = (r * PARTS + (p ^ (VALUES ? value_turn(r) : key_turn<D>(r)))) * 16;
+      tile_dma16(codes, (uint32_t)source, lds + (buffer * 2 + VALUES) * BYTES + load * 1024);
+    }
+  };
+  auto load_keys = [&](int page, int buffer) { load_part(page, buffer, std::false_type{}); };
+  auto load_values = [&](int page, int buffer) { load_part(page, buffer, std::true_type{}); };
+
+  // Scores of the block in a buffer.
+  auto score = [&](f32x16 (&s)[2], int buffer) {
+    const uint8_t* keys = shared.block[split][buffer * 2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = ((column >> 2) & 1) * 32 + t * 16 + (column >> 3) * 4 + (column & 3);
+#pragma unroll
+      for (int c = 0; c < PAIRS; ++c) {
+        const u32x4 raw = *reinterpret_cast<const u32x4*>(keys + key * D + ((c * 2 + half) ^ key_turn<D>(key)) * 16);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s[t] = mfma32(e4m3_operand<T>(raw[2 * e], raw[2 * e + 1], 1.0f), q[c][e], c + e == 0 ? (f32x16)(0.0f) : s[t]);
       }
     }
-    if (a.chunks > 1 && split == 0 && quarter == 0) {
-      float* statistics = a.statistics + (place * a.chunks + chunk) * 2;
-      statistics[0] = most[t];
-      statistics[1] = sum[t];
+  };
+  f16x8 p[4];
+  auto add_up = [&](const f32x16 (&s)[2]) {  // the weights in fp16, and their sums
+    const f16x2 ones = {(f16)1.0f, (f16)1.0f};
+    float sums[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[u][e] = (f16)s[u / 2][u % 2 * 8 + e];
+      sums[u] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        sums[u] = __builtin_amdgcn_fdot2((f16x2){p[u][e], p[u][e + 1]}, ones, sums[u], false);
+    }
+    sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  };
+  auto value_operand = [&](int buffer, int f, int u, float scale) {
+    const int d = f * 32 + column;
+    const u32x2 raw = *reinterpret_cast<const u32x2*>(&shared.block[split][buffer * 2 + 1][0] + d * kBlockTokens +
+                                                      ((half * 2 + u / 2) ^ value_turn(d)) * 16 + u % 2 * 8);
+    return e4m3_operand<f16>(raw[0], raw[1], scale);
+  };
+
+  // The group's blocks, 64 at a time: a lane each looks up the page and its scales.  A
+  // page outside the cache is loaded as the first one, and not used.
+  int pages = -1;
+  float key_scales = 0.0f, value_scales = 0.0f;
+  auto look_up = [&](int first) {
+    const int mine = from + split + (first + lane) * SPLIT;
+    pages = -1;
+    if (mine < coded_to) pages = a.table[b * a.max_blocks + mine];
+    if (pages < 0 || pages >= a.blocks) pages = -1;
+    if (pages >= 0) {
+      key_scales = a.key_scales[(int64_t)pages * a.kv_heads + h];
+      value_scales = a.value_scales[(int64_t)pages * a.kv_heads + h];
+    }
+  };
+  auto page_of = [&](int i) {
+    const int page = __builtin_amdgcn_readlane(pages, i);
+    return page < 0 ? 0 : page;
+  };
+  // Block i of this look-up, AHEAD: its scores in s; those of block i + 1 go to next
+  // while this one's weights are formed and used.
+  auto step = [&](int first, int i, int here, f32x16 (&s)[2], f32x16 (&next)[2]) {
+    // Loads under way, in order: (keys i,) values i, keys i + 1, values i + 1.
+    if (i + 1 < here)
+      wait_loads<(AHEAD ? 1 : 2) * (LOADS / ROWS)>();
+    else
+      wait_loads<0>();
+    if (AHEAD) wait_lds();  // keys i are read
+    if (ROWS > 1) tile_barrier();  // every wave's part of the loads has come
+    if (AHEAD && i + 2 < here) load_keys(page_of(i + 2), i & 1);
+    if (!AHEAD) score(s, i & 1);
+    const int block = from + split + (first + i) * SPLIT;
+    const bool held = __builtin_amdgcn_readlane(pages, i) >= 0;
+    const bool seen = block < coded_to && block * kBlockTokens <= last_position;
+    const bool whole = block * kBlockTokens + (kBlockTokens - 1) <= least_position;
+    // never 0, which would make NaN of a masked score
+    const float factor =
+        fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(key_scales), i)) * a.scale_log2, 1.17549435e-38f);
+    const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
+    const float top = largest(s, factor);
+    // Nearly all blocks: seen whole, no base or unit to raise, codes times the ratio of
+    // scales exact in fp16.  They have a copy of their own without branches, in which the
+    // outputs stay where they are and the next block's products run beside the weights.
+    if (seen && held && whole && !__any(top > most + kWeightMargin) && scale_bits <= unit &&
+        power_ratio(scale_bits, unit) >= 0x1p-15f) {
+      if (AHEAD) score(next, (i + 1) & 1);
+      weigh(s, factor);
+      add_up(s);
+      const float ratio = power_ratio(scale_bits, unit);
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) out[f] = mfma32(value_operand(i & 1, f, u, ratio), p[u], out[f]);
+    } else {
+      if (seen && !held) {  // a page outside the cache
+        if (sees >= block * kBlockTokens) sum = __builtin_nanf("");
+      } else if (seen) {
+        if (!whole) hide(s, block);
+        const float row_top = whole ? top : largest(s, factor);
+        if (__any(row_top > most + kWeightMargin)) raise_base(row_top);
+        weigh(s, factor);
+        add_up(s);
+        raise_unit(scale_bits);
+        const float ratio = power_ratio(scale_bits, unit);
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) {
+          f32x16 add = (f32x16)(0.0f);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) add = mfma32(value_operand(i & 1, f, u, 1.0f), p[u], add);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) out[f][r] = fmaf(add[r], ratio, out[f][r]);
+        }
+      }
+      if (AHEAD) score(next, (i + 1) & 1);
+    }
+    if (i + 2 < here) {
+      wait_lds();
+      if (ROWS > 1) tile_barrier();  // values i (and keys i) are read
+      if (!AHEAD) load_keys(page_of(i + 2), i & 1);
+      load_values(page_of(i + 2), i & 1);
+    }
+  };
+  if (a.blocks == 0) {  // no cache to read
+    if (turns > 0 && sees >= (from + split) * kBlockTokens && from + split < coded_to) sum = __builtin_nanf("");
+  } else {
+    for (int first = 0; first < turns; first += 64) {
+      look_up(first);
+      const int here = turns - first < 64 ? turns - first : 64;
+      if (first != 0) {  // the buffers' last blocks are read
+        wait_lds();
+        if (ROWS > 1) tile_barrier();
+      }
+      load_keys(page_of(0), 0);
+      load_values(page_of(0), 0);
+      if (here > 1) {
+        load_keys(page_of(1), 1);
+        load_values(page_of(1), 1);
+        if (AHEAD) wait_loads<3 * (LOADS / ROWS)>();
+      } else {
+        wait_loads<0>();
+      }
+      f32x16 even[2], odd[2];
+      if (AHEAD) {
+        if (ROWS > 1) tile_barrier();
+        score(even, 0);
+      }
+      for (int i = 0; i < here; i += 2) {
+        step(first, i, here, even, odd);
+        if (i + 1 < here) step(first, i + 1, here, odd, even);
+      }
+    }
+  }
+
+  // The incomplete block, as above.
+  if (tail_block >= from && tail_block < to && (tail_block - from) % SPLIT == split &&
+      last_position >= tail_block * kBlockTokens) {
+    const int held = first_position + count - tail_block * kBlockTokens;
+    const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
+    const T* keys = static_cast<const T*>(a.key_tail) + tail_at + half * 16;
+    const T* values = static_cast<const T*>(a.value_tail) + tail_at + half * 32;
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = ((column >> 2) & 1) * 32 + t * 16 + (column >> 3) * 4 + (column & 3);
+#pragma unroll
+      for (int c = 0; c < PAIRS; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s[t] = mfma32(*reinterpret_cast<const V8*>(keys + key * D + c * 32 + e * 8), q[c][e],
+                        c + e == 0 ? (f32x16)(0.0f) : s[t]);
+    }
+    constexpr int SHIFT_BITS = (127 + (int)kWeightShift) << 23;
+    constexpr bool WIDE = std::is_same<T, bf16>::value;
+    raise_unit(SHIFT_BITS);
+    const float ratio = power_ratio(SHIFT_BITS, unit);
+    const float factor = fmaxf(a.scale_log2, 1.17549435e-38f);
+    hide(s, tail_block);
+    const float top = largest(s, factor);
+    if (__any(top > most + kWeightMargin)) raise_base(top);
+    weigh(s, factor);
+    V8 p[4], rest[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float weight = s[u / 2][u % 2 * 8 + e];
+        sum += weight;
+        const float w = weight * (WIDE ? kUnshift : 1.0f);
+        p[u][e] = (T)w;
+        rest[u][e] = (T)(w - (float)p[u][e]);
+      }
+#pragma unroll
+    for (int f = 0; f < FEATURES; ++f) {
+      f32x16 add = (f32x16)(0.0f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        V8 v = *reinterpret_cast<const V8*>(values + (f * 32 + column) * kBlockTokens + u * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (half * 32 + u * 8 + e >= held) v[e] = (T)0.0f;  // what stands behind the last token
+        add = mfma32(v, p[u], add);
+        if constexpr (WIDE) add = mfma32(v, rest[u], add);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[f][r] = fmaf(WIDE ? add[r] : add[r] * kUnshift, ratio, out[f][r]);
+    }
+  }
+
+  // Merge and store, 32 features at a time: the group's SPLIT waves of the same rows
+  // weigh their outputs as above, and rows leave in runs of 32 features.
+  sum += __shfl_xor(sum, 32);
+  const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+  const float unit_value = __int_as_float(unit);
+  if (half == 0) {
+    stats[wave][column][0] = most;
+    stats[wave][column][1] = sum;
+  }
+  for (int f = 0; f < FEATURES; ++f) {
+    __syncthreads();  // the blocks, or the last tile, are read
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = out[0][k * 4 + j];
+#pragma unroll
+        for (int g = 1; g < FEATURES; ++g) x = f == g ? out[g][k * 4 + j] : x;
+        v[j] = x * inverse * unit_value;
+      }
+      *reinterpret_cast<f32x4*>(&shared.part[wave][column * PITCH + k * 8 + half * 4]) = v;
+    }
+    __syncthreads();
+    for (int i = split * 64 + lane; i < 32 * 8; i += SPLIT * 64) {
+      const int r = i / 8, feature = i % 8 * 4;
+      float top = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, stats[w * ROWS + row_wave][r][0]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      f32x4 merged = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < SPLIT; ++w) {
+        const float part_sum = stats[w * ROWS + row_wave][r][1];
+        const float weight = part_sum != 0.0f ? part_sum * exp2_fast(stats[w * ROWS + row_wave][r][0] - base) : 0.0f;
+        total += weight;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(&shared.part[w * ROWS + row_wave][r * PITCH + feature]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) merged[j] = fmaf(v[j], weight, merged[j]);
+      }
+      const float scale = total != 0.0f ? 1.0f / total : 0.0f;
+      const uint32_t its_row = first_row + r;
+      const int its_token = (int)(its_row / (uint32_t)a.group);
+      const int head = h * a.group + (int)(its_row - (uint32_t)its_token * (uint32_t)a.group);
+      if (its_token >= a.seq_len) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) merged[j] = its_token < count ? merged[j] * scale : 0.0f;  // rows without a query
+      if (a.chunks == 1) {
+        typename Vec8<T>::half_type v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (T)merged[j];
+        *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + its_token * a.o_ss +
+                                                        (int64_t)head * D + f * 32 + feature) = v;
+      } else {
+        const int64_t place = ((b * a.seq_len + its_token) * a.heads + head) * a.chunks + chunk;
+        *reinterpret_cast<f32x4*>(a.partial + place * D + f * 32 + feature) = merged;
+        if (f == 0 && feature == 0) {
+          a.statistics[place * 2] = top;
+          a.statistics[place * 2 + 1] = its_token < count ? total : 0.0f;
+        }
+      }
     }
   }
 }
@@ -507,53 +858,56 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int feature = (lane % LANES) * 4;
+  const f32x2* statistics = reinterpret_cast<const f32x2*>(a.statistics) + row * a.chunks;
+  const float* partial = a.partial + row * a.chunks * D + feature;
+  // (a sum of 0: a chunk behind the row's last token, or a row without a query)
+  const f32x2 nothing = {-INFINITY, 0.0f};
+  const f32x2 own = lane < a.chunks ? statistics[lane] : nothing;
+  float top = own[0];
+  for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, statistics[c][0]);
+  f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
+  float total = 0.0f;
+  for (int first = 0; first < a.chunks; first += 64) {
+    const int here = a.chunks - first < 64 ? a.chunks - first : 64;
+    f32x4 v[4];
+    auto load = [&](int c) {  // the parts' outputs do not wait for their weights
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int mine = c + u * PARTS + lane / LANES;
+        v[u] = *reinterpret_cast<const f32x4*>(partial + (int64_t)(first + (mine < here ? mine : here - 1)) * D);
+      }
+    };
+    load(0);
+    if (first == 0) {
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    }
+    const f32x2 s = first == 0 ? own : first + lane < a.chunks ? statistics[first + lane] : nothing;
+    const float weight = s[1] != 0.0f ? s[1] * exp2_fast(s[0] - (top == -INFINITY ? 0.0f : top)) : 0.0f;
+    total += weight;
+    for (int c = 0; c < here; c += 4 * PARTS) {
+      if (c != 0) load(c);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = __shfl(weight, c + u * PARTS + lane / LANES);  // 0 behind the last chunk
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = fmaf(v[u][j], w, out[j]);
+      }
+    }
+  }
+  total = wave_sum(total);
+  const float inverse = total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+  for (int m = LANES; m < 64; m <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] += __shfl_xor(out[j], m);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] *= inverse;
+  if (lane >= LANES) return;
   const int64_t token_row = row / a.heads;
   const int head = (int)(row - token_row * a.heads);
   const int64_t b = token_row / a.seq_len;
   const int64_t token = token_row - b * a.seq_len;
-  const int count = a.counts != nullptr ? a.counts[b] : a.seq_len;
-  const bool live = a.starts[b] >= 0 && token < count;
-
-  f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (live) {
-    const f32x2* statistics = reinterpret_cast<const f32x2*>(a.statistics) + row * a.chunks;
-    const float* partial = a.partial + row * a.chunks * D + feature;
-    float top = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, statistics[c][0]);
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f;
-    for (int first = 0; first < a.chunks; first += 64) {
-      float weight = 0.0f;
-      if (first + lane < a.chunks) {
-        const f32x2 s = statistics[first + lane];
-        if (s[1] != 0.0f) weight = s[1] * exp2_fast(s[0] - base);  // 0: a chunk behind the row's last token
-      }
-      total += weight;
-      const int here = a.chunks - first < 64 ? a.chunks - first : 64;
-      for (int c = 0; c < here; c += 4 * PARTS) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int mine = c + u * PARTS + lane / LANES;
-          const float w = __shfl(weight, mine);  // 0 behind the last chunk, whose output is then read again
-          const int read = first + (mine < here ? mine : here - 1);
-          const f32x4 v = *reinterpret_cast<const f32x4*>(partial + (int64_t)read * D);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) out[j] = fmaf(v[j], w, out[j]);
-        }
-      }
-    }
-    total = wave_sum(total);
-    const float inverse = total != 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll
-    for (int m = LANES; m < 64; m <<= 1)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) out[j] += __shfl_xor(out[j], m);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] *= inverse;
-  }
-  if (lane >= LANES) return;
   typename Vec8<T>::half_type v;
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = (T)out[j];
@@ -561,29 +915,36 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
                                                   (int64_t)head * D + feature) = v;
 }
 
-// How a call is laid out: row tiles of a wave, waves that split the tokens (the
-// rest of a workgroup's four take other rows), workgroups of rows and chunks.
+// How a call is laid out: rows of a wave (16, the decoding kernel, or 32, the chunk
+// kernel), groups of waves that split the tokens of the same rows, waves of a group,
+// workgroups of rows and chunks.
 struct Layout {
-  int tiles, split;
+  int wave_rows, split, rows;
   int64_t row_groups;
   int chunks, chunk_blocks;
 };
-
-constexpr int kWaves = 4;
 
 Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group, int64_t head_dim,
                  int64_t max_length) {
   Layout l{};
   const int64_t rows = seq_len * group;
-  l.tiles = rows <= 16 ? 1 : 2;
-  // waves that the registers leave room for, on all compute units
-  const int64_t room = (int64_t)kUnits * 4 * (head_dim == 128 && l.tiles == 2 ? 1 : head_dim == 64 && l.tiles == 1 ? 3 : 2);
-  const int64_t waves = batch * kv_heads * ceil_div(rows, 16 * l.tiles);
   const int64_t blocks = max_length / kBlockTokens + 1;
-  l.split = waves >= room ? 1 : l.tiles == 1 && blocks <= 32 ? 8 : 4;
-  if (l.tiles == 1 && l.split == 1) l.split = 4;
-  l.row_groups = ceil_div(rows, (int64_t)16 * l.tiles * (l.split == 1 ? kWaves : 1));
-  int64_t chunks = room / (waves * l.split);
+  l.wave_rows = rows <= 16 ? 16 : 32;
+  // waves that the registers leave room for, on all compute units
+  const int64_t room = (int64_t)kUnits * 4 * (head_dim == 64 && l.wave_rows == 16 ? 3 : 2);
+  // The waves of a workgroup split the tokens, which leaves fewer parts to merge through
+  // memory; short histories go to eight of them, in one launch.  Heads of 128 have the
+  // registers for one block's scores, and more to gain from blocks shared by four waves
+  // of other rows (2 x 512 rows behind 7680 tokens, 16 / 4 heads, us: heads of 128
+  // 123 / 111 shared, heads of 64 63 / 66).
+  l.split = l.wave_rows == 16 && blocks <= 32 ? 8 : 4;
+  l.rows = 1;
+  if (head_dim == 128 && rows > 64) {
+    l.split = 2;
+    l.rows = 4;
+  }
+  l.row_groups = ceil_div(rows, (int64_t)l.wave_rows * l.rows);
+  int64_t chunks = room / (batch * kv_heads * l.row_groups * l.rows * l.split);
   const int64_t most = ceil_div(blocks, 4 * l.split);
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
@@ -594,15 +955,17 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
 
 template <typename T, int D>
 int launch_attention(AttentionArgs& a, const Layout& l, int64_t batch, unsigned grid, hipStream_t stream) {
-#define SAH_ATTENTION_CASE(TILES, SPLIT, ROWS)                                                               \
-  if (l.tiles == TILES && l.split == SPLIT)                                                                  \
-    hipLaunchKernelGGL((cached_attention_kernel<T, D, TILES, SPLIT, ROWS>), dim3(grid), dim3(SPLIT * ROWS * 64), 0, \
-                       stream, a);
-  SAH_ATTENTION_CASE(1, 4, 1)
-  SAH_ATTENTION_CASE(1, 8, 1)
-  SAH_ATTENTION_CASE(2, 4, 1)
-  SAH_ATTENTION_CASE(2, 1, 4)
-#undef SAH_ATTENTION_CASE
+  const dim3 blocks(grid), threads((unsigned)(l.split * l.rows * 64));
+  if (l.wave_rows == 16) {
+    if (l.split == 8)
+      hipLaunchKernelGGL((cached_attention_kernel<T, D, 8>), blocks, threads, 0, stream, a);
+    else
+      hipLaunchKernelGGL((cached_attention_kernel<T, D, 4>), blocks, threads, 0, stream, a);
+  } else if (l.rows == 1) {
+    hipLaunchKernelGGL((chunk_attention_kernel<T, D, 4, 1>), blocks, threads, 0, stream, a);
+  } else {
+    if constexpr (D == 128) hipLaunchKernelGGL((chunk_attention_kernel<T, D, 2, 4>), blocks, threads, 0, stream, a);
+  }
   int status = check_hip(hipGetLastError(), "cached attention launch");
   if (status != SAH_OK || l.chunks == 1) return status;
   const int64_t rows = batch * a.seq_len * a.heads;

@@ -88,13 +88,13 @@ def stored_tokens(key, value):
 def attention(query, keys, values, position, scale):
     """One query row [D] over the tokens [T, D] up to ``position``: the answer, the
     same weights' sum of the values' magnitudes (what its errors are relative to),
-    and 2^-37 of the largest weight on every value (a weight below 2^-26 of it is a
-    subnormal fp16, in steps of 2^-36)."""
+    and 2^-36 of the largest weight on every value (a weight below 2^-25 of it is a
+    subnormal fp16, in steps of 2^-24 / 2^11)."""
 
     scores = keys[: position + 1] @ query * scale
     weights = torch.softmax(scores, 0)
     sizes = values[: position + 1].abs()
-    return weights @ values[: position + 1], (weights @ sizes, 2.0**-37 * weights.max() * sizes.sum(0))
+    return weights @ values[: position + 1], (weights @ sizes, 2.0**-36 * weights.max() * sizes.sum(0))
 
 
 def attention_bound(answer, sizes, query, keys, position, scale, dtype):
