@@ -515,6 +515,74 @@ def test_cache_of_more_than_four_gigabytes(gpu_device):
     _check_attention(t, _rand((2, 16, 1, 64), 142, BF16), [129, 69])
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (64, F16), (128, F16), (128, BF16)])
+@pytest.mark.parametrize("seq", [1, 9, 40])
+def test_more_blocks_than_one_look_up_of_a_wave(gpu_device, seq, dim, dtype):
+    """Histories far beyond max_length: every wave's blocks come in more than one look-up of 64."""
+
+    starts = [36_000, 9_000 if seq == 1 else 17_500]
+    t = _Tokens(gpu_device, [s + seq for s in starts], 1, dim, dtype, seed=211).fill()
+    query = _rand((2, 2, seq, dim), 212, dtype)
+    _check_attention(t, query, starts, rows=[0, seq - 1], max_length=1)
+    if seq == 1:
+        return
+    # a page outside the cache in the second look-up, which every row sees
+    t.cache.block_table[0, 550] = -1
+    t.cache.block_table[1, 265] = t.cache.key_codes.shape[0]
+    assert bool(_attend(t, query, starts, max_length=1).isnan().all())
+
+
+@pytest.mark.parametrize("heads", [40, 96])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_query_heads_a_key_head(gpu_device, heads, dim):
+    lengths = [1, 63, 64, 700]
+    t = _Tokens(gpu_device, lengths, 1, dim, BF16, seed=heads).fill()
+    _check_attention(t, _rand((4, heads, 1, dim), 213, BF16), [n - 1 for n in lengths])
+
+
+@pytest.mark.parametrize("seq", [1, 3, 40])
+def test_padded_rows_are_not_read(gpu_device, seq):
+    """Queries behind the counts may hold anything; their outputs are zeros."""
+
+    starts, counts = [70, 20, 300, 64], [seq, 0, max(1, seq // 2), 1]
+    t = _Tokens(gpu_device, [a + b for a, b in zip(starts, counts)], 2, 64, BF16, seed=221).fill()
+    query = _rand((4, 8, seq, 64), 222, BF16)
+    for b, count in enumerate(counts):
+        query[b, :, count:] = math.nan
+    _check_attention(t, query, starts, counts, rows=[0, 1, seq - 1])
+
+
+@pytest.mark.parametrize("width", [0, 2])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_caches_without_blocks(gpu_device, dim, width):
+    """Up to 63 tokens need no block; complete blocks have no place, and who sees one gets NaN."""
+
+    from solution.kernels.attention import BlockCache, hip_block_cache_append
+
+    t = _Tokens(gpu_device, [63, 17, 1], 2, dim, BF16, seed=231)
+    table = torch.full((3, width), 0, dtype=torch.int32, device=gpu_device)
+    t.cache = BlockCache.allocate(3, 2, dim, max_tokens=63, num_blocks=0, dtype=BF16, device=gpu_device, block_table=table)
+    assert t.cache.max_tokens == 63 + 64 * width
+    t.append([0] * 3, [40, 17, 1])
+    t.append([40, 17, 1], [23, 0, 0])
+    t.check()
+    for seq in (1, 17):
+        _check_attention(t, _rand((3, 8, seq, dim), 232, BF16), [63 - seq, max(0, 17 - seq), 0], [seq, seq, 1])
+    kv = torch.ones((3, 2, 5, dim), dtype=BF16, device=gpu_device)
+    starts = torch.tensor([63, 17, 1], dtype=torch.int32, device=gpu_device)
+    with torch.inference_mode():
+        hip_block_cache_append(t.cache, kv, kv, starts)
+    for seq in (1, 5, 20):
+        first = max(0, 22 - seq)
+        query = _rand((3, 8, seq, dim), 233, BF16)
+        out = _attend(t, query, [68 - seq, first, 0], [seq, min(seq, 22), min(seq, 6)])
+        # the block of the first 64 tokens, which is lost, is seen by every row of the first sequence
+        assert bool(out[0].isnan().all()) and not bool(out[1:].isnan().any())
+    key, value = t.read([60, 0, 0], [68, 22, 6], 8)
+    assert bool(key[0, :, :4].isnan().all()) and bool(value[0, :, :4].isnan().all())
+    assert not bool(key[0, :, 4:].isnan().any()) and not bool(key[1:].isnan().any())
+
+
 def test_attention_refusals(gpu_device):
     from solution.kernels.attention import hip_block_cache_append, hip_block_cache_attention, hip_block_cache_read
 
