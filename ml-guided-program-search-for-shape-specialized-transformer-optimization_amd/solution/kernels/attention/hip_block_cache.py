@@ -166,44 +166,59 @@ def hip_block_cache_available() -> bool:
     return library_available()
 
 
-def _lengths_ok(lengths: torch.Tensor | None, cache: BlockCache) -> bool:
-    tail = cache.key_tail
+def _lengths_ok(lengths: torch.Tensor | None, batch: int, index: int) -> bool:
     return lengths is None or (
         lengths.dtype is torch.int32
-        and lengths.shape == tail.shape[:1]
+        and lengths.shape == (batch,)
         and lengths.is_contiguous()
-        and lengths.device == tail.device
+        and lengths.get_device() == index
     )
 
 
-def _rows_ok(value: torch.Tensor, cache: BlockCache) -> bool:
-    """A [batch, heads, seq_len, head_dim] view of the cache's type that the kernels read in place."""
+def _strides(value: torch.Tensor, size: torch.Size) -> tuple[int, int, int] | None:
+    """Strides of the first three axes, 0 for an axis of size 1 (never stepped), or
+    None for a tensor that the kernels do not read in place."""
 
-    tail = cache.key_tail
-    if value.dtype is not tail.dtype or value.device != tail.device:
-        return False
-    size, stride, of_tail = value.shape, value.stride(), tail.shape
-    if len(size) != 4 or size[0] != of_tail[0] or size[3] != of_tail[3]:
-        return False
-    return not (
-        stride[3] != 1
-        or (stride[0] % 8 and size[0] != 1)
-        or (stride[1] % 8 and size[1] != 1)
-        or (stride[2] % 8 and size[2] != 1)
-        or value.data_ptr() % 16
-        or (value.requires_grad and torch.is_grad_enabled())
-    )
+    b, h, s, feature = value.stride()
+    if size[0] == 1:
+        b = 0
+    if size[1] == 1:
+        h = 0
+    if size[2] == 1:
+        s = 0
+    if feature != 1 or b % 8 or h % 8 or s % 8 or value.data_ptr() % 16:
+        return None
+    if value.requires_grad and torch.is_grad_enabled():
+        return None
+    return b, h, s
 
 
-def _strides(value: torch.Tensor) -> tuple[int, int, int]:
-    """Strides of the first three axes, 0 for an axis of size 1 (never stepped)."""
+def _append_request(
+    cache: BlockCache,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    starts: torch.Tensor,
+    counts: torch.Tensor | None,
+) -> tuple[int, ...] | None:
+    """The strides of key and value where the append kernel takes the request, else None."""
 
-    size, stride = value.shape, value.stride()
-    return (
-        stride[0] if size[0] != 1 else 0,
-        stride[1] if size[1] != 1 else 0,
-        stride[2] if size[2] != 1 else 0,
-    )
+    tail, size = cache.key_tail, key.shape
+    dtype, index = tail.dtype, tail.get_device()
+    if key.dtype is not dtype or value.dtype is not dtype or len(size) != 4 or value.shape != size:
+        return None
+    batch, heads, _, dim = tail.shape
+    if size[0] != batch or size[1] != heads or size[3] != dim:
+        return None
+    if key.get_device() != index or value.get_device() != index:
+        return None
+    key_strides, value_strides = _strides(key, size), _strides(value, size)
+    if key_strides is None or value_strides is None or starts is None:
+        return None
+    if not (_lengths_ok(starts, batch, index) and _lengths_ok(counts, batch, index)):
+        return None
+    if not (is_gfx950(tail.device) and library_available()):
+        return None
+    return key_strides + value_strides
 
 
 def can_use_hip_block_cache_append(
@@ -215,17 +230,7 @@ def can_use_hip_block_cache_append(
 ) -> bool:
     """Whether the append kernel takes these tensors."""
 
-    return (
-        _rows_ok(key, cache)
-        and key.shape[1] == cache.key_tail.shape[1]
-        and value.shape == key.shape
-        and _rows_ok(value, cache)
-        and starts is not None
-        and _lengths_ok(starts, cache)
-        and _lengths_ok(counts, cache)
-        and is_gfx950(key.device)
-        and library_available()
-    )
+    return _append_request(cache, key, value, starts, counts) is not None
 
 
 def hip_block_cache_append(
@@ -245,7 +250,8 @@ def hip_block_cache_append(
     value makes NaN of every query that attends to it, and of no other.
     """
 
-    if not can_use_hip_block_cache_append(cache, key, value, starts, counts):
+    strides = _append_request(cache, key, value, starts, counts)
+    if strides is None:
         raise RuntimeError("HIP block cache append is ineligible for the requested inputs")
     batch, heads, seq_len, dim = key.shape
     try:
@@ -262,8 +268,7 @@ def hip_block_cache_append(
             heads,
             seq_len,
             dim,
-            *_strides(key),
-            *_strides(value),
+            *strides,
             cache.key_codes.shape[0],
             cache.block_table.shape[1],
             dtype_code(key.dtype),
@@ -278,15 +283,17 @@ def can_use_hip_block_cache_read(
 ) -> bool:
     """Whether the read kernel takes these tensors."""
 
+    tail = cache.key_tail
+    batch, index = tail.shape[0], tail.get_device()
     return (
         isinstance(tokens, int)
         and not isinstance(tokens, bool)
         and tokens >= 0
         and firsts is not None
         and lengths is not None
-        and _lengths_ok(firsts, cache)
-        and _lengths_ok(lengths, cache)
-        and is_gfx950(cache.key_tail.device)
+        and _lengths_ok(firsts, batch, index)
+        and _lengths_ok(lengths, batch, index)
+        and is_gfx950(tail.device)
         and library_available()
     )
 
@@ -302,7 +309,7 @@ def hip_block_cache_read(
         raise RuntimeError("HIP block cache read is ineligible for the requested inputs")
     tail = cache.key_tail
     batch, heads, _, dim = tail.shape
-    key = torch.empty((batch, heads, tokens, dim), dtype=tail.dtype, device=tail.device)
+    key = tail.new_empty((batch, heads, tokens, dim))
     value = torch.empty_like(key)
     try:
         launch(
@@ -327,6 +334,34 @@ def hip_block_cache_read(
     return key, value, HIP_BLOCK_CACHE_READ_BACKEND
 
 
+def _attention_request(
+    query: torch.Tensor,
+    cache: BlockCache,
+    starts: torch.Tensor,
+    counts: torch.Tensor | None,
+    scale: float | None,
+    max_length: int | None,
+) -> tuple[int, int, int] | None:
+    """The query's strides where the attention kernel takes the request, else None."""
+
+    tail, size = cache.key_tail, query.shape
+    index = tail.get_device()
+    if query.dtype is not tail.dtype or len(size) != 4 or query.get_device() != index:
+        return None
+    batch, kv_heads, _, dim = tail.shape
+    if size[0] != batch or size[3] != dim or size[1] < 1 or size[1] % kv_heads:
+        return None
+    if scale is not None and not math.isfinite(scale):
+        return None
+    if max_length is not None and not (isinstance(max_length, int) and 0 <= max_length <= _MAX_LENGTH):
+        return None
+    if starts is None or not (_lengths_ok(starts, batch, index) and _lengths_ok(counts, batch, index)):
+        return None
+    if not (is_gfx950(tail.device) and library_available()):
+        return None
+    return _strides(query, size)
+
+
 def can_use_hip_block_cache_attention(
     query: torch.Tensor,
     cache: BlockCache,
@@ -338,18 +373,7 @@ def can_use_hip_block_cache_attention(
 ) -> bool:
     """Whether the attention kernel takes these tensors."""
 
-    return (
-        _rows_ok(query, cache)
-        and query.shape[1] > 0
-        and query.shape[1] % cache.key_tail.shape[1] == 0
-        and starts is not None
-        and _lengths_ok(starts, cache)
-        and _lengths_ok(counts, cache)
-        and (scale is None or math.isfinite(scale))
-        and (max_length is None or 0 <= max_length <= _MAX_LENGTH)
-        and is_gfx950(query.device)
-        and library_available()
-    )
+    return _attention_request(query, cache, starts, counts, scale, max_length) is not None
 
 
 def hip_block_cache_attention(
@@ -373,13 +397,14 @@ def hip_block_cache_attention(
     parts of histories that no sequence has.  Longer ones are still computed whole.
     """
 
-    if not can_use_hip_block_cache_attention(query, cache, starts, counts, scale=scale, max_length=max_length):
+    strides = _attention_request(query, cache, starts, counts, scale, max_length)
+    if strides is None:
         raise RuntimeError("HIP block cache attention is ineligible for the requested inputs")
     batch, heads, seq_len, dim = query.shape
     kv_heads = cache.key_tail.shape[1]
-    dtype, device = query.dtype, query.device
-    most = cache.max_tokens if max_length is None else min(max_length, cache.max_tokens)
-    output = torch.empty((batch, seq_len, heads * dim), dtype=dtype, device=device)
+    device, max_blocks = query.device, cache.block_table.shape[1]
+    most = min(max_blocks * BLOCK_TOKENS + BLOCK_TOKENS - 1, _MAX_LENGTH if max_length is None else max_length)
+    output = query.new_empty((batch, seq_len, heads * dim))
     try:
         library = load_library()
         size = library.sah_block_cache_attention_workspace_bytes(batch, seq_len, heads, kv_heads, dim, most)
@@ -398,14 +423,14 @@ def hip_block_cache_attention(
             kv_heads,
             seq_len,
             dim,
-            *_strides(query),
+            *strides,
             seq_len * heads * dim,
             heads * dim,
             cache.key_codes.shape[0],
-            cache.block_table.shape[1],
+            max_blocks,
             most,
             dim**-0.5 if scale is None else float(scale),
-            dtype_code(dtype),
+            dtype_code(query.dtype),
             None if workspace is None else workspace.data_ptr(),
             size,
         )

@@ -51,46 +51,42 @@ def hip_qk_norm_rotary_available() -> bool:
     return library_available()
 
 
-def _heads_ok(value: torch.Tensor, unit: int) -> bool:
-    size, stride = value.shape, value.stride()
-    return not (
-        stride[3] != 1
-        or (stride[0] % unit and size[0] != 1)
-        or (stride[1] % unit and size[1] != 1)
-        or (stride[2] % unit and size[2] != 1)
-        or value.data_ptr() % 16
-        or (value.requires_grad and torch.is_grad_enabled())
-    )
+def _strides(value: torch.Tensor, size: torch.Size, unit: int) -> tuple[int, int, int] | None:
+    """Strides of the first three axes, 0 for an axis of size 1 (never stepped), or
+    None for a tensor that the kernel does not read in place."""
+
+    b, h, s, feature = value.stride()
+    if size[0] == 1:
+        b = 0
+    if size[1] == 1:
+        h = 0
+    if size[2] == 1:
+        s = 0
+    if feature != 1 or b % unit or h % unit or s % unit or value.data_ptr() % 16:
+        return None
+    if value.requires_grad and torch.is_grad_enabled():
+        return None
+    return b, h, s
 
 
-def _strides(value: torch.Tensor) -> tuple[int, int, int]:
-    """Strides of the first three axes, 0 for an axis of size 1 (never stepped)."""
-
-    size, stride = value.shape, value.stride()
-    return (
-        stride[0] if size[0] != 1 else 0,
-        stride[1] if size[1] != 1 else 0,
-        stride[2] if size[2] != 1 else 0,
-    )
-
-
-def _param_dtype(parameters: tuple[torch.Tensor | None, ...], like: torch.Tensor) -> torch.dtype | None:
+def _param_dtype(
+    parameters: tuple[torch.Tensor | None, ...], dim: int, index: int, like: torch.dtype
+) -> torch.dtype | None:
     """The one dtype of the parameters given (fp32 for none), or None where a
     parameter is not one the kernel reads."""
 
     found = None
-    dim, device = like.shape[3], like.device
     for parameter in parameters:
         if parameter is None:
             continue
         dtype = parameter.dtype
         if (
             parameter.shape != (dim,)
-            or parameter.device != device
+            or parameter.get_device() != index
             or not parameter.is_contiguous()
             or parameter.data_ptr() % 16
             or (parameter.requires_grad and torch.is_grad_enabled())
-            or (dtype is not torch.float32 and dtype is not like.dtype)
+            or (dtype is not torch.float32 and dtype is not like)
             or (found is not None and dtype is not found)
         ):
             return None
@@ -107,20 +103,20 @@ def _request(
     eps: float,
     norm: str,
     interleaved: bool,
-) -> torch.dtype | None:
-    """The parameters' dtype of a request that the kernel takes, else None."""
+) -> tuple[torch.dtype, tuple[int, int, int], tuple[int, int, int]] | None:
+    """The parameters' dtype and both strides of a request that the kernel takes, else None."""
 
-    dtype, size, device = query.dtype, query.shape, query.device
-    key_size = key.shape
+    dtype, size, key_size, index = query.dtype, query.shape, key.shape, query.get_device()
     if dtype not in SUPPORTED_DTYPES or dtype is not key.dtype or len(size) != 4 or len(key_size) != 4:
         return None
     batch, heads, seq_len, dim = size
     if dim not in SUPPORTED_HEAD_DIMS or key_size[0] != batch or key_size[2] != seq_len or key_size[3] != dim:
         return None
-    if heads < 1 or key_size[1] < 1 or device != key.device or batch * seq_len >= 2**31:
+    if heads < 1 or key_size[1] < 1 or index != key.get_device() or batch * seq_len >= 2**31:
         return None
     unit = 4 if dtype is torch.float32 else 8
-    if not (_heads_ok(query, unit) and _heads_ok(key, unit)) or norm not in NORM_KINDS or not eps >= 0:
+    strides, key_strides = _strides(query, size, unit), _strides(key, key_size, unit)
+    if strides is None or key_strides is None or norm not in NORM_KINDS or not eps >= 0:
         return None
     if table is not None:
         rows = table.shape
@@ -129,7 +125,7 @@ def _request(
             or not 0 < rows[1] <= dim
             or rows[1] % (8 if interleaved else 16)
             or table.dtype is not torch.float32
-            or table.device != device
+            or table.get_device() != index
             or not table.is_contiguous()
             or table.data_ptr() % 16
             or table.requires_grad
@@ -138,13 +134,14 @@ def _request(
     if starts is not None and (
         starts.dtype is not torch.int32
         or starts.shape != (batch,)
-        or starts.device != device
+        or starts.get_device() != index
         or not starts.is_contiguous()
     ):
         return None
-    if not (is_gfx950(device) and library_available()):
+    if not (is_gfx950(query.device) and library_available()):
         return None
-    return _param_dtype(parameters, query)
+    param_dtype = _param_dtype(parameters, dim, index, dtype)
+    return None if param_dtype is None else (param_dtype, strides, key_strides)
 
 
 def can_use_hip_qk_norm_rotary(
@@ -195,17 +192,17 @@ def hip_qk_norm_rotary(
     """
 
     parameters = (query_weight, query_bias, key_weight, key_bias)
-    param_dtype = _request(query, key, parameters, table, starts, eps, norm, interleaved)
-    if param_dtype is None:
+    request = _request(query, key, parameters, table, starts, eps, norm, interleaved)
+    if request is None:
         raise RuntimeError("HIP query/key norm with rotation is ineligible for the requested inputs")
+    param_dtype, strides, key_strides = request
     batch, heads, seq_len, dim = query.shape
-    kv_heads = key.shape[1]
-    dtype, device = query.dtype, query.device
-    query_out = torch.empty((batch, heads, seq_len, dim), dtype=dtype, device=device)
-    key_out = torch.empty((batch, kv_heads, seq_len, dim), dtype=dtype, device=device)
+    rows, rotary_dim = (0, 0) if table is None else table.shape
+    query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
     try:
         launch(
-            device,
+            query.device,
             load_library().sah_qk_norm_rotary,
             "sah_qk_norm_rotary",
             query.data_ptr(),
@@ -218,16 +215,16 @@ def hip_qk_norm_rotary(
             batch,
             seq_len,
             heads,
-            kv_heads,
+            key.shape[1],
             dim,
-            *_strides(query),
-            *_strides(key),
-            0 if table is None else table.shape[1],
-            0 if table is None else table.shape[0],
+            *strides,
+            *key_strides,
+            rotary_dim,
+            rows,
             1 if interleaved else 0,
             NORM_KINDS[norm],
             float(eps),
-            dtype_code(dtype),
+            dtype_code(query.dtype),
             dtype_code(param_dtype),
         )
     except HipLibraryError as exc:

@@ -142,32 +142,46 @@ def can_use_hip_linear_w4(
 ) -> bool:
     """Whether the kernel takes this request."""
 
+    return _request(value, weight, bias, activation) is not None
+
+
+def _request(
+    value: torch.Tensor, weight: PackedLinearW4, bias: torch.Tensor | None, activation: str
+) -> tuple[int, int, int, int] | None:
+    """in_features, out_features, group size and row stride of a request that the
+    kernel takes, else None."""
+
     scales = weight.scales
-    if value.ndim < 1 or value.dtype is not scales.dtype or value.device != scales.device:
-        return False
-    if value.shape[-1] != weight.in_features or activation not in ACTIVATIONS or value.data_ptr() % 16:
-        return False
+    dtype, index, shape = scales.dtype, scales.get_device(), value.shape
+    groups, out_features = scales.shape
+    in_features = weight.in_features
+    if value.dtype is not dtype or value.get_device() != index or not shape or shape[-1] != in_features:
+        return None
+    if activation not in ACTIVATIONS or value.data_ptr() % 16:
+        return None
     if value.requires_grad and torch.is_grad_enabled():
-        return False
-    if _row_stride(value) is None:
-        return False
+        return None
+    stride = _row_stride(shape, value.stride())
+    if stride is None:
+        return None
     if bias is not None and (
-        bias.shape != scales.shape[1:]
-        or bias.dtype is not scales.dtype
-        or bias.device != scales.device
+        bias.shape != (out_features,)
+        or bias.dtype is not dtype
+        or bias.get_device() != index
         or not bias.is_contiguous()
         or bias.data_ptr() % 8
         or (bias.requires_grad and torch.is_grad_enabled())
     ):
-        return False
-    return is_gfx950(value.device) and library_available()
+        return None
+    if not (is_gfx950(value.device) and library_available()):
+        return None
+    return in_features, out_features, in_features // groups, stride
 
 
-def _row_stride(value: torch.Tensor) -> int | None:
-    """The stride of ``value``'s rows, taken as one axis; None where they are not
+def _row_stride(shape: tuple[int, ...], strides: tuple[int, ...]) -> int | None:
+    """The stride of a tensor's rows, taken as one axis; None where they are not
     at one stride that the kernel reads."""
 
-    shape, strides = value.shape, value.stride()
     if strides[-1] != 1:
         return None
     stride, span = shape[-1], None
@@ -195,14 +209,14 @@ def hip_linear_w4(
     is "none" or "gelu" (exact).  Any number of rows is right; it is meant for up to
     a few dozen."""
 
-    if not can_use_hip_linear_w4(value, weight, bias, activation=activation):
+    request = _request(value, weight, bias, activation)
+    if request is None:
         raise RuntimeError("HIP 4-bit linear is ineligible for the requested inputs")
-    in_features, out_features = weight.in_features, weight.out_features
-    dtype, device = value.dtype, value.device
-    output = torch.empty((*value.shape[:-1], out_features), dtype=dtype, device=device)
+    in_features, out_features, group_size, stride = request
+    output = value.new_empty((*value.shape[:-1], out_features))
     try:
         launch(
-            device,
+            value.device,
             load_library().sah_linear_w4,
             "sah_linear_w4",
             value.data_ptr(),
@@ -213,10 +227,10 @@ def hip_linear_w4(
             value.numel() // in_features,
             in_features,
             out_features,
-            in_features // weight.scales.shape[0],
-            _row_stride(value),
+            group_size,
+            stride,
             out_features,
-            dtype_code(dtype),
+            dtype_code(value.dtype),
             ACTIVATIONS[activation],
         )
     except HipLibraryError as exc:
