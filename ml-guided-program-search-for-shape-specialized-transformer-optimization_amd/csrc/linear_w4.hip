@@ -21,11 +21,13 @@
 #include <type_traits>
 
 #include "decode_common.hpp"
+#include "gemm_mainloop.hpp"
 
 namespace sah {
 namespace {
 
 constexpr int kUnitK = 128;  // inputs of a tile
+constexpr int64_t kMaxRowStride = (int64_t)1 << 25;
 
 struct LinearW4Args {
   const void* x;
@@ -46,24 +48,34 @@ __device__ __forceinline__ typename Vec8<T>::type code_operand(uint32_t word) {
 }
 
 // A workgroup takes OUTS x 16 outputs of TILES x 16 rows; its SPLIT waves share the
-// inputs among them, a tile of 128 at a time, and load the next tile while they work
-// on this one.  Rows of x are read in whole lines and pass through the wave's own
-// part of LDS on their way to the operands (STAGED): a load straight in the operands'
-// order touches a line a lane.  Few rows do without.
+// inputs among them, a unit of 128 at a time, the next unit's codes, scales and rows of
+// x under way while this one is worked on.  Rows pass through the wave's own part of
+// LDS on their way to the operands (STAGED), by direct-to-LDS loads of whole lines: a
+// load in the operands' order touches a line a lane.  One row does without.  16-byte
+// parts of a row change places by its number, so that the 16 rows of an operand meet no
+// bank twice.  A place in LDS is loaded anew when its operands are read, which are the
+// unit's, or half of it where the sums leave no registers for more.
+//
+// Few rows are bound by the codes' latency and way from memory, many by the vector
+// units (conversions and scales, 290 of them beside 64 matrix instructions a unit of
+// 64 rows and 64 outputs) and the rows' way from L2, 512 KiB a workgroup.
 template <typename T, int GROUP, int TILES, int OUTS, int SPLIT, bool STAGED>
 __global__ __launch_bounds__(SPLIT * 64) void linear_w4_kernel(const LinearW4Args a) {
   typedef typename Vec8<T>::type V8;
   typedef typename Vec8<T>::half_type V4;
   constexpr int GROUPS = kUnitK / GROUP;
-  constexpr int STEPS = GROUP / 32;  // products of a group
+  constexpr int HALF = kUnitK / 2;                 // inputs that x comes in
+  constexpr int RUN = GROUP < HALF ? GROUP : HALF;  // inputs summed before their scale
+  constexpr int STEPS = RUN / 32;                  // products of a run
+  constexpr int RUNS = HALF / RUN;
   constexpr int PARTS = SPLIT < 4 ? SPLIT : 4;
-  constexpr int PITCH = kUnitK + 8;  // values of a row in LDS: operands' rows fall on different banks
-  constexpr int STAGE = STAGED ? TILES * 16 * PITCH : 8;
+  constexpr bool WHOLE = TILES * OUTS <= 8;  // registers for a unit's operands at once
+  constexpr int DMAS = TILES * 2;  // loads of 8 rows of a half
   union Shared {
     f32x4 part[PARTS][TILES * OUTS][64];
-    T stage[SPLIT][STAGE];
+    T stage[STAGED ? SPLIT : 1][2][STAGED ? TILES * 16 * HALF : 8];
   };
-  __shared__ Shared shared;
+  __shared__ __align__(16) Shared shared;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15, quarter = lane >> 4;
@@ -74,15 +86,15 @@ __global__ __launch_bounds__(SPLIT * 64) void linear_w4_kernel(const LinearW4Arg
 
   const u32x4* codes = reinterpret_cast<const u32x4*>(a.codes) + (int64_t)out_tile * a.in_tiles * 64 + lane;
   const T* scales = static_cast<const T*>(a.scales) + (int64_t)out_tile * 16 + quarter * 4;
-  // Places without a row take the last one's.
-  constexpr int LOADS = STAGED ? TILES * 4 : TILES;
-  const T* x[LOADS];
+  // Places without a row take the last one's.  Offsets are below 64 rows of at most 2^25.
+  const T* x = static_cast<const T*>(a.x) + first_row * a.x_stride;
+  uint32_t offset[DMAS];
 #pragma unroll
-  for (int t = 0; t < LOADS; ++t) {
-    const int64_t row = first_row + (STAGED ? t * 4 + lane / 16 : t * 16 + column);
-    x[t] = static_cast<const T*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride +
-           (STAGED ? lane % 16 : quarter) * 8;
+  for (int i = 0; i < DMAS; ++i) {
+    const int64_t row = i * 8 + lane / 8, last = a.rows - 1 - first_row;
+    offset[i] = (uint32_t)((row < last ? row : last) * a.x_stride * 2) + ((lane ^ (lane >> 4) ^ (i % 2 * 4)) & 7) * 16;
   }
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)&shared.stage[STAGED ? wave : 0][0][0];
 
   f32x4 sums[TILES][OUTS];
 #pragma unroll
@@ -90,67 +102,100 @@ __global__ __launch_bounds__(SPLIT * 64) void linear_w4_kernel(const LinearW4Arg
 #pragma unroll
     for (int o = 0; o < OUTS; ++o) sums[t][o] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-  u32x4 next_codes[OUTS];
-  V4 next_scales[OUTS][GROUPS];
-  V8 next_x[TILES * 4];
-  auto load = [&](int unit) {
+  u32x4 words[2][OUTS];
+  V4 scale[2][OUTS][GROUPS];
+  V8 rows[STAGED ? 1 : 4];
+  auto load_codes = [&](auto of_buffer, int unit) {
+    constexpr int B = decltype(of_buffer)::value;
 #pragma unroll
     for (int o = 0; o < OUTS; ++o) {
-      next_codes[o] = codes[((int64_t)o * a.in_tiles + unit) * 64];
+      words[B][o] = codes[((int64_t)o * a.in_tiles + unit) * 64];
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
-        next_scales[o][g] = *reinterpret_cast<const V4*>(scales + ((int64_t)unit * GROUPS + g) * out_features + o * 16);
+        scale[B][o][g] = *reinterpret_cast<const V4*>(scales + ((int64_t)unit * GROUPS + g) * out_features + o * 16);
     }
-#pragma unroll
-    for (int i = 0; i < TILES * 4; ++i)
-      next_x[i] = *reinterpret_cast<const V8*>(x[STAGED ? i : i / 4] + (int64_t)unit * kUnitK + (STAGED ? 0 : i % 4 * 32));
   };
-  T* stage = shared.stage[wave];
-  if (wave < a.in_tiles) load(wave);
-  for (int unit = wave; unit < a.in_tiles; unit += SPLIT) {
-    u32x4 words[OUTS];
-    V4 scale[OUTS][GROUPS];
-    V8 rows[STAGED ? 1 : TILES * 4];
+  auto load_x = [&](int half, int unit) {
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int i = 0; i < DMAS; ++i)
+        tile_dma16(x + (int64_t)unit * kUnitK + half * HALF, offset[i], lds + half * (TILES * 16 * HALF * 2) + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = half * 2; i < half * 2 + 2; ++i)
+        rows[i] = *reinterpret_cast<const V8*>(x + (int64_t)unit * kUnitK + i * 32 + quarter * 8);
+    }
+  };
+  auto step = [&](int unit, auto of_buffer, auto has_next) {
+    constexpr int B = decltype(of_buffer)::value;
+    constexpr bool NEXT = decltype(has_next)::value;
+    // All of the unit has come.  (The compiler, which does not count the direct loads,
+    // would wait for the codes after some of the next unit's have been issued.)
+    if (STAGED) wait_loads<0>();
 #pragma unroll
     for (int o = 0; o < OUTS; ++o) {
-      words[o] = next_codes[o];
+      asm volatile("" : "+v"(words[B][o]));
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) scale[o][g] = next_scales[o][g];
+      for (int g = 0; g < GROUPS; ++g) asm volatile("" : "+v"(scale[B][o][g]));
     }
+    V8 operand[4][TILES];
 #pragma unroll
-    for (int i = 0; i < TILES * 4; ++i) {
-      if (STAGED)
-        *reinterpret_cast<V8*>(stage + (i * 4 + lane / 16) * PITCH + lane % 16 * 8) = next_x[i];
-      else
-        rows[i] = next_x[i];
-    }
-    if (unit + SPLIT < a.in_tiles) load(unit + SPLIT);
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      V8 operand[STEPS][TILES];
+      for (int i = half * 2; i < (WHOLE ? 4 - half * 2 : half * 2 + 2); ++i)
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-          operand[i][t] = STAGED ? *reinterpret_cast<const V8*>(stage + (t * 16 + column) * PITCH +
-                                                                (g * STEPS + i) * 32 + quarter * 8)
-                                 : rows[STAGED ? 0 : t * 4 + g * STEPS + i];
+        for (int t = 0; t < TILES; ++t) {
+          if constexpr (STAGED)
+            operand[i][t] = *reinterpret_cast<const V8*>(&shared.stage[wave][i / 2][0] + (t * 16 + column) * HALF +
+                                                         (((i % 2 * 4 + quarter) ^ (column >> 1)) & 7) * 8);
+          else
+            operand[i][t] = rows[i];
+        }
+      if (NEXT && !(WHOLE && half == 1)) {
+        if (STAGED) wait_lds();
+        load_x(half, unit + SPLIT);
+        if (half == 0) load_codes(std::integral_constant<int, 1 - B>{}, unit + SPLIT);
+        if (WHOLE) load_x(1, unit + SPLIT);
+      }
 #pragma unroll
       for (int o = 0; o < OUTS; ++o) {
-        f32x4 group[TILES];
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          const V8 w = code_operand<T>(words[o][g * STEPS + i]);
+        for (int r = 0; r < RUNS; ++r) {
+          const int g = (half * HALF + r * RUN) / GROUP;
+          f32x4 group[TILES];
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            const V8 w = code_operand<T>(words[B][o][half * 2 + r * STEPS + i]);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+              group[t] = mfma16(w, operand[half * 2 + r * STEPS + i][t], i == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : group[t]);
+          }
 #pragma unroll
           for (int t = 0; t < TILES; ++t)
-            group[t] = mfma16(w, operand[i][t], i == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : group[t]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[t][o][j] = fmaf(group[t][j], to_f32(scale[B][o][g][j]), sums[t][o][j]);
         }
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sums[t][o][j] = fmaf(group[t][j], to_f32(scale[o][g][j]), sums[t][o][j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+  };
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> odd{};
+  int unit = wave;
+  if (unit < a.in_tiles) {
+    load_x(0, unit);
+    load_codes(even, unit);
+    load_x(1, unit);
+  }
+  for (; unit + 2 * SPLIT < a.in_tiles; unit += 2 * SPLIT) {
+    step(unit, even, std::true_type{});
+    step(unit + SPLIT, odd, std::true_type{});
+  }
+  if (unit + SPLIT < a.in_tiles) {
+    step(unit, even, std::true_type{});
+    step(unit + SPLIT, odd, std::false_type{});
+  } else if (unit < a.in_tiles) {
+    step(unit, even, std::false_type{});
   }
   __syncthreads();  // the sums take the stages' place
 
@@ -213,12 +258,15 @@ int launch_tiles(const LinearW4Args& a, hipStream_t stream) {
 // Row tiles by the row count; 16-output tiles of a workgroup by how many there are:
 // x is read anew by every workgroup, so as many outputs as still leave the compute
 // units one each.  One row reads x in the operands' order (all its lanes read the
-// same line).  Measured, us, OUTS 1 / 2 / 4 (SPLIT 8 up to 2, then 4):
-//   16 rows  4096 ->  4096   5.5 /  5.9         64 rows  4096 ->  4096  11.5 / 12.9 / 16.1
-//    8 rows  4096 ->  8192   7.8 /  6.5         64 rows  4096 ->  8192  23.0 / 13.0 / 16.5
-//   16 rows  4096 -> 16384  14.7 / 11.3         64 rows  4096 -> 16384  42.7 / 24.1 / 21.0
-//   32 rows  4096 ->  8192  12.4 /  9.1 / 11.0  32 rows  4096 -> 16384  21.6 / 14.4 / 12.5
-// and without / with the stage: 1 row 4096 -> 4096 5.05 / 5.33, 13 rows 6.3 / 5.5.
+// same line).  Measured, us, OUTS 1 / 2 / 4 as instantiated below, group 128, weights
+// from memory:
+//    1 row   4096 ->  4096   4.9 /  5.5 /  7.5    4096 -> 16384  13.1 / 10.7 / 10.0
+//   16 rows  4096 ->  4096   5.6 /  6.2 /  8.0    4096 -> 16384  14.8 / 12.1 / 10.5
+//   32 rows  4096 ->  8192  11.8 /  8.6 / 11.5    4096 -> 16384  21.2 / 14.8 / 13.1
+//   64 rows  4096 ->  4096  10.7 / 11.4 / 14.2    4096 -> 16384  38.1 / 21.3 / 17.0
+//   64 rows  4096 ->  8192  19.6 / 12.2 / 14.9
+// (the last of 64 rows: 36 MB, 2.1 TB/s, 505 TFLOP/s), and 1 row 4096 -> 4096 without
+// / with the stage 5.05 / 5.33, 13 rows 6.3 / 5.5.
 template <typename T, int GROUP>
 int launch_linear_w4(const LinearW4Args& a, hipStream_t stream) {
   const int64_t row_tiles = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
@@ -226,9 +274,13 @@ int launch_linear_w4(const LinearW4Args& a, hipStream_t stream) {
   const bool two = tiles >= 512 && a.out_tiles % 2 == 0;
   const bool four = tiles >= 1024 && a.out_tiles % 4 == 0;
   if (a.rows == 1)
-    return two ? launch_tiles<T, GROUP, 1, 2, 8, false>(a, stream) : launch_tiles<T, GROUP, 1, 1, 8, false>(a, stream);
+    return four  ? launch_tiles<T, GROUP, 1, 4, 8, false>(a, stream)
+           : two ? launch_tiles<T, GROUP, 1, 2, 8, false>(a, stream)
+                 : launch_tiles<T, GROUP, 1, 1, 8, false>(a, stream);
   if (row_tiles == 1)
-    return two ? launch_tiles<T, GROUP, 1, 2, 8, true>(a, stream) : launch_tiles<T, GROUP, 1, 1, 8, true>(a, stream);
+    return four  ? launch_tiles<T, GROUP, 1, 4, 8, true>(a, stream)
+           : two ? launch_tiles<T, GROUP, 1, 2, 8, true>(a, stream)
+                 : launch_tiles<T, GROUP, 1, 1, 8, true>(a, stream);
   if (row_tiles == 2)
     return four  ? launch_tiles<T, GROUP, 2, 4, 4, true>(a, stream)
            : two ? launch_tiles<T, GROUP, 2, 2, 8, true>(a, stream)
@@ -272,6 +324,8 @@ extern "C" int sah_linear_w4(const void* x, const void* codes, const void* scale
   if (!aligned16(x) || !aligned16(codes) || !aligned16(scales) || !aligned16(y) ||
       (reinterpret_cast<uintptr_t>(bias) & 7u) != 0)
     return fail(SAH_ERR_INVALID_ARGUMENT, "sah_linear_w4: tensors must be 16-byte aligned, bias 8-byte");
+  if (rows > 1 && (x_row_stride < 0 || x_row_stride > kMaxRowStride))
+    return fail(SAH_ERR_UNSUPPORTED, "sah_linear_w4: rows of x %lld elements apart", (long long)x_row_stride);
   if (x_row_stride % 8 != 0 || y_row_stride % 8 != 0)
     return fail(SAH_ERR_INVALID_ARGUMENT, "sah_linear_w4: row strides must be multiples of 8 elements");
   LinearW4Args a{};

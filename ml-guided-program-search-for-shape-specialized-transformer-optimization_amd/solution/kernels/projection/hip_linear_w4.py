@@ -29,6 +29,7 @@ SUPPORTED_GROUP_SIZES = frozenset({32, 64, 128})
 SUPPORTED_DTYPES = frozenset({torch.bfloat16, torch.float16})
 ACTIVATIONS = {"none": SAH_ACTIVATION_NONE, "gelu": SAH_ACTIVATION_GELU_EXACT}
 _TILE_IN = 128
+_MAX_ROW_STRIDE = 2**25
 _TILE_OUT = 16
 _LARGEST_CODE = 7
 
@@ -194,7 +195,7 @@ def _row_stride(shape: tuple[int, ...], strides: tuple[int, ...]) -> int | None:
         elif step != span:
             return None
         span = step * size
-    return stride if stride % 8 == 0 and stride >= 0 else None
+    return stride if stride % 8 == 0 and 0 <= stride <= _MAX_ROW_STRIDE else None
 
 
 def hip_linear_w4(
