@@ -24,15 +24,15 @@
 // type; the weights are fp16 (times 2^11, so that none above 2^-25 of the largest is
 // subnormal), the scales, maxima, sums and outputs fp32.
 //
-// A long history is split over workgroups (and over the waves of one); a second
-// launch merges their outputs with their maxima and sums.
+// A long history is split over workgroups (and over the waves of one), which take its
+// blocks in turn; a second launch merges their outputs with their maxima and sums.
 //
 // Bounds.  For a single token every feature of a held token is 2 bytes to read for
 // 4 * group operations, so the codes' way from memory bounds it: 4 sequences of 90000
-// to 100000 tokens, 16 heads of 64, 779 MB in 139 us, 5.6 TB/s (a copy moves 4.9), and
-// 4.7 us for the merge of their chunks.  32 ragged sequences of 100 to 4095 tokens,
-// 32 / 8 heads of 128 (138 MB), take 38 us and 4.6, one of 777 tokens 7.5: there the
-// longest wave's chain of loads bounds it.
+// to 100000 tokens, 16 heads of 64, 779 MB in 136 us, 5.7 TB/s (a copy moves 4.9), and
+// 4.9 us for the merge of their parts.  32 sequences of 100 to 4095 tokens, 32 / 8 heads
+// of 128 (138 MB), take 33 us and 4.9, one of 777 tokens 7.5: there the longest wave's
+// chain of loads bounds it.
 
 #include <type_traits>
 
@@ -66,8 +66,8 @@ struct AttentionArgs {
   int64_t q_sb, q_sh, q_ss, o_sb, o_ss;
   int64_t blocks, max_blocks;
   int seq_len, heads, kv_heads, group;
-  int chunks, chunk_blocks;
-  uint32_t row_groups;
+  int chunks;
+  uint32_t row_groups, batch;
   float scale_log2;   // |scale| log2(e); log2(e) for a zero scale
   uint32_t sign;      // 0x80008000 where the scale is negative
   uint32_t keep;      // 0 for a zero scale: a zero query at scale 1
@@ -123,12 +123,13 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   const int h = common((int)(at % (uint32_t)a.kv_heads));
   const int64_t b = common((int)(at / (uint32_t)a.kv_heads));
 
-  // The table entries of this wave's first blocks are asked for before its lengths are
-  // known; those behind the sequence's blocks are not used.
-  const int64_t from64 = (int64_t)chunk * a.chunk_blocks;
+  // The waves of all chunks take the blocks of a sequence in turn, whatever its length:
+  // this one `first`, first + stride, ...  Their table entries are asked for before the
+  // length is known; those behind the sequence's blocks are not used.
+  const int first = chunk * SPLIT + split, stride = a.chunks * SPLIT;
   int first_pages = -1;
-  if (from64 + split + lane * SPLIT < a.max_blocks)
-    first_pages = a.table[b * a.max_blocks + from64 + split + lane * SPLIT];
+  if (first + (int64_t)lane * stride < a.max_blocks)
+    first_pages = a.table[b * a.max_blocks + first + (int64_t)lane * stride];
 
   const int64_t start = common(a.starts[b]);
   int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
@@ -160,11 +161,8 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
       q[hh][kk] = __builtin_bit_cast(V8, raw);
     }
 
-  // Blocks of this workgroup: the sequence's, in chunks, the last chunk with the rest.
   const int all_blocks = count == 0 || beyond ? 0 : last_position / kBlockTokens + 1;
-  const int from = from64 < all_blocks ? (int)from64 : all_blocks;
-  const int to = chunk == a.chunks - 1 || all_blocks - from < a.chunk_blocks ? all_blocks : from + a.chunk_blocks;
-  const int coded_to = to < tail_block ? to : tail_block;
+  const int coded_to = all_blocks < tail_block ? all_blocks : tail_block;
 
   // Outputs are held in units of a power of two, the largest value scale so far.
   f32x4 out[FEATURES];
@@ -232,17 +230,17 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   };
 
   // A wave's blocks, 64 at a time: a lane each looks up the page and its scales.
-  for (int base = from + split; base < coded_to; base += 64 * SPLIT) {
-    const int mine = base + lane * SPLIT;
+  for (int base = first; base < coded_to; base += 64 * stride) {
+    const int mine = base + lane * stride;
     int pages = first_pages;
-    if (base != from + split && mine < coded_to) pages = a.table[b * a.max_blocks + mine];
+    if (base != first && mine < coded_to) pages = a.table[b * a.max_blocks + mine];
     if (mine >= coded_to || pages < 0 || pages >= a.blocks) pages = -1;
     float key_scales = 0.0f, value_scales = 0.0f;
     if (pages >= 0) {
       key_scales = a.key_scales[(int64_t)pages * a.kv_heads + h];
       value_scales = a.value_scales[(int64_t)pages * a.kv_heads + h];
     }
-    const int left = (coded_to - base + SPLIT - 1) / SPLIT;
+    const int left = (coded_to - base + stride - 1) / stride;
     const int here = left < 64 ? left : 64;
     int page = __builtin_amdgcn_readlane(pages, 0);
     if (page >= 0) {
@@ -250,7 +248,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
       load_values(page);
     }
     for (int i = 0; i < here; ++i) {
-      const int block = base + i * SPLIT;
+      const int block = base + i * stride;
       const bool held = page >= 0;
       page = i + 1 < here ? __builtin_amdgcn_readlane(pages, i + 1) : -1;
       f32x4 s[4];
@@ -302,7 +300,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
 
   // The incomplete block, in the tensors' own type: weights without the shift, in a
   // unit of at least 2^11 (the shift), so that large values do not overflow.
-  if (tail_block >= from && tail_block < to && (tail_block - from) % SPLIT == split) {
+  if (tail_block < all_blocks && tail_block % stride == first) {
     const int held = first_position + count - tail_block * kBlockTokens;  // tokens in it
     const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
     const T* tail_keys = static_cast<const T*>(a.key_tail) + tail_at + quarter * 16;
@@ -429,7 +427,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
 // The vector units bound it (60% busy: 32 weights and 64 conversions a lane and block
 // beside 32 matrix instructions of 16 cycles), so with heads of 64 the products of the
 // next block are issued beside this one's weights.  2 x 512 tokens behind 7680, 16 / 4
-// heads: heads of 64 64 us, 33.3 GFLOP at 520 TFLOP/s; heads of 128 112 us, 595 TFLOP/s.
+// heads: heads of 64 63 us, 33.3 GFLOP at 530 TFLOP/s; heads of 128 110 us, 605 TFLOP/s.
 template <int D>
 __device__ __forceinline__ int key_turn(int t) {
   return D == 64 ? (((t >> 1) ^ (t >> 2)) & 1) | (((t >> 5) & 1) << 1)
@@ -462,12 +460,13 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
   const int split = wave / ROWS, row_wave = wave % ROWS;
 
   uint32_t at = blockIdx.x;
-  const int chunk = common((int)(at % (uint32_t)a.chunks));
-  at /= (uint32_t)a.chunks;
-  const uint32_t group_row = (uint32_t)common((int)(at % a.row_groups)) * (ROWS * 32);  // rows are below 2^31
-  at /= a.row_groups;
+  // Key heads next to one another on the dies, so that each die's L2 keeps few of them.
+  const int64_t b = common((int)(at % a.batch));
+  at /= a.batch;
   const int h = common((int)(at % (uint32_t)a.kv_heads));
-  const int64_t b = common((int)(at / (uint32_t)a.kv_heads));
+  at /= (uint32_t)a.kv_heads;
+  const int chunk = common((int)(at % (uint32_t)a.chunks));
+  const uint32_t group_row = (uint32_t)common((int)(at / (uint32_t)a.chunks)) * (ROWS * 32);  // rows are below 2^31
 
   const int64_t start = common(a.starts[b]);
   int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
@@ -505,13 +504,12 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
       q[c][e] = __builtin_bit_cast(V8, raw);
     }
 
-  // Blocks of the workgroup's rows in this chunk; group `split` takes every SPLIT-th.
+  // The groups of all chunks take the blocks that the workgroup's rows see in turn; all
+  // groups of a workgroup do as many turns, the last ones perhaps without a block.
   const int all_blocks = group_last < 0 || beyond ? 0 : group_last / kBlockTokens + 1;
-  const int64_t from64 = (int64_t)chunk * a.chunk_blocks;
-  const int from = from64 < all_blocks ? (int)from64 : all_blocks;
-  const int to = chunk == a.chunks - 1 || all_blocks - from < a.chunk_blocks ? all_blocks : from + a.chunk_blocks;
-  const int coded_to = to < tail_block ? to : tail_block;
-  const int turns = coded_to > from ? (coded_to - from + SPLIT - 1) / SPLIT : 0;
+  const int coded_to = all_blocks < tail_block ? all_blocks : tail_block;
+  const int first_block = chunk * SPLIT + split, stride = a.chunks * SPLIT;
+  const int turns = coded_to > chunk * SPLIT ? (coded_to - chunk * SPLIT + stride - 1) / stride : 0;
 
   f32x16 out[FEATURES];
   int unit = 0;
@@ -620,7 +618,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
   int pages = -1;
   float key_scales = 0.0f, value_scales = 0.0f;
   auto look_up = [&](int first) {
-    const int mine = from + split + (first + lane) * SPLIT;
+    const int64_t mine = first_block + (int64_t)(first + lane) * stride;
     pages = -1;
     if (mine < coded_to) pages = a.table[b * a.max_blocks + mine];
     if (pages < 0 || pages >= a.blocks) pages = -1;
@@ -645,7 +643,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
     if (ROWS > 1) tile_barrier();  // every wave's part of the loads has come
     if (AHEAD && i + 2 < here) load_keys(page_of(i + 2), i & 1);
     if (!AHEAD) score(s, i & 1);
-    const int block = from + split + (first + i) * SPLIT;
+    const int block = first_block + (first + i) * stride;
     const bool held = __builtin_amdgcn_readlane(pages, i) >= 0;
     const bool seen = block < coded_to && block * kBlockTokens <= last_position;
     const bool whole = block * kBlockTokens + (kBlockTokens - 1) <= least_position;
@@ -697,7 +695,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
     }
   };
   if (a.blocks == 0) {  // no cache to read
-    if (turns > 0 && sees >= (from + split) * kBlockTokens && from + split < coded_to) sum = __builtin_nanf("");
+    if (first_block < coded_to && sees >= first_block * kBlockTokens) sum = __builtin_nanf("");
   } else {
     for (int first = 0; first < turns; first += 64) {
       look_up(first);
@@ -728,8 +726,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
   }
 
   // The incomplete block, as above.
-  if (tail_block >= from && tail_block < to && (tail_block - from) % SPLIT == split &&
-      last_position >= tail_block * kBlockTokens) {
+  if (last_position >= tail_block * kBlockTokens && tail_block % stride == first_block) {
     const int held = first_position + count - tail_block * kBlockTokens;
     const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
     const T* keys = static_cast<const T*>(a.key_tail) + tail_at + half * 16;
@@ -921,7 +918,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
 struct Layout {
   int wave_rows, split, rows;
   int64_t row_groups;
-  int chunks, chunk_blocks;
+  int chunks;
 };
 
 Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group, int64_t head_dim,
@@ -948,8 +945,7 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
   const int64_t most = ceil_div(blocks, 4 * l.split);
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
-  l.chunk_blocks = (int)ceil_div(blocks, chunks);
-  l.chunks = (int)ceil_div(blocks, l.chunk_blocks);
+  l.chunks = (int)chunks;
   return l;
 }
 
@@ -1069,8 +1065,8 @@ extern "C" int sah_block_cache_attention(
   a.kv_heads = (int)kv_heads;
   a.group = (int)(heads / kv_heads);
   a.chunks = l.chunks;
-  a.chunk_blocks = l.chunk_blocks;
   a.row_groups = (uint32_t)l.row_groups;
+  a.batch = (uint32_t)batch;
   a.sign = scale < 0.0f ? 0x80008000u : 0u;
   a.keep = scale == 0.0f ? 0u : ~0u;
   a.scale_log2 = scale == 0.0f ? 1.44269504f : scale_log2;
