@@ -31,8 +31,8 @@
 // 4 * group operations, so the codes' way from memory bounds it: 4 sequences of 90000
 // to 100000 tokens, 16 heads of 64, 779 MB in 136 us, 5.7 TB/s (a copy moves 4.9), and
 // 4.9 us for the merge of their parts.  32 sequences of 100 to 4095 tokens, 32 / 8 heads
-// of 128 (138 MB), take 33 us and 4.9, one of 777 tokens 7.5: there the longest wave's
-// chain of loads bounds it.
+// of 128 (138 MB), take 36 us, one of 777 tokens 7.5: there the longest wave's chain of
+// loads bounds it.
 
 #include <type_traits>
 
@@ -930,11 +930,13 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
   // waves that the registers leave room for, on all compute units
   const int64_t room = (int64_t)kUnits * 4 * (head_dim == 64 && l.wave_rows == 16 ? 3 : 2);
   // The waves of a workgroup split the tokens, which leaves fewer parts to merge through
-  // memory; short histories go to eight of them, in one launch.  Heads of 128 have the
-  // registers for one block's scores, and more to gain from blocks shared by four waves
-  // of other rows (2 x 512 rows behind 7680 tokens, 16 / 4 heads, us: heads of 128
-  // 123 / 111 shared, heads of 64 63 / 66).
-  l.split = l.wave_rows == 16 && blocks <= 32 ? 8 : 4;
+  // memory.  Eight of them do in one launch what four leave to a second one, but leave
+  // registers unused with heads of 64 (tokens of a sequence, us with both launches, eight
+  // / four: 64 x 2000 14.6 / 20.1, 64 x 8000 49.6 / 54.8; 8 x 20000 28.4 / 25.2, 4 x
+  // 100000 160 / 142).  Heads of 128 have the registers for one block's scores, and more
+  // to gain from blocks shared by four waves of other rows (2 x 512 rows behind 7680
+  // tokens, 16 / 4 heads: heads of 128 123 / 111 shared, heads of 64 63 / 66).
+  l.split = l.wave_rows == 16 && blocks <= 128 ? 8 : 4;
   l.rows = 1;
   if (head_dim == 128 && rows > 64) {
     l.split = 2;
@@ -942,6 +944,8 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
   }
   l.row_groups = ceil_div(rows, (int64_t)l.wave_rows * l.rows);
   int64_t chunks = room / (batch * kv_heads * l.row_groups * l.rows * l.split);
+  // A wave has at least four blocks (1 x 1000 tokens 6.7, with two blocks and a second
+  // launch 19.9).
   const int64_t most = ceil_div(blocks, 4 * l.split);
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
