@@ -532,6 +532,16 @@ def test_more_blocks_than_one_look_up_of_a_wave(gpu_device, seq, dim, dtype):
     assert bool(_attend(t, query, starts, max_length=1).isnan().all())
 
 
+def test_many_look_ups_in_parts(gpu_device):
+    """Four waves a workgroup and several parts, with more than 64 blocks a wave."""
+
+    t = _Tokens(gpu_device, [150_000], 1, 64, BF16, seed=215).fill()
+    query = _rand((1, 2, 1, 64), 216, BF16)
+    _check_attention(t, query, [149_999], max_length=8_300)
+    t.cache.block_table[0, 2_330] = -1
+    assert bool(_attend(t, query, [149_999], max_length=8_300).isnan().all())
+
+
 @pytest.mark.parametrize("heads", [40, 96])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_many_query_heads_a_key_head(gpu_device, heads, dim):
