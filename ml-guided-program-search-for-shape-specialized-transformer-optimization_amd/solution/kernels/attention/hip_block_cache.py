@@ -27,10 +27,9 @@ import torch
 from ..hip._library import (
     HipLibraryError,
     dtype_code,
-    is_gfx950,
     launch,
     library_available,
-    load_library,
+    library_for,
 )
 
 HIP_BLOCK_CACHE_APPEND_BACKEND = "hip_block_cache_append"
@@ -199,8 +198,9 @@ def _append_request(
     value: torch.Tensor,
     starts: torch.Tensor,
     counts: torch.Tensor | None,
-) -> tuple[int, ...] | None:
-    """The strides of key and value where the append kernel takes the request, else None."""
+) -> tuple | None:
+    """The library, the device and the strides of key and value where the append kernel
+    takes the request, else None."""
 
     tail, size = cache.key_tail, key.shape
     dtype, index = tail.dtype, tail.get_device()
@@ -216,9 +216,8 @@ def _append_request(
         return None
     if not (_lengths_ok(starts, batch, index) and _lengths_ok(counts, batch, index)):
         return None
-    if not (is_gfx950(tail.device) and library_available()):
-        return None
-    return key_strides + value_strides
+    library = library_for(index)
+    return None if library is None else (library, index, key_strides, value_strides)
 
 
 def can_use_hip_block_cache_append(
@@ -250,14 +249,15 @@ def hip_block_cache_append(
     value makes NaN of every query that attends to it, and of no other.
     """
 
-    strides = _append_request(cache, key, value, starts, counts)
-    if strides is None:
+    request = _append_request(cache, key, value, starts, counts)
+    if request is None:
         raise RuntimeError("HIP block cache append is ineligible for the requested inputs")
+    library, index, key_strides, value_strides = request
     batch, heads, seq_len, dim = key.shape
     try:
         launch(
-            key.device,
-            load_library().sah_block_cache_append,
+            index,
+            library.sah_block_cache_append,
             "sah_block_cache_append",
             key.data_ptr(),
             value.data_ptr(),
@@ -268,7 +268,8 @@ def hip_block_cache_append(
             heads,
             seq_len,
             dim,
-            *strides,
+            *key_strides,
+            *value_strides,
             cache.key_codes.shape[0],
             cache.block_table.shape[1],
             dtype_code(key.dtype),
@@ -293,8 +294,7 @@ def can_use_hip_block_cache_read(
         and lengths is not None
         and _lengths_ok(firsts, batch, index)
         and _lengths_ok(lengths, batch, index)
-        and is_gfx950(tail.device)
-        and library_available()
+        and library_for(index) is not None
     )
 
 
@@ -309,12 +309,13 @@ def hip_block_cache_read(
         raise RuntimeError("HIP block cache read is ineligible for the requested inputs")
     tail = cache.key_tail
     batch, heads, _, dim = tail.shape
+    index = tail.get_device()
     key = tail.new_empty((batch, heads, tokens, dim))
     value = torch.empty_like(key)
     try:
         launch(
-            tail.device,
-            load_library().sah_block_cache_read,
+            index,
+            library_for(index).sah_block_cache_read,
             "sah_block_cache_read",
             *cache._pointers(),
             firsts.data_ptr(),
@@ -341,8 +342,9 @@ def _attention_request(
     counts: torch.Tensor | None,
     scale: float | None,
     max_length: int | None,
-) -> tuple[int, int, int] | None:
-    """The query's strides where the attention kernel takes the request, else None."""
+) -> tuple | None:
+    """The library, the device and the query's strides where the attention kernel takes
+    the request, else None."""
 
     tail, size = cache.key_tail, query.shape
     index = tail.get_device()
@@ -357,9 +359,8 @@ def _attention_request(
         return None
     if starts is None or not (_lengths_ok(starts, batch, index) and _lengths_ok(counts, batch, index)):
         return None
-    if not (is_gfx950(tail.device) and library_available()):
-        return None
-    return _strides(query, size)
+    strides, library = _strides(query, size), library_for(index)
+    return None if strides is None or library is None else (library, index, strides)
 
 
 def can_use_hip_block_cache_attention(
@@ -397,20 +398,19 @@ def hip_block_cache_attention(
     parts of histories that no sequence has.  Longer ones are still computed whole.
     """
 
-    strides = _attention_request(query, cache, starts, counts, scale, max_length)
-    if strides is None:
+    request = _attention_request(query, cache, starts, counts, scale, max_length)
+    if request is None:
         raise RuntimeError("HIP block cache attention is ineligible for the requested inputs")
+    library, index, strides = request
     batch, heads, seq_len, dim = query.shape
-    kv_heads = cache.key_tail.shape[1]
-    device, max_blocks = query.device, cache.block_table.shape[1]
+    kv_heads, max_blocks = cache.key_tail.shape[1], cache.block_table.shape[1]
     most = min(max_blocks * BLOCK_TOKENS + BLOCK_TOKENS - 1, _MAX_LENGTH if max_length is None else max_length)
     output = query.new_empty((batch, seq_len, heads * dim))
     try:
-        library = load_library()
         size = library.sah_block_cache_attention_workspace_bytes(batch, seq_len, heads, kv_heads, dim, most)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        workspace = torch.empty(size, dtype=torch.uint8, device=query.device) if size else None
         launch(
-            device,
+            index,
             library.sah_block_cache_attention,
             "sah_block_cache_attention",
             query.data_ptr(),

@@ -209,15 +209,15 @@ def stream_handle(device: torch.device) -> int:
     return int(torch._C._cuda_getCurrentRawStream(_device_index(device)))
 
 
-def launch(device: torch.device, function, what: str, *args) -> None:
-    """Call a C entry on ``device``'s current stream (its last argument), with that
-    device as the current one, and raise :class:`HipLibraryError` on a status."""
+def launch(index: int, function, what: str, *args) -> None:
+    """Call a C entry on device ``index``'s current stream (its last argument), with
+    that device as the current one, and raise :class:`HipLibraryError` on a status."""
 
-    if device.index == torch._C._cuda_getDevice():
-        status = function(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if index == torch._C._cuda_getDevice():
+        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            status = function(*args, stream_handle(device))
+        with torch.cuda.device(index):
+            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
     if status != SAH_OK:
         check_status(status, what)
 
@@ -246,6 +246,16 @@ def is_gfx950(device: torch.device) -> bool:
     return known
 
 
+def library_for(index: int) -> ctypes.CDLL | None:
+    """The library, where device ``index`` (-1: the CPU) is a gfx950 GPU and it loads."""
+
+    if _library is not None and _GFX950_BY_INDEX.get(index):
+        return _library
+    if index < 0 or not is_gfx950(torch.device("cuda", index)) or not library_available():
+        return None
+    return load_library()
+
+
 __all__ = [
     "ABI_VERSION",
     "EXPORTED_SYMBOLS",
@@ -262,6 +272,7 @@ __all__ = [
     "is_gfx950",
     "launch",
     "library_available",
+    "library_for",
     "load_library",
     "stream_handle",
 ]

@@ -15,10 +15,9 @@ from ..hip._library import (
     SAH_NORM_RMS,
     HipLibraryError,
     dtype_code,
-    is_gfx950,
     launch,
     library_available,
-    load_library,
+    library_for,
 )
 
 HIP_QK_NORM_ROTARY_BACKEND = "hip_qk_norm_rotary"
@@ -103,8 +102,9 @@ def _request(
     eps: float,
     norm: str,
     interleaved: bool,
-) -> tuple[torch.dtype, tuple[int, int, int], tuple[int, int, int]] | None:
-    """The parameters' dtype and both strides of a request that the kernel takes, else None."""
+) -> tuple | None:
+    """The library, the device, the parameters' dtype and both strides of a request that
+    the kernel takes, else None."""
 
     dtype, size, key_size, index = query.dtype, query.shape, key.shape, query.get_device()
     if dtype not in SUPPORTED_DTYPES or dtype is not key.dtype or len(size) != 4 or len(key_size) != 4:
@@ -138,10 +138,9 @@ def _request(
         or not starts.is_contiguous()
     ):
         return None
-    if not (is_gfx950(query.device) and library_available()):
-        return None
     param_dtype = _param_dtype(parameters, dim, index, dtype)
-    return None if param_dtype is None else (param_dtype, strides, key_strides)
+    library = library_for(index)
+    return None if param_dtype is None or library is None else (library, index, param_dtype, strides, key_strides)
 
 
 def can_use_hip_qk_norm_rotary(
@@ -195,15 +194,15 @@ def hip_qk_norm_rotary(
     request = _request(query, key, parameters, table, starts, eps, norm, interleaved)
     if request is None:
         raise RuntimeError("HIP query/key norm with rotation is ineligible for the requested inputs")
-    param_dtype, strides, key_strides = request
+    library, index, param_dtype, strides, key_strides = request
     batch, heads, seq_len, dim = query.shape
     rows, rotary_dim = (0, 0) if table is None else table.shape
     query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
     try:
         launch(
-            query.device,
-            load_library().sah_qk_norm_rotary,
+            index,
+            library.sah_qk_norm_rotary,
             "sah_qk_norm_rotary",
             query.data_ptr(),
             key.data_ptr(),

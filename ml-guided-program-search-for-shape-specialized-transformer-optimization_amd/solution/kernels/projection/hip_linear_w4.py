@@ -18,10 +18,9 @@ from ..hip._library import (
     SAH_ACTIVATION_NONE,
     HipLibraryError,
     dtype_code,
-    is_gfx950,
     launch,
     library_available,
-    load_library,
+    library_for,
 )
 
 HIP_LINEAR_W4_BACKEND = "hip_linear_w4"
@@ -148,9 +147,9 @@ def can_use_hip_linear_w4(
 
 def _request(
     value: torch.Tensor, weight: PackedLinearW4, bias: torch.Tensor | None, activation: str
-) -> tuple[int, int, int, int] | None:
-    """in_features, out_features, group size and row stride of a request that the
-    kernel takes, else None."""
+) -> tuple | None:
+    """The library, the device, in_features, out_features, group size and row stride of
+    a request that the kernel takes, else None."""
 
     scales = weight.scales
     dtype, index, shape = scales.dtype, scales.get_device(), value.shape
@@ -174,9 +173,8 @@ def _request(
         or (bias.requires_grad and torch.is_grad_enabled())
     ):
         return None
-    if not (is_gfx950(value.device) and library_available()):
-        return None
-    return in_features, out_features, in_features // groups, stride
+    library = library_for(index)
+    return None if library is None else (library, index, in_features, out_features, in_features // groups, stride)
 
 
 def _row_stride(shape: tuple[int, ...], strides: tuple[int, ...]) -> int | None:
@@ -213,12 +211,12 @@ def hip_linear_w4(
     request = _request(value, weight, bias, activation)
     if request is None:
         raise RuntimeError("HIP 4-bit linear is ineligible for the requested inputs")
-    in_features, out_features, group_size, stride = request
+    library, index, in_features, out_features, group_size, stride = request
     output = value.new_empty((*value.shape[:-1], out_features))
     try:
         launch(
-            value.device,
-            load_library().sah_linear_w4,
+            index,
+            library.sah_linear_w4,
             "sah_linear_w4",
             value.data_ptr(),
             weight.codes.data_ptr(),
