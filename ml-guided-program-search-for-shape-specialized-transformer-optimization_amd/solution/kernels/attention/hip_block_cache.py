@@ -244,9 +244,10 @@ def hip_block_cache_append(
     ``key`` and ``value`` are [batch, kv_heads, seq_len, head_dim] (any strides,
     head_dim contiguous); sequence b holds ``starts[b]`` tokens and takes the first
     ``counts[b]`` rows, or all ``seq_len`` without ``counts``.  A block is coded when
-    its 64th token comes.  Blocks without a place in the cache are dropped, and the
-    attention that would read them answers NaN.  A token with a non-finite key or
-    value makes NaN of every query that attends to it, and of no other.
+    its 64th token comes, at a place that no other sequence of the call completes
+    one at.  Blocks without a place in the cache are dropped, and the attention that
+    would read them answers NaN.  A token with a non-finite key or value makes NaN of
+    every query that attends to it, and of no other.
     """
 
     request = _append_request(cache, key, value, starts, counts)

@@ -4,6 +4,8 @@ the 4-bit format against a plain decoder."""
 
 from __future__ import annotations
 
+import importlib
+
 import pytest
 import torch
 
@@ -195,10 +197,33 @@ LINEAR = dict(
         ({"x_stride": 257}, INVALID),
         ({"y_stride": 36}, INVALID),
         ({"rows": 1 << 39}, UNSUPPORTED),
+        ({"x_stride": -256}, UNSUPPORTED),
+        ({"x_stride": 2**25 + 8}, UNSUPPORTED),
     ],
 )
 def test_linear_w4_entry_refuses_before_launch(changes, status):
     assert _call("sah_linear_w4", LINEAR, **changes) == status
+
+
+@pytest.mark.parametrize(
+    "shape,strides,want",
+    [
+        ((128,), (1,), 128),
+        ((3, 128), (136, 1), 136),
+        ((3, 128), (0, 1), 0),
+        ((1, 128), (2**26, 1), 128),
+        ((2, 128), (2**25, 1), 2**25),
+        ((2, 128), (2**25 + 8, 1), None),
+        ((2, 128), (132, 1), None),
+        ((2, 128), (128, 2), None),
+        ((2, 3, 128), (384, 128, 1), 128),
+        ((2, 3, 128), (512, 128, 1), None),
+        ((2, 1, 128), (512, 7, 1), 512),
+    ],
+)
+def test_linear_w4_rows_at_one_stride(shape, strides, want):
+    module = importlib.import_module("solution.kernels.projection.hip_linear_w4")
+    assert module._row_stride(shape, strides) == want
 
 
 def _cpu_cache(**changes):

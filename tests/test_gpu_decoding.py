@@ -533,11 +533,13 @@ def test_more_blocks_than_one_look_up_of_a_wave(gpu_device, seq, dim, dtype):
 
 
 def test_many_look_ups_in_parts(gpu_device):
-    """Four waves a workgroup and several parts, with more than 64 blocks a wave."""
+    """Four waves a workgroup and several parts, with more than 64 blocks a wave; and
+    more than 64 parts."""
 
     t = _Tokens(gpu_device, [150_000], 1, 64, BF16, seed=215).fill()
     query = _rand((1, 2, 1, 64), 216, BF16)
     _check_attention(t, query, [149_999], max_length=8_300)
+    _check_attention(t, query, [149_999])
     t.cache.block_table[0, 2_330] = -1
     assert bool(_attend(t, query, [149_999], max_length=8_300).isnan().all())
 
