@@ -12,9 +12,10 @@
 // heads of one token (the packed projection's output is read in whole lines), and
 // the wave goes over up to STEPS such groups with one read of the table row.  All its
 // loads are issued before the first sum.
-//   2 x 50001 tokens, 16 + 16 heads of 64, bf16 (846 MB): 208 us, 4.1 TB/s (228 with
+//   2 x 50001 tokens, 16 + 16 heads of 64, bf16 (846 MB): 206 us, 4.1 TB/s (228 with
 //   cached loads and stores)
-//   1 token of the same: 3.4 us (4.8 with four groups of heads a wave)
+//   3 x 777 tokens, 12 + 4 heads of 128, fp32 (38 MB): 12.4 us; 1 token, 16 + 16 heads of
+//   64, bf16: 3.3 us (4.8 with four groups of heads a wave)
 
 #include <type_traits>
 
