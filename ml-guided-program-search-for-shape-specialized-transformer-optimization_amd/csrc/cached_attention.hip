@@ -43,7 +43,8 @@ namespace sah {
 namespace {
 
 // Weights are 2^(score - base + kWeightShift); a row's base is raised to its maximum
-// when that exceeds it by kWeightMargin, so no weight is above 2^15.
+// when that exceeds it by kWeightMargin, or in chunks when a weight leaves fp16's range
+// (scores 5 above the base), so no weight is above 2^16.
 constexpr float kWeightShift = 11.0f;
 constexpr float kWeightMargin = 4.0f;
 constexpr float kUnshift = 0x1p-11f;  // 2^-kWeightShift
@@ -424,10 +425,12 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
 // value_turn), so that the operands' reads of 8 and of 16 rows meet no bank twice.
 // SPLIT groups of such waves take blocks in turn and merge in LDS at the end.
 //
-// The vector units bound it (60% busy: 32 weights and 64 conversions a lane and block
-// beside 32 matrix instructions of 16 cycles), so with heads of 64 the products of the
-// next block are issued beside this one's weights.  2 x 512 tokens behind 7680, 16 / 4
-// heads: heads of 64 63 us, 33.3 GFLOP at 530 TFLOP/s; heads of 128 110 us, 605 TFLOP/s.
+// The vector units bound it (busy 75% of the time, 32 weights and 64 conversions a
+// lane and block; the matrix cores 25%, 16 instructions of 32 cycles), so with heads of
+// 64 the products of the next block are issued beside this one's weights.  2 x 512
+// tokens behind 7680, 16 / 4 heads: heads of 64 62 us, 33.3 GFLOP at 540 TFLOP/s; heads
+// of 128 95 us, 700 TFLOP/s (107 with a row's maximum asked for in every block, which
+// left too few registers).
 template <int D>
 __device__ __forceinline__ int key_turn(int t) {
   return D == 64 ? (((t >> 1) ^ (t >> 2)) & 1) | (((t >> 5) & 1) << 1)
@@ -436,7 +439,7 @@ __device__ __forceinline__ int key_turn(int t) {
 __device__ __forceinline__ int value_turn(int d) { return (((d >> 1) ^ (d >> 3)) & 1) | (((d >> 2) & 1) << 1); }
 
 template <typename T, int D, int SPLIT, int ROWS>
-__global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_attention_kernel(const AttentionArgs a) {
   typedef typename Vec8<T>::type V8;
   constexpr int WAVES = SPLIT * ROWS;
   constexpr int PAIRS = D / 32;      // 16-byte parts of a key row a lane
@@ -444,8 +447,10 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
   constexpr int BYTES = kBlockTokens * D;  // of a block's keys, and of its values
   constexpr int LOADS = BYTES / 1024;      // wave loads of them
   constexpr int PITCH = 36;
-  // Heads of 128 leave no registers for the scores of two blocks.
+  // Heads of 128 leave no registers for the scores of two blocks.  (The bound of 256
+  // registers keeps two waves a SIMD.)
   constexpr bool AHEAD = D == 64;
+  static_assert(!AHEAD || 2 * PAIRS == 4, "a part of the next scores beside every eight weights");
   static_assert(LOADS % ROWS == 0, "every wave loads the same number of parts");
   union Shared {
     uint8_t block[SPLIT][4][BYTES];  // keys and values, twice
@@ -551,11 +556,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
     for (int f = 0; f < FEATURES; ++f) out[f] *= change;
     most = now;
   };
-  auto weigh = [&](f32x16 (&s)[2], float factor) {
-    const float shift = kWeightShift - (most == -INFINITY ? 0.0f : most);
-#pragma unroll
-    for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = exp2_fast(fmaf(s[r / 16][r % 16], factor, shift));
-  };
+  auto shift_of = [&] { return kWeightShift - (most == -INFINITY ? 0.0f : most); };
 
   // This wave's part of the loads of a block's keys or values: slots of 16 bytes, its
   // lane's one each.
@@ -576,35 +577,29 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
   auto load_keys = [&](int page, int buffer) { load_part(page, buffer, std::false_type{}); };
   auto load_values = [&](int page, int buffer) { load_part(page, buffer, std::true_type{}); };
 
-  // Scores of the block in a buffer.
-  auto score = [&](f32x16 (&s)[2], int buffer) {
-    const uint8_t* keys = shared.block[split][buffer * 2];
+  // Scores of the block in a buffer, 32 tokens times 32 features at once.
+  auto score_part = [&](f32x16 (&s)[2], int buffer, int part) {
+    const int t = part / PAIRS, c = part % PAIRS;
+    const int key = ((column >> 2) & 1) * 32 + t * 16 + (column >> 3) * 4 + (column & 3);
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(&shared.block[split][buffer * 2][0] + key * D +
+                                                      ((c * 2 + half) ^ key_turn<D>(key)) * 16);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key = ((column >> 2) & 1) * 32 + t * 16 + (column >> 3) * 4 + (column & 3);
-#pragma unroll
-      for (int c = 0; c < PAIRS; ++c) {
-        const u32x4 raw = *reinterpret_cast<const u32x4*>(keys + key * D + ((c * 2 + half) ^ key_turn<D>(key)) * 16);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          s[t] = mfma32(e4m3_operand<T>(raw[2 * e], raw[2 * e + 1], 1.0f), q[c][e], c + e == 0 ? (f32x16)(0.0f) : s[t]);
-      }
-    }
+    for (int e = 0; e < 2; ++e)
+      s[t] = mfma32(e4m3_operand<T>(raw[2 * e], raw[2 * e + 1], 1.0f), q[c][e], c + e == 0 ? (f32x16)(0.0f) : s[t]);
   };
-  f16x8 p[4];
-  auto add_up = [&](const f32x16 (&s)[2]) {  // the weights in fp16, and their sums
+  auto score = [&](f32x16 (&s)[2], int buffer) {
+#pragma unroll
+    for (int part = 0; part < 2 * PAIRS; ++part) score_part(s, buffer, part);
+  };
+  // Eight weights of the lane in fp16, and their sum.
+  auto weigh_part = [&](const f32x16 (&s)[2], int u, float factor, float shift, f16x8& p) {
     const f16x2 ones = {(f16)1.0f, (f16)1.0f};
-    float sums[4];
+    float added = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int e = 0; e < 8; ++e) p[e] = (f16)exp2_fast(fmaf(s[u / 2][u % 2 * 8 + e], factor, shift));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[u][e] = (f16)s[u / 2][u % 2 * 8 + e];
-      sums[u] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; e += 2)
-        sums[u] = __builtin_amdgcn_fdot2((f16x2){p[u][e], p[u][e + 1]}, ones, sums[u], false);
-    }
-    sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    for (int e = 0; e < 8; e += 2) added = __builtin_amdgcn_fdot2((f16x2){p[e], p[e + 1]}, ones, added, false);
+    return added;
   };
   auto value_operand = [&](int buffer, int f, int u, float scale) {
     const int d = f * 32 + column;
@@ -651,41 +646,54 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
     const float factor =
         fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(key_scales), i)) * a.scale_log2, 1.17549435e-38f);
     const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
-    const float top = largest(s, factor);
+    const float ratio = power_ratio(scale_bits, unit);
+    f16x8 p[4];
+    bool done = false;
     // Nearly all blocks: seen whole, no base or unit to raise, codes times the ratio of
-    // scales exact in fp16.  They have a copy of their own without branches, in which the
-    // outputs stay where they are and the next block's products run beside the weights.
-    if (seen && held && whole && !__any(top > most + kWeightMargin) && scale_bits <= unit &&
-        power_ratio(scale_bits, unit) >= 0x1p-15f) {
-      if (AHEAD) score(next, (i + 1) & 1);
-      weigh(s, factor);
-      add_up(s);
-      const float ratio = power_ratio(scale_bits, unit);
+    // scales exact in fp16.  The next block's products run beside the weights, and the
+    // row's maximum is not asked for: a weight that left fp16's range is infinite, and so
+    // is the sum.  Then the block is done again below.
+    if (seen && held && whole && scale_bits <= unit && ratio >= 0x1p-15f) {
+      const float shift = shift_of();
+      float added[4];
 #pragma unroll
-      for (int f = 0; f < FEATURES; ++f)
+      for (int u = 0; u < 4; ++u) {
+        if (AHEAD) score_part(next, (i + 1) & 1, u);
+        added[u] = weigh_part(s, u, factor, shift, p[u]);
+      }
+      const float all = (added[0] + added[1]) + (added[2] + added[3]);
+      if (!__any(!(all < INFINITY))) {
+        sum += all;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) out[f] = mfma32(value_operand(i & 1, f, u, ratio), p[u], out[f]);
-    } else {
-      if (seen && !held) {  // a page outside the cache
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int f = 0; f < FEATURES; ++f) out[f] = mfma32(value_operand(i & 1, f, u, ratio), p[u], out[f]);
+        done = true;
+      }
+    } else if (AHEAD) {
+      score(next, (i + 1) & 1);
+    }
+    if (!done && seen) {
+      if (!held) {  // a page outside the cache
         if (sees >= block * kBlockTokens) sum = __builtin_nanf("");
-      } else if (seen) {
+      } else {
         if (!whole) hide(s, block);
-        const float row_top = whole ? top : largest(s, factor);
-        if (__any(row_top > most + kWeightMargin)) raise_base(row_top);
-        weigh(s, factor);
-        add_up(s);
+        const float top = largest(s, factor);
+        if (__any(top > most + kWeightMargin)) raise_base(top);
+        const float shift = shift_of();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum += weigh_part(s, u, factor, shift, p[u]);
         raise_unit(scale_bits);
-        const float ratio = power_ratio(scale_bits, unit);
+        const float to_unit = power_ratio(scale_bits, unit);
 #pragma unroll
         for (int f = 0; f < FEATURES; ++f) {
           f32x16 add = (f32x16)(0.0f);
 #pragma unroll
           for (int u = 0; u < 4; ++u) add = mfma32(value_operand(i & 1, f, u, 1.0f), p[u], add);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) out[f][r] = fmaf(add[r], ratio, out[f][r]);
+          for (int r = 0; r < 16; ++r) out[f][r] = fmaf(add[r], to_unit, out[f][r]);
         }
       }
-      if (AHEAD) score(next, (i + 1) & 1);
     }
     if (i + 2 < here) {
       wait_lds();
@@ -750,13 +758,13 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64) void chunk_attention_kernel(cons
     hide(s, tail_block);
     const float top = largest(s, factor);
     if (__any(top > most + kWeightMargin)) raise_base(top);
-    weigh(s, factor);
+    const float shift = shift_of();
     V8 p[4], rest[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float weight = s[u / 2][u % 2 * 8 + e];
+        const float weight = exp2_fast(fmaf(s[u / 2][u % 2 * 8 + e], factor, shift));
         sum += weight;
         const float w = weight * (WIDE ? kUnshift : 1.0f);
         p[u][e] = (T)w;
@@ -935,7 +943,7 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
   // / four: 64 x 2000 14.6 / 20.1, 64 x 8000 49.6 / 54.8; 8 x 20000 28.4 / 25.2, 4 x
   // 100000 160 / 142).  Heads of 128 have the registers for one block's scores, and more
   // to gain from blocks shared by four waves of other rows (2 x 512 rows behind 7680
-  // tokens, 16 / 4 heads: heads of 128 123 / 111 shared, heads of 64 63 / 66).
+  // tokens, 16 / 4 heads: heads of 128 112 / 95 shared, heads of 64 62 / 68).
   l.split = l.wave_rows == 16 && blocks <= 128 ? 8 : 4;
   l.rows = 1;
   if (head_dim == 128 && rows > 64) {

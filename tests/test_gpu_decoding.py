@@ -442,6 +442,20 @@ def test_blocks_of_very_different_sizes(gpu_device):
     _check_attention(t, _rand((1, 3, 329, 64), 97, BF16), [0], [329], rows=[0, 63, 64, 127, 200, 255, 256, 328])
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (64, F16), (128, BF16)])
+@pytest.mark.parametrize("seq", [1, 5, 40])
+def test_scores_that_grow_and_fall_along_the_history(gpu_device, seq, dim, dtype):
+    """Every block's largest scores far above all before it, then far below."""
+
+    sizes = (0.25, 1.0, 3.0, 8.0, 20.0, 40.0, 1.0, 0.1, 60.0, 2.0)
+    length = 64 * len(sizes) * 5 + 7
+    t = _Tokens(gpu_device, [length, length - 70], 1, dim, dtype, seed=241)
+    for block in range(length // 64):
+        t.key[:, :, 64 * block : 64 * block + 64] *= sizes[block // 5]
+    t.fill()
+    _check_attention(t, _rand((2, 4, seq, dim), 242, dtype), [length - seq, length - 70 - seq], rows=[0, seq - 1], max_length=1)
+
+
 def test_strided_queries_and_broadcast_heads(gpu_device):
     from solution.kernels.attention import hip_block_cache_attention
 
