@@ -63,7 +63,7 @@ struct AttentionArgs {
   const int32_t* starts;
   const int32_t* counts;
   float* partial;     // [batch, seq, heads, chunks, D]
-  float* statistics;  // [batch, seq, heads, chunks, 2]: maximum, sum
+  float* statistics;  // [batch, seq, heads, chunks, 2]: base, sum
   int64_t q_sb, q_sh, q_ss, o_sb, o_ss;
   int64_t blocks, max_blocks;
   int seq_len, heads, kv_heads, group;
