@@ -473,6 +473,28 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   const int chunk = common((int)(at % (uint32_t)a.chunks));
   const uint32_t group_row = (uint32_t)common((int)(at / (uint32_t)a.chunks)) * (ROWS * 32);  // rows are below 2^31
 
+  // The queries and this wave's first table entries are asked for before its lengths
+  // are known; those that do not count are not used.
+  const uint32_t first_row = group_row + row_wave * 32;
+  const uint32_t row = first_row + column;
+  const int token = (int)(row / (uint32_t)a.group);
+  V8 q[PAIRS][2];
+  u32x4 loaded[PAIRS][2];
+#pragma unroll
+  for (int c = 0; c < PAIRS; ++c)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      loaded[c][e] = (u32x4){0u, 0u, 0u, 0u};
+      if (token < a.seq_len) {
+        const int head = h * a.group + (int)(row - (uint32_t)token * (uint32_t)a.group);
+        loaded[c][e] = load16(static_cast<const T*>(a.query) + b * a.q_sb + head * a.q_sh + token * a.q_ss + c * 32 + half * 16 + e * 8);
+      }
+    }
+  const int first_block = chunk * SPLIT + split, stride = a.chunks * SPLIT;
+  int first_pages = -1;
+  if (first_block + (int64_t)lane * stride < a.max_blocks)
+    first_pages = a.table[b * a.max_blocks + first_block + (int64_t)lane * stride];
+
   const int64_t start = common(a.starts[b]);
   int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
   if (count > a.seq_len) count = a.seq_len;
@@ -487,33 +509,23 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
     const int high = common((int)((first + rows - 1) / (uint32_t)a.group));
     return low < count ? first_position + (high < count ? high : count - 1) : -1;
   };
-  const uint32_t first_row = group_row + row_wave * 32;
   const int last_position = last_of(first_row, 32);
   const int group_last = last_of(group_row, ROWS * 32);
   const int least_position = first_position + common((int)(first_row / (uint32_t)a.group));
-  const uint32_t row = first_row + column;
-  const int token = (int)(row / (uint32_t)a.group);
   const bool live = token < count;
   const int sees = live ? first_position + token : last_position;
-  V8 q[PAIRS][2];
 #pragma unroll
   for (int c = 0; c < PAIRS; ++c)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      u32x4 raw = {0u, 0u, 0u, 0u};
-      if (live) {
-        const int head = h * a.group + (int)(row - (uint32_t)token * (uint32_t)a.group);
-        raw = load16(static_cast<const T*>(a.query) + b * a.q_sb + head * a.q_sh + token * a.q_ss + c * 32 + half * 16 + e * 8);
-        raw = (raw ^ a.sign) & a.keep;
-      }
-      q[c][e] = __builtin_bit_cast(V8, raw);
+      const u32x4 raw = (loaded[c][e] ^ a.sign) & a.keep;
+      q[c][e] = __builtin_bit_cast(V8, live ? raw : (u32x4){0u, 0u, 0u, 0u});
     }
 
   // The groups of all chunks take the blocks that the workgroup's rows see in turn; all
   // groups of a workgroup do as many turns, the last ones perhaps without a block.
   const int all_blocks = group_last < 0 || beyond ? 0 : group_last / kBlockTokens + 1;
   const int coded_to = all_blocks < tail_block ? all_blocks : tail_block;
-  const int first_block = chunk * SPLIT + split, stride = a.chunks * SPLIT;
   const int turns = coded_to > chunk * SPLIT ? (coded_to - chunk * SPLIT + stride - 1) / stride : 0;
 
   f32x16 out[FEATURES];
@@ -614,8 +626,9 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   float key_scales = 0.0f, value_scales = 0.0f;
   auto look_up = [&](int first) {
     const int64_t mine = first_block + (int64_t)(first + lane) * stride;
-    pages = -1;
-    if (mine < coded_to) pages = a.table[b * a.max_blocks + mine];
+    pages = first == 0 ? first_pages : -1;
+    if (first != 0 && mine < coded_to) pages = a.table[b * a.max_blocks + mine];
+    if (mine >= coded_to) pages = -1;
     if (pages < 0 || pages >= a.blocks) pages = -1;
     if (pages >= 0) {
       key_scales = a.key_scales[(int64_t)pages * a.kv_heads + h];
@@ -797,7 +810,8 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
     stats[wave][column][1] = sum;
   }
   for (int f = 0; f < FEATURES; ++f) {
-    __syncthreads();  // the blocks, or the last tile, are read
+    wait_lds();  // (a full barrier would wait for the last tile's stores)
+    tile_barrier();  // the blocks, or the last tile, are read
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       f32x4 v;
@@ -810,7 +824,8 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
       }
       *reinterpret_cast<f32x4*>(&shared.part[wave][column * PITCH + k * 8 + half * 4]) = v;
     }
-    __syncthreads();
+    wait_lds();
+    tile_barrier();
     for (int i = split * 64 + lane; i < 32 * 8; i += SPLIT * 64) {
       const int r = i / 8, feature = i % 8 * 4;
       float top = -INFINITY, total = 0.0f;
@@ -935,29 +950,54 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
   const int64_t rows = seq_len * group;
   const int64_t blocks = max_length / kBlockTokens + 1;
   l.wave_rows = rows <= 16 ? 16 : 32;
+  l.rows = 1;
   // waves that the registers leave room for, on all compute units
   const int64_t room = (int64_t)kUnits * 4 * (head_dim == 64 && l.wave_rows == 16 ? 3 : 2);
-  // The waves of a workgroup split the tokens, which leaves fewer parts to merge through
-  // memory.  Eight of them do in one launch what four leave to a second one, but leave
-  // registers unused with heads of 64 (tokens of a sequence, us with both launches, eight
-  // / four: 64 x 2000 14.6 / 20.1, 64 x 8000 49.6 / 54.8; 8 x 20000 28.4 / 25.2, 4 x
-  // 100000 160 / 142).  Heads of 128 have the registers for one block's scores, and more
-  // to gain from blocks shared by four waves of other rows (2 x 512 rows behind 7680
-  // tokens, 16 / 4 heads: heads of 128 112 / 95 shared, heads of 64 62 / 68).
-  l.split = l.wave_rows == 16 && blocks <= 128 ? 8 : 4;
-  l.rows = 1;
-  if (head_dim == 128 && rows > 64) {
-    l.split = 2;
-    l.rows = 4;
+  if (l.wave_rows == 16) {
+    // The waves of a workgroup split the tokens, which leaves fewer parts to merge
+    // through memory.  Eight of them do in one launch what four leave to a second one,
+    // but leave registers unused with heads of 64 (tokens of a sequence, us with both
+    // launches, eight / four: 64 x 2000 14.6 / 20.1, 64 x 8000 49.6 / 54.8; 8 x 20000
+    // 28.4 / 25.2, 4 x 100000 160 / 142).
+    l.split = blocks <= 128 ? 8 : 4;
+    l.row_groups = 1;
+    int64_t chunks = room / (batch * kv_heads * l.split);
+    // A wave has at least four blocks (1 x 1000 tokens 6.7, with two blocks and a second
+    // launch 19.9).
+    const int64_t most = ceil_div(blocks, 4 * l.split);
+    if (chunks > most) chunks = most;
+    l.chunks = chunks < 1 ? 1 : (int)chunks;
+    return l;
   }
-  l.row_groups = ceil_div(rows, (int64_t)l.wave_rows * l.rows);
-  int64_t chunks = room / (batch * kv_heads * l.row_groups * l.rows * l.split);
-  // A wave has at least four blocks (1 x 1000 tokens 6.7, with two blocks and a second
-  // launch 19.9).
-  const int64_t most = ceil_div(blocks, 4 * l.split);
-  if (chunks > most) chunks = most;
-  if (chunks < 1) chunks = 1;
-  l.chunks = (int)chunks;
+  // Heads of 128 have the registers for one block's scores only, and more to gain from
+  // blocks shared by four waves of other rows (2 x 512 rows behind 7680 tokens, 16 / 4
+  // heads: heads of 128 112 / 95 shared, heads of 64 62 / 68).
+  const bool shared = head_dim == 128 && rows > 64;
+  if (shared) l.rows = 4;
+  l.row_groups = ceil_div(rows, (int64_t)32 * l.rows);
+  const int64_t waves = batch * kv_heads * l.row_groups * l.rows;
+  // Rows' waves split their tokens to fill the units, further over workgroups with a
+  // second launch.  In blocks of 64 tokens, 2 us each: a wave's start and end cost six,
+  // the second launch five and its parts' way through memory.  (24 x 479 rows behind 225
+  // to 445, 8 heads of 64: one wave 46 us, four 64; 2 x 512 rows behind 7680 as above: two
+  // waves and a second launch 72, four 62; 3 x 394, 12 / 1 heads of 128 behind 73 to 359:
+  // one launch 28, two 33.)
+  double least = INFINITY;
+  for (int split = shared ? 2 : 4; split >= (head_dim == 128 && !shared ? 4 : 1); split /= 2) {
+    int64_t most = room / (waves * split);
+    if (most > ceil_div(blocks, 4 * split)) most = ceil_div(blocks, 4 * split);
+    for (int second = 0; second < (most > 1 ? 2 : 1); ++second) {
+      const int64_t chunks = second ? most : 1;
+      const double parts = (double)split * (double)chunks, rounds = (double)waves * parts / (double)room;
+      double cost = (rounds > 1.0 ? rounds : 1.0) * (6.0 + (double)blocks / parts);
+      if (second) cost += 5.0 + (double)(batch * rows * kv_heads * chunks * head_dim) * 8.0 / 9.8e6;
+      if (cost < least) {
+        least = cost;
+        l.split = split;
+        l.chunks = (int)chunks;
+      }
+    }
+  }
   return l;
 }
 
@@ -969,10 +1009,20 @@ int launch_attention(AttentionArgs& a, const Layout& l, int64_t batch, unsigned 
       hipLaunchKernelGGL((cached_attention_kernel<T, D, 8>), blocks, threads, 0, stream, a);
     else
       hipLaunchKernelGGL((cached_attention_kernel<T, D, 4>), blocks, threads, 0, stream, a);
-  } else if (l.rows == 1) {
-    hipLaunchKernelGGL((chunk_attention_kernel<T, D, 4, 1>), blocks, threads, 0, stream, a);
+  } else if constexpr (D == 64) {
+    if (l.split == 1)
+      hipLaunchKernelGGL((chunk_attention_kernel<T, D, 1, 1>), blocks, threads, 0, stream, a);
+    else if (l.split == 2)
+      hipLaunchKernelGGL((chunk_attention_kernel<T, D, 2, 1>), blocks, threads, 0, stream, a);
+    else
+      hipLaunchKernelGGL((chunk_attention_kernel<T, D, 4, 1>), blocks, threads, 0, stream, a);
   } else {
-    if constexpr (D == 128) hipLaunchKernelGGL((chunk_attention_kernel<T, D, 2, 4>), blocks, threads, 0, stream, a);
+    if (l.rows == 1)
+      hipLaunchKernelGGL((chunk_attention_kernel<T, D, 4, 1>), blocks, threads, 0, stream, a);
+    else if (l.split == 2)
+      hipLaunchKernelGGL((chunk_attention_kernel<T, D, 2, 4>), blocks, threads, 0, stream, a);
+    else
+      hipLaunchKernelGGL((chunk_attention_kernel<T, D, 1, 4>), blocks, threads, 0, stream, a);
   }
   int status = check_hip(hipGetLastError(), "cached attention launch");
   if (status != SAH_OK || l.chunks == 1) return status;

@@ -415,6 +415,18 @@ def test_chunks_over_ragged_histories(gpu_device, seq, heads, kv_heads, dim, dty
     _check_attention(t, query, starts, counts, rows=rows)
 
 
+@pytest.mark.parametrize("batch", [20, 64])
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (64, F16)])
+def test_chunks_of_many_rows_over_short_histories(gpu_device, batch, dim, dtype):
+    """Rows that fill the card: one or two waves share a row's tokens."""
+
+    seq = 100
+    starts = [(37 * b) % 131 for b in range(batch)]
+    counts = [seq if b % 3 else (b * 7) % (seq + 1) for b in range(batch)]
+    t = _Tokens(gpu_device, [a + b for a, b in zip(starts, counts)], 8, dim, dtype, seed=251).fill()
+    _check_attention(t, _rand((batch, 8, seq, dim), 252, dtype), starts, counts, rows=[0, 31, 57, 99])
+
+
 @pytest.mark.parametrize("max_length", [None, 1, 500, 5000])
 @pytest.mark.parametrize("seq", [1, 20, 80])
 def test_long_histories_in_parts(gpu_device, seq, max_length):
