@@ -450,11 +450,12 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   // Heads of 128 leave no registers for the scores of two blocks.  (The bound of 256
   // registers keeps two waves a SIMD.)
   constexpr bool AHEAD = D == 64;
+  constexpr int TILES = D == 64 ? FEATURES : 1;  // that leave together
   static_assert(!AHEAD || 2 * PAIRS == 4, "a part of the next scores beside every eight weights");
   static_assert(LOADS % ROWS == 0, "every wave loads the same number of parts");
   union Shared {
     uint8_t block[SPLIT][4][BYTES];  // keys and values, twice
-    float part[WAVES][32 * PITCH];
+    float part[WAVES][TILES][32 * PITCH];
   };
   __shared__ __align__(16) Shared shared;
   __shared__ float stats[WAVES][32][2];
@@ -800,67 +801,72 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
     }
   }
 
-  // Merge and store, 32 features at a time: the group's SPLIT waves of the same rows
-  // weigh their outputs as above, and rows leave in runs of 32 features.
+  // Merge and store: the SPLIT waves of the same rows weigh their outputs by their share
+  // of the row's sum, as above, and their sums leave in runs of 32 features.
   sum += __shfl_xor(sum, 32);
-  const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
-  const float unit_value = __int_as_float(unit);
   if (half == 0) {
     stats[wave][column][0] = most;
     stats[wave][column][1] = sum;
   }
-  for (int f = 0; f < FEATURES; ++f) {
-    wait_lds();  // (a full barrier would wait for the last tile's stores)
-    tile_barrier();  // the blocks, or the last tile, are read
+  __syncthreads();  // also: the blocks are read
+  float top = -INFINITY, total = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f32x4 v;
+  for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, stats[w * ROWS + row_wave][column][0]);
+  const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float x = out[0][k * 4 + j];
+  for (int w = 0; w < SPLIT; ++w) {
+    const float part_sum = stats[w * ROWS + row_wave][column][1];
+    total += part_sum != 0.0f ? part_sum * exp2_fast(stats[w * ROWS + row_wave][column][0] - base) : 0.0f;
+  }
+  const float share = sum != 0.0f && total != 0.0f ? exp2_fast(most - base) / total : 0.0f;
+  const float unit_value = __int_as_float(unit);
+  if (a.chunks > 1 && split == 0 && half == 0 && token < a.seq_len) {
+    const int head = h * a.group + (int)(row - (uint32_t)token * (uint32_t)a.group);
+    const int64_t place = ((b * a.seq_len + token) * a.heads + head) * a.chunks + chunk;
+    *reinterpret_cast<f32x2*>(a.statistics + place * 2) = (f32x2){top, live ? total : 0.0f};
+  }
+  for (int pass = 0; pass < FEATURES / TILES; ++pass) {
+    if (pass != 0) __syncthreads();  // the last tiles are read
 #pragma unroll
-        for (int g = 1; g < FEATURES; ++g) x = f == g ? out[g][k * 4 + j] : x;
-        v[j] = x * inverse * unit_value;
+    for (int f = 0; f < TILES; ++f)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = out[f][k * 4 + e];
+#pragma unroll
+          for (int g = 1; g < FEATURES / TILES; ++g) x = pass == g ? out[g * TILES + f][k * 4 + e] : x;
+          v[e] = x * share * unit_value;
+        }
+        *reinterpret_cast<f32x4*>(&shared.part[wave][f][column * PITCH + k * 8 + half * 4]) = v;
       }
-      *reinterpret_cast<f32x4*>(&shared.part[wave][column * PITCH + k * 8 + half * 4]) = v;
-    }
-    wait_lds();
-    tile_barrier();
+    __syncthreads();
+#pragma unroll
     for (int i = split * 64 + lane; i < 32 * 8; i += SPLIT * 64) {
       const int r = i / 8, feature = i % 8 * 4;
-      float top = -INFINITY, total = 0.0f;
-#pragma unroll
-      for (int w = 0; w < SPLIT; ++w) top = fmaxf(top, stats[w * ROWS + row_wave][r][0]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      f32x4 merged = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int w = 0; w < SPLIT; ++w) {
-        const float part_sum = stats[w * ROWS + row_wave][r][1];
-        const float weight = part_sum != 0.0f ? part_sum * exp2_fast(stats[w * ROWS + row_wave][r][0] - base) : 0.0f;
-        total += weight;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(&shared.part[w * ROWS + row_wave][r * PITCH + feature]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) merged[j] = fmaf(v[j], weight, merged[j]);
-      }
-      const float scale = total != 0.0f ? 1.0f / total : 0.0f;
       const uint32_t its_row = first_row + r;
       const int its_token = (int)(its_row / (uint32_t)a.group);
       const int head = h * a.group + (int)(its_row - (uint32_t)its_token * (uint32_t)a.group);
       if (its_token >= a.seq_len) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) merged[j] = its_token < count ? merged[j] * scale : 0.0f;  // rows without a query
-      if (a.chunks == 1) {
-        typename Vec8<T>::half_type v;
+      for (int f = 0; f < TILES; ++f) {
+        f32x4 merged = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (its_token < count) {  // rows without a query stay zeros
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (T)merged[j];
-        *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + its_token * a.o_ss +
-                                                        (int64_t)head * D + f * 32 + feature) = v;
-      } else {
-        const int64_t place = ((b * a.seq_len + its_token) * a.heads + head) * a.chunks + chunk;
-        *reinterpret_cast<f32x4*>(a.partial + place * D + f * 32 + feature) = merged;
-        if (f == 0 && feature == 0) {
-          a.statistics[place * 2] = top;
-          a.statistics[place * 2 + 1] = its_token < count ? total : 0.0f;
+          for (int w = 0; w < SPLIT; ++w)
+            merged += *reinterpret_cast<const f32x4*>(&shared.part[w * ROWS + row_wave][f][r * PITCH + feature]);
+        }
+        const int at = (pass * TILES + f) * 32 + feature;
+        if (a.chunks == 1) {
+          typename Vec8<T>::half_type v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (T)merged[e];
+          *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + its_token * a.o_ss +
+                                                          (int64_t)head * D + at) = v;
+        } else {
+          const int64_t place = ((b * a.seq_len + its_token) * a.heads + head) * a.chunks + chunk;
+          *reinterpret_cast<f32x4*>(a.partial + place * D + at) = merged;
         }
       }
     }
