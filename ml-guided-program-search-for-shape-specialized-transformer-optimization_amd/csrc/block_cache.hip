@@ -263,7 +263,7 @@ __device__ __forceinline__ T held_value(float code, float scale) {
 // HBM-bound: codes are read once, 16-bit keys and values written once.  A workgroup
 // takes one block of (sequence, head), whose values turn in LDS, a feature's tokens an
 // odd number of places apart, on their way to the output's rows:
-//   4 x 8001 tokens, 8 heads of 128, fp16 (197 MB): 40 us, 4.9 TB/s (41.5 with features
+//   4 x 8001 tokens, 8 heads of 128, fp16 (197 MB): 39 us, 5.0 TB/s (41 with features
 //   68 places apart); 64 x 64 tokens, 16 heads of 64: 8.4 us
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void block_read_kernel(const ReadArgs a) {

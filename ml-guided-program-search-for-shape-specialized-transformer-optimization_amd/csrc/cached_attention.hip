@@ -428,7 +428,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
 // The vector units bound it (busy 75% of the time, 32 weights and 64 conversions a
 // lane and block; the matrix cores 25%, 16 instructions of 32 cycles), so with heads of
 // 64 the products of the next block are issued beside this one's weights.  2 x 512
-// tokens behind 7680, 16 / 4 heads: heads of 64 62 us, 33.3 GFLOP at 540 TFLOP/s; heads
+// tokens behind 7680, 16 / 4 heads: heads of 64 61 us, 33.3 GFLOP at 545 TFLOP/s; heads
 // of 128 95 us, 700 TFLOP/s (107 with a row's maximum asked for in every block, which
 // left too few registers).
 template <int D>
