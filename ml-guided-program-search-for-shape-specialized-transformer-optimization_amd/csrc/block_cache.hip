@@ -77,7 +77,8 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
 // are read at the same time, and past the caches:
 //   4 x 8001 tokens, 8 heads of 128, fp16 (197 MB): 41 us, 4.7 TB/s (48 through the
 //   caches); 8 x 4001 tokens, 16 heads of 64: 43 us (66 block by block of a head)
-//   64 x 1 token, 16 heads of 64: 4.0 us, 6.4 where some blocks are completed
+//   33 x 1 token, 8 heads of 128: 3.3 us, 6.3 where a block is completed (8.6 with the
+//   tail's values read token by token); 52 x 43 tokens: 16 us (25)
 //
 // One workgroup takes one block of (sequence, head): it codes the block if the
 // append completes it, from the tail's old tokens and the new ones.  The first
@@ -91,7 +92,11 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
   constexpr int PASSES = kBlockTokens / TOKENS;
   constexpr int ROW = kBlockTokens + 4;        // bytes of a feature in LDS: features on different banks
   __shared__ float largest_of[2][kThreads / 64];
-  __shared__ __align__(4) uint8_t turned[D * ROW];
+  constexpr int WIDE_ROW = kBlockTokens + 1;   // values of a feature in LDS, an odd number
+  __shared__ __align__(16) union {
+    uint8_t codes[D * ROW];
+    T values[D * WIDE_ROW];
+  } turned;
 
   const uint32_t pair = blockIdx.x / (uint32_t)a.cache.heads;
   const int h = (int)(blockIdx.x - pair * (uint32_t)a.cache.heads);
@@ -133,6 +138,18 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
     V8 k[PASSES], v[PASSES];
     bool bad[PASSES];
     float k_largest = 0.0f, v_largest = 0.0f;
+    if (index == 0 && start % kBlockTokens != 0) {  // the tail's values turn in LDS
+      const int old = (int)(start % kBlockTokens);
+#pragma unroll
+      for (int i = tid; i < D * 8; i += kThreads) {
+        const int slot = i % 8 * 8;
+        if (slot >= old) continue;
+        const V8 part = *reinterpret_cast<const V8*>(value_tail + i * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) turned.values[i / 8 * WIDE_ROW + slot + e] = part[e];
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int slot = token0 * PASSES + p;
@@ -140,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
       if (position < start) {  // index 0 only: an older token of this block
         k[p] = *reinterpret_cast<const V8*>(key_tail + slot * D + feature);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[p][e] = value_tail[(feature + e) * kBlockTokens + slot];
+        for (int e = 0; e < 8; ++e) v[p][e] = turned.values[(feature + e) * WIDE_ROW + slot];
       } else {
         const int64_t at = position - start;
         k[p] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(key + at * a.k_ss));
@@ -199,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
       uint32_t codes = 0;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) codes |= (value_coded[p][e / 4] >> (8 * (e % 4)) & 0xffu) << (8 * p);
-      uint8_t* to = turned + (feature + e) * ROW + token0 * PASSES;
+      uint8_t* to = turned.codes + (feature + e) * ROW + token0 * PASSES;
       if constexpr (PASSES == 4)
         *reinterpret_cast<uint32_t*>(to) = codes;
       else
@@ -209,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
     if (held) {
 #pragma unroll
       for (int i = tid; i < D * 4; i += kThreads) {
-        const uint32_t* from = reinterpret_cast<const uint32_t*>(turned + (i / 4) * ROW + (i % 4) * 16);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(turned.codes + (i / 4) * ROW + (i % 4) * 16);
         const u32x4 part = {from[0], from[1], from[2], from[3]};
         store16(a.cache.value_codes + code_at + i * 16, part);
       }
@@ -221,24 +238,38 @@ __global__ __launch_bounds__(kThreads) void block_append_kernel(const AppendArgs
   }
 
   // The tail: the new tokens of the last, incomplete block.  Every old token that
-  // the block above needs is in registers (the barriers above).
-  if (index == 0) {
-    const int64_t last = end / kBlockTokens * kBlockTokens;
-    const int64_t from = start > last ? start : last;
-    for (int64_t position = from + token0; position < end; position += TOKENS) {
-      const int slot = (int)(position - last);
-      const int64_t at = position - start;
-      V8 k = *reinterpret_cast<const V8*>(key + at * a.k_ss);
-      V8 v = *reinterpret_cast<const V8*>(value + at * a.v_ss);
-      if (bad_token(k, v)) {  // asked of the lanes of one token, which are here together
+  // the block above needs is in registers (the barriers above).  Values of several
+  // tokens turn in LDS too and leave a feature's tokens side by side.
+  if (index != 0) return;
+  const int64_t last = end / kBlockTokens * kBlockTokens;
+  const int64_t from = start > last ? start : last;
+  const bool several = end - from >= 8;
+  if (several) __syncthreads();  // the codes above are read
+  for (int64_t position = from + token0; position < end; position += TOKENS) {
+    const int slot = (int)(position - last);
+    const int64_t at = position - start;
+    V8 k = *reinterpret_cast<const V8*>(key + at * a.k_ss);
+    V8 v = *reinterpret_cast<const V8*>(value + at * a.v_ss);
+    if (bad_token(k, v)) {  // asked of the lanes of one token, which are here together
 #pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = (T)__builtin_nanf(""), v[e] = (T)0.0f;
-      }
-      *reinterpret_cast<V8*>(key_tail + slot * D + feature) = k;
+      for (int e = 0; e < 8; ++e) k[e] = (T)__builtin_nanf(""), v[e] = (T)0.0f;
+    }
+    *reinterpret_cast<V8*>(key_tail + slot * D + feature) = k;
+    if (several) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) turned.values[(feature + e) * WIDE_ROW + slot] = v[e];
+    } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) value_tail[(feature + e) * kBlockTokens + slot] = v[e];
     }
   }
+  if (!several) return;
+  __syncthreads();
+  const int slot = tid % kBlockTokens;
+  if (slot < from - last || slot >= end - last) return;
+#pragma unroll
+  for (int d = tid / kBlockTokens; d < D; d += kThreads / kBlockTokens)
+    value_tail[d * kBlockTokens + slot] = turned.values[d * WIDE_ROW + slot];
 }
 
 struct ReadArgs {

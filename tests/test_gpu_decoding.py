@@ -253,6 +253,21 @@ def test_cache_does_not_depend_on_the_steps(gpu_device, dtype, dim):
         assert torch.equal(whole.cache.value_tail[b, ..., :n], steps.cache.value_tail[b, ..., :n])
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 64), (BF16, 128)])
+def test_appends_of_few_and_several_tokens(gpu_device, dtype, dim):
+    """Within a block, up to its end, over it and over several, a few tokens and many."""
+
+    steps = [(5, 8), (20, 7), (9, 1), (30, 47), (1, 2), (64, 63), (7, 1), (100, 9), (8, 70), (0, 3), (63, 8), (13, 64)]
+    lengths = [sum(s[b] for s in steps) for b in range(2)]
+    t = _Tokens(gpu_device, lengths, 2, dim, dtype, seed=261)
+    t.key[0, 1, 24, 3], t.value[1, 0, 14, 5] = math.inf, math.nan
+    held = [0, 0]
+    for step in steps:
+        t.append(held, list(step))
+        held = [a + b for a, b in zip(held, step)]
+        t.check(held)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_scales_of_extreme_blocks(gpu_device, dtype):
     t = _Tokens(gpu_device, [64 * 6 + 1], 1, 64, dtype, seed=11)
