@@ -17,8 +17,8 @@
 // that these 16 tokens are neighbours: the value codes, feature by feature in the
 // cache, are then 16 bytes a lane, as the key codes are.  A wave loads its blocks
 // straight into registers, the next block's keys and values as soon as this one's are
-// used; nothing but the final merge goes through LDS.  More than 16 rows (a chunk of
-// tokens) go to a kernel of their own further down.
+// used; nothing but the final merge goes through LDS.  Many rows (a chunk of tokens) go
+// to a kernel of their own further down.
 //
 // Precision.  Codes are exact in both types, so Q K^T takes them in the queries'
 // type; the weights are fp16 (times 2^11, so that none above 2^-25 of the largest is
@@ -121,6 +121,8 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   uint32_t at = blockIdx.x;
   const int chunk = common((int)(at % (uint32_t)a.chunks));
   at /= (uint32_t)a.chunks;
+  const uint32_t group_row = (uint32_t)common((int)(at % a.row_groups)) * 16;
+  at /= a.row_groups;
   const int h = common((int)(at % (uint32_t)a.kv_heads));
   const int64_t b = common((int)(at / (uint32_t)a.kv_heads));
 
@@ -141,9 +143,10 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   const int first_position = beyond ? 0 : (int)start;
   const int tail_block = beyond ? 0 : (int)((start + count) / kBlockTokens);
 
-  // This lane's row: token column / group of the chunk, query head h * group + column % group.
-  const int token = column / a.group;
-  const int head = h * a.group + (column - token * a.group);
+  // This lane's row: token row / group of the chunk, query head h * group + row % group.
+  const uint32_t row = group_row + column;
+  const int token = (int)(row / (uint32_t)a.group);
+  const int head = h * a.group + (int)(row - (uint32_t)token * (uint32_t)a.group);
   const bool live = token < count;
   const int last_position = first_position + count - 1;  // -1 or less: no query
   // The position up to which the row sees; a row without a query sees as far as the last.
@@ -955,10 +958,16 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
   Layout l{};
   const int64_t rows = seq_len * group;
   const int64_t blocks = max_length / kBlockTokens + 1;
-  l.wave_rows = rows <= 16 ? 16 : 32;
   l.rows = 1;
   // waves that the registers leave room for, on all compute units
-  const int64_t room = (int64_t)kUnits * 4 * (head_dim == 64 && l.wave_rows == 16 ? 3 : 2);
+  const int64_t few = (int64_t)kUnits * 4 * (head_dim == 64 ? 3 : 2), room = (int64_t)kUnits * 4 * 2;
+  // A few groups of 16 rows, while eight waves of each fit the units, are done sooner by
+  // the kernel without LDS on the blocks' way than by the one for chunks, which does more
+  // rows a conversion (us, 16 / 32 rows a wave: 19 x 48 rows behind 2944 tokens, 4 key
+  // heads of 128 30.7 / 41.4; 1 x 32 behind 629 9.5 / 13.8; 64 x 40 behind 1000, 8 heads
+  // of 64 49 / 26).
+  l.row_groups = ceil_div(rows, 16);
+  l.wave_rows = rows <= 16 || (rows <= 64 && batch * kv_heads * l.row_groups * 8 <= few) ? 16 : 32;
   if (l.wave_rows == 16) {
     // The waves of a workgroup split the tokens, which leaves fewer parts to merge
     // through memory.  Eight of them do in one launch what four leave to a second one,
@@ -966,8 +975,7 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
     // launches, eight / four: 64 x 2000 14.6 / 20.1, 64 x 8000 49.6 / 54.8; 8 x 20000
     // 28.4 / 25.2, 4 x 100000 160 / 142).
     l.split = blocks <= 128 ? 8 : 4;
-    l.row_groups = 1;
-    int64_t chunks = room / (batch * kv_heads * l.split);
+    int64_t chunks = few / (batch * kv_heads * l.row_groups * l.split);
     // A wave has at least four blocks (1 x 1000 tokens 6.7, with two blocks and a second
     // launch 19.9).
     const int64_t most = ceil_div(blocks, 4 * l.split);

@@ -420,7 +420,7 @@ def test_one_token_over_ragged_histories(gpu_device, heads, kv_heads, dtype, dim
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 4, 64, BF16), (8, 2, 64, F16), (4, 1, 128, BF16), (3, 3, 128, F16)])
-@pytest.mark.parametrize("seq", [2, 5, 17, 33, 70, 150])
+@pytest.mark.parametrize("seq", [2, 5, 17, 33, 64, 70, 150])
 def test_chunks_over_ragged_histories(gpu_device, seq, heads, kv_heads, dim, dtype):
     counts = [seq, 1, max(1, seq // 2), 0, seq]
     starts = [0, 130, 61, 40, 700]
@@ -430,16 +430,15 @@ def test_chunks_over_ragged_histories(gpu_device, seq, heads, kv_heads, dim, dty
     _check_attention(t, query, starts, counts, rows=rows)
 
 
-@pytest.mark.parametrize("batch", [20, 64])
+@pytest.mark.parametrize("batch,seq", [(20, 100), (64, 100), (64, 40)])
 @pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (64, F16)])
-def test_chunks_of_many_rows_over_short_histories(gpu_device, batch, dim, dtype):
+def test_chunks_of_many_rows_over_short_histories(gpu_device, batch, seq, dim, dtype):
     """Rows that fill the card: one or two waves share a row's tokens."""
 
-    seq = 100
     starts = [(37 * b) % 131 for b in range(batch)]
     counts = [seq if b % 3 else (b * 7) % (seq + 1) for b in range(batch)]
     t = _Tokens(gpu_device, [a + b for a, b in zip(starts, counts)], 8, dim, dtype, seed=251).fill()
-    _check_attention(t, _rand((batch, 8, seq, dim), 252, dtype), starts, counts, rows=[0, 31, 57, 99])
+    _check_attention(t, _rand((batch, 8, seq, dim), 252, dtype), starts, counts, rows=[0, 31, 39, 57, 99])
 
 
 @pytest.mark.parametrize("max_length", [None, 1, 500, 5000])
