@@ -254,12 +254,14 @@ __device__ __forceinline__ V8 lds_read_tr16_pair(const void* lo, const void* hi)
 // base + offset land at LDS byte lds + 16 i (base and lds wave-uniform,
 // moved to scalar registers here).  Written as assembly so the compiler does
 // not treat it as an LDS write (it would wait for it before every LDS read);
-// the tile loop waits for it explicitly.
+// the tile loop waits for it explicitly.  A write of m0 needs one wait state before
+// the load that takes its place from it; base comes of scalar arithmetic, whose
+// registers need none.
 __device__ __forceinline__ void dma16(const void* base, uint32_t offset, uint32_t lds) {
   const uint64_t b = (uint64_t)(uintptr_t)base;
   const uint64_t sbase = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
                : "v"(offset), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "memory", "m0");

@@ -33,15 +33,29 @@ constexpr int kTileRowBytes = kTileK * 2;
 
 __device__ __forceinline__ int tile_swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
+// A wave-uniform address in scalar registers.  A vector instruction that writes a
+// scalar register (v_readfirstlane) needs five wait states before a vector memory
+// instruction reads it.  The compiler does not see that the assembly below is one, so
+// where an address may come out of vector registers the states stand here, once.
+__device__ __forceinline__ const char* scalar_base(const void* p) {
+  const uint64_t b = (uint64_t)(uintptr_t)p;
+  uint64_t s = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
+               (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
+  asm volatile("s_nop 4" : "+s"(s));
+  return reinterpret_cast<const char*>((uintptr_t)s);
+}
+
 // One 16-byte direct-to-LDS load per lane: lane i's bytes from base + offset
 // land at LDS byte lds + 16 i (base and lds wave-uniform).  Assembly, so that
 // the compiler does not wait for it before unrelated LDS reads; the loops
-// below wait explicitly.
+// below wait explicitly.  A write of m0 needs one wait state before the load that
+// takes its place from it.  (All five that a base in vector registers would need
+// cost the projections up to 7%: 16384 x 4096 -> 1024 110.8 / 103.9 us.)
 __device__ __forceinline__ void tile_dma16(const void* base, uint32_t offset, uint32_t lds) {
   const uint64_t b = (uint64_t)(uintptr_t)base;
   const uint64_t sbase = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
                : "v"(offset), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "memory", "m0");
@@ -109,12 +123,12 @@ struct GemmTile {
     static_assert(XL % 2 == 0 && WL % 2 == 0, "loads alternate between the two lane offsets");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    xb = reinterpret_cast<const char*>(x);
+    xb = scalar_base(x);
     x_last = (uint32_t)(valid_rows - 1);
     x_stride = (uint32_t)x_ld * 2;
     x_row = wave * XL * 8 + (lane >> 3);
     w_step = (uint32_t)k * 16;
-    wb = reinterpret_cast<const char*>(w) + (int64_t)wave * WL * w_step;
+    wb = scalar_base(reinterpret_cast<const char*>(w) + (int64_t)wave * WL * w_step);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t chunk = (uint32_t)((lane & 7) ^ tile_swizzle(i * 8 + (lane >> 3))) * 16;

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import re
+import subprocess
 from pathlib import Path
 
 import pytest
@@ -367,3 +368,60 @@ def test_linear_sizes_take_the_kernels_they_are_tests_of(kernel):
         assert library.sah_linear_kernel(*case) == kernel, case
     for case in [(0, 64, 256, 0), (1, 32, 256, 0), (1, 64, 128, 0)]:
         assert library.sah_linear_kernel(*case) is None
+
+
+OBJDUMP = Path("/opt/rocm/llvm/bin/llvm-objdump")
+
+
+def _unwaited_direct_loads(listing: str) -> tuple[int, list[str]]:
+    """How many direct-to-LDS loads a listing holds, and those that come too soon: within
+    five wait states of a vector instruction that writes the scalar registers of their
+    address, or none after a write of m0, which names their place in LDS."""
+
+    written = re.compile(r"(?:v_readfirstlane_b32|v_readlane_b32|v_cmp\w*) s\[?(\d+)(?::(\d+))?")
+    load = re.compile(r"global_load_lds_dword\w* v\[?[\d:]+\]?, (?:s\[(\d+):(\d+)\]|off)")
+    count, found, before = 0, [], []  # the instructions before, the last one first
+    for line in listing.splitlines():
+        text = line.split("//")[0].strip()
+        if not text or text.endswith(":"):
+            continue
+        match = load.match(text)
+        if match:
+            count += 1
+            registers = set(range(int(match[1]), int(match[2]) + 1)) if match[1] else set()
+            states = 0
+            for earlier in before:
+                if states == 0 and re.match(r"s_\w+ m0,", earlier):
+                    found.append(f"{earlier}; {text}")
+                name = written.match(earlier)
+                if name and registers & set(range(int(name[1]), int(name[2] or name[1]) + 1)):
+                    found.append(f"{earlier}; {states} wait states; {text}")
+                idle = re.match(r"s_nop (\d+)", earlier)
+                states += int(idle[1]) + 1 if idle else 1
+                if states >= 5:
+                    break
+        before = [text, *before[:4]]
+    return count, found
+
+
+def test_direct_loads_have_their_wait_states(tmp_path):
+    """The compiler keeps no wait states for the loads that the kernels write as assembly."""
+
+    if not OBJDUMP.exists():
+        pytest.skip(f"no {OBJDUMP}")
+    listed = "s_mov_b32 m0, s3\n{}global_load_lds_dwordx4 v1, s[4:5]\n"
+    assert _unwaited_direct_loads(listed.format("s_nop 0\n")) == (1, [])
+    assert len(_unwaited_direct_loads(listed.format(""))[1]) == 1
+    assert len(_unwaited_direct_loads("v_readfirstlane_b32 s5, v0\n" + listed.format("s_nop 0\n"))[1]) == 1
+    assert _unwaited_direct_loads("v_readfirstlane_b32 s5, v0\n" + listed.format("s_nop 3\n")) == (1, [])
+    library = tmp_path / "library.so"
+    library.write_bytes(_library.LIBRARY_PATH.read_bytes())
+    subprocess.run([str(OBJDUMP), "--offloading", str(library)], check=True, capture_output=True, cwd=tmp_path)
+    total = 0
+    for image in sorted(tmp_path.glob("library.so.*gfx950")):
+        options = ("-d", "--no-show-raw-insn", "--no-leading-addr")
+        listing = subprocess.run([str(OBJDUMP), *options, str(image)], check=True, capture_output=True, text=True)
+        count, found = _unwaited_direct_loads(listing.stdout)
+        assert not found, (image.name, len(found), found[:3])
+        total += count
+    assert total > 0
