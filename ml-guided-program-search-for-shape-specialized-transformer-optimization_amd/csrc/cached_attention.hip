@@ -102,10 +102,37 @@ __device__ __forceinline__ float halves_max(float x) {
   return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
 }
 
-// Powers of two by their fp32 bits: 2^a / 2^b, 2^-126 where it is less.
+// Powers of two by their fp32 bits: 2^a / 2^b, 0 where it is below 2^-126.
 __device__ __forceinline__ float power_ratio(int a_bits, int b_bits) {
   const int bits = 0x3f800000 + (a_bits - b_bits);
-  return __int_as_float(bits < 0x00800000 ? 0x00800000 : bits);
+  return __int_as_float(bits < 0x00800000 ? 0 : bits);
+}
+
+// Whether any weight of an operand is not zero.
+template <typename V8>
+__device__ __forceinline__ bool any_weight(const V8 (&p)[2]) {
+  const u32x4 bits = __builtin_bit_cast(u32x4, p[0]) | __builtin_bit_cast(u32x4, p[1]);
+  return ((bits[0] | bits[1]) | (bits[2] | bits[3])) != 0;
+}
+template <typename V8>
+__device__ __forceinline__ bool any_weight(const V8 (&p)[4]) {
+  const u32x4 bits = (__builtin_bit_cast(u32x4, p[0]) | __builtin_bit_cast(u32x4, p[1])) |
+                     (__builtin_bit_cast(u32x4, p[2]) | __builtin_bit_cast(u32x4, p[3]));
+  return ((bits[0] | bits[1]) | (bits[2] | bits[3])) != 0;
+}
+
+// A row's outputs are held in a unit, the largest value scale so far of a block that it
+// has weights in.  Rows of a wave share it (its bits; -1 where they do not), but a row
+// that gives a block no weight, seen or not, does not follow it up by more than 2^60:
+// what it holds would leave fp32.  What a row with a weight there loses is less than
+// 2^-60 of the block's largest value.
+constexpr int kUnitRise = 60 << 23;
+__device__ __forceinline__ bool unit_rises(int unit, int bits, bool weighs) {
+  return bits > unit && (unit == 0 || weighs || bits - unit <= kUnitRise);
+}
+__device__ __forceinline__ int common_unit(int unit) {
+  const int first = common(unit);
+  return __any(unit != first) ? -1 : first;
 }
 
 template <typename T, int D, int SPLIT>
@@ -168,21 +195,24 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   const int all_blocks = count == 0 || beyond ? 0 : last_position / kBlockTokens + 1;
   const int coded_to = all_blocks < tail_block ? all_blocks : tail_block;
 
-  // Outputs are held in units of a power of two, the largest value scale so far.
   f32x4 out[FEATURES];
-  int unit = 0;  // its bits; 0 before the first block
+  int unit = 0;  // the row's, 0 before the first block
+  int wave_unit = 0;
   float most = -INFINITY;
   float sum = beyond && count != 0 ? __builtin_nanf("") : 0.0f;
 #pragma unroll
   for (int f = 0; f < FEATURES; ++f) out[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  auto raise_unit = [&](int bits) {
-    if (bits <= unit) return;
-    if (unit != 0) {
-      const float change = power_ratio(unit, bits);
+  auto raise_unit = [&](int bits, const auto& p) {
+    if (bits <= wave_unit) return;
+    uint64_t weighs = __ballot(any_weight(p));
+    weighs |= weighs >> 32;
+    weighs |= weighs >> 16;
+    const bool rises = unit_rises(unit, bits, (weighs >> column & 1) != 0);
+    const float change = rises ? power_ratio(unit, bits) : 1.0f;  // of nothing, before the first block
 #pragma unroll
-      for (int f = 0; f < FEATURES; ++f) out[f] *= change;
-    }
-    unit = bits;
+    for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+    if (rises) unit = bits;
+    wave_unit = common_unit(unit);
   };
 
   // The weights of the row for one block, from its scores (16 tokens of it in this
@@ -278,21 +308,22 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
 #pragma unroll
           for (int e = 0; e < 8; ++e) p[k][e] = (f16)s[2 * k + e / 4][e % 4];
         const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
-        raise_unit(scale_bits);
-        const float ratio = power_ratio(scale_bits, unit);
-        if (ratio >= 0x1p-15f) {  // codes times the ratio are exact in fp16
+        raise_unit(scale_bits, p);
+        const float ratio = power_ratio(scale_bits, wave_unit);
+        if (scale_bits <= wave_unit && ratio >= 0x1p-15f) {  // codes times the ratio are exact in fp16
 #pragma unroll
           for (int f = 0; f < FEATURES; ++f) {
             out[f] = mfma16(e4m3_operand<f16>(values[f][0], values[f][1], ratio), p[0], out[f]);
             out[f] = mfma16(e4m3_operand<f16>(values[f][2], values[f][3], ratio), p[1], out[f]);
           }
         } else {
+          const float to_unit = power_ratio(scale_bits, unit);
 #pragma unroll
           for (int f = 0; f < FEATURES; ++f) {
             f32x4 add = mfma16(e4m3_operand<f16>(values[f][0], values[f][1], 1.0f), p[0], (f32x4){0.0f, 0.0f, 0.0f, 0.0f});
             add = mfma16(e4m3_operand<f16>(values[f][2], values[f][3], 1.0f), p[1], add);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[f][j] = fmaf(add[j], ratio, out[f][j]);
+            for (int j = 0; j < 4; ++j) out[f][j] = fmaf(add[j], to_unit, out[f][j]);
           }
         }
       } else if (sees >= block * kBlockTokens) {  // a page outside the cache: NaN of every row that sees it
@@ -328,8 +359,6 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
                                                      hh * 64 + kk * 8),
                         q[hh][kk], hh + kk == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : s[r]);
     asm volatile("" ::: "memory");  // the values are under way with the keys
-    raise_unit(SHIFT_BITS);
-    const float ratio = power_ratio(SHIFT_BITS, unit);
     softmax_step(s, fmaxf(a.scale_log2, 1.17549435e-38f), tail_block);
     // bf16 weights keep 16 bits of precision as a sum of two; fp16 ones the shift
     V8 p[2], rest[2];
@@ -341,6 +370,8 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
         p[k][e] = (T)w;
         rest[k][e] = (T)(w - (float)p[k][e]);
       }
+    raise_unit(SHIFT_BITS, p);
+    const float ratio = power_ratio(SHIFT_BITS, unit);
 #pragma unroll
     for (int f = 0; f < FEATURES; ++f) {
       f32x4 add = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -533,19 +564,21 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   const int turns = coded_to > chunk * SPLIT ? (coded_to - chunk * SPLIT + stride - 1) / stride : 0;
 
   f32x16 out[FEATURES];
-  int unit = 0;
+  int unit = 0, wave_unit = 0;
   float most = -INFINITY;
   float sum = beyond && last_position >= 0 ? __builtin_nanf("") : 0.0f;
 #pragma unroll
   for (int f = 0; f < FEATURES; ++f) out[f] = (f32x16)(0.0f);
-  auto raise_unit = [&](int bits) {
-    if (bits <= unit) return;
-    if (unit != 0) {
-      const float change = power_ratio(unit, bits);
+  auto raise_unit = [&](int bits, const auto& p) {
+    if (bits <= wave_unit) return;
+    uint64_t weighs = __ballot(any_weight(p));
+    weighs |= weighs >> 32;
+    const bool rises = unit_rises(unit, bits, (weighs >> column & 1) != 0);
+    const float change = rises ? power_ratio(unit, bits) : 1.0f;
 #pragma unroll
-      for (int f = 0; f < FEATURES; ++f) out[f] *= change;
-    }
-    unit = bits;
+    for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+    if (rises) unit = bits;
+    wave_unit = common_unit(unit);
   };
   // The largest of a row's scores, times the factor (common to the lanes that share it).
   auto largest = [&](const f32x16 (&s)[2], float factor) {
@@ -663,14 +696,14 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
     const float factor =
         fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(key_scales), i)) * a.scale_log2, 1.17549435e-38f);
     const int scale_bits = __builtin_amdgcn_readlane(__float_as_int(value_scales), i);
-    const float ratio = power_ratio(scale_bits, unit);
+    const float ratio = power_ratio(scale_bits, wave_unit);
     f16x8 p[4];
     bool done = false;
     // Nearly all blocks: seen whole, no base or unit to raise, codes times the ratio of
     // scales exact in fp16.  The next block's products run beside the weights, and the
     // row's maximum is not asked for: a weight that left fp16's range is infinite, and so
     // is the sum.  Then the block is done again below.
-    if (seen && held && whole && scale_bits <= unit && ratio >= 0x1p-15f) {
+    if (seen && held && whole && scale_bits <= wave_unit && ratio >= 0x1p-15f) {
       const float shift = shift_of();
       float added[4];
 #pragma unroll
@@ -700,7 +733,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
         const float shift = shift_of();
 #pragma unroll
         for (int u = 0; u < 4; ++u) sum += weigh_part(s, u, factor, shift, p[u]);
-        raise_unit(scale_bits);
+        raise_unit(scale_bits, p);
         const float to_unit = power_ratio(scale_bits, unit);
 #pragma unroll
         for (int f = 0; f < FEATURES; ++f) {
@@ -769,8 +802,6 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
     }
     constexpr int SHIFT_BITS = (127 + (int)kWeightShift) << 23;
     constexpr bool WIDE = std::is_same<T, bf16>::value;
-    raise_unit(SHIFT_BITS);
-    const float ratio = power_ratio(SHIFT_BITS, unit);
     const float factor = fmaxf(a.scale_log2, 1.17549435e-38f);
     hide(s, tail_block);
     const float top = largest(s, factor);
@@ -787,6 +818,8 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
         p[u][e] = (T)w;
         rest[u][e] = (T)(w - (float)p[u][e]);
       }
+    raise_unit(SHIFT_BITS, p);
+    const float ratio = power_ratio(SHIFT_BITS, unit);
 #pragma unroll
     for (int f = 0; f < FEATURES; ++f) {
       f32x16 add = (f32x16)(0.0f);
