@@ -471,41 +471,45 @@ def test_blocks_of_very_different_sizes(gpu_device):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,start,seq", [(1, 13, 150), (3, 5, 140), (2, 50, 90), (1, 40, 300)])
 def test_later_blocks_leave_earlier_rows_alone(gpu_device, heads, start, seq, dim):
-    """Value scales more than 2^126 apart, rows of one wave on both sides of a block's border."""
+    """Value scales more than 2^126 apart, rows of one wave on both sides of a block's
+    border, and 16 blocks before it, so that every wave has met the small values."""
 
+    border, start = 64 * 17, 64 * 16 + start
     t = _Tokens(gpu_device, [start + seq], 1, dim, BF16, seed=271)
-    for block, size in enumerate((1e-20, 1e30, 1e-10, 1e34, 1.0)):
-        t.value[0, 0, 64 * block : 64 * block + 64] *= size
+    t.value[0, 0, :border] *= 1e-20
+    t.value[0, 0, border:] *= 1e30
     t.fill()
     query = _rand((1, heads, seq, dim), 272, BF16)
-    _check_attention(t, query, [start], rows=[0, 62 - start, 63 - start, 64 - start, 65 - start, 127 - start, 128 - start, seq - 1])
+    last = border - 1 - start
+    rows = [0, last - 2, last - 1, last, last + 1, last + 2, seq - 1]
+    _check_attention(t, query, [start], rows=rows, max_length=1)
 
 
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,seq", [(1, 1), (6, 2), (1, 150), (3, 120)])
-@pytest.mark.parametrize("last", [64 * 4, 64 * 4 + 9])
+@pytest.mark.parametrize("last", [64 * 27, 64 * 27 + 9])
 def test_blocks_without_weight_leave_small_outputs_alone(gpu_device, last, heads, seq, dim):
     """A row whose weights of a block are all zero answers from the others, whatever the block holds."""
 
     t = _Tokens(gpu_device, [last], 1, dim, BF16, seed=281)
-    ones = torch.ones(dim)
-    t.key[0, 0] = (t.key[0, 0].float() * 0.25 + 8.0 * ones).to(BF16)
-    t.key[0, 0, 64:] = (t.key[0, 0, 64:].float() - 16.0 * ones).to(BF16)  # scores some 16 dim^0.5 below
-    for block, size in enumerate((1e-25, 1e30, 1e-28, 1e36, 1.0)):
-        t.value[0, 0, 64 * block : 64 * block + 64] *= size
+    near = 64 * 17  # the tokens before it have all the weight
+    t.key[0, 0] = (t.key[0, 0].float() * 0.25 + 8.0).to(BF16)
+    t.key[0, 0, near:] = (t.key[0, 0, near:].float() - 16.0).to(BF16)  # scores some 16 dim^0.5 below
+    t.value[0, 0, :near] *= 1e-20
+    t.value[0, 0, near:] *= 1e30
     t.fill()
     query = (torch.ones(1, heads, seq, dim) + 0.1 * _rand((1, heads, seq, dim), 282, F32)).to(BF16)
     start = last - seq
-    out = _attend(t, query, [start]).reshape(seq, heads, dim)
+    out = _attend(t, query, [start], max_length=1).reshape(seq, heads, dim)
     keys, values = t.stored(0, 0)
     for h in range(heads):
         for i in {0, seq // 2, seq - 1}:
             q = query[0, h, i].double()
             scores = keys[: start + i + 1] @ q * dim**-0.5
-            assert float(scores[:64].max() - scores[64:].max()) > 100.0  # weights below 2^-144: none in 32 bits
-            weights = torch.softmax(scores[:64], 0)
-            want, sizes = weights @ values[:64], weights @ values[:64].abs()
-            inner = 2 * (2.0**-11 + 2 * (dim + 4) * 2.0**-24 * float((keys[:64].abs() @ q.abs()).max()) * dim**-0.5 + 2.0**-20)
+            assert float(scores[:near].max() - scores[near:].max()) > 100.0  # weights below 2^-144
+            weights = torch.softmax(scores[:near], 0)
+            want, sizes = weights @ values[:near], weights @ values[:near].abs()
+            inner = 2 * (2.0**-11 + 2 * (dim + 4) * 2.0**-24 * float((keys[:near].abs() @ q.abs()).max()) * dim**-0.5 + 2.0**-20)
             _near(out[i, h], want, 2.0**-8 * want.abs() + (1 + 2.0**-8) * inner * sizes, f"head {h} row {i}")
 
 
