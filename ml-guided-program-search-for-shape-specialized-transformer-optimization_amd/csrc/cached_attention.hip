@@ -135,6 +135,14 @@ __device__ __forceinline__ int common_unit(int unit) {
   return __any(unit != first) ? -1 : first;
 }
 
+// How many of a sequence's `count` new rows see only blocks that its table has room for
+// (the others answer NaN).  Their positions, and the tail's, are below 2^31.
+__device__ __forceinline__ int rows_in_table(int64_t start, int count, int64_t max_blocks) {
+  if ((start + count) / kBlockTokens <= max_blocks) return count;
+  const int64_t room = max_blocks * kBlockTokens - start;  // below count
+  return room < 0 ? 0 : (int)room;
+}
+
 template <typename T, int D, int SPLIT>
 __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const AttentionArgs a) {
   typedef typename Vec8<T>::type V8;
@@ -165,26 +173,25 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
   if (count > a.seq_len) count = a.seq_len;
   if (start < 0 || count < 0) count = 0;
-  // More tokens than the table can name: NaN.  Otherwise positions are below 2^31.
-  const bool beyond = (start + count) / kBlockTokens > a.max_blocks;
-  const int first_position = beyond ? 0 : (int)start;
-  const int tail_block = beyond ? 0 : (int)((start + count) / kBlockTokens);
+  const int known = rows_in_table(start, count, a.max_blocks);
+  const int first_position = known == 0 ? 0 : (int)start;
+  const int tail_block = (first_position + known) / kBlockTokens;
 
   // This lane's row: token row / group of the chunk, query head h * group + row % group.
   const uint32_t row = group_row + column;
   const int token = (int)(row / (uint32_t)a.group);
   const int head = h * a.group + (int)(row - (uint32_t)token * (uint32_t)a.group);
   const bool live = token < count;
-  const int last_position = first_position + count - 1;  // -1 or less: no query
+  const int last_position = first_position + known - 1;  // -1: no query
   // The position up to which the row sees; a row without a query sees as far as the last.
-  const int sees = live ? first_position + token : last_position;
+  const int sees = token < known ? first_position + token : last_position;
   V8 q[HALVES][2];
 #pragma unroll
   for (int hh = 0; hh < HALVES; ++hh)
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       u32x4 raw = {0u, 0u, 0u, 0u};
-      if (live) {
+      if (token < known) {
         raw = load16(static_cast<const T*>(a.query) + b * a.q_sb + head * a.q_sh + token * a.q_ss + hh * 64 +
                      quarter * 16 + kk * 8);
         raw = (raw ^ a.sign) & a.keep;
@@ -192,14 +199,14 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
       q[hh][kk] = __builtin_bit_cast(V8, raw);
     }
 
-  const int all_blocks = count == 0 || beyond ? 0 : last_position / kBlockTokens + 1;
+  const int all_blocks = known == 0 ? 0 : last_position / kBlockTokens + 1;
   const int coded_to = all_blocks < tail_block ? all_blocks : tail_block;
 
   f32x4 out[FEATURES];
   int unit = 0;  // the row's, 0 before the first block
   int wave_unit = 0;
   float most = -INFINITY;
-  float sum = beyond && count != 0 ? __builtin_nanf("") : 0.0f;
+  float sum = live && token >= known ? __builtin_nanf("") : 0.0f;
 #pragma unroll
   for (int f = 0; f < FEATURES; ++f) out[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   auto raise_unit = [&](int bits, const auto& p) {
@@ -336,7 +343,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   // The incomplete block, in the tensors' own type: weights without the shift, in a
   // unit of at least 2^11 (the shift), so that large values do not overflow.
   if (tail_block < all_blocks && tail_block % stride == first) {
-    const int held = first_position + count - tail_block * kBlockTokens;  // tokens in it
+    const int held = first_position + known - tail_block * kBlockTokens;  // tokens in it
     const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
     const T* tail_keys = static_cast<const T*>(a.key_tail) + tail_at + quarter * 16;
     const T* tail_values = static_cast<const T*>(a.value_tail) + tail_at + quarter * 16;
@@ -534,39 +541,39 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   int count = common(a.counts != nullptr ? a.counts[b] : a.seq_len);
   if (count > a.seq_len) count = a.seq_len;
   if (start < 0 || count < 0) count = 0;
-  const bool beyond = (start + count) / kBlockTokens > a.max_blocks;
-  const int first_position = beyond ? 0 : (int)start;
-  const int tail_block = beyond ? 0 : (int)((start + count) / kBlockTokens);
+  const int known = rows_in_table(start, count, a.max_blocks);
+  const int first_position = known == 0 ? 0 : (int)start;
+  const int tail_block = (first_position + known) / kBlockTokens;
 
   // The last position that rows first .. first + rows - 1 see, -1 where none has a query.
   auto last_of = [&](uint32_t first, int rows) {
     const int low = common((int)(first / (uint32_t)a.group));
     const int high = common((int)((first + rows - 1) / (uint32_t)a.group));
-    return low < count ? first_position + (high < count ? high : count - 1) : -1;
+    return low < known ? first_position + (high < known ? high : known - 1) : -1;
   };
   const int last_position = last_of(first_row, 32);
   const int group_last = last_of(group_row, ROWS * 32);
   const int least_position = first_position + common((int)(first_row / (uint32_t)a.group));
   const bool live = token < count;
-  const int sees = live ? first_position + token : last_position;
+  const int sees = token < known ? first_position + token : last_position;
 #pragma unroll
   for (int c = 0; c < PAIRS; ++c)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const u32x4 raw = (loaded[c][e] ^ a.sign) & a.keep;
-      q[c][e] = __builtin_bit_cast(V8, live ? raw : (u32x4){0u, 0u, 0u, 0u});
+      q[c][e] = __builtin_bit_cast(V8, token < known ? raw : (u32x4){0u, 0u, 0u, 0u});
     }
 
   // The groups of all chunks take the blocks that the workgroup's rows see in turn; all
   // groups of a workgroup do as many turns, the last ones perhaps without a block.
-  const int all_blocks = group_last < 0 || beyond ? 0 : group_last / kBlockTokens + 1;
+  const int all_blocks = group_last < 0 ? 0 : group_last / kBlockTokens + 1;
   const int coded_to = all_blocks < tail_block ? all_blocks : tail_block;
   const int turns = coded_to > chunk * SPLIT ? (coded_to - chunk * SPLIT + stride - 1) / stride : 0;
 
   f32x16 out[FEATURES];
   int unit = 0, wave_unit = 0;
   float most = -INFINITY;
-  float sum = beyond && last_position >= 0 ? __builtin_nanf("") : 0.0f;
+  float sum = live && token >= known ? __builtin_nanf("") : 0.0f;
 #pragma unroll
   for (int f = 0; f < FEATURES; ++f) out[f] = (f32x16)(0.0f);
   auto raise_unit = [&](int bits, const auto& p) {
@@ -785,7 +792,7 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
 
   // The incomplete block, as above.
   if (last_position >= tail_block * kBlockTokens && tail_block % stride == first_block) {
-    const int held = first_position + count - tail_block * kBlockTokens;
+    const int held = first_position + known - tail_block * kBlockTokens;
     const int64_t tail_at = (b * a.kv_heads + h) * (int64_t)(kBlockTokens * D);
     const T* keys = static_cast<const T*>(a.key_tail) + tail_at + half * 16;
     const T* values = static_cast<const T*>(a.value_tail) + tail_at + half * 32;

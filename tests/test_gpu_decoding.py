@@ -374,6 +374,33 @@ def test_lengths_beyond_the_table_and_sequences_without_tokens(gpu_device):
     assert bool(out[:2].isnan().all()) and bool(out[2].isfinite().all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,seq", [(2, 170), (8, 150), (2, 70), (16, 66)])
+def test_rows_before_the_end_of_the_table_answer(gpu_device, heads, seq, dim):
+    """A chunk that passes the table's room: rows that see only blocks with a place answer, the others are NaN."""
+
+    starts = [127, 100, 0, 64, 128, 150]
+    counts = [seq, max(seq - 10, 92), seq, 0, 64, seq]
+    counts = [min(c, seq) for c in counts]
+    t = _Tokens(gpu_device, [s + c for s, c in zip(starts, counts)], 2, dim, BF16, room=127, seed=291)
+    assert t.cache.block_table.shape[1] == 2
+    t.append(starts=[0] * 6, counts=starts)
+    t.append(starts, counts)
+    query = _rand((6, heads, seq, dim), 292, BF16)
+    out = _attend(t, query, starts, counts)
+    for b, (start, count) in enumerate(zip(starts, counts)):
+        lost = (start + torch.arange(seq) >= 128) & (torch.arange(seq) < count) & (start + count >= 192)
+        assert bool(out[b].isnan().all(-1).eq(lost).all()) and bool(out[b].isnan().any(-1).eq(lost).all()), b
+        seen = [i for i in (0, 1, 27, 28, 63, 64, 127) if i < count and not lost[i]]
+        for h in range(heads):
+            keys, values = t.stored(b, h // (heads // 2), start + count)
+            for i in seen:
+                q = query[b, h, i].double()
+                want, size = plain.attention(q, keys, values, start + i, dim**-0.5)
+                bound = plain.attention_bound(want, size, q, keys, start + i, dim**-0.5, BF16)
+                _near(out[b, i].reshape(heads, dim)[h], want, bound, f"sequence {b} head {h} row {i}")
+
+
 # ---------------------------------------------------------------------------
 # attention over the cache
 
