@@ -477,6 +477,23 @@ def test_long_histories_in_parts(gpu_device, seq, max_length):
     _check_attention(t, query, starts, rows=[0, 7, seq - 1], max_length=max_length)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (64, F16), (128, BF16), (128, F16)])
+@pytest.mark.parametrize("seq", [1, 20, 80, 150])
+def test_parts_of_every_type_and_head_dim(gpu_device, seq, dim, dtype):
+    """More than one part a row and their merge, in each kernel, beyond 8192 tokens and before."""
+
+    from solution.kernels.hip import load_library
+
+    starts, counts = [12_000 - seq, 63, 2_500, 0], [seq, seq, max(1, seq // 2), 1]
+    t = _Tokens(gpu_device, [s + c for s, c in zip(starts, counts)], 1, dim, dtype, room=12_500, seed=301).fill()
+    query = _rand((4, 2, seq, dim), 302, dtype)
+    for max_length in (None, 4_000):
+        most = t.cache.max_tokens if max_length is None else max_length
+        parts = load_library().sah_block_cache_attention_workspace_bytes(4, seq, 2, 1, dim, most) // (4 * seq * 2 * (dim + 2) * 4)
+        assert parts > 1
+        _check_attention(t, query, starts, counts, rows=[0, 7, 33, seq - 1], max_length=max_length)
+
+
 @pytest.mark.parametrize("scale", [0.5, -0.125, 0.0, 1e-30, 3.0])
 @pytest.mark.parametrize("seq", [1, 40])
 def test_scales_of_the_scores(gpu_device, scale, seq):
