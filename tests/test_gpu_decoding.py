@@ -494,6 +494,24 @@ def test_parts_of_every_type_and_head_dim(gpu_device, seq, dim, dtype):
         _check_attention(t, query, starts, counts, rows=[0, 7, 33, seq - 1], max_length=max_length)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,seq", [(64, 1), (4, 8), (2, 150)])
+def test_values_all_alike_come_back_exactly(gpu_device, heads, seq, dtype, dim):
+    """The weights that the values take are those that the row's sum adds up.  1.875 is a
+    code of every block scale; half a step of fp16 there is 2.6e-4 of it, the rounding of
+    a weight to fp16 up to 4.9e-4."""
+
+    lengths = [3000 + 37 * b for b in range(8)]
+    t = _Tokens(gpu_device, lengths, 1, dim, dtype, seed=311)
+    t.value[:] = 1.875
+    t.fill()
+    query = _rand((8, heads, seq, dim), 312, dtype)
+    for scale in (0.25, 1.0, 2.0):
+        out = _attend(t, query, [n - seq for n in lengths], scale=scale, max_length=1)
+        assert bool((out == 1.875).all()), scale
+
+
 @pytest.mark.parametrize("scale", [0.5, -0.125, 0.0, 1e-30, 3.0])
 @pytest.mark.parametrize("seq", [1, 40])
 def test_scales_of_the_scores(gpu_device, scale, seq):
