@@ -26,6 +26,7 @@ import torch
 
 from ..hip._library import (
     HipLibraryError,
+    differentiated,
     dtype_code,
     launch,
     library_available,
@@ -86,7 +87,7 @@ class BlockCache:
         for tensor, shape, dtype in expected:
             if tuple(tensor.shape) != shape or tensor.dtype != dtype:
                 raise ValueError(f"the cache's tensors do not belong together: expected {dtype} {shape}")
-            if not tensor.is_contiguous() or tensor.device != tail.device or tensor.requires_grad:
+            if not tensor.is_contiguous() or tensor.device != tail.device or tensor.requires_grad or differentiated(tensor):
                 raise ValueError("the cache's tensors must be contiguous, on one device and need no gradient")
         for tensor in (self.key_codes, self.value_codes, self.key_tail, self.value_tail):
             if tensor.data_ptr() % 16:
@@ -187,7 +188,7 @@ def _strides(value: torch.Tensor, size: torch.Size) -> tuple[int, int, int] | No
         s = 0
     if feature != 1 or b % 8 or h % 8 or s % 8 or value.data_ptr() % 16:
         return None
-    if value.requires_grad and torch.is_grad_enabled():
+    if differentiated(value):
         return None
     return b, h, s
 

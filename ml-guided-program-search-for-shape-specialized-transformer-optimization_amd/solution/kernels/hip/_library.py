@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 PACKAGE_ROOT = Path(__file__).resolve().parents[3]
 LIBRARY_PATH = PACKAGE_ROOT / "lib" / "libshape_aware_hip.so"
@@ -222,6 +223,15 @@ def launch(index: int, function, what: str, *args) -> None:
         check_status(status, what)
 
 
+def differentiated(value: torch.Tensor) -> bool:
+    """Whether autograd would follow ``value`` into a call: it asks for a gradient, or
+    carries a tangent (which it does under no_grad too)."""
+
+    if value.requires_grad and torch.is_grad_enabled():
+        return True
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(value).tangent is not None
+
+
 # gfx950 or not, per device index: device properties do not change within a
 # process, and every operator's eligibility check asks.
 _GFX950_BY_INDEX: dict[int, bool] = {}
@@ -268,6 +278,7 @@ __all__ = [
     "SAH_NORM_LAYER",
     "SAH_NORM_RMS",
     "check_status",
+    "differentiated",
     "dtype_code",
     "is_gfx950",
     "launch",

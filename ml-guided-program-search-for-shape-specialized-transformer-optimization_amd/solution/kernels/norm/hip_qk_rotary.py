@@ -14,6 +14,7 @@ from ..hip._library import (
     SAH_NORM_LAYER,
     SAH_NORM_RMS,
     HipLibraryError,
+    differentiated,
     dtype_code,
     launch,
     library_available,
@@ -63,7 +64,7 @@ def _strides(value: torch.Tensor, size: torch.Size, unit: int) -> tuple[int, int
         s = 0
     if feature != 1 or b % unit or h % unit or s % unit or value.data_ptr() % 16:
         return None
-    if value.requires_grad and torch.is_grad_enabled():
+    if differentiated(value):
         return None
     return b, h, s
 
@@ -84,7 +85,7 @@ def _param_dtype(
             or parameter.get_device() != index
             or not parameter.is_contiguous()
             or parameter.data_ptr() % 16
-            or (parameter.requires_grad and torch.is_grad_enabled())
+            or differentiated(parameter)
             or (dtype is not torch.float32 and dtype is not like)
             or (found is not None and dtype is not found)
         ):
@@ -129,6 +130,7 @@ def _request(
             or not table.is_contiguous()
             or table.data_ptr() % 16
             or table.requires_grad
+            or differentiated(table)
         ):
             return None
     if starts is not None and (

@@ -17,6 +17,7 @@ from ..hip._library import (
     SAH_ACTIVATION_GELU_EXACT,
     SAH_ACTIVATION_NONE,
     HipLibraryError,
+    differentiated,
     dtype_code,
     launch,
     library_available,
@@ -55,7 +56,7 @@ class PackedLinearW4:
         if not scales.shape[0] or self.in_features % scales.shape[0] or self.group_size not in SUPPORTED_GROUP_SIZES:
             raise ValueError("the group size must be 32, 64 or 128")
         for tensor in (codes, scales):
-            if not tensor.is_contiguous() or tensor.device != codes.device or tensor.requires_grad:
+            if not tensor.is_contiguous() or tensor.device != codes.device or tensor.requires_grad or differentiated(tensor):
                 raise ValueError("codes and scales must be contiguous, on one device and need no gradient")
             if tensor.data_ptr() % 16:
                 raise ValueError("codes and scales must be 16-byte aligned")
@@ -159,7 +160,7 @@ def _request(
         return None
     if activation not in ACTIVATIONS or value.data_ptr() % 16:
         return None
-    if value.requires_grad and torch.is_grad_enabled():
+    if differentiated(value):
         return None
     stride = _row_stride(shape, value.stride())
     if stride is None:
@@ -170,7 +171,7 @@ def _request(
         or bias.get_device() != index
         or not bias.is_contiguous()
         or bias.data_ptr() % 8
-        or (bias.requires_grad and torch.is_grad_enabled())
+        or differentiated(bias)
     ):
         return None
     library = library_for(index)

@@ -9,10 +9,23 @@ import importlib
 import pytest
 import torch
 
-from solution.kernels.attention import BlockCache, hip_block_cache_append, hip_block_cache_attention, hip_block_cache_read
+from solution.kernels.attention import (
+    BlockCache,
+    can_use_hip_block_cache_append,
+    can_use_hip_block_cache_attention,
+    hip_block_cache_append,
+    hip_block_cache_attention,
+    hip_block_cache_read,
+)
 from solution.kernels.hip import _library
-from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
-from solution.kernels.projection import PackedLinearW4, hip_linear_w4, pack_linear_w4_codes, quantize_linear_w4
+from solution.kernels.norm import can_use_hip_qk_norm_rotary, hip_qk_norm_rotary, rotary_table
+from solution.kernels.projection import (
+    PackedLinearW4,
+    can_use_hip_linear_w4,
+    hip_linear_w4,
+    pack_linear_w4_codes,
+    quantize_linear_w4,
+)
 
 # An address that the host checks may look at and no kernel reads: every call below
 # is refused, or has nothing to do, before a launch.
@@ -354,3 +367,62 @@ def test_quantized_weights_are_within_half_a_step():
 def test_weights_that_cannot_be_packed(make):
     with pytest.raises(ValueError):
         make()
+
+
+@pytest.fixture
+def without_a_gpu(monkeypatch):
+    """The operators' eligibility checks on CPU tensors: everything but the device."""
+
+    for name in ("attention.hip_block_cache", "norm.hip_qk_rotary", "projection.hip_linear_w4"):
+        monkeypatch.setattr(importlib.import_module(f"solution.kernels.{name}"), "library_for", lambda index: object())
+
+
+def _requests():
+    """For each operator its check, the arguments of a call that it takes, and those that may be differentiated."""
+
+    cache = _cpu_cache()
+    starts = torch.zeros(2, dtype=torch.int32)
+    kv = torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)
+    weight, bias = torch.ones(64), torch.zeros(64)
+    packed = quantize_linear_w4(torch.ones(16, 128, dtype=torch.bfloat16))
+    x, b = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(16, dtype=torch.bfloat16)
+    return {
+        "append": (can_use_hip_block_cache_append, dict(cache=cache, key=kv, value=kv, starts=starts), ("key", "value")),
+        "attention": (can_use_hip_block_cache_attention, dict(query=kv, cache=cache, starts=starts), ("query",)),
+        "rotary": (
+            can_use_hip_qk_norm_rotary,
+            dict(query=kv, key=kv, query_weight=weight, key_weight=weight, table=rotary_table(4, 64, device="cpu"),
+                 starts=starts, query_bias=bias, key_bias=bias),
+            ("query", "key", "query_weight", "key_weight", "query_bias", "key_bias", "table"),
+        ),
+        "linear": (can_use_hip_linear_w4, dict(value=x, weight=packed, bias=b), ("value", "bias")),
+    }
+
+
+@pytest.mark.parametrize("operator", ["append", "attention", "rotary", "linear"])
+def test_inputs_with_tangents_are_refused(without_a_gpu, operator):
+    """A dual tensor asks for no gradient and keeps its tangent under no_grad: answering
+    without the tangent would drop it."""
+
+    check, arguments, names = _requests()[operator]
+    assert check(**arguments)
+    with torch.no_grad(), torch.autograd.forward_ad.dual_level():
+        assert check(**arguments)
+        for name in names:
+            value = arguments[name]
+            dual = torch.autograd.forward_ad.make_dual(value, torch.ones_like(value))
+            assert not check(**{**arguments, name: dual}), name
+    with torch.no_grad():
+        assert check(**arguments)
+
+
+def test_caches_and_weights_with_tangents_are_refused():
+    cache, packed = _cpu_cache(), quantize_linear_w4(torch.ones(16, 128, dtype=torch.bfloat16))
+    parts = {field: getattr(cache, field) for field in cache.__dataclass_fields__}
+    with torch.autograd.forward_ad.dual_level():
+        make_dual = torch.autograd.forward_ad.make_dual
+        for name in ("key_scales", "value_tail"):
+            with pytest.raises(ValueError):
+                BlockCache(**{**parts, name: make_dual(parts[name], torch.ones_like(parts[name]))})
+        with pytest.raises(ValueError):
+            PackedLinearW4(packed.codes, make_dual(packed.scales, torch.ones_like(packed.scales)))
