@@ -19,7 +19,6 @@ and after the step's last layer ``starts += 1`` (or ``+= counts``).
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -41,6 +40,7 @@ BLOCK_TOKENS = 64
 SUPPORTED_HEAD_DIMS = frozenset({64, 128})
 SUPPORTED_DTYPES = frozenset({torch.bfloat16, torch.float16})
 _MAX_LENGTH = 2**31 - 1
+_MAX_SCALE = 2.0**127  # times log2(e) still in fp32's range
 
 
 @dataclass(frozen=True, eq=False)
@@ -355,7 +355,7 @@ def _attention_request(
     batch, kv_heads, _, dim = tail.shape
     if size[0] != batch or size[3] != dim or size[1] < 1 or size[1] % kv_heads:
         return None
-    if scale is not None and not math.isfinite(scale):
+    if scale is not None and not abs(scale) <= _MAX_SCALE:
         return None
     if max_length is not None and not (isinstance(max_length, int) and 0 <= max_length <= _MAX_LENGTH):
         return None
@@ -395,9 +395,10 @@ def hip_block_cache_attention(
     position ``starts[b] + i`` and attends to all positions up to its own, with
     ``starts`` and ``counts`` those of the append.  Returns [batch, seq_len, heads *
     head_dim]; rows from ``counts[b]`` on are zeros.  ``scale`` defaults to
-    head_dim ** -0.5.  ``max_length``, where the program knows one, bounds the
-    sequences' lengths below what the table has room for: it spares launching the
-    parts of histories that no sequence has.  Longer ones are still computed whole.
+    head_dim ** -0.5 (2 ** 127 is the largest).  ``max_length``, where the program
+    knows one, bounds the sequences' lengths below what the table has room for: it
+    spares launching the parts of histories that no sequence has.  Longer ones are
+    still computed whole.
     """
 
     request = _attention_request(query, cache, starts, counts, scale, max_length)

@@ -426,3 +426,12 @@ def test_caches_and_weights_with_tangents_are_refused():
                 BlockCache(**{**parts, name: make_dual(parts[name], torch.ones_like(parts[name]))})
         with pytest.raises(ValueError):
             PackedLinearW4(packed.codes, make_dual(packed.scales, torch.ones_like(packed.scales)))
+
+
+@pytest.mark.parametrize("scale,taken", [(0.0, True), (-3.0, True), (2.0**127, True), (1e39, False), (3e38, False),
+                                         (-1e39, False), (float("inf"), False), (float("nan"), False)])
+def test_scales_that_the_attention_takes(without_a_gpu, scale, taken):
+    check, arguments, _ = _requests()["attention"]
+    assert check(**arguments, scale=scale) is taken
+    if taken:  # the C entry takes it too (of a batch of none, for which nothing is launched)
+        assert _call("sah_block_cache_attention", ATTENTION, scale=scale, batch=0) == OK
