@@ -5,6 +5,8 @@ the 4-bit format against a plain decoder."""
 from __future__ import annotations
 
 import importlib
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -435,3 +437,53 @@ def test_scales_that_the_attention_takes(without_a_gpu, scale, taken):
     assert check(**arguments, scale=scale) is taken
     if taken:  # the C entry takes it too (of a batch of none, for which nothing is launched)
         assert _call("sah_block_cache_attention", ATTENTION, scale=scale, batch=0) == OK
+
+
+def _parameters(entry):
+    """A C entry's parameter names, from the header."""
+
+    header = (Path(__file__).resolve().parents[1] / "include" / "shape_aware_hip.h").read_text()
+    declared = re.search(rf"\b{entry}\((.*?)\);", re.sub(r"/\*.*?\*/", "", header, flags=re.S), flags=re.S)[1]
+    return [re.findall(r"\w+", parameter)[-1] for parameter in declared.split(",")]
+
+
+def _example(entry, values):
+    """The call of ``entry`` in INTEGRATION.md: its arguments by name, numbers evaluated."""
+
+    text = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
+    call = re.search(rf"rc = {entry}\((.*?)\);", re.sub(r"/\*.*?\*/", "", text, flags=re.S), flags=re.S)[1]
+    arguments = [part.strip() for part in call.replace("(sah_stream_t)", "").split(",")]
+    names = _parameters(entry)
+    assert len(arguments) == len(names)
+    number = lambda text: eval(text, {}, values) if re.fullmatch(r"[\w +*()]*\w[\w +*()]*", text) else text  # noqa: E731
+    known = lambda text: all(w.isdigit() or w in values for w in re.findall(r"\w+", text))  # noqa: E731
+    return {name: number(text) if known(text) else text for name, text in zip(names, arguments)}
+
+
+def test_the_documented_step_stays_in_its_tensors():
+    """The C example's strides reach the last element of each tensor, and not beyond."""
+
+    sizes = dict(B=3, S=5, H=6, Hkv=2, D=256, N=(6 + 2 * 2) * 64, num_blocks=9, max_blocks=4, max_length=300, table_rows=400)
+    batch, seq, heads, kv_heads, width = (sizes[name] for name in ("B", "S", "H", "Hkv", "N"))
+    starts_at = {"q": 0, "k": heads * 64, "v": (heads + kv_heads) * 64}  # in packed
+    elements = {"x": batch * seq * 256, "packed": batch * seq * width, "q_out": batch * heads * seq * 64,
+                "k_out": batch * kv_heads * seq * 64, "context": batch * seq * heads * 64}
+
+    def ends(tensor, counts, strides, row=64):
+        last = starts_at.get(tensor, 0) + sum((n - 1) * stride for n, stride in zip(counts, strides)) + row
+        packed_end = {"q": elements["packed"] - 2 * kv_heads * 64, "k": elements["packed"] - kv_heads * 64, "v": elements["packed"]}
+        assert last == {**elements, **packed_end}[tensor], tensor
+
+    linear = _example("sah_linear_w4", sizes)
+    ends(linear["x"], [linear["rows"]], [linear["x_row_stride"]], linear["in_features"])
+    ends(linear["y"], [linear["rows"]], [linear["y_row_stride"]], linear["out_features"])
+    rotary = _example("sah_qk_norm_rotary", sizes)
+    append = _example("sah_block_cache_append", sizes)
+    attention = _example("sah_block_cache_attention", sizes)
+    strides = lambda call, p: [call[f"{p}_stride_{axis}"] for axis in "bhs"]  # noqa: E731
+    ends(rotary["query"], [batch, rotary["heads"], seq], strides(rotary, "q"))
+    ends(rotary["key"], [batch, rotary["kv_heads"], seq], strides(rotary, "k"))
+    ends(append["key"], [batch, append["kv_heads"], append["seq_len"]], strides(append, "k"))
+    ends(append["value"], [batch, append["kv_heads"], append["seq_len"]], strides(append, "v"))
+    ends(attention["query"], [batch, attention["heads"], attention["seq_len"]], strides(attention, "q"))
+    ends(attention["output"], [batch, seq], [attention["o_stride_b"], attention["o_stride_s"]], heads * 64)
