@@ -511,6 +511,10 @@ int sah_qk_norm_rotary(
  * non-finite key or value is held as a key of NaN and a value of zeros: queries
  * that attend to it answer NaN, others are not touched by it.
  *
+ * Tokens may be taken back by lowering starts, within the incomplete block or to a
+ * multiple of 64.  Anywhere else below the incomplete block is not allowed: the tail
+ * holds a later block's tokens by then, and they would be taken for the earlier one's.
+ *
  * head_dim 64 or 128; dtype f16 or bf16; codes and tails contiguous and 16-byte
  * aligned, the rest 4-byte.
  */

@@ -249,6 +249,12 @@ def hip_block_cache_append(
     one at.  Blocks without a place in the cache are dropped, and the attention that
     would read them answers NaN.  A token with a non-finite key or value makes NaN of
     every query that attends to it, and of no other.
+
+    Tokens are taken back by lowering ``starts``: within the sequence's incomplete
+    block, or to a multiple of 64.  Not elsewhere below that block, whose tokens stand
+    where the earlier block's stood before it was coded (to go back there, read the
+    block's first tokens with :func:`hip_block_cache_read` and append them anew, from
+    the multiple of 64 on).
     """
 
     request = _append_request(cache, key, value, starts, counts)

@@ -268,6 +268,30 @@ def test_appends_of_few_and_several_tokens(gpu_device, dtype, dim):
         t.check(held)
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 128)])
+def test_tokens_taken_back(gpu_device, dtype, dim):
+    """Within the incomplete block, to a multiple of 64, and elsewhere by way of the read:
+    the cache then holds what it would without the tokens that were taken back."""
+
+    t = _Tokens(gpu_device, [200, 200, 130], 2, dim, dtype, seed=321)
+    t.append([0, 0, 0], [200, 200, 130])
+    held = [195, 64, 128]  # the second goes back to a border two blocks below, the third to its own block's first token
+    fresh = _rand((3, 2, 200, dim), 322, dtype)
+    for b, n in enumerate(held):
+        t.key[b, :, n:] = fresh[b, :, n:]
+        t.value[b, :, n:] = -fresh[b, :, n:]
+    t.check(held)
+    t.append(held, [3, 70, 1])
+    held = [198, 134, 129]
+    t.check(held)
+    _check_attention(t, _rand((3, 4, 1, dim), 323, dtype), [n - 1 for n in held], [1, 1, 1])
+    # back to 100 of the first sequence's tokens: its second block's first 36 are coded ones by now
+    key, value = t.read([64, 0, 0], held, 36)
+    t.key[0, :, 64:100], t.value[0, :, 64:100] = key[0].to(dtype), value[0].to(dtype)
+    t.append([64, 134, 129], [36, 0, 0])
+    t.check([100, 134, 129])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_scales_of_extreme_blocks(gpu_device, dtype):
     t = _Tokens(gpu_device, [64 * 6 + 1], 1, 64, dtype, seed=11)
