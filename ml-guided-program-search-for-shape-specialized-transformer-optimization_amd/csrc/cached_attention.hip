@@ -1172,7 +1172,7 @@ extern "C" int sah_block_cache_attention(
   const int64_t units = batch * kv_heads;
   const int64_t most = (int64_t)(UINT32_MAX / 512);
   if (l.row_groups > most / l.chunks || units > most / (l.row_groups * l.chunks) ||
-      batch * seq_len * heads > most * 8 - 8)
+      (l.chunks > 1 && batch * seq_len * heads > most * 8 - 8))  // the merge, four rows a workgroup
     return fail(SAH_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
 
   AttentionArgs a{};

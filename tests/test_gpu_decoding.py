@@ -715,6 +715,29 @@ def test_many_look_ups_in_parts(gpu_device):
     assert bool(_attend(t, query, [149_999], max_length=8_300).isnan().all())
 
 
+def test_more_rows_than_a_merge_takes(gpu_device):
+    """2^26 padded rows and more, of which few have a query: the others are zeros."""
+
+    batch, heads, seq, counts = 8, 64, 131_080, [5, 0, 70, 1, 33, 2, 64, 9]
+    t = _Tokens(gpu_device, [100 + c for c in counts], 8, 64, BF16, seed=331).fill()
+    query = _rand((batch, heads, 70, 64), 332, BF16)
+    padded = torch.empty((batch, seq, heads, 64), dtype=BF16, device=gpu_device).transpose(1, 2)
+    padded[:, :, :70] = query.to(gpu_device)
+    starts, lengths = (torch.tensor(v, dtype=torch.int32, device=gpu_device) for v in ([100] * batch, counts))
+    from solution.kernels.attention import hip_block_cache_attention
+
+    with torch.inference_mode():
+        out = hip_block_cache_attention(padded, t.cache, starts, lengths)[0]
+        few = hip_block_cache_attention(query.to(gpu_device), t.cache, starts, lengths)[0]
+    assert out.shape == (batch, seq, heads * 64) and not bool(out[:, 70:].any())
+    for b, count in enumerate(counts):
+        assert not bool(out[b, count:].any())
+        for i in range(count):  # the same rows, the tokens split otherwise
+            want = few[b, i].double()
+            # two roundings of the output, and of weights (2^-11 each) on values of about 1
+            assert float(((out[b, i].double() - want).abs() - 2.0**-7 * want.abs()).max()) <= 2.0**-9
+
+
 @pytest.mark.parametrize("heads", [40, 96])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_many_query_heads_a_key_head(gpu_device, heads, dim):
