@@ -936,9 +936,9 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   }
 }
 
-// Merge of the chunks, a wave a row: chunk c's output weighs sum_c 2^(most_c - top).
-// A lane first looks at one chunk's statistics, then D / 4 lanes take a chunk's
-// output each time, 256 / D chunks at once.
+// Merge of the chunks, a wave a row: chunk c's output weighs its share of the chunks'
+// sum_c 2^(most_c - top).  A lane first looks at one chunk's statistics, then D / 4 lanes
+// take a chunk's output each time, 256 / D chunks at once.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64_t rows) {
   constexpr int LANES = D / 4;
@@ -955,7 +955,10 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
   float top = own[0];
   for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, statistics[c][0]);
   f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
-  float total = 0.0f;
+  auto weight_of = [&](f32x2 s) {
+    return s[1] != 0.0f ? s[1] * exp2_fast(s[0] - (top == -INFINITY ? 0.0f : top)) : 0.0f;
+  };
+  float inverse = 0.0f;
   for (int first = 0; first < a.chunks; first += 64) {
     const int here = a.chunks - first < 64 ? a.chunks - first : 64;
     f32x4 v[4];
@@ -970,10 +973,13 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
     if (first == 0) {
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+      float total = weight_of(own);
+      for (int c = lane + 64; c < a.chunks; c += 64) total += weight_of(statistics[c]);
+      total = wave_sum(total);
+      inverse = total != 0.0f ? 1.0f / total : 0.0f;
     }
     const f32x2 s = first == 0 ? own : first + lane < a.chunks ? statistics[first + lane] : nothing;
-    const float weight = s[1] != 0.0f ? s[1] * exp2_fast(s[0] - (top == -INFINITY ? 0.0f : top)) : 0.0f;
-    total += weight;
+    const float weight = weight_of(s) * inverse;
     for (int c = 0; c < here; c += 4 * PARTS) {
       if (c != 0) load(c);
 #pragma unroll
@@ -984,14 +990,10 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
       }
     }
   }
-  total = wave_sum(total);
-  const float inverse = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
   for (int m = LANES; m < 64; m <<= 1)
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] += __shfl_xor(out[j], m);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) out[j] *= inverse;
   if (lane >= LANES) return;
   const int64_t token_row = row / a.heads;
   const int head = (int)(row - token_row * a.heads);

@@ -599,6 +599,18 @@ def test_blocks_without_weight_leave_small_outputs_alone(gpu_device, last, heads
             _near(out[i, h], want, 2.0**-8 * want.abs() + (1 + 2.0**-8) * inner * sizes, f"head {h} row {i}")
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("seq", [1, 150])
+@pytest.mark.parametrize("size", [1e36, 1e-30])
+def test_large_and_small_values_in_parts(gpu_device, size, seq, dim):
+    """Parts are merged by their shares: outputs far from 1 neither overflow nor lose bits."""
+
+    t = _Tokens(gpu_device, [9000, 5000], 1, dim, BF16, seed=351)
+    t.value *= size
+    t.fill()
+    _check_attention(t, _rand((2, 2, seq, dim), 352, BF16), [9000 - seq, 5000 - seq], rows=[0, seq - 1])
+
+
 @pytest.mark.parametrize("dim,dtype", [(64, BF16), (64, F16), (128, BF16)])
 @pytest.mark.parametrize("seq", [1, 5, 40])
 def test_scores_that_grow_and_fall_along_the_history(gpu_device, seq, dim, dtype):
