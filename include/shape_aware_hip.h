@@ -558,6 +558,7 @@ int sah_block_cache_read(
  * (starts and counts are those of the append): row i of sequence b attends to
  * positions 0 .. starts[b] + i.
  *   output = round_to(dtype, softmax(scale q K^T) V), fp32 softmax and accumulation
+ * (beyond dtype's range, where codes of its largest values are rounded up: the largest).
  * query [batch, heads, seq_len, head_dim] by strides (multiples of 8 elements,
  * head_dim contiguous); query head j reads key head j / (heads / kv_heads); output
  * [batch, seq_len, heads * head_dim] by strides, overlapping no input.  Rows from

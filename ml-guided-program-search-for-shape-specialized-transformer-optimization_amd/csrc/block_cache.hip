@@ -282,15 +282,6 @@ struct ReadArgs {
   uint32_t span;
 };
 
-// A code times its scale in T.  A value whose rounding up left T's range (within
-// half a step of its largest) takes the largest.
-template <typename T>
-__device__ __forceinline__ T held_value(float code, float scale) {
-  constexpr float kMost = std::is_same<T, f16>::value ? 65504.0f : 3.38953139e38f;
-  const float v = code * scale;
-  return from_f32<T>(v != v ? v : fminf(fmaxf(v, -kMost), kMost));
-}
-
 // HBM-bound: codes are read once, 16-bit keys and values written once.  A workgroup
 // takes one block of (sequence, head), whose values turn in LDS, a feature's tokens an
 // odd number of places apart, on their way to the output's rows:
@@ -338,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void block_read_kernel(const ReadArgs a) 
         if (held) raw = *reinterpret_cast<const u32x2*>(a.cache.value_codes + code_at + feature * kBlockTokens + slot);
         const V8 codes = e4m3_operand<T>(raw[0], raw[1], 1.0f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = held_value<T>(to_f32(codes[e]), v_scale);
+        for (int e = 0; e < 8; ++e) v[e] = in_range<T>(to_f32(codes[e]) * v_scale);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) turned[feature * ROW + slot + e] = v[e];
@@ -364,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void block_read_kernel(const ReadArgs a) 
         if (held) raw = *reinterpret_cast<const u32x2*>(a.cache.key_codes + code_at + slot * D + feature);
         const V8 codes = e4m3_operand<T>(raw[0], raw[1], 1.0f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = held_value<T>(to_f32(codes[e]), k_scale);
+        for (int e = 0; e < 8; ++e) k[e] = in_range<T>(to_f32(codes[e]) * k_scale);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = turned[(feature + e) * ROW + slot];

@@ -116,6 +116,12 @@ __device__ __forceinline__ float power_ratio(int a_bits, int b_bits) {
   return __int_as_float(bits < 0x00800000 ? 0 : bits);
 }
 
+// A part's output that is weighed further: fp32's largest value where the type's largest
+// ones were coded higher.  (A NaN row's weights are NaN, whatever its parts.)
+__device__ __forceinline__ float finite_part(float x) {
+  return __builtin_amdgcn_fmed3f(x, -3.40282347e38f, 3.40282347e38f);
+}
+
 // Whether any weight of an operand is not zero.
 template <typename V8>
 __device__ __forceinline__ bool any_weight(const V8 (&p)[2]) {
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
 #pragma unroll
   for (int f = 0; f < FEATURES; ++f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[f][j] = out[f][j] * inverse * unit_value;
+    for (int j = 0; j < 4; ++j) out[f][j] = finite_part(out[f][j] * inverse * unit_value);
     *reinterpret_cast<f32x4*>(&part[split][column * PITCH + f * 16 + quarter * 4]) = out[f];
   }
   __syncthreads();
@@ -462,10 +468,12 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
     if (a.chunks == 1) {
       typename Vec8<T>::half_type v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (T)merged[j];
+      for (int j = 0; j < 4; ++j) v[j] = in_range<T>(merged[j]);
       *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + token * a.o_ss +
                                                       (int64_t)head * D + f * 16 + quarter * 4) = v;
     } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) merged[j] = finite_part(merged[j]);
       *reinterpret_cast<f32x4*>(a.partial + place * D + f * 16 + quarter * 4) = merged;
     }
   }
@@ -924,11 +932,13 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
         if (a.chunks == 1) {
           typename Vec8<T>::half_type v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (T)merged[e];
+          for (int e = 0; e < 4; ++e) v[e] = in_range<T>(merged[e]);
           *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + its_token * a.o_ss +
                                                           (int64_t)head * D + at) = v;
         } else {
           const int64_t place = ((b * a.seq_len + its_token) * a.heads + head) * a.chunks + chunk;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) merged[e] = finite_part(merged[e]);
           *reinterpret_cast<f32x4*>(a.partial + place * D + at) = merged;
         }
       }
@@ -1001,7 +1011,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const AttentionArgs a, int64
   const int64_t token = token_row - b * a.seq_len;
   typename Vec8<T>::half_type v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = (T)out[j];
+  for (int j = 0; j < 4; ++j) v[j] = in_range<T>(out[j]);
   *reinterpret_cast<typename Vec8<T>::half_type*>(static_cast<T*>(a.output) + b * a.o_sb + token * a.o_ss +
                                                   (int64_t)head * D + feature) = v;
 }

@@ -3,6 +3,8 @@
 // conversion of e4m3 bytes to its operands.
 #pragma once
 
+#include <type_traits>
+
 #include "sah_common.hpp"
 
 namespace sah {
@@ -38,6 +40,15 @@ __device__ __forceinline__ f16x8 e4m3_operand<f16>(uint32_t lo, uint32_t hi, flo
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false)),
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true))};
   return __builtin_bit_cast(f16x8, v);
+}
+
+// fp32 in T, where rounded codes times their scale may have left T's range though the
+// values that they stand for did not (within half a code's step of its largest, which
+// is taken then).  NaN stays.
+template <typename T>
+__device__ __forceinline__ T in_range(float v) {
+  constexpr float kMost = std::is_same<T, f16>::value ? 65504.0f : 3.38953139e38f;
+  return from_f32<T>(v != v ? v : fminf(fmaxf(v, -kMost), kMost));
 }
 
 // Tokens of one block of the key/value cache.

@@ -599,6 +599,21 @@ def test_blocks_without_weight_leave_small_outputs_alone(gpu_device, last, heads
             _near(out[i, h], want, 2.0**-8 * want.abs() + (1 + 2.0**-8) * inner * sizes, f"head {h} row {i}")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,seq,max_length", [(1, 1, None), (2, 150, None), (1, 1, 1), (2, 150, 1)])
+def test_the_types_largest_values(gpu_device, heads, seq, max_length, dtype):
+    """Their codes stand for more than the type holds; the answer stays in its range."""
+
+    most = torch.finfo(dtype).max
+    t = _Tokens(gpu_device, [6000], 1, 64, dtype, seed=341)
+    t.value[..., :32], t.value[..., 32:] = most, -most
+    t.fill()
+    out = _attend(t, _rand((1, heads, seq, 64), 342, dtype), [6000 - seq], max_length=max_length).reshape(seq, heads, 64)
+    # rounding of a code up (by 2^-4 at most) and back, and of weights; the tail holds the values themselves
+    assert bool((out[..., :32] >= most * (1 - 2.0**-7)).all()) and bool((out[..., 32:] <= -most * (1 - 2.0**-7)).all())
+    assert bool(out.isfinite().all())
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("seq", [1, 150])
 @pytest.mark.parametrize("size", [1e36, 1e-30])
