@@ -19,8 +19,9 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Eight e4m3 bytes, in order, times a power of two, as one operand: exact in
-// both types for the scales used here (1 and 2^9).
+// Eight e4m3 bytes, in order, times a power of two, as one operand: exact in both
+// types for the scales used here (1; 1/2 on whole numbers up to 7 * 2^-9; and from 1 down
+// to 2^-15 in fp16, whose smallest subnormal is the smallest code's then).
 template <typename T>
 __device__ __forceinline__ typename Vec8<T>::type e4m3_operand(uint32_t lo, uint32_t hi, float scale);
 template <>

@@ -9,8 +9,9 @@
 //
 // A code is a sign and three bits of magnitude.  As an e4m3 byte these four bits are
 // sign * magnitude * 2^-9 (a subnormal, linear in the magnitude), which the
-// conversion with a scale of 2^9 takes to the exact whole number in the operand's
-// type.  The word holds the first four codes at bits 0-2 and 7 of its bytes and the
+// conversion with a scale of 1/2 takes to the code times 2^-10, exact in the operand's
+// type; the outputs take the 2^10 back.  (A group of whole codes times the largest bf16
+// values would leave fp32 where its scale brings it back in: 7 * 128 < 2^10.)  The word holds the first four codes at bits 0-2 and 7 of its bytes and the
 // other four the same way, turned left by four bits: one AND, one turn and AND, and
 // four conversions of two make an operand of eight, with no offset to correct.
 // Products and groups are summed in fp32, a group's sum is scaled by its scale there.
@@ -44,7 +45,7 @@ template <typename T>
 __device__ __forceinline__ typename Vec8<T>::type code_operand(uint32_t word) {
   const uint32_t low = word & 0x87878787u;
   const uint32_t high = __builtin_rotateright32(word, 4) & 0x87878787u;
-  return e4m3_operand<T>(low, high, 512.0f);
+  return e4m3_operand<T>(low, high, 0.5f);
 }
 
 // A workgroup takes OUTS x 16 outputs of TILES x 16 rows; its SPLIT waves share the
@@ -232,6 +233,8 @@ __global__ __launch_bounds__(SPLIT * 64) void linear_w4_kernel(const LinearW4Arg
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += other[j];
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= 1024.0f;
     const int64_t n = ((int64_t)out_tile + i % OUTS) * 16 + quarter * 4;
     if (a.bias != nullptr) {
       const V4 bias = *reinterpret_cast<const V4*>(static_cast<const T*>(a.bias) + n);

@@ -922,6 +922,27 @@ def test_linear_w4_layouts_and_extremes(gpu_device):
         hip_linear_w4(one, packed, activation="relu")
 
 
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("group", [32, 128])
+def test_linear_w4_of_large_inputs(gpu_device, rows, group):
+    """Inputs of up to bf16's largest: a group's sum of whole codes would leave fp32."""
+
+    from solution.kernels.projection import hip_linear_w4, pack_linear_w4_codes
+
+    generator = torch.Generator().manual_seed(rows)
+    codes = torch.randint(-7, 8, (48, 256), generator=generator)
+    codes[:16] = codes[:16].abs()  # sums without cancellation
+    scales = torch.full((48, 256 // group), 2.0**-12).to(BF16)
+    packed = pack_linear_w4_codes(codes.to(gpu_device), scales.to(gpu_device))
+    x = (torch.rand((rows, 256), generator=generator) + 1).to(BF16) * 2.0**126
+    with torch.inference_mode():
+        got = hip_linear_w4(x.to(gpu_device), packed)[0]
+    weight = codes.double() * 2.0**-12
+    want, size = plain.linear(x.double(), weight, None, False)
+    assert float(want.abs().max()) < torch.finfo(BF16).max
+    _near(got, want, plain.linear_bound(want, size, 256, False, BF16), f"large inputs, {rows} rows")
+
+
 # ---------------------------------------------------------------------------
 # a decoding step
 
