@@ -225,6 +225,15 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   for (int f = 0; f < FEATURES; ++f) out[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   auto raise_unit = [&](int bits, const auto& p) {
     if (bits <= wave_unit) return;
+    if (wave_unit == 0 || (wave_unit > 0 && bits - wave_unit <= kUnitRise)) {  // every row follows
+      if (wave_unit != 0) {
+        const float change = power_ratio(wave_unit, bits);
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+      }
+      unit = wave_unit = bits;
+      return;
+    }
     uint64_t weighs = __ballot(any_weight(p));
     weighs |= weighs >> 32;
     weighs |= weighs >> 16;
@@ -606,6 +615,15 @@ __global__ __launch_bounds__(SPLIT * ROWS * 64, 8 / (SPLIT * ROWS)) void chunk_a
   for (int f = 0; f < FEATURES; ++f) out[f] = (f32x16)(0.0f);
   auto raise_unit = [&](int bits, const auto& p) {
     if (bits <= wave_unit) return;
+    if (wave_unit == 0 || (wave_unit > 0 && bits - wave_unit <= kUnitRise)) {  // every row follows
+      if (wave_unit != 0) {
+        const float change = power_ratio(wave_unit, bits);
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) out[f] *= change;
+      }
+      unit = wave_unit = bits;
+      return;
+    }
     uint64_t weighs = __ballot(any_weight(p));
     weighs |= weighs >> 32;
     const bool rises = unit_rises(unit, bits, (weighs >> column & 1) != 0);
