@@ -598,9 +598,9 @@ size_t sah_block_cache_attention_workspace_bytes(
  * + 7; code e >= 4 stands as code e - 4, turned left by 4 bits.  scales
  * [in_features / group_size, out_features] and bias [out_features] (or NULL) in
  * dtype; x [rows, in_features] and y [rows, out_features] by row strides (multiples
- * of 8 elements; rows of x 0 to 2^25 apart), y overlapping no input.  dtype f16 or
- * bf16; group_size 32, 64 or 128; in_features a multiple of 128, out_features of 16;
- * tensors 16-byte aligned, bias 8-byte.
+ * of 8 elements; rows of x 0 to 2^25 apart, of y at least out_features), y overlapping
+ * no input.  dtype f16 or bf16; group_size 32, 64 or 128; in_features a multiple of
+ * 128, out_features of 16; tensors 16-byte aligned, bias 8-byte.
  */
 int sah_linear_w4(
     const void* x, const void* codes, const void* scales, const void* bias, void* y,

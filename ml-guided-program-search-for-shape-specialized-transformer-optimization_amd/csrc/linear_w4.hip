@@ -331,6 +331,9 @@ extern "C" int sah_linear_w4(const void* x, const void* codes, const void* scale
     return fail(SAH_ERR_UNSUPPORTED, "sah_linear_w4: rows of x %lld elements apart", (long long)x_row_stride);
   if (x_row_stride % 8 != 0 || y_row_stride % 8 != 0)
     return fail(SAH_ERR_INVALID_ARGUMENT, "sah_linear_w4: row strides must be multiples of 8 elements");
+  if (rows > 1 && y_row_stride < out_features)
+    return fail(SAH_ERR_INVALID_ARGUMENT, "sah_linear_w4: rows of y overlap (%lld elements apart)",
+                (long long)y_row_stride);
   LinearW4Args a{};
   a.x = x;
   a.codes = static_cast<const uint32_t*>(codes);

@@ -220,6 +220,12 @@ def test_linear_w4_entry_refuses_before_launch(changes, status):
     assert _call("sah_linear_w4", LINEAR, **changes) == status
 
 
+@pytest.mark.parametrize("changes,status", [({"y_stride": 24}, INVALID), ({"y_stride": 0}, INVALID), ({"y_stride": -32}, INVALID),
+                                            ({"rows": 0, "y_stride": 0}, OK)])
+def test_linear_w4_entry_refuses_rows_of_y_that_overlap(changes, status):
+    assert _call("sah_linear_w4", LINEAR, **changes) == status
+
+
 @pytest.mark.parametrize(
     "shape,strides,want",
     [
