@@ -182,6 +182,8 @@ def _row_stride(shape: tuple[int, ...], strides: tuple[int, ...]) -> int | None:
     """The stride of a tensor's rows, taken as one axis; None where they are not
     at one stride that the kernel reads."""
 
+    if 0 in shape:  # no rows
+        return shape[-1]
     if strides[-1] != 1:
         return None
     stride, span = shape[-1], None

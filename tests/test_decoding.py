@@ -493,3 +493,9 @@ def test_the_documented_step_stays_in_its_tensors():
     ends(append["value"], [batch, append["kv_heads"], append["seq_len"]], strides(append, "v"))
     ends(attention["query"], [batch, attention["heads"], attention["seq_len"]], strides(attention, "q"))
     ends(attention["output"], [batch, seq], [attention["o_stride_b"], attention["o_stride_s"]], heads * 64)
+
+
+@pytest.mark.parametrize("shape", [(0, 128), (2, 0, 128), (0, 3, 128), (2, 0, 3, 128)])
+def test_linear_w4_takes_no_rows(without_a_gpu, shape):
+    check, arguments, _ = _requests()["linear"]
+    assert check(**{**arguments, "value": torch.zeros(shape, dtype=torch.bfloat16)})
