@@ -1056,6 +1056,74 @@ def test_captured_steps_replay_as_eager_ones(gpu_device):
         assert torch.equal(getattr(layers[0].cache, name), getattr(layers[1].cache, name)), name
 
 
+def test_calls_without_tokens(gpu_device):
+    """No sequences, no tokens, no rows: outputs of their shapes, and the cache as it was."""
+
+    from solution.kernels.attention import BlockCache, hip_block_cache_append, hip_block_cache_attention, hip_block_cache_read
+    from solution.kernels.norm import hip_qk_norm_rotary, rotary_table
+    from solution.kernels.projection import hip_linear_w4, quantize_linear_w4
+
+    weight = quantize_linear_w4(_rand((32, 128), 361, BF16).to(gpu_device))
+    table = rotary_table(8, 64, device=gpu_device)
+    with torch.inference_mode():
+        for batch, seq in ((0, 3), (2, 0), (0, 0)):
+            t = _Tokens(gpu_device, [70] * 2, 2, 64, BF16, seed=362).fill()
+            cache = t.cache if batch else BlockCache.allocate(0, 2, 64, max_tokens=200, device=gpu_device)
+            before = {n: getattr(t.cache, n).clone() for n in ("key_codes", "value_codes", "key_tail", "value_tail")}
+            starts = torch.full((batch,), 70, dtype=torch.int32, device=gpu_device)
+            q, kv = (torch.zeros(batch, h, seq, 64, dtype=BF16, device=gpu_device) for h in (4, 2))
+            out = hip_qk_norm_rotary(q, kv, None, None, table, starts)
+            assert out[0].shape == q.shape and out[1].shape == kv.shape
+            hip_block_cache_append(cache, kv, kv, starts)
+            assert hip_block_cache_attention(q, cache, starts)[0].shape == (batch, seq, 256)
+            assert hip_block_cache_read(cache, starts, starts, seq)[0].shape == (batch, 2, seq, 64)
+            assert hip_linear_w4(torch.zeros(batch, seq, 128, dtype=BF16, device=gpu_device), weight)[0].shape == (batch, seq, 32)
+            for name, want in before.items():
+                assert torch.equal(getattr(t.cache, name), want), name
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_captured_chunks_replay_as_eager_ones(gpu_device, dim):
+    """Chunks in parts from one graph, at other places and of other lengths each time."""
+
+    from solution.kernels.attention import hip_block_cache_append, hip_block_cache_attention
+
+    seq, lengths = 90, [9_000, 4_000, 130]
+    tokens = [_Tokens(gpu_device, lengths, 1, dim, BF16, seed=371) for _ in range(2)]
+    for t in tokens:
+        t.append([0] * 3, [8_000, 64, 0])
+    query = _rand((3, 4, seq, dim), 372, BF16).to(gpu_device)
+    kv = _rand((2, 3, 1, seq, dim), 373, BF16).to(gpu_device)
+    to = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu_device)  # noqa: E731
+    starts, counts = to([8_000, 64, 0]), to([seq, 1, 0])
+
+    def step(cache, key, value, starts, counts):
+        hip_block_cache_append(cache, key, value, starts, counts)
+        return hip_block_cache_attention(query, cache, starts, counts)[0]
+
+    with torch.inference_mode():
+        key, value = kv[0].clone(), kv[1].clone()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+            out = step(tokens[0].cache, key, value, starts, counts)
+            starts += counts
+        torch.cuda.current_stream().wait_stream(stream)
+        held = [8_000, 64, 0]
+        for i, new in enumerate(([seq, 1, 0], [3, 64, 20], [0, 0, 44], [64, seq, 1], [seq, 0, 65])):
+            fresh = kv.roll(i, dims=3)
+            want = step(tokens[1].cache, fresh[0], fresh[1], to(held), to(new))
+            key.copy_(fresh[0]), value.copy_(fresh[1]), counts.copy_(to(new))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), i
+            held = [a + b for a, b in zip(held, new)]
+        assert starts.tolist() == held
+    for name in ("key_codes", "value_codes", "key_scales", "value_scales", "key_tail", "value_tail"):
+        assert torch.equal(getattr(tokens[0].cache, name), getattr(tokens[1].cache, name)), name
+
+
 def test_two_streams_at_once(gpu_device):
     """Calls that overlap on two streams have workspaces of their own."""
 
