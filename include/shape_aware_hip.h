@@ -563,7 +563,8 @@ int sah_block_cache_read(
  * head_dim contiguous); query head j reads key head j / (heads / kv_heads); output
  * [batch, seq_len, heads * head_dim] by strides, overlapping no input.  Rows from
  * counts[b] on, and all rows of a sequence with a negative start, are zeros; rows
- * that see a block without a place in the cache are NaN.
+ * that see a block without a place in the cache are NaN.  A score is summed over a
+ * block's codes before its scale: 448 * head_dim times the largest |q| stays below 2^127.
  * max_length bounds starts + counts; it lays out the
  * launch and sizes the workspace.  Longer sequences are still computed whole.
  * workspace: device memory of sah_block_cache_attention_workspace_bytes(), 16-byte

@@ -438,7 +438,7 @@ __global__ __launch_bounds__(SPLIT * 64) void cached_attention_kernel(const Atte
   // Merge of the waves: wave w's output weighs sum_w 2^(most_w - top).  Each wave merges
   // the tiles of 16 features f % SPLIT == split.
   constexpr int PITCH = D + 4;
-  __shared__ float part[SPLIT][16 * PITCH];
+  __shared__ __align__(16) float part[SPLIT][16 * PITCH];
   __shared__ float stats[SPLIT][16][2];
   if (quarter == 0) {
     stats[split][column][0] = most;
@@ -1063,11 +1063,15 @@ Layout layout_of(int64_t batch, int64_t seq_len, int64_t kv_heads, int64_t group
     // through memory.  Eight of them do in one launch what four leave to a second one,
     // but leave registers unused with heads of 64 (tokens of a sequence, us with both
     // launches, eight / four: 64 x 2000 14.6 / 20.1, 64 x 8000 49.6 / 54.8; 8 x 20000
-    // 28.4 / 25.2, 4 x 100000 160 / 142).
+    // 28.4 / 25.2, 4 x 100000 160 / 142).  `blocks` counts the incomplete one: at a room of
+    // 8192 tokens four begin (16 / 4 heads of 64: 1 x 8000 13.3 / 11.3, 32 x 2000 18.5 /
+    // 13.8, 32 x 8000 35.7 / 28.5, 64 x 2000 14.7 / 22.1).
     l.split = blocks <= 128 ? 8 : 4;
     int64_t chunks = few / (batch * kv_heads * l.row_groups * l.split);
-    // A wave has at least four blocks (1 x 1000 tokens 6.7, with two blocks and a second
-    // launch 19.9).
+    // A part for every four blocks a wave, and one for what is left over: two from 33
+    // blocks on, a room of 2048 tokens, where the second launch costs what it gives (us,
+    // two parts / one, one sequence of 1500 / 2000 / 4000 tokens: 16 / 4 heads of 64 10.6 / 9.4,
+    // 10.8 / 10.9, 13.6 / 16.5; 32 / 8 heads of 128 14.8 / 14.8, 14.9 / 17.6, 20.1 / 28.0).
     const int64_t most = ceil_div(blocks, 4 * l.split);
     if (chunks > most) chunks = most;
     l.chunks = chunks < 1 ? 1 : (int)chunks;
