@@ -37,9 +37,9 @@
 //
 // Bounds.  For a single token every feature of a held token is 2 bytes to read for
 // 4 * group operations, so the codes' way from memory bounds it: 4 sequences of 90000
-// to 100000 tokens, 16 heads of 64, 779 MB in 136 us, 5.7 TB/s (a copy moves 4.9), and
-// 4.9 us for the merge of their parts.  32 sequences of 100 to 4095 tokens, 32 / 8 heads
-// of 128 (138 MB), take 36 us, one of 777 tokens 7.5: there the longest wave's chain of
+// to 100000 tokens, 16 heads of 64, 779 MB in 141 us, 5.5 TB/s (a copy moves 4.9), and
+// 4.6 us for the merge of their parts.  32 sequences of 100 to 4095 tokens, 32 / 8 heads
+// of 128 (138 MB), take 39 us, one of 777 tokens 8.1: there the longest wave's chain of
 // loads bounds it.
 
 #include <type_traits>
