@@ -112,7 +112,7 @@ __device__ __forceinline__ float halves_max(float x) {
 
 // Powers of two by their fp32 bits: 2^a / 2^b, 0 where it is below 2^-126.
 __device__ __forceinline__ float power_ratio(int a_bits, int b_bits) {
-  const int bits = 0x3f800000 + (a_bits - b_bits);
+  const int bits = (int)(0x3f800000u + (uint32_t)a_bits - (uint32_t)b_bits);  // used where a is at most b
   return __int_as_float(bits < 0x00800000 ? 0 : bits);
 }
 

@@ -454,7 +454,7 @@ def _parameters(entry):
 
 
 def _example(entry, values):
-    """The call of ``entry`` in INTEGRATION.md: its arguments by name, numbers evaluated."""
+    """The documented call of ``entry``: its arguments by name, numbers evaluated."""
 
     text = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
     call = re.search(rf"rc = {entry}\((.*?)\);", re.sub(r"/\*.*?\*/", "", text, flags=re.S), flags=re.S)[1]
