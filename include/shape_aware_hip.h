@@ -512,8 +512,9 @@ int sah_qk_norm_rotary(
  * that attend to it answer NaN, others are not touched by it.
  *
  * Tokens may be taken back by lowering starts, within the incomplete block or to a
- * multiple of 64.  Anywhere else below the incomplete block is not allowed: the tail
- * holds a later block's tokens by then, and they would be taken for the earlier one's.
+ * multiple of 64.  Anywhere else below the incomplete block the tail holds a later
+ * block's tokens, which would be taken for the earlier one's:
+ * sah_block_cache_take_back() fetches that block's own tokens first.
  *
  * head_dim 64 or 128; dtype f16 or bf16; codes and tails contiguous and 16-byte
  * aligned, the rest 4-byte.
@@ -607,6 +608,163 @@ int sah_linear_w4(
     const void* x, const void* codes, const void* scales, const void* bias, void* y,
     int64_t rows, int64_t in_features, int64_t out_features, int64_t group_size,
     int64_t x_row_stride, int64_t y_row_stride, int dtype, int activation,
+    sah_stream_t stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   y[b][s] = round_to(dtype, base[b][s] + scale_a (x[b][s] down_a^T) up_a^T),
+ * a = indices[b], with fp32 accumulation in both products.  The middle factor enters the
+ * second product as two 16-bit numbers (off by 2^-16 of itself in bf16, 2^-22 in fp16).
+ * A sequence whose index is outside [0, adapters), and rows from counts[b] on (counts
+ * NULL: none), take base as it is.
+ *
+ * x [batch, seq_len, in_features], base and y [batch, seq_len, out_features] by
+ * strides (multiples of 8 elements, features contiguous); y is base itself (same
+ * address and strides) or overlaps no input, and no row of y overlaps another.  down
+ * [adapters, rank, in_features] and up [adapters, out_features, rank] contiguous;
+ * scales [adapters] fp32 (NULL: 1).  ranks [adapters] (NULL: rank of all): adapter a has
+ * directions 0 .. ranks[a] - 1, rounded up to a multiple of 8 (those between are zeros)
+ * and at most rank; what lies behind is not read, and 0 or less is no adapter.  dtype f16 or
+ * bf16; in_features, out_features and rank multiples of 8, rank at most 128; tensors
+ * 16-byte aligned.
+ * workspace: device memory of sah_low_rank_adapters_workspace_bytes(), 16-byte aligned,
+ * NULL when that is 0; calls that share one must not overlap.
+ */
+int sah_low_rank_adapters(
+    const void* x, const void* base, const void* down, const void* up, const float* scales,
+    const int32_t* ranks, const int32_t* indices, const int32_t* counts, void* y,
+    int64_t batch, int64_t seq_len, int64_t in_features, int64_t out_features,
+    int64_t adapters, int64_t rank,
+    int64_t x_stride_b, int64_t x_stride_s, int64_t base_stride_b, int64_t base_stride_s,
+    int64_t y_stride_b, int64_t y_stride_s, int dtype,
+    void* workspace, size_t workspace_bytes, sah_stream_t stream);
+
+/* Bytes of the partial sums of few tokens; 0 for many. */
+size_t sah_low_rank_adapters_workspace_bytes(
+    int64_t batch, int64_t seq_len, int64_t in_features, int64_t out_features, int64_t rank);
+
+/*
+ * Verification of drafted tokens against the target's probabilities, from given random
+ * numbers.  target [batch, drafts + 1, vocab] holds the logits of the model that answers,
+ * row i after the first i drafted tokens; tokens [batch, drafts] what another one
+ * drafted, and draft [batch, drafts, vocab] the logits that each was drawn from, or
+ * NULL where a draft was certain (a look-up, the draft's most likely token).  With
+ *   p_i = softmax(target_i / temperature),  q_i = softmax(draft_i / temperature)
+ * (q_i all at token x_i without draft), draft i stands where the drafts before it stand
+ * and u_i q_i(x_i) < p_i(x_i), u_i = uniforms[b][i] in [0, 1).  The token after the ones
+ * that stand is drawn by u = uniforms[b][drafts] from max(p - q, 0) at the first that
+ * does not stand, from p where all do: the lowest v for which the sum of the weights up
+ * to v is above u times the sum of all.  In fp64 throughout.
+ *   accepted[b]  the drafts that stand
+ *   answer[b]    [drafts + 1]: these, the token drawn, -1 behind
+ * temperatures[b] (NULL: 1) not above 0 (or NaN) asks for the likeliest token: a draft
+ * stands where it is the target's (ties: the lowest), which also is the token drawn.
+ * counts[b] (NULL: drafts) is the number of the request's drafts, at most drafts; below 0
+ * the request takes no part: accepted and answer are -1.  A draft outside [0, vocab)
+ * does not stand.  Logits of -inf have no weight.  A row that is asked for, of target
+ * or draft, with a logit of NaN or +inf, or none above -inf, ends the request's answer:
+ * -1 is the token drawn.  So is it where max(p - q, 0) is 0 everywhere.
+ *
+ * Logits f32, f16 or bf16 by strides in elements (any), vocab contiguous; the rest
+ * contiguous; tensors aligned to their elements; at most 1024 drafts.  workspace:
+ * device memory of sah_verify_draft_workspace_bytes() (sampled: draft is not NULL),
+ * 16-byte aligned; calls that share one must not overlap.
+ */
+int sah_verify_draft(
+    const void* target, const void* draft, const int64_t* tokens, const float* uniforms,
+    const int32_t* counts, const float* temperatures, int64_t* answer, int32_t* accepted,
+    int64_t batch, int64_t drafts, int64_t vocab,
+    int64_t target_stride_b, int64_t target_stride_s,
+    int64_t draft_stride_b, int64_t draft_stride_s, int dtype,
+    void* workspace, size_t workspace_bytes, sah_stream_t stream);
+
+size_t sah_verify_draft_workspace_bytes(int64_t batch, int64_t drafts, int64_t vocab, int sampled);
+
+/*
+ * Book-keeping of the block cache's places on the device.  holders [num_blocks] (int32)
+ * counts the entries of block_table [batch, max_blocks] that name a place; a place
+ * without holders is free, an entry of -1 names none.  Layers of the same sequences
+ * share one table and one book.  Results do not depend on the schedule.  All tensors
+ * contiguous, 4-byte aligned.
+ */
+
+/*
+ * Names a place for every block that appending counts[b] tokens (NULL: tokens; more
+ * count as tokens) behind starts[b] completes and whose entry names none: the lowest free
+ * places in order, sequence by sequence and block by block.  A sequence with a
+ * negative start takes none.  missing[b]: its blocks that found no free place, or
+ * lie behind max_blocks; the append drops them, and they may be reserved later only if
+ * nothing was appended to them.  workspace of
+ * sah_block_pool_reserve_workspace_bytes(), 4-byte aligned, not shared by calls that overlap.
+ */
+int sah_block_pool_reserve(
+    int32_t* block_table, int32_t* holders, const int32_t* starts, const int32_t* counts,
+    int32_t* missing, int64_t batch, int64_t max_blocks, int64_t num_blocks, int64_t tokens,
+    void* workspace, size_t workspace_bytes, sah_stream_t stream);
+size_t sah_block_pool_reserve_workspace_bytes(
+    int64_t batch, int64_t max_blocks, int64_t num_blocks, int64_t tokens);
+
+/* Gives up every block of sequence b but the first lengths[b] / 64 (negative: none). */
+int sah_block_pool_release(
+    int32_t* block_table, int32_t* holders, const int32_t* lengths,
+    int64_t batch, int64_t max_blocks, int64_t num_blocks, sah_stream_t stream);
+
+/*
+ * Sequence b goes on as a copy of sequence sources[b], of which lengths[sources[b]]
+ * tokens are held: it gives up its own blocks and shares the complete ones of its source
+ * (every source as it was before the call, so sequences may change places).  A source
+ * outside [0, batch), or b itself, leaves b as it is.  At most 1024 sequences.  The
+ * tails follow with sah_block_cache_fork(), the lengths by the caller.
+ */
+int sah_block_pool_fork(
+    int32_t* block_table, int32_t* holders, const int32_t* sources, const int32_t* lengths,
+    int64_t batch, int64_t max_blocks, int64_t num_blocks, sah_stream_t stream);
+
+/*
+ * Brings the places that have holders to the front: used[0] counts them, the held places
+ * from there on are renamed to the free ones below, in order, and origins[place]
+ * [num_blocks] is the place whose contents each of these takes (-1 elsewhere), for
+ * sah_block_cache_copy().  Every table that names the places must be this one.
+ * workspace of sah_block_pool_compact_workspace_bytes(), 4-byte aligned, not shared by
+ * calls that overlap.
+ */
+int sah_block_pool_compact(
+    int32_t* block_table, int32_t* holders, int32_t* origins, int32_t* used,
+    int64_t batch, int64_t max_blocks, int64_t num_blocks,
+    void* workspace, size_t workspace_bytes, sah_stream_t stream);
+size_t sah_block_pool_compact_workspace_bytes(int64_t num_blocks);
+
+/*
+ * Copies complete blocks within one layer's cache: place t takes the codes and scales of
+ * place origins[t], where that is another place of [0, num_blocks).  One place may be
+ * the origin of several; a place whose origin is itself to be written keeps what it holds.
+ */
+int sah_block_cache_copy(
+    void* key_codes, void* value_codes, float* key_scales, float* value_scales,
+    const int32_t* origins, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+    sah_stream_t stream);
+
+/* The tails of sequence sources[b], as they were before the call, go to sequence b;
+ * sources as in sah_block_pool_fork(). */
+int sah_block_cache_fork(
+    void* key_tail, void* value_tail, const int32_t* sources,
+    int64_t batch, int64_t kv_heads, int64_t head_dim, sah_stream_t stream);
+
+/*
+ * Makes sequences of lengths[b] tokens ready to go on from ends[b] (at most
+ * lengths[b]): where ends[b] falls into a complete block, and not on its first token, the
+ * tail takes that block's values (its codes times their scale, in dtype; NaN for a block
+ * without a place).  Other tails stay.  Before the block's place is given up or used
+ * again.  What is appended next is coded anew with these values, which are off by one
+ * rounding already.
+ */
+int sah_block_cache_take_back(
+    const void* key_codes, const void* value_codes,
+    const float* key_scales, const float* value_scales,
+    void* key_tail, void* value_tail, const int32_t* block_table,
+    const int32_t* lengths, const int32_t* ends,
+    int64_t batch, int64_t kv_heads, int64_t head_dim,
+    int64_t num_blocks, int64_t max_blocks, int dtype,
     sah_stream_t stream);
 
 #ifdef __cplusplus

@@ -40,6 +40,9 @@ SOURCES = (
     "block_cache.hip",
     "cached_attention.hip",
     "linear_w4.hip",
+    "block_pool.hip",
+    "low_rank.hip",
+    "verify_draft.hip",
 )
 OFFLOAD_ARCH = "gfx950"
 

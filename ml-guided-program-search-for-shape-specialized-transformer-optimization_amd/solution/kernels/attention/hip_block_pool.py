@@ -1,0 +1,441 @@
+"""Book-keeping of the block cache's places on gfx950: reserving, freeing, forking,
+compacting, and the data that moves with it.
+
+No counterpart in the reference.  :class:`BlockPool` holds what the layers of a model share,
+the table of the sequences' blocks and a count of each place's holders, on the device:
+nothing here waits for the host, so a captured step may hold any of it.  Sequences that
+go on from the same tokens share the places of their complete blocks, which are never
+written again.
+
+A step with drafts, of ``drafts + 1`` new tokens a sequence, for every layer::
+
+    hip_block_pool_reserve(pool, starts, drafts + 1)
+    ...                                            # append, attention, the model's logits
+    answer, accepted, _ = hip_verify_draft(logits, tokens, uniforms, draft_logits)
+    lengths, ends = starts + drafts + 1, starts + 1 + accepted
+    for cache in caches:
+        hip_block_cache_take_back(cache, lengths, ends)
+    hip_block_pool_release(pool, ends)
+    starts = ends
+
+Beams and parallel samples go on from ``sources`` [batch]::
+
+    hip_block_pool_fork(pool, sources, lengths)
+    for cache in caches:
+        hip_block_cache_fork(cache, sources)
+    lengths = lengths[sources]
+
+and a pool is compacted, for a smaller one or a copy elsewhere, by::
+
+    origins, used, _ = hip_block_pool_compact(pool)
+    for cache in caches:
+        hip_block_cache_copy(cache, origins)
+
+csrc/block_pool.hip holds the kernels, include/shape_aware_hip.h the definitions.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ..hip._library import (
+    HipLibraryError,
+    dtype_code,
+    launch,
+    library_available,
+    library_for,
+)
+from .hip_block_cache import BLOCK_TOKENS, BlockCache
+
+HIP_BLOCK_POOL_RESERVE_BACKEND = "hip_block_pool_reserve"
+HIP_BLOCK_POOL_RELEASE_BACKEND = "hip_block_pool_release"
+HIP_BLOCK_POOL_FORK_BACKEND = "hip_block_pool_fork"
+HIP_BLOCK_POOL_COMPACT_BACKEND = "hip_block_pool_compact"
+HIP_BLOCK_CACHE_COPY_BACKEND = "hip_block_cache_copy"
+HIP_BLOCK_CACHE_FORK_BACKEND = "hip_block_cache_fork"
+HIP_BLOCK_CACHE_TAKE_BACK_BACKEND = "hip_block_cache_take_back"
+
+MAX_FORKED_SEQUENCES = 1024
+_MAX_TOKENS = 2**31 - 1
+
+
+@dataclass(frozen=True, eq=False)
+class BlockPool:
+    """Which place holds each block of each sequence, and how many entries name a place.
+
+    ``block_table`` [batch, max_blocks] (int32) is the table of the layers'
+    :class:`BlockCache` (-1: no place), ``holders`` [num_blocks] (int32) the number of its
+    entries that name a place.  A place without holders is free.
+    """
+
+    block_table: torch.Tensor
+    holders: torch.Tensor
+
+    def __post_init__(self) -> None:
+        table, holders = self.block_table, self.holders
+        if table.ndim != 2 or holders.ndim != 1 or table.dtype != torch.int32 or holders.dtype != torch.int32:
+            raise ValueError("a pool is block_table [batch, max_blocks] and holders [num_blocks], both int32")
+        if not table.is_contiguous() or not holders.is_contiguous() or holders.device != table.device:
+            raise ValueError("the pool's tensors must be contiguous and on one device")
+
+    @classmethod
+    def allocate(
+        cls, batch: int, *, max_tokens: int, num_blocks: int, device: torch.device | str = "cuda"
+    ) -> "BlockPool":
+        """A pool of free places, for sequences of up to ``max_tokens``."""
+
+        return cls(
+            torch.full((batch, max_tokens // BLOCK_TOKENS), -1, dtype=torch.int32, device=device),
+            torch.zeros((num_blocks,), dtype=torch.int32, device=device),
+        )
+
+    @classmethod
+    def from_table(cls, block_table: torch.Tensor, num_blocks: int) -> "BlockPool":
+        """The pool of a table that names places already."""
+
+        places = block_table[(block_table >= 0) & (block_table < num_blocks)].long()
+        return cls(block_table, torch.bincount(places, minlength=num_blocks).to(torch.int32))
+
+    @property
+    def batch(self) -> int:
+        return self.block_table.shape[0]
+
+    @property
+    def max_blocks(self) -> int:
+        return self.block_table.shape[1]
+
+    @property
+    def num_blocks(self) -> int:
+        return self.holders.shape[0]
+
+
+def hip_block_pool_available() -> bool:
+    """Whether the gfx950 library loads in this process."""
+
+    return library_available()
+
+
+def _words_ok(words: torch.Tensor | None, size: int, index: int) -> bool:
+    return (
+        words is not None
+        and words.dtype is torch.int32
+        and words.shape == (size,)
+        and words.is_contiguous()
+        and words.get_device() == index
+    )
+
+
+def _pool_library(pool: BlockPool, *lengths: torch.Tensor | None):
+    """The library and the device where the kernels take a pool and whole numbers
+    [batch], else None."""
+
+    index = pool.block_table.get_device()
+    if not all(_words_ok(words, pool.batch, index) for words in lengths):
+        return None
+    library = library_for(index)
+    return None if library is None else (library, index)
+
+
+def _reserve_request(pool: BlockPool, starts: torch.Tensor, tokens: int, counts: torch.Tensor | None):
+    if not isinstance(tokens, int) or isinstance(tokens, bool) or not 0 <= tokens <= _MAX_TOKENS:
+        return None
+    return _pool_library(pool, starts, *(() if counts is None else (counts,)))
+
+
+def can_use_hip_block_pool_reserve(
+    pool: BlockPool, starts: torch.Tensor, tokens: int, counts: torch.Tensor | None = None
+) -> bool:
+    """Whether the reserve kernel takes these tensors."""
+
+    return _reserve_request(pool, starts, tokens, counts) is not None
+
+
+def hip_block_pool_reserve(
+    pool: BlockPool, starts: torch.Tensor, tokens: int, counts: torch.Tensor | None = None
+) -> tuple[torch.Tensor, str]:
+    """Name a place for every block that appending ``tokens`` rows (``counts[b]`` of them)
+    behind ``starts`` completes: the lowest free ones, sequence by sequence.
+
+    Before the append.  Returns ``missing`` [batch] (int32), the blocks that found no free
+    place or lie behind the table: the append drops those.
+    """
+
+    request = _reserve_request(pool, starts, tokens, counts)
+    if request is None:
+        raise RuntimeError("HIP block pool reserve is ineligible for the requested inputs")
+    library, index = request
+    sizes = (pool.batch, pool.max_blocks, pool.num_blocks, tokens)
+    missing = torch.empty_like(starts)
+    try:
+        size = library.sah_block_pool_reserve_workspace_bytes(*sizes)
+        workspace = torch.empty(size, dtype=torch.uint8, device=starts.device) if size else None
+        launch(
+            index,
+            library.sah_block_pool_reserve,
+            "sah_block_pool_reserve",
+            pool.block_table.data_ptr(),
+            pool.holders.data_ptr(),
+            starts.data_ptr(),
+            None if counts is None else counts.data_ptr(),
+            missing.data_ptr(),
+            *sizes,
+            None if workspace is None else workspace.data_ptr(),
+            size,
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block pool reserve execution failed") from exc
+    return missing, HIP_BLOCK_POOL_RESERVE_BACKEND
+
+
+def can_use_hip_block_pool_release(pool: BlockPool, lengths: torch.Tensor) -> bool:
+    """Whether the release kernel takes these tensors."""
+
+    return _pool_library(pool, lengths) is not None
+
+
+def hip_block_pool_release(pool: BlockPool, lengths: torch.Tensor) -> str:
+    """Give up every block of a sequence but its first ``lengths[b] // 64`` (0 frees a
+    sequence that has ended, a negative length leaves it)."""
+
+    request = _pool_library(pool, lengths)
+    if request is None:
+        raise RuntimeError("HIP block pool release is ineligible for the requested inputs")
+    library, index = request
+    try:
+        launch(
+            index,
+            library.sah_block_pool_release,
+            "sah_block_pool_release",
+            pool.block_table.data_ptr(),
+            pool.holders.data_ptr(),
+            lengths.data_ptr(),
+            pool.batch,
+            pool.max_blocks,
+            pool.num_blocks,
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block pool release execution failed") from exc
+    return HIP_BLOCK_POOL_RELEASE_BACKEND
+
+
+def can_use_hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.Tensor) -> bool:
+    """Whether the fork kernel takes these tensors."""
+
+    return pool.batch <= MAX_FORKED_SEQUENCES and _pool_library(pool, sources, lengths) is not None
+
+
+def hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.Tensor) -> str:
+    """Let sequence b go on as a copy of sequence ``sources[b]`` of ``lengths[sources[b]]``
+    tokens: it gives up its own blocks and shares the source's complete ones.
+
+    All sources are as they were before the call, so sequences may change places; a
+    source outside [0, batch), or b itself, leaves b as it is.  Each layer's
+    tails follow with :func:`hip_block_cache_fork`.  Up to 1024 sequences.
+    """
+
+    if not can_use_hip_block_pool_fork(pool, sources, lengths):
+        raise RuntimeError("HIP block pool fork is ineligible for the requested inputs")
+    library, index = _pool_library(pool, sources, lengths)
+    try:
+        launch(
+            index,
+            library.sah_block_pool_fork,
+            "sah_block_pool_fork",
+            pool.block_table.data_ptr(),
+            pool.holders.data_ptr(),
+            sources.data_ptr(),
+            lengths.data_ptr(),
+            pool.batch,
+            pool.max_blocks,
+            pool.num_blocks,
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block pool fork execution failed") from exc
+    return HIP_BLOCK_POOL_FORK_BACKEND
+
+
+def can_use_hip_block_pool_compact(pool: BlockPool) -> bool:
+    """Whether the compaction kernels take this pool."""
+
+    return _pool_library(pool) is not None
+
+
+def hip_block_pool_compact(pool: BlockPool) -> tuple[torch.Tensor, torch.Tensor, str]:
+    """Rename the places in use to the pool's lowest ones: ``(origins, used, marker)``.
+
+    ``origins`` [num_blocks] (int32) names the place whose contents each renamed place
+    takes (-1: keeps its own), for :func:`hip_block_cache_copy` of every layer before the
+    cache is read or appended to; ``used`` [1] (int32) counts the places in use.
+    """
+
+    request = _pool_library(pool)
+    if request is None:
+        raise RuntimeError("HIP block pool compact is ineligible for the requested inputs")
+    library, index = request
+    origins = torch.empty_like(pool.holders)
+    used = pool.holders.new_empty((1,))
+    try:
+        size = library.sah_block_pool_compact_workspace_bytes(pool.num_blocks)
+        workspace = torch.empty(size, dtype=torch.uint8, device=origins.device)
+        launch(
+            index,
+            library.sah_block_pool_compact,
+            "sah_block_pool_compact",
+            pool.block_table.data_ptr(),
+            pool.holders.data_ptr(),
+            origins.data_ptr(),
+            used.data_ptr(),
+            pool.batch,
+            pool.max_blocks,
+            pool.num_blocks,
+            workspace.data_ptr(),
+            size,
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block pool compact execution failed") from exc
+    return origins, used, HIP_BLOCK_POOL_COMPACT_BACKEND
+
+
+def _cache_library(cache: BlockCache, size: int, *words: torch.Tensor):
+    """The library and the device where the kernels take a cache and whole numbers
+    [size], else None."""
+
+    index = cache.key_tail.get_device()
+    if not all(_words_ok(word, size, index) for word in words):
+        return None
+    library = library_for(index)
+    return None if library is None else (library, index)
+
+
+def can_use_hip_block_cache_copy(cache: BlockCache, origins: torch.Tensor) -> bool:
+    """Whether the copy kernel takes these tensors."""
+
+    return _cache_library(cache, cache.key_codes.shape[0], origins) is not None
+
+
+def hip_block_cache_copy(cache: BlockCache, origins: torch.Tensor) -> str:
+    """Copy complete blocks within the cache: place t takes what place ``origins[t]``
+    holds, where that is another place (``origins`` [num_blocks], int32).
+
+    Several places may have one origin.  A place whose origin is itself to be written by
+    the call keeps what it holds.
+    """
+
+    request = _cache_library(cache, cache.key_codes.shape[0], origins)
+    if request is None:
+        raise RuntimeError("HIP block cache copy is ineligible for the requested inputs")
+    library, index = request
+    try:
+        launch(
+            index,
+            library.sah_block_cache_copy,
+            "sah_block_cache_copy",
+            *cache._pointers()[:4],
+            origins.data_ptr(),
+            cache.kv_heads,
+            cache.head_dim,
+            cache.key_codes.shape[0],
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block cache copy execution failed") from exc
+    return HIP_BLOCK_CACHE_COPY_BACKEND
+
+
+def can_use_hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> bool:
+    """Whether the fork kernel takes these tensors."""
+
+    return cache.batch <= MAX_FORKED_SEQUENCES and _cache_library(cache, cache.batch, sources) is not None
+
+
+def hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> str:
+    """Copy the incomplete block of sequence ``sources[b]``, as it was before the call, to
+    sequence b, with the sources of :func:`hip_block_pool_fork`."""
+
+    if not can_use_hip_block_cache_fork(cache, sources):
+        raise RuntimeError("HIP block cache fork is ineligible for the requested inputs")
+    library, index = _cache_library(cache, cache.batch, sources)
+    try:
+        launch(
+            index,
+            library.sah_block_cache_fork,
+            "sah_block_cache_fork",
+            cache.key_tail.data_ptr(),
+            cache.value_tail.data_ptr(),
+            sources.data_ptr(),
+            cache.batch,
+            cache.kv_heads,
+            cache.head_dim,
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block cache fork execution failed") from exc
+    return HIP_BLOCK_CACHE_FORK_BACKEND
+
+
+def can_use_hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> bool:
+    """Whether the take-back kernel takes these tensors."""
+
+    return _cache_library(cache, cache.batch, lengths, ends) is not None
+
+
+def hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> str:
+    """Make sequences of ``lengths[b]`` tokens ready to go on from ``ends[b]``, anywhere
+    up to that.
+
+    Where ``ends[b]`` falls into a complete block, the tail takes that block's values
+    back: its codes times their scale, so these tokens are coded a second time once
+    their block is complete again.  Call it before the block's place is released or
+    written; ``starts = ends`` from then on.
+    """
+
+    request = _cache_library(cache, cache.batch, lengths, ends)
+    if request is None:
+        raise RuntimeError("HIP block cache take back is ineligible for the requested inputs")
+    library, index = request
+    try:
+        launch(
+            index,
+            library.sah_block_cache_take_back,
+            "sah_block_cache_take_back",
+            *cache._pointers(),
+            lengths.data_ptr(),
+            ends.data_ptr(),
+            cache.batch,
+            cache.kv_heads,
+            cache.head_dim,
+            cache.key_codes.shape[0],
+            cache.block_table.shape[1],
+            dtype_code(cache.key_tail.dtype),
+        )
+    except HipLibraryError as exc:
+        raise RuntimeError("HIP block cache take back execution failed") from exc
+    return HIP_BLOCK_CACHE_TAKE_BACK_BACKEND
+
+
+__all__ = [
+    "BlockPool",
+    "HIP_BLOCK_CACHE_COPY_BACKEND",
+    "HIP_BLOCK_CACHE_FORK_BACKEND",
+    "HIP_BLOCK_CACHE_TAKE_BACK_BACKEND",
+    "HIP_BLOCK_POOL_COMPACT_BACKEND",
+    "HIP_BLOCK_POOL_FORK_BACKEND",
+    "HIP_BLOCK_POOL_RELEASE_BACKEND",
+    "HIP_BLOCK_POOL_RESERVE_BACKEND",
+    "MAX_FORKED_SEQUENCES",
+    "can_use_hip_block_cache_copy",
+    "can_use_hip_block_cache_fork",
+    "can_use_hip_block_cache_take_back",
+    "can_use_hip_block_pool_compact",
+    "can_use_hip_block_pool_fork",
+    "can_use_hip_block_pool_release",
+    "can_use_hip_block_pool_reserve",
+    "hip_block_cache_copy",
+    "hip_block_cache_fork",
+    "hip_block_cache_take_back",
+    "hip_block_pool_available",
+    "hip_block_pool_compact",
+    "hip_block_pool_fork",
+    "hip_block_pool_release",
+    "hip_block_pool_reserve",
+]

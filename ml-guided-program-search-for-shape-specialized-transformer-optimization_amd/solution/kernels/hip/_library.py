@@ -120,6 +120,22 @@ _SIGNATURES: dict[str, tuple[list[object], object]] = {
     ),
     "sah_block_cache_attention_workspace_bytes": ([_i64] * 6, ctypes.c_size_t),
     "sah_linear_w4": ([_ptr] * 5 + [_i64] * 6 + [_int] * 2 + [_ptr], _int),
+    "sah_low_rank_adapters": ([_ptr] * 9 + [_i64] * 6 + [_i64] * 6 + [_int, _ptr, ctypes.c_size_t, _ptr], _int),
+    "sah_low_rank_adapters_workspace_bytes": ([_i64] * 5, ctypes.c_size_t),
+    "sah_verify_draft": (
+        [_ptr] * 8 + [_i64] * 3 + [_i64] * 4 + [_int, _ptr, ctypes.c_size_t, _ptr],
+        _int,
+    ),
+    "sah_verify_draft_workspace_bytes": ([_i64] * 3 + [_int], ctypes.c_size_t),
+    "sah_block_pool_reserve": ([_ptr] * 5 + [_i64] * 4 + [_ptr, ctypes.c_size_t, _ptr], _int),
+    "sah_block_pool_reserve_workspace_bytes": ([_i64] * 4, ctypes.c_size_t),
+    "sah_block_pool_release": ([_ptr] * 3 + [_i64] * 3 + [_ptr], _int),
+    "sah_block_pool_fork": ([_ptr] * 4 + [_i64] * 3 + [_ptr], _int),
+    "sah_block_pool_compact": ([_ptr] * 4 + [_i64] * 3 + [_ptr, ctypes.c_size_t, _ptr], _int),
+    "sah_block_pool_compact_workspace_bytes": ([_i64], ctypes.c_size_t),
+    "sah_block_cache_copy": ([_ptr] * 5 + [_i64] * 3 + [_ptr], _int),
+    "sah_block_cache_fork": ([_ptr] * 3 + [_i64] * 3 + [_ptr], _int),
+    "sah_block_cache_take_back": ([_ptr] * 9 + [_i64] * 5 + [_int, _ptr], _int),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 # SAH_ATTENTION_STATIC_WORKSPACE_BYTES of the header: the device array behind
