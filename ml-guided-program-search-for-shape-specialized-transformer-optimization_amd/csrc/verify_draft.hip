@@ -9,15 +9,27 @@
 //
 // A token is chosen at a border between two, of which there are as many as tokens: sums
 // wrong by 1e-7, as fp32 leaves them, choose another token once in 10^7 / vocabulary
-// requests.  Exponentials, sums and weights are fp64 (v_fma_f64 issues at fp32's rate
-// here): the choice is that of exact arithmetic but for borders closer than 1e-15 or so
-// of the whole.
+// requests.  The choice here is that of exact arithmetic, but for borders closer than some
+// 1e-14 of the whole:
+//   1. rows: a chunk of a row's largest logit and sum of exponentials, in fp32 (a row's
+//      sum comes out right to kFastError).  The one pass over all logits, bound by them;
+//   2. decide: p_i(x_i), q_i(x_i) from these; where the test's two sides lie within
+//      that error, from sums in fp64.  j is known;
+//   3. weigh: of row j alone, in fp64.  With e_p, e_q the exponentials and r = sum e_p /
+//      sum e_q, the weights are in proportion to max(e_p - r e_q, 0).  r is known to
+//      fp32's precision; a chunk adds up e_p, e_q, and both over the tokens S where
+//      e_p > r e_q.  Its weight is then sum_S e_p - r sum_S e_q for the r that the
+//      sums of all chunks give: a token that changes sides between one r and the other
+//      has a weight of their distance at most, and so many do, which leaves the
+//      distance's square;
+//   4. pick: r, the chunk in which the sum passes the border, the token.
 //
-// Bound by the logits, read once (rows that count alone), in three parts:
-//   1. a workgroup's chunk of a row: largest logit, its place, sum of exponentials;
-//   2. each chunk of the chosen row: every workgroup finds j by itself from the parts,
-//      then the sum of its chunk's weights;
-//   3. the workgroup of a request that comes last finds the chunk, then the token.
+// 64 requests, 7 drafts, 131072 tokens, bf16 (252 MB, 51 us at a large copy's rate): rows
+// 56 us, decide 7, weigh 22, pick 6.  fp64's v_fma issues at fp32's rate here, but with
+// all rows in fp64 the vector units took 126 us for them.  The draw's two parts in one
+// launch, by the request's last workgroup, took 106 us instead of 27: each of the 4096
+// releases its L2's lines.  For one request (4 drafts, 32000 tokens) each part is a
+// launch's latency, 4 us.
 
 #include <type_traits>
 
@@ -26,18 +38,39 @@
 namespace sah {
 namespace {
 
+constexpr int kVec = 8;  // logits of one access
 constexpr int kRowThreads = 256;
-constexpr int kVec = 8;         // logits of one access
-constexpr int kAccesses = 4;    // of a thread
-constexpr int kChunk = kRowThreads * kVec * kAccesses;
-constexpr int kPickThreads = kChunk / kVec;
+constexpr int kAccesses = 4;  // of a thread
+constexpr int kRowChunk = kRowThreads * kVec * kAccesses;
+constexpr int kDecideThreads = 1024;
+constexpr int kPickThreads = 256;
+constexpr int kPickChunk = kPickThreads * kVec;
 constexpr int kMaxDrafts = 1024;
 constexpr double kLog2e = 1.4426950408889634074;
+// A row's sum in fp32, relative: an exponent |x| <= 64 (what lies below adds less than
+// 2^-33) is off by its difference's, its factor's and its product's rounding, 3 * 64 *
+// 2^-24 ln 2 = 8e-6; v_exp_f32 by 2^-22, 32 additions by 2e-6.  Two rows: 2^-15.
+constexpr double kFastError = 1.0 / 32768.0;
 
 struct RowPart {
-  double sum;   // of exp2((l - top) c)
-  float top;    // the largest logit; NaN where one is NaN
-  int32_t at;   // its lowest place
+  double sum;  // of exp2((l - top) c); NaN where a logit is NaN or +inf
+  float top;   // the largest logit
+  int32_t at;  // its lowest place (greedy requests)
+};
+
+// What the decision leaves for the draw, of one request.
+struct Choice {
+  int32_t row;      // the first draft that does not stand, or the number of drafts
+  int32_t mode;     // how the next token is drawn
+  float p_top, q_top;
+  double ratio;     // sum e_p / sum e_q, about
+  double c;         // log2(e) / temperature
+};
+enum { kDone = 0, kFromTarget = 1, kWithout = 2, kResample = 3 };
+
+struct Weights {
+  double p, q;          // sums of e_p, e_q
+  double p_over, q_over;  // where e_p > ratio e_q
 };
 
 struct VerifyArgs {
@@ -50,33 +83,34 @@ struct VerifyArgs {
   int64_t* answer;
   int32_t* accepted;
   int64_t t_sb, t_ss, d_sb, d_ss;
-  RowPart* parts;        // [batch][drafts + 1 (+ drafts)][chunks]
-  double* weights;       // [batch][chunks]
-  uint32_t* tickets;     // [batch]
-  int batch, drafts, vocab, chunks;
+  RowPart* parts;     // [batch][drafts + 1 (+ drafts)][row_chunks]
+  Weights* weights;   // [batch][pick_chunks]
+  Choice* choices;    // [batch]
+  int batch, drafts, vocab, row_chunks, pick_chunks;
 };
 
-// 2^x for x <= 0, 0 from below the smallest number on: x = n + f with |f| <= 1/2, and
-// 2^f = e^(f ln 2) as its series, whose first term left out is (ln 2 / 2)^13 / 13!,
-// below 2^-52.
+// 2^x for x <= 0, 0 from below the smallest number on (and for NaN, which no row that is
+// drawn from has): x = n + f with |f| <= 1/2, and for 2^f the polynomial that meets it at
+// the 11 Chebyshev points of that interval, off by 2^-51 of it.
 __device__ __forceinline__ double exp2_upto0(double x) {
-  x = x < -1100.0 ? -1100.0 : x;
+  x = fmax(x, -1100.0);
   const double n = __builtin_rint(x);
-  const double f = (x - n) * 0.69314718055994530942;
-  double y = 1.0 / 479001600.0;
-  y = fma(y, f, 1.0 / 39916800.0);
-  y = fma(y, f, 1.0 / 3628800.0);
-  y = fma(y, f, 1.0 / 362880.0);
-  y = fma(y, f, 1.0 / 40320.0);
-  y = fma(y, f, 1.0 / 5040.0);
-  y = fma(y, f, 1.0 / 720.0);
-  y = fma(y, f, 1.0 / 120.0);
-  y = fma(y, f, 1.0 / 24.0);
-  y = fma(y, f, 1.0 / 6.0);
-  y = fma(y, f, 0.5);
-  y = fma(y, f, 1.0);
+  const double f = x - n;
+  double y = 0x1.e6063f7217bc6p-28;
+  y = fma(y, f, 0x1.b675bca4eeebbp-24);
+  y = fma(y, f, 0x1.62bfd47773353p-20);
+  y = fma(y, f, 0x1.ffcb54062e698p-17);
+  y = fma(y, f, 0x1.430913096fd9fp-13);
+  y = fma(y, f, 0x1.5d87fe9d7a584p-10);
+  y = fma(y, f, 0x1.3b2ab6fba1ddap-7);
+  y = fma(y, f, 0x1.c6b08d703ce49p-5);
+  y = fma(y, f, 0x1.ebfbdff82c598p-3);
+  y = fma(y, f, 0x1.62e42fefa3a19p-1);
   y = fma(y, f, 1.0);
   return ldexp(y, (int)n);
+}
+__device__ __forceinline__ double weight_of(float logit, float top, double c) {
+  return exp2_upto0(((double)logit - (double)top) * c);
 }
 
 // log2(e) / temperature, and whether the request answers greedily instead (a temperature
@@ -114,68 +148,144 @@ __device__ __forceinline__ void load_logits(const T* row, int64_t at, int64_t vo
   }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+// Values of other lanes: within 16 by DPP (lane ^ 1, lane ^ 2, 7 - lane of 8, 15 - lane),
+// which takes no trip through LDS; across 16 and 32 by the lane swaps, whose two results
+// are the two partners of every lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(dpp<CTRL>(__float_as_uint(v)));
+}
+template <int CTRL>
+__device__ __forceinline__ int32_t dpp(int32_t v) {
+  return (int32_t)dpp<CTRL>((uint32_t)v);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(double, (u32x2){dpp<CTRL>(w[0]), dpp<CTRL>(w[1])});
+}
+template <int LANES>
+__device__ __forceinline__ void swap_lanes(uint32_t v, uint32_t& a, uint32_t& b) {
+  const u32x2 r = LANES == 16 ? __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(v, v, false, false))
+                              : __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+  a = r[0];
+  b = r[1];
+}
+template <int LANES>
+__device__ __forceinline__ void swap_lanes(float v, float& a, float& b) {
+  uint32_t x, y;
+  swap_lanes<LANES>(__float_as_uint(v), x, y);
+  a = __uint_as_float(x);
+  b = __uint_as_float(y);
+}
+template <int LANES>
+__device__ __forceinline__ void swap_lanes(int32_t v, int32_t& a, int32_t& b) {
+  uint32_t x, y;
+  swap_lanes<LANES>((uint32_t)v, x, y);
+  a = (int32_t)x;
+  b = (int32_t)y;
+}
+template <int LANES>
+__device__ __forceinline__ void swap_lanes(double v, double& a, double& b) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  u32x2 x, y;
+  uint32_t x0, x1, y0, y1;
+  swap_lanes<LANES>(w[0], x0, y0);
+  swap_lanes<LANES>(w[1], x1, y1);
+  x = (u32x2){x0, x1};
+  y = (u32x2){y0, y1};
+  a = __builtin_bit_cast(double, x);
+  b = __builtin_bit_cast(double, y);
+}
+// op over the wave, in every lane.
+template <typename V, typename Op>
+__device__ __forceinline__ V wave_reduce(V v, Op op) {
+  v = op(v, dpp<0xB1>(v));
+  v = op(v, dpp<0x4E>(v));
+  v = op(v, dpp<0x141>(v));
+  v = op(v, dpp<0x140>(v));
+  V a, b;
+  swap_lanes<16>(v, a, b);
+  v = op(a, b);
+  swap_lanes<32>(v, a, b);
+  return op(a, b);
+}
+template <typename V>
+__device__ __forceinline__ V wave_add(V v) {
+  return wave_reduce(v, [](V a, V b) { return a + b; });
+}
+__device__ __forceinline__ float wave_largest(float v) {
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ int32_t wave_lowest(int32_t v) {
+  return wave_reduce(v, [](int32_t a, int32_t b) { return b < a ? b : a; });
+}
+// The sum over the lanes up to this one: within 16 by shifts, then the last lanes of the
+// 16 and the 32 before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  const u32x2 r = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[0], CTRL, ROWS, 0xF, false),
+                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[1], CTRL, ROWS, 0xF, false)};
+  return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double wave_up_to(double v) {
+  v += dpp_or_zero<0x111, 0xF>(v);
+  v += dpp_or_zero<0x112, 0xF>(v);
+  v += dpp_or_zero<0x114, 0xF>(v);
+  v += dpp_or_zero<0x118, 0xF>(v);
+  v += dpp_or_zero<0x142, 0xA>(v);
+  v += dpp_or_zero<0x143, 0xC>(v);
   return v;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(const VerifyArgs a) {
-  __shared__ float tops[kRowThreads / 64];
-  __shared__ int32_t bads[kRowThreads / 64];
-  __shared__ double totals[kRowThreads / 64];
-  __shared__ int32_t places[kRowThreads / 64];
+  constexpr int WAVES = kRowThreads / 64;
+  __shared__ float tops[WAVES];
+  __shared__ float sums[WAVES];
+  __shared__ int32_t places[WAVES];
   const int rows = a.drafts + 1 + (a.draft != nullptr ? a.drafts : 0);
-  const uint32_t chunk = blockIdx.x % (uint32_t)a.chunks;
-  const uint32_t request_row = blockIdx.x / (uint32_t)a.chunks;
+  const uint32_t chunk = blockIdx.x % (uint32_t)a.row_chunks;
+  const uint32_t request_row = blockIdx.x / (uint32_t)a.row_chunks;
   const int64_t b = request_row / (uint32_t)rows;
   const int r = (int)(request_row % (uint32_t)rows);
   const int tid = threadIdx.x, wave = tid >> 6;
-  if (r == 0 && chunk == 0 && tid == 0) a.tickets[b] = 0;
   const int count = drafts_of(a, b);
   const bool is_draft = r > a.drafts;
   if (is_draft ? r - a.drafts - 1 >= count : r > count) return;
-  double c;
-  const bool greedy = is_greedy(a, b, c);
+  double factor;
+  const bool greedy = is_greedy(a, b, factor);
   if (greedy && is_draft) return;  // a greedy request's draft stands by the target alone
   const T* row = is_draft ? static_cast<const T*>(a.draft) + b * a.d_sb + (r - a.drafts - 1) * a.d_ss
                           : static_cast<const T*>(a.target) + b * a.t_sb + r * a.t_ss;
-  const int64_t first = (int64_t)chunk * kChunk + tid * kVec;
+  const int64_t first = (int64_t)chunk * kRowChunk + tid * kVec;
   float l[kAccesses][kVec];
 #pragma unroll
   for (int i = 0; i < kAccesses; ++i) load_logits<T>(row, first + (int64_t)i * kRowThreads * kVec, a.vocab, l[i]);
   float top = -INFINITY;
-  bool bad = false;
 #pragma unroll
   for (int i = 0; i < kAccesses; ++i)
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      top = fmaxf(top, l[i][e]);
-      bad = bad || l[i][e] != l[i][e];
-    }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const bool any_bad = __ballot(bad) != 0;
-  if ((tid & 63) == 0) {
-    tops[wave] = top;
-    bads[wave] = any_bad ? 1 : 0;
-  }
+    for (int e = 0; e < kVec; ++e) top = fmaxf(top, l[i][e]);
+  top = wave_largest(top);
+  if ((tid & 63) == 0) tops[wave] = top;
   __syncthreads();
-  int32_t nan = 0;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 64; ++w) {
-    top = fmaxf(top, tops[w]);
-    nan |= bads[w];
-  }
-  double sum = 0.0;
-  if (top > -INFINITY && top < INFINITY) {
-    const double base = (double)top;
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
+  // Differences of -inf from -inf would be NaN, which stands for a bad logit; from +inf
+  // they are meant to be.
+  const float base = top == -INFINITY ? 0.0f : top;
+  const float c = fminf((float)factor, 3e38f);
+  float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kAccesses; ++i)
+  for (int i = 0; i < kAccesses; ++i)
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum += exp2_upto0(((double)l[i][e] - base) * c);
-  }
+    for (int e = 0; e < kVec; ++e) sum += __builtin_amdgcn_exp2f((l[i][e] - base) * c);
   int32_t at = INT32_MAX;
   if (greedy) {
 #pragma unroll
@@ -183,91 +293,92 @@ __global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(const VerifyAr
 #pragma unroll
       for (int e = kVec - 1; e >= 0; --e)
         if (l[i][e] == top) at = (int32_t)(first + (int64_t)i * kRowThreads * kVec + e);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int32_t other = __shfl_xor(at, d);
-      at = other < at ? other : at;
-    }
+    at = wave_lowest(at);
   }
-  sum = wave_sum(sum);
+  sum = wave_add(sum);
   if ((tid & 63) == 0) {
-    totals[wave] = sum;
+    sums[wave] = sum;
     places[wave] = at;
   }
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kRowThreads / 64; ++w) {
-      sum += totals[w];
+    double total = (double)sum;
+    for (int w = 1; w < WAVES; ++w) {
+      total += (double)sums[w];
       at = places[w] < at ? places[w] : at;
     }
-    RowPart* part = a.parts + (int64_t)request_row * a.chunks + chunk;
-    part->sum = sum;
-    part->top = nan != 0 ? NAN : top;
+    RowPart* part = a.parts + (int64_t)request_row * a.row_chunks + chunk;
+    part->sum = total;
+    part->top = top;
     part->at = at;
   }
 }
 
-// A row's statistics from its chunks', by one wave: the largest logit (not finite: the
-// row has no distribution), its place and the sum.
+// A row's statistics from its chunks', by one wave.
 struct RowSum {
   double sum;
   float top;
   int32_t at;
+  __device__ bool there() const { return top > -INFINITY && top < INFINITY && sum == sum; }
 };
 __device__ __forceinline__ RowSum merge_row(const RowPart* parts, int chunks, double c) {
   const int lane = threadIdx.x & 63;
-  float top = -INFINITY;
-  bool bad = false;
-  for (int i = lane; i < chunks; i += 64) {
-    const float t = parts[i].top;
-    bad = bad || t != t;
-    top = fmaxf(top, t);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  if (__ballot(bad) != 0) top = NAN;
+  RowPart part{0.0, -INFINITY, INT32_MAX};
+  if (lane < chunks) part = parts[lane];
+  float top = part.top;
+  for (int i = lane + 64; i < chunks; i += 64) top = fmaxf(top, parts[i].top);
+  top = wave_largest(top);
   double sum = 0.0;
   int32_t at = INT32_MAX;
-  if (top > -INFINITY && top < INFINITY)
-    for (int i = lane; i < chunks; i += 64) {
-      const RowPart p = parts[i];
-      if (p.top > -INFINITY) sum += p.sum * exp2_upto0(((double)p.top - (double)top) * c);
-      if (p.top == top && p.at < at) at = p.at;
-    }
-  sum = wave_sum(sum);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int32_t other = __shfl_xor(at, d);
-    at = other < at ? other : at;
+  for (int i = lane; i < chunks; i += 64) {
+    if (i != lane) part = parts[i];
+    // (a sum that is NaN stays it)
+    if (part.sum != 0.0) sum += part.sum * weight_of(part.top, top, c);
+    if (part.top == top && part.at < at) at = part.at;
   }
-  return {sum, top, at};
+  return {wave_add(sum), top, wave_lowest(at)};
 }
 
-struct Chosen {
-  int row;         // the first draft that does not stand, or the number of drafts
-  int resample;    // 1: from max(p - q, 0)
-  float p_top, q_top;
-  double p_sum, q_sum;
-  int32_t at;      // place of the largest logit of target's row
-  int32_t none;    // 1: no distribution to draw from
-};
-
+// A row's sum of exponentials in fp64, by the workgroup.
 template <typename T>
-__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
-  constexpr int WAVES = kPickThreads / 64;
-  __shared__ Chosen found[WAVES];
-  __shared__ double totals[WAVES];
-  __shared__ int32_t is_last, chosen_chunk;
-  __shared__ double border[2];
-  const uint32_t chunk = blockIdx.x % (uint32_t)a.chunks;
-  const int64_t b = blockIdx.x / (uint32_t)a.chunks;
+__device__ double exact_sum(const T* row, float top, double c, int64_t vocab, double* waves) {
+  double sum = 0.0;
+  for (int64_t at = (int64_t)threadIdx.x * kVec; at < vocab; at += kDecideThreads * kVec) {
+    float l[kVec];
+    load_logits<T>(row, at, vocab, l);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum += weight_of(l[e], top, c);
+  }
+  sum = wave_add(sum);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < kDecideThreads / 64; ++w) sum += waves[w];
+  return sum;
+}
+
+// A workgroup a request; a wave a row of the target, with the draft's beside it.  16 rows
+// at a time, up to the first draft that does not stand.
+template <typename T>
+__global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(const VerifyArgs a) {
+  constexpr int WAVES = kDecideThreads / 64;
+  struct Seen {
+    RowSum p, q;
+    int32_t stands;   // 1: the draft stands, 0: it does not, -1: too near to say
+    int32_t none;     // 1: no distribution to draw from
+  };
+  __shared__ Seen seen[WAVES];
+  __shared__ double sums[WAVES];
+  const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int count = drafts_of(a, b);
   int64_t* answer = a.answer + b * (a.drafts + 1);
   if (count < 0) {
-    if (chunk == 0) {
-      for (int i = tid; i <= a.drafts; i += kPickThreads) answer[i] = -1;
-      if (tid == 0) a.accepted[b] = -1;
+    for (int i = tid; i <= a.drafts; i += kDecideThreads) answer[i] = -1;
+    if (tid == 0) {
+      a.accepted[b] = -1;
+      a.choices[b].mode = kDone;
     }
     return;
   }
@@ -275,226 +386,258 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   const bool greedy = is_greedy(a, b, c);
   const bool sampled = a.draft != nullptr && !greedy;
   const int rows = a.drafts + 1 + (a.draft != nullptr ? a.drafts : 0);
-  const RowPart* parts = a.parts + b * rows * a.chunks;
+  const RowPart* parts = a.parts + b * rows * a.row_chunks;
   const T* target = static_cast<const T*>(a.target) + b * a.t_sb;
   const T* draft = static_cast<const T*>(a.draft) + b * a.d_sb;
+  const int64_t* tokens = a.tokens + b * a.drafts;
+  const float* uniforms = a.uniforms + b * (a.drafts + 1);
 
-  // The waves take the rows in turn until one finds the first that does not stand; a
-  // wave's own first is the lowest of its rows, and the lowest of them all is j.
-  Chosen mine{count + 1, 0, 0.0f, 0.0f, 1.0, 1.0, 0, 0};
-  for (int i = wave; i <= count; i += WAVES) {
-    const RowSum p = merge_row(parts + (int64_t)i * a.chunks, a.chunks, c);
-    const bool p_there = p.top > -INFINITY && p.top < INFINITY;
-    RowSum q{1.0, 0.0f, 0};
-    bool q_there = true;
-    bool stands = false;
-    if (i < count) {
-      const int64_t token = a.tokens[b * a.drafts + i];
+  int j = -1;
+  Seen found{};
+  for (int first = 0; j < 0; first += WAVES) {
+    const int i = first + wave;
+    if (i <= count) {
+      const int64_t token = i < count ? tokens[i] : -1;
       const bool known = token >= 0 && token < a.vocab;
-      if (sampled) {
-        q = merge_row(parts + (int64_t)(a.drafts + 1 + i) * a.chunks, a.chunks, c);
-        q_there = q.top > -INFINITY && q.top < INFINITY;
-      }
-      if (p_there && q_there && known) {
+      float p_logit = 0.0f, q_logit = 0.0f;
+      if (known) p_logit = to_f32(target[i * a.t_ss + token]);
+      if (known && sampled) q_logit = to_f32(draft[i * a.d_ss + token]);
+      Seen mine{};
+      mine.p = merge_row(parts + (int64_t)i * a.row_chunks, a.row_chunks, c);
+      mine.q = {1.0, 0.0f, 0};
+      if (sampled && i < count) mine.q = merge_row(parts + (int64_t)(a.drafts + 1 + i) * a.row_chunks, a.row_chunks, c);
+      mine.none = mine.p.there() && mine.q.there() ? 0 : 1;
+      if (mine.none == 0 && known) {
         if (greedy) {
-          stands = p.at == token;
+          mine.stands = mine.p.at == token ? 1 : 0;
         } else {
-          const double chance = exp2_upto0(((double)to_f32(target[i * a.t_ss + token]) - (double)p.top) * c) / p.sum;
-          double other = 1.0;
-          if (sampled) other = exp2_upto0(((double)to_f32(draft[i * a.d_ss + token]) - (double)q.top) * c) / q.sum;
-          stands = (double)a.uniforms[b * (a.drafts + 1) + i] * other < chance;
+          const double p = weight_of(p_logit, mine.p.top, c) / mine.p.sum;
+          double q = (double)uniforms[i];
+          if (sampled) q *= weight_of(q_logit, mine.q.top, c) / mine.q.sum;
+          mine.stands = fabs(q - p) <= kFastError * p && p > 0.0 ? -1 : q < p ? 1 : 0;
         }
       }
+      if (lane == 0) seen[wave] = mine;
     }
-    if (!stands) {
-      mine = {i, i < count ? 1 : 0, p.top, q.top, p.sum, q.sum, p.at, p_there && q_there ? 0 : 1};
-      break;
-    }
-  }
-  if (lane == 0) found[wave] = mine;
-  __syncthreads();
-  Chosen at = found[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w)
-    if (found[w].row < at.row) at = found[w];
-  const int j = at.row;
-
-  auto write = [&](int64_t token) {  // by the workgroup's every thread
-    for (int i = tid; i <= a.drafts; i += kPickThreads)
-      answer[i] = i < j ? a.tokens[b * a.drafts + i] : i == j ? token : -1;
-    if (tid == 0) a.accepted[b] = j;
-  };
-  if (greedy || at.none != 0) {
-    if (chunk == 0) write(at.none != 0 ? -1 : at.at);
-    return;
-  }
-
-  // The weights of 8 tokens; zeros behind the row's end.
-  const bool resample = at.resample != 0;
-  const int64_t drafted = resample ? a.tokens[b * a.drafts + j] : -1;
-  const T* p_row = target + j * a.t_ss;
-  const T* q_row = draft + j * a.d_ss;
-  auto weigh = [&](int64_t first, double* w) {
-    float l[kVec];
-    load_logits<T>(p_row, first, a.vocab, l);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e)
-      w[e] = exp2_upto0(((double)l[e] - (double)at.p_top) * c) / at.p_sum;
-    if (!resample) return;
-    if (sampled) {
-      load_logits<T>(q_row, first, a.vocab, l);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const double less = w[e] - exp2_upto0(((double)l[e] - (double)at.q_top) * c) / at.q_sum;
-        w[e] = less > 0.0 ? less : 0.0;
+    __syncthreads();
+    for (int w = 0; w < WAVES && j < 0; ++w) {
+      const int at = first + w;
+      int stands = seen[w].stands;
+      if (stands < 0) {  // (the same for every thread)
+        const int64_t token = tokens[at];
+        const Seen& it = seen[w];
+        const T* p_row = target + at * a.t_ss;
+        const double p = weight_of(to_f32(p_row[token]), it.p.top, c) / exact_sum<T>(p_row, it.p.top, c, a.vocab, sums);
+        double q = (double)uniforms[at];
+        if (sampled) {
+          const T* q_row = draft + at * a.d_ss;
+          q *= weight_of(to_f32(q_row[token]), it.q.top, c) / exact_sum<T>(q_row, it.q.top, c, a.vocab, sums);
+        }
+        stands = q < p ? 1 : 0;
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (first + e == drafted) w[e] = 0.0;
+      if (stands == 0 || at == count) {
+        j = at;
+        found = seen[w];
+      }
     }
-  };
+    __syncthreads();
+  }
 
-  double w[kVec];
-  weigh((int64_t)chunk * kChunk + tid * kVec, w);
-  double sum = 0.0;
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) sum += w[e];
-  sum = wave_sum(sum);
-  if (lane == 0) totals[wave] = sum;
-  __syncthreads();
-  double* weights = a.weights + b * a.chunks;
+  const bool done = greedy || found.none != 0;
+  for (int i = tid; i <= a.drafts; i += kDecideThreads) {
+    if (i < j)
+      answer[i] = tokens[i];
+    else if (i > j || done)  // answer[j] is the draw's otherwise
+      answer[i] = i == j && found.none == 0 ? found.p.at : -1;
+  }
   if (tid == 0) {
-    double total = 0.0;
-#pragma unroll
-    for (int k = 0; k < WAVES; ++k) total += totals[k];
-    __hip_atomic_store(weights + chunk, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const uint32_t ticket = __hip_atomic_fetch_add(a.tickets + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    is_last = ticket + 1 == (uint32_t)a.chunks ? 1 : 0;
+    a.accepted[b] = j;
+    Choice choice{j, kDone, found.p.top, found.q.top, 0.0, c};
+    if (!done) choice.mode = j == count ? kFromTarget : sampled ? kResample : kWithout;
+    if (choice.mode == kResample) choice.ratio = found.p.sum / found.q.sum;
+    a.choices[b] = choice;
   }
-  __syncthreads();
-  if (is_last == 0) return;
+}
 
-  // The last workgroup: the chunk in which the sum passes u times the whole.
-  if (wave == 0) {
-    double whole = 0.0;
-    for (int i = 0; i < a.chunks; i += 64) {
-      const double v = i + lane < a.chunks
-                           ? __hip_atomic_load(weights + i + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                           : 0.0;
-      whole += wave_sum(v);
-    }
-    const double bound = (double)a.uniforms[b * (a.drafts + 1) + a.drafts] * whole;
-    double before = 0.0, last_before = 0.0;
-    int chosen = -1, last = -1;
-    for (int i = 0; i < a.chunks && chosen < 0; i += 64) {
-      const double v = i + lane < a.chunks
-                           ? __hip_atomic_load(weights + i + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                           : 0.0;
-      double up_to = v;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double other = __shfl_up(up_to, d);
-        if (lane >= d) up_to += other;
-      }
-      const uint64_t some = __ballot(v > 0.0);
-      const uint64_t above = __ballot(v > 0.0 && before + up_to > bound);
-      const double mine_before = before + (up_to - v);
-      if (some != 0) {
-        const int k = 63 - __clzll((long long)some);
-        last = i + k;
-        last_before = __shfl(mine_before, k);
-      }
-      if (above != 0) {
-        const int k = __ffsll((unsigned long long)above) - 1;
-        chosen = i + k;
-        last_before = __shfl(mine_before, k);
-      }
-      before += __shfl(up_to, 63);
-    }
-    if (lane == 0) {
-      chosen_chunk = chosen >= 0 ? chosen : last;  // (a border of rounding: the last weight)
-      border[0] = last_before;
-      border[1] = bound;
-    }
+// e_p and e_q of 8 tokens (e_q: 0 where it takes no part); zeros behind the row's end.
+template <typename T>
+struct Rows {
+  const T* p_row;
+  const T* q_row;
+  int64_t drafted;  // the token that a certain draft takes out
+  __device__ Rows(const VerifyArgs& a, int64_t b, const Choice& it) {
+    p_row = static_cast<const T*>(a.target) + b * a.t_sb + it.row * a.t_ss;
+    q_row = static_cast<const T*>(a.draft) + b * a.d_sb + it.row * a.d_ss;
+    drafted = it.mode == kWithout ? a.tokens[b * a.drafts + it.row] : -1;
   }
+  __device__ __forceinline__ void weigh(const VerifyArgs& a, const Choice& it, int64_t first, double* p, double* q) const {
+    float pl[kVec], ql[kVec];
+    load_logits<T>(p_row, first, a.vocab, pl);
+    if (it.mode == kResample) load_logits<T>(q_row, first, a.vocab, ql);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) p[e] = first + e == drafted ? 0.0 : weight_of(pl[e], it.p_top, it.c);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) q[e] = it.mode == kResample ? weight_of(ql[e], it.q_top, it.c) : 0.0;
+  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(kPickThreads) void verify_weigh_kernel(const VerifyArgs a) {
+  constexpr int WAVES = kPickThreads / 64;
+  __shared__ Weights waves[WAVES];
+  const uint32_t chunk = blockIdx.x % (uint32_t)a.pick_chunks;
+  const int64_t b = blockIdx.x / (uint32_t)a.pick_chunks;
+  const Choice it = a.choices[b];
+  if (it.mode == kDone) return;
+  const Rows<T> rows(a, b, it);
+  double p[kVec], q[kVec];
+  rows.weigh(a, it, (int64_t)chunk * kPickChunk + threadIdx.x * kVec, p, q);
+  Weights sum{0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    sum.p += p[e];
+    sum.q += q[e];
+    const bool over = p[e] > it.ratio * q[e];
+    sum.p_over += over ? p[e] : 0.0;
+    sum.q_over += over ? q[e] : 0.0;
+  }
+  sum.p_over = wave_add(sum.p_over);
+  if (it.mode == kResample) {
+    sum.p = wave_add(sum.p);
+    sum.q = wave_add(sum.q);
+    sum.q_over = wave_add(sum.q_over);
+  }
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
   __syncthreads();
-  const int where = chosen_chunk;
-  const double start = border[0], bound = border[1];
-  if (where < 0) {  // the drafted token had all of the target's weight, and did not stand
-    write(-1);
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < WAVES; ++w) {
+    sum.p += waves[w].p;
+    sum.q += waves[w].q;
+    sum.p_over += waves[w].p_over;
+    sum.q_over += waves[w].q_over;
+  }
+  a.weights[b * a.pick_chunks + chunk] = sum;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
+  constexpr int WAVES = kPickThreads / 64;
+  __shared__ double sums[WAVES];
+  __shared__ int32_t picks[WAVES], lasts[WAVES];
+  const int64_t b = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Choice it = a.choices[b];
+  if (it.mode == kDone) return;
+  const Weights* weights = a.weights + b * a.pick_chunks;
+
+  // Every wave for itself: the ratio, the whole, and the chunk in which the sum passes
+  // u times the whole.
+  double ratio = 0.0;
+  if (it.mode == kResample) {
+    double p = 0.0, q = 0.0;
+    for (int i = lane; i < a.pick_chunks; i += 64) {
+      p += weights[i].p;
+      q += weights[i].q;
+    }
+    ratio = wave_add(p) / wave_add(q);
+  }
+  auto weight = [&](int i) {
+    if (i >= a.pick_chunks) return 0.0;
+    const double w = weights[i].p_over - ratio * weights[i].q_over;
+    return w > 0.0 ? w : 0.0;
+  };
+  double whole = 0.0;
+  for (int i = lane; i < a.pick_chunks; i += 64) whole += weight(i);
+  whole = wave_add(whole);
+  const double bound = (double)a.uniforms[b * (a.drafts + 1) + a.drafts] * whole;
+  double before = 0.0, start = 0.0;
+  int chosen = -1;
+  for (int at = 0; at < a.pick_chunks; at += 64) {
+    const double w = weight(at + lane);
+    const double up_to = wave_up_to(w);
+    const uint64_t some = __ballot(w > 0.0);
+    const uint64_t above = __ballot(w > 0.0 && before + up_to > bound);
+    if (some != 0) {  // (the last one with a weight, should none pass the border)
+      const int k = above != 0 ? __ffsll((unsigned long long)above) - 1 : 63 - __clzll((long long)some);
+      chosen = at + k;
+      start = __shfl(before + (up_to - w), k);
+    }
+    if (above != 0) break;
+    before += __shfl(up_to, 63);
+  }
+  int64_t* answer = a.answer + b * (a.drafts + 1) + it.row;
+  if (chosen < 0) {  // nothing has a weight
+    if (tid == 0) *answer = -1;
     return;
   }
-  const int64_t first = (int64_t)where * kChunk + tid * kVec;
-  weigh(first, w);
-  double own_sum = 0.0;
+
+  const int64_t first = (int64_t)chosen * kPickChunk + tid * kVec;
+  const Rows<T> rows(a, b, it);
+  double p[kVec], q[kVec];
+  rows.weigh(a, it, first, p, q);
+  double own = 0.0;
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) own_sum += w[e];
-  double up_to = own_sum;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double other = __shfl_up(up_to, d);
-    if (lane >= d) up_to += other;
+  for (int e = 0; e < kVec; ++e) {
+    p[e] -= ratio * q[e];
+    p[e] = p[e] > 0.0 ? p[e] : 0.0;
+    own += p[e];
   }
+  const double up_to = wave_up_to(own);
+  if (lane == 63) sums[wave] = up_to;
   __syncthreads();
-  if (lane == 63) totals[wave] = up_to;
-  __syncthreads();
-  double run = start + (up_to - own_sum);
-  for (int k = 0; k < wave; ++k) run += totals[k];
+  double run = start + (up_to - own);
+  for (int w = 0; w < wave; ++w) run += sums[w];
   int32_t pick = INT32_MAX, last = -1;
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
-    run += w[e];
-    if (w[e] > 0.0) {
+    run += p[e];
+    if (p[e] > 0.0) {
       last = (int32_t)(first + e);
       if (run > bound && pick == INT32_MAX) pick = last;
     }
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int32_t p = __shfl_xor(pick, d), q = __shfl_xor(last, d);
-    pick = p < pick ? p : pick;
-    last = q > last ? q : last;
-  }
-  __shared__ int32_t picks[WAVES], lasts[WAVES];
+  pick = wave_lowest(pick);
+  last = -wave_lowest(-last);
   if (lane == 0) {
     picks[wave] = pick;
     lasts[wave] = last;
   }
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < WAVES; ++k) {
-    pick = picks[k] < pick ? picks[k] : pick;
-    last = lasts[k] > last ? lasts[k] : last;
+  if (tid != 0) return;
+  for (int w = 1; w < WAVES; ++w) {
+    pick = picks[w] < pick ? picks[w] : pick;
+    last = lasts[w] > last ? lasts[w] : last;
   }
-  write(pick != INT32_MAX ? pick : last);
+  *answer = pick != INT32_MAX ? pick : last;
 }
 
 struct Layout {
-  int64_t chunks, rows;
-  size_t parts, weights, tickets, bytes;
+  int64_t row_chunks, pick_chunks, rows;
+  size_t weights, choices, bytes;
 };
 // Where the parts stand in the workspace; false for sizes that no launch takes.
 bool lay_out(int64_t batch, int64_t drafts, int64_t vocab, bool sampled, Layout& out) {
-  if (batch < 0 || drafts < 0 || drafts > kMaxDrafts || vocab <= 0 || vocab > INT32_MAX - kChunk) return false;
-  out.chunks = ceil_div(vocab, kChunk);
+  if (batch < 0 || drafts < 0 || drafts > kMaxDrafts || vocab <= 0 || vocab > INT32_MAX - kRowChunk) return false;
+  out.row_chunks = ceil_div(vocab, kRowChunk);
+  out.pick_chunks = ceil_div(vocab, kPickChunk);
   out.rows = drafts + 1 + (sampled ? drafts : 0);
-  const int64_t most = (int64_t)(UINT32_MAX / kPickThreads);
-  if (batch > most / (out.rows * out.chunks)) return false;
-  out.parts = 0;
-  out.weights = (size_t)(batch * out.rows * out.chunks) * sizeof(RowPart);
-  out.tickets = out.weights + (size_t)(batch * out.chunks) * sizeof(double);
-  out.bytes = out.tickets + (size_t)batch * sizeof(uint32_t);
+  const int64_t most = (int64_t)(UINT32_MAX / kDecideThreads);
+  if (batch > most / (out.rows * out.row_chunks) || batch > most / out.pick_chunks) return false;
+  out.weights = (size_t)(batch * out.rows * out.row_chunks) * sizeof(RowPart);
+  out.choices = out.weights + (size_t)(batch * out.pick_chunks) * sizeof(Weights);
+  out.bytes = out.choices + (size_t)batch * sizeof(Choice);
   return true;
 }
 
 template <typename T>
 int launch(const VerifyArgs& a, const Layout& layout, hipStream_t stream) {
-  hipLaunchKernelGGL(verify_rows_kernel<T>, dim3((unsigned)(a.batch * layout.rows * layout.chunks)), dim3(kRowThreads),
-                     0, stream, a);
-  const int status = check_hip(hipGetLastError(), "verify draft launch");
-  if (status != SAH_OK) return status;
-  hipLaunchKernelGGL(verify_pick_kernel<T>, dim3((unsigned)(a.batch * layout.chunks)), dim3(kPickThreads), 0, stream, a);
+  const unsigned batch = (unsigned)a.batch;
+  hipLaunchKernelGGL(verify_rows_kernel<T>, dim3((unsigned)(batch * layout.rows * layout.row_chunks)),
+                     dim3(kRowThreads), 0, stream, a);
+  hipLaunchKernelGGL(verify_decide_kernel<T>, dim3(batch), dim3(kDecideThreads), 0, stream, a);
+  hipLaunchKernelGGL(verify_weigh_kernel<T>, dim3((unsigned)(batch * layout.pick_chunks)), dim3(kPickThreads), 0,
+                     stream, a);
+  hipLaunchKernelGGL(verify_pick_kernel<T>, dim3(batch), dim3(kPickThreads), 0, stream, a);
   return check_hip(hipGetLastError(), "verify draft launch");
 }
 
@@ -549,13 +692,14 @@ extern "C" int sah_verify_draft(const void* target, const void* draft, const int
   a.d_sb = draft_stride_b;
   a.d_ss = draft_stride_s;
   char* space = static_cast<char*>(workspace);
-  a.parts = reinterpret_cast<RowPart*>(space + layout.parts);
-  a.weights = reinterpret_cast<double*>(space + layout.weights);
-  a.tickets = reinterpret_cast<uint32_t*>(space + layout.tickets);
+  a.parts = reinterpret_cast<RowPart*>(space);
+  a.weights = reinterpret_cast<Weights*>(space + layout.weights);
+  a.choices = reinterpret_cast<Choice*>(space + layout.choices);
   a.batch = (int)batch;
   a.drafts = (int)drafts;
   a.vocab = (int)vocab;
-  a.chunks = (int)layout.chunks;
+  a.row_chunks = (int)layout.row_chunks;
+  a.pick_chunks = (int)layout.pick_chunks;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == SAH_DTYPE_BF16) return launch<bf16>(a, layout, s);
   if (dtype == SAH_DTYPE_F16) return launch<f16>(a, layout, s);

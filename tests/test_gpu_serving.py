@@ -176,6 +176,28 @@ def test_verify_extreme_random_numbers(gpu_device, value):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("vocab", [50, 9001])
+def test_verify_random_numbers_at_the_border(gpu_device, dtype, sampled, vocab):
+    """Numbers next to p / q, where fp32 cannot say whether a draft stands: that of either
+    side, in rows of which one after the other is so near."""
+
+    batch, drafts = 24, 18
+    target, draft, tokens, uniforms = _drafted(batch, drafts, vocab, dtype, 19 + vocab)
+    if not sampled:
+        tokens = target[:, :drafts].float().argmax(-1)
+    p = torch.softmax(target[:, :drafts].double(), -1).gather(-1, tokens[..., None])[..., 0]
+    q = torch.softmax(draft.double(), -1).gather(-1, tokens[..., None])[..., 0] if sampled else torch.ones_like(p)
+    border = (p / q).clamp(max=0.999).float()
+    step = torch.randint(-1, 2, border.shape, generator=_generator(20))
+    step[:, : drafts // 2] = -1  # the first of them stand
+    border = torch.where(step < 0, torch.nextafter(border, torch.zeros(())), border)
+    uniforms[:, :drafts] = torch.where(step > 0, torch.nextafter(border, torch.ones(())), border)
+    want = _verify(gpu_device, target, tokens, uniforms, draft if sampled else None)
+    assert min(want[1]) >= drafts // 2 - 1 and min(want[1]) < drafts
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_verify_logits_of_any_strides(gpu_device, dtype):
     target, draft, tokens, uniforms = _drafted(3, 2, 1001, dtype, 17)
     want = _verify(gpu_device, target, tokens, uniforms, draft)
