@@ -30,6 +30,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kGroup = 64;  // outputs of a wave at a time
 constexpr int kMaxRank = 128;
+constexpr int kFusedTiles = 2;  // tiles of 16 tokens of a workgroup that does both products
 
 struct LowRankArgs {
   const void* x;
@@ -84,42 +85,34 @@ __device__ __forceinline__ int down_row(int t, int m, int used) {
   const int row = NP == 0 ? m : 32 * (t / 2) + 8 * (m / 4) + 4 * (t & 1) + (m & 3);
   return row < used ? row : 0;
 }
-template <int NP>
-__device__ __forceinline__ bool tile_used(int t, int used) {
-  return NP == 0 || 32 * (t / 2) < used;
-}
-
-// h += down x over inputs [32 first, 32 last), a step of 32 inputs after the other, each
-// `stride` steps apart.  x: each tile's token row; w: each tile's row of down.
+// h += down x over inputs [32 first, 32 last).  x: each tile's token row; w: each tile's
+// row of down.
 template <typename T, int NP, int TT, int UNROLL>
-__device__ __forceinline__ void shrink(const T* const (&x)[TT], const T* const (&w)[kTiles<NP>], int used, int64_t in,
-                                       int64_t first, int64_t last, int stride, f32x4 (&h)[TT][kTiles<NP>]) {
+__device__ __forceinline__ void shrink(const T* const (&x)[TT], const T* const (&w)[kTiles<NP>], int64_t in,
+                                       int64_t first, int64_t last, f32x4 (&h)[TT][kTiles<NP>]) {
   typedef typename Vec8<T>::type V8;
   constexpr int N = kTiles<NP>;
   const int quarter = (threadIdx.x & 63) >> 4;
   const int64_t whole = in / 32 < last ? in / 32 : last;  // steps without a ragged end
   int64_t step = first;
-  for (; step + (int64_t)(UNROLL - 1) * stride < whole; step += (int64_t)UNROLL * stride) {
+  for (; step + UNROLL <= whole; step += UNROLL) {
     V8 xs[UNROLL][TT], ws[UNROLL][N];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int64_t k = (step + (int64_t)u * stride) * 32 + quarter * 8;
+      const int64_t k = (step + u) * 32 + quarter * 8;
 #pragma unroll
       for (int i = 0; i < TT; ++i) xs[u][i] = *reinterpret_cast<const V8*>(x[i] + k);
 #pragma unroll
-      for (int t = 0; t < N; ++t)
-        if (tile_used<NP>(t, used)) ws[u][t] = *reinterpret_cast<const V8*>(w[t] + k);
+      for (int t = 0; t < N; ++t) ws[u][t] = *reinterpret_cast<const V8*>(w[t] + k);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
       for (int t = 0; t < N; ++t)
-        if (tile_used<NP>(t, used)) {
 #pragma unroll
-          for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws[u][t], xs[u][i], h[i][t]);
-        }
+        for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws[u][t], xs[u][i], h[i][t]);
   }
-  for (; step < last; step += stride) {
+  for (; step < last; ++step) {
     const int64_t k = step * 32 + quarter * 8;
     const bool there = k < in;
     V8 xs[TT];
@@ -130,15 +123,14 @@ __device__ __forceinline__ void shrink(const T* const (&x)[TT], const T* const (
       if (there) xs[i] = *reinterpret_cast<const V8*>(x[i] + k);
     }
 #pragma unroll
-    for (int t = 0; t < N; ++t)
-      if (tile_used<NP>(t, used)) {
-        V8 ws;
+    for (int t = 0; t < N; ++t) {
+      V8 ws;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ws[e] = (T)0.0f;
-        if (there) ws = *reinterpret_cast<const V8*>(w[t] + k);
+      for (int e = 0; e < 8; ++e) ws[e] = (T)0.0f;
+      if (there) ws = *reinterpret_cast<const V8*>(w[t] + k);
 #pragma unroll
-        for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws, xs[i], h[i][t]);
-      }
+      for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws, xs[i], h[i][t]);
+    }
   }
 }
 
@@ -195,75 +187,106 @@ __device__ __forceinline__ Hidden<T, NP> make_hidden(const f32x4 (&h)[kTiles<NP>
   return out;
 }
 
-// Outputs [64 group, 64 group + 64) of the tiles' tokens: base + scale (up h).  A lane's
-// token is column lane % 16; its outputs 16 (lane / 16) + 0..15 of the group.  Tokens
-// that the adapter is not added to take base as it is, tokens behind the sequence nothing.
+// What outputs [64 group, 64 group + 64) of a wave's tokens need: the rows of up, and
+// base.  A lane's token is column lane % 16; its outputs 8 (lane / 16) + 0..7 of either
+// half of the group, so that an access takes 64 bytes of a token.  Places outside the tensors read the nearest inside.
 template <typename T, int NP, int TT>
-__device__ __forceinline__ void expand_group(const T* up, int64_t rank, int64_t out, int used, int64_t group, float scale,
-                                             const Hidden<T, NP> (&h)[TT], const T* const (&base)[TT], T* const (&y)[TT],
-                                             const bool (&live)[TT], const bool (&added)[TT]) {
+struct Group {
   typedef typename Vec8<T>::type V8;
   typedef typename Vec8<T>::half_type V4;
-  const int lane = threadIdx.x & 63, quarter = lane >> 4, m = lane & 15;
-  const int64_t mine = group * kGroup + quarter * 16;
+  static constexpr int S = NP == 0 ? 1 : NP;
   V8 held[TT][2];
+  V8 w[4][S];
+
+  __device__ __forceinline__ void load(const T* up, int64_t rank, int64_t out, int used, int64_t group,
+                                       const T* const (&base)[TT]) {
+    const int lane = threadIdx.x & 63, quarter = lane >> 4, m = lane & 15;
 #pragma unroll
-  for (int i = 0; i < TT; ++i)
+    for (int p = 0; p < 2; ++p) {
+      const int64_t asked = group * kGroup + 32 * p + 8 * quarter;
+      const int64_t at = asked < out ? asked : out - 8;
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-      if (live[i] && mine + 8 * p < out) held[i][p] = *reinterpret_cast<const V8*>(base[i] + mine + 8 * p);
-  f32x4 sums[TT][4];
+      for (int i = 0; i < TT; ++i) held[i][p] = *reinterpret_cast<const V8*>(base[i] + at);
+    }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t asked = group * kGroup + 16 * (m / 4) + 4 * t + (m & 3);
-    const T* row = up + (asked < out ? asked : out - 1) * rank;
+    for (int t = 0; t < 4; ++t) {
+      const int64_t asked = group * kGroup + 32 * (t / 2) + 8 * (m / 4) + 4 * (t & 1) + (m & 3);
+      const T* row = up + (asked < out ? asked : out - 1) * rank;
+      if constexpr (NP == 0) {
+        const V4 half = *reinterpret_cast<const V4*>(row + (4 * quarter < used ? 4 * quarter : 0));
+        w[t][0] = __builtin_shufflevector(half, half, 0, 1, 2, 3, 0, 1, 2, 3);
+      } else {
 #pragma unroll
-    for (int i = 0; i < TT; ++i) sums[i][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (NP == 0) {
-      const V4 half = *reinterpret_cast<const V4*>(row + (4 * quarter < used ? 4 * quarter : 0));
-      const V8 w = __builtin_shufflevector(half, half, 0, 1, 2, 3, 0, 1, 2, 3);
-#pragma unroll
-      for (int i = 0; i < TT; ++i) sums[i][t] = mfma16(w, h[i].high[0], sums[i][t]);
-    } else {
-#pragma unroll
-      for (int s = 0; s < NP; ++s)
-        if (32 * s < used) {
+        for (int s = 0; s < NP; ++s) {
           const int at = 32 * s + 8 * quarter;
-          const V8 w = *reinterpret_cast<const V8*>(row + (at < used ? at : 0));
+          w[t][s] = *reinterpret_cast<const V8*>(row + (at < used ? at : 0));
+        }
+      }
+    }
+  }
+
+  // base + scale (up h).  Tokens that the adapter is not added to take base as it is,
+  // tokens behind the sequence nothing.
+  __device__ __forceinline__ void finish(int64_t out, int64_t group, float scale, const Hidden<T, NP> (&h)[TT],
+                                         T* const (&y)[TT], const bool (&live)[TT], const bool (&added)[TT]) {
+    const int quarter = (threadIdx.x & 63) >> 4;
+    f32x4 sums[TT][4];
 #pragma unroll
-          for (int i = 0; i < TT; ++i) {
-            sums[i][t] = mfma16(w, h[i].low[s], sums[i][t]);
-            sums[i][t] = mfma16(w, h[i].high[s], sums[i][t]);
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < TT; ++i) sums[i][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          if constexpr (NP != 0) sums[i][t] = mfma16(w[t][s], h[i].low[s], sums[i][t]);
+          sums[i][t] = mfma16(w[t][s], h[i].high[s], sums[i][t]);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int64_t at = group * kGroup + 32 * p + 8 * quarter;
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+        if (live[i] && at < out) {
+          V8 sum = held[i][p];
+          if (added[i]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              sum[e] = from_f32<T>(fmaf(scale, ldexpf(sums[i][2 * p + e / 4][e % 4], -h[i].power), to_f32(held[i][p][e])));
           }
+          *reinterpret_cast<V8*>(y[i] + at) = sum;
         }
     }
   }
-#pragma unroll
-  for (int i = 0; i < TT; ++i)
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-      if (live[i] && mine + 8 * p < out) {
-        V8 sum = held[i][p];
-        if (added[i]) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sum[e] = from_f32<T>(fmaf(scale, ldexpf(sums[i][2 * p + e / 4][e % 4], -h[i].power), to_f32(held[i][p][e])));
-        }
-        *reinterpret_cast<V8*>(y[i] + mine + 8 * p) = sum;
-      }
-}
+};
 
-// Tokens without an adapter: base as it is.
-template <typename T, int TT>
-__device__ __forceinline__ void copy_group(int64_t out, int64_t group, const T* const (&base)[TT], T* const (&y)[TT],
-                                           const bool (&live)[TT]) {
+// Tokens without an adapter, groups first, first + step, ..: base as it is.
+template <typename T, int TT, int DEEP>
+__device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t groups, int64_t step,
+                                            const T* const (&base)[TT], T* const (&y)[TT], const bool (&live)[TT]) {
   const int quarter = (threadIdx.x & 63) >> 4;
-  const int64_t mine = group * kGroup + quarter * 16;
+  for (int64_t g = first; g < groups; g += DEEP * step) {
+    u32x4 held[DEEP][TT][2];
 #pragma unroll
-  for (int i = 0; i < TT; ++i)
+    for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-      if (live[i] && mine + 8 * p < out && y[i] != base[i]) store16(y[i] + mine + 8 * p, load16(base[i] + mine + 8 * p));
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int64_t at = (g + d * step) * kGroup + 32 * p + 8 * quarter;
+          held[d][i][p] = load16(base[i] + (at < out ? at : out - 8));
+        }
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int64_t at = (g + d * step) * kGroup + 32 * p + 8 * quarter;
+          if (live[i] && at < out && y[i] != base[i]) store16(y[i] + at, held[d][i][p]);
+        }
+  }
 }
 
 template <typename T, int TT>
@@ -290,38 +313,66 @@ __device__ __forceinline__ Tokens<T, TT> tokens_of(const LowRankArgs& a, int64_t
   return out;
 }
 
+// A workgroup takes 16 TT tokens.  Its waves share `in` for h, add their sums up in order
+// through LDS, and share `out`, the next group's loads under way while one is worked on.
 template <typename T, int NP, int TT>
 __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankArgs a) {
   constexpr int N = kTiles<NP>;
+  __shared__ f32x4 sums[kWaves][TT * N][64];
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tile = (int64_t)blockIdx.x * kWaves + wave;
-  if (tile >= a.tiles) return;
+  const int64_t tile = blockIdx.x;
   const int64_t b = tile / a.tiles_of_seq;
   const int64_t first = (tile - b * a.tiles_of_seq) * (16 * TT);
   const Adapter it = adapter_of(a, b);
   const Tokens<T, TT> tokens = tokens_of<T, TT>(a, b, first, it.count);
   const int64_t groups = (a.out + kGroup - 1) / kGroup;
   if (it.used == 0 || first >= it.count) {
-    for (int64_t g = 0; g < groups; ++g) copy_group<T, TT>(a.out, g, tokens.base, tokens.y, tokens.live);
+    copy_groups<T, TT, 4>(a.out, wave, groups, kWaves, tokens.base, tokens.y, tokens.live);
     return;
   }
   const T* down = static_cast<const T*>(a.down) + it.index * a.rank * a.in;
   const T* w[N];
 #pragma unroll
-  for (int t = 0; t < N; ++t) w[t] = down + (int64_t)down_row<NP>(t, threadIdx.x & 15, it.used) * a.in;
+  for (int t = 0; t < N; ++t) w[t] = down + (int64_t)down_row<NP>(t, lane & 15, it.used) * a.in;
   f32x4 h[TT][N];
 #pragma unroll
   for (int i = 0; i < TT; ++i)
 #pragma unroll
     for (int t = 0; t < N; ++t) h[i][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  shrink<T, NP, TT, (N * 2 + TT * 2 > 12 ? 2 : 4)>(tokens.x, w, it.used, a.in, 0, (a.in + 31) / 32, 1, h);
-  const float scale = a.scales != nullptr ? a.scales[it.index] : 1.0f;
+  const int64_t steps = (a.in + 31) / 32, share = (steps + kWaves - 1) / kWaves;
+  const int64_t to = (wave + 1) * share;
+  shrink<T, NP, TT, (N + TT > 6 ? 2 : 4)>(tokens.x, w, a.in, wave * share, to < steps ? to : steps, h);
+#pragma unroll
+  for (int i = 0; i < TT; ++i)
+#pragma unroll
+    for (int t = 0; t < N; ++t) sums[wave][i * N + t][lane] = h[i][t];
+  __syncthreads();
   Hidden<T, NP> hidden[TT];
 #pragma unroll
-  for (int i = 0; i < TT; ++i) hidden[i] = make_hidden<T, NP>(h[i], it.used);
+  for (int i = 0; i < TT; ++i) {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      h[i][t] = sums[0][i * N + t][lane];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) h[i][t] += sums[k][i * N + t][lane];
+    }
+    hidden[i] = make_hidden<T, NP>(h[i], it.used);
+  }
+  const float scale = a.scales != nullptr ? a.scales[it.index] : 1.0f;
   const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
-  for (int64_t g = 0; g < groups; ++g)
-    expand_group<T, NP, TT>(up, a.rank, a.out, it.used, g, scale, hidden, tokens.base, tokens.y, tokens.live, tokens.added);
+  Group<T, NP, TT> buffer[2];
+  int64_t g = wave;
+  if (g < groups) buffer[0].load(up, a.rank, a.out, it.used, g, tokens.base);
+  while (g < groups) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (g >= groups) break;
+      if (g + kWaves < groups) buffer[1 - k].load(up, a.rank, a.out, it.used, g + kWaves, tokens.base);
+      buffer[k].finish(a.out, g, scale, hidden, tokens.y, tokens.live, tokens.added);
+      g += kWaves;
+    }
+  }
 }
 
 // Partial sums of h: workgroup (tile, part) takes the part's steps, its waves in turn.
@@ -348,7 +399,9 @@ __global__ __launch_bounds__(kThreads) void low_rank_shrink_kernel(const LowRank
   const int64_t steps = (a.in + 31) / 32;
   const int64_t from = (int64_t)part * a.steps_of_part;
   const int64_t to = from + a.steps_of_part < steps ? from + a.steps_of_part : steps;
-  shrink<T, NP, 1, (N > 4 ? 2 : 4)>(tokens.x, w, it.used, a.in, from + wave, to, kWaves, h);
+  const int64_t share = (to - from + kWaves - 1) / kWaves;
+  const int64_t mine = from + wave * share;
+  shrink<T, NP, 1, (N > 4 ? 2 : 4)>(tokens.x, w, a.in, mine, mine + share < to ? mine + share : to, h);
   if (wave != 0) {
 #pragma unroll
     for (int t = 0; t < N; ++t) sums[wave - 1][t][lane] = h[0][t];
@@ -358,7 +411,6 @@ __global__ __launch_bounds__(kThreads) void low_rank_shrink_kernel(const LowRank
   f32x4* partial = reinterpret_cast<f32x4*>(a.partial) + ((int64_t)part * a.tiles + tile) * N * 64;
 #pragma unroll
   for (int t = 0; t < N; ++t) {
-    if (!tile_used<NP>(t, it.used)) continue;
     f32x4 sum = h[0][t];
 #pragma unroll
     for (int k = 0; k < kWaves - 1; ++k) sum += sums[k][t][lane];
@@ -381,23 +433,25 @@ __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRank
   const Adapter it = adapter_of(a, b);
   const Tokens<T, 1> tokens = tokens_of<T, 1>(a, b, first, it.count);
   if (it.used == 0 || first >= it.count) {
-    copy_group<T, 1>(a.out, group, tokens.base, tokens.y, tokens.live);
+    copy_groups<T, 1, 1>(a.out, group, group + 1, 1, tokens.base, tokens.y, tokens.live);
     return;
   }
+  Group<T, NP, 1> data;
+  data.load(static_cast<const T*>(a.up) + it.index * a.out * a.rank, a.rank, a.out, it.used, group, tokens.base);
   f32x4 h[N];
 #pragma unroll
   for (int t = 0; t < N; ++t) h[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   if (tokens.added[0]) {
     const f32x4* partial = reinterpret_cast<const f32x4*>(a.partial) + tile * N * 64 + lane;
+    // (of tiles that no row of down fills, what is read is not used)
+#pragma unroll 4
     for (int p = 0; p < a.parts; ++p)
 #pragma unroll
-      for (int t = 0; t < N; ++t)
-        if (tile_used<NP>(t, it.used)) h[t] += partial[(int64_t)p * a.tiles * N * 64 + t * 64];
+      for (int t = 0; t < N; ++t) h[t] += partial[(int64_t)p * a.tiles * N * 64 + t * 64];
   }
   const float scale = a.scales != nullptr ? a.scales[it.index] : 1.0f;
   const Hidden<T, NP> hidden[1] = {make_hidden<T, NP>(h, it.used)};
-  const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
-  expand_group<T, NP, 1>(up, a.rank, a.out, it.used, group, scale, hidden, tokens.base, tokens.y, tokens.live, tokens.added);
+  data.finish(a.out, group, scale, hidden, tokens.y, tokens.live, tokens.added);
 }
 
 // How a call is launched.
@@ -409,7 +463,7 @@ struct Plan {
   int rank_tiles;
   size_t bytes;
 };
-constexpr int64_t kFusedTiles = 1024;   // of 16 tokens: from here on a wave does both products
+constexpr int64_t kManyTiles = 1024;  // of 16 tokens: from here on one launch does both products
 
 Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t rank) {
   Plan p{};
@@ -417,8 +471,13 @@ Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t rank) {
   p.tokens = 16;
   p.tiles_of_seq = ceil_div(seq, 16);
   p.tiles = batch * p.tiles_of_seq;
-  p.fused = p.tiles >= kFusedTiles;
-  if (p.fused) return p;
+  p.fused = p.tiles >= kManyTiles;
+  if (p.fused) {
+    p.tokens = 16 * kFusedTiles;
+    p.tiles_of_seq = ceil_div(seq, p.tokens);
+    p.tiles = batch * p.tiles_of_seq;
+    return p;
+  }
   const int64_t steps = ceil_div(in, 32);
   int64_t parts = ceil_div(1024, p.tiles);
   const int64_t most = ceil_div(steps, 4 * kWaves);
@@ -432,8 +491,7 @@ Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t rank) {
 template <typename T, int NP>
 int launch(const LowRankArgs& a, const Plan& p, hipStream_t stream) {
   if (p.fused) {
-    const unsigned grid = (unsigned)ceil_div(p.tiles, kWaves);
-    hipLaunchKernelGGL((low_rank_fused_kernel<T, NP, 1>), dim3(grid), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((low_rank_fused_kernel<T, NP, kFusedTiles>), dim3((unsigned)p.tiles), dim3(kThreads), 0, stream, a);
     return check_hip(hipGetLastError(), "low-rank adapters launch");
   }
   hipLaunchKernelGGL((low_rank_shrink_kernel<T, NP>), dim3((unsigned)(p.tiles * p.parts)), dim3(kThreads), 0, stream, a);
