@@ -2,22 +2,30 @@
 //
 //   y[b, s] = base[b, s] + scale_a (x[b, s] down_a^T) up_a^T,   a = index[b]
 //
-// Two products a token: h = down x (rank x in) and up h (out x rank), both with the
-// adapter's weights as rows and 16 tokens as columns of 16 x 16 x 32 products.  A lane
-// then holds, of its token's h, four numbers a tile of 16 rows; the rows of `down` are
-// dealt to the tiles so that two tiles give a lane eight neighbouring ones, which is its
-// part of the second product's operand: h never leaves its registers.  The rows of `up`
-// are dealt so that a lane ends with 16 neighbouring outputs of its token.
+// Two products a token, h = down x (rank x in) and up h (out x rank), on 16 x 16 x 32
+// products whose operands hold 16 bytes of row lane % 16 a lane.  The rows of `down` are
+// dealt to tiles of 16 so that two tiles leave a lane with eight neighbouring numbers of
+// its token's h, which is its part of the second product's operand: h never leaves its
+// registers.
+//
+// Memory is read in another order than the operands': four lanes in a row take 64 bytes of
+// a row (the address units work on four lanes at a time, and in the operands' order, one
+// row a lane, they were the bound: 91% busy).  Rows of x and `down` change places within
+// four lanes in registers, rows of `up` through the wave's own part of LDS, and the second
+// product's columns are outputs 4 n + t, so that 16 lanes take 128 bytes of base and y.
 //
 // h is fp32.  It enters the second product as the sum of two 16-bit numbers, off by
 // 2^-16 (bf16) or 2^-22 (fp16) of itself: one number's 2^-9 would be as much as the
 // output's own rounding.  A token's h is taken in a power of two of its own, its largest
 // below 2^15, so that fp16 reaches.
 //
-// Many tokens are bound by x, base and y: a wave does both products of its tokens (fused).
-// Few tokens are bound by the adapters' bytes, and a wave a token would leave most of
-// the chip idle: one launch shares `in` among workgroups and leaves partial sums of h,
-// another adds them up in order and shares `out`.
+// Few tokens are bound by the adapters' bytes and by latency, and a workgroup a token would
+// leave most of the chip idle: one launch shares `in` among workgroups and leaves partial
+// sums of h, another adds them up in order and shares `out`.  Many tokens are bound by x,
+// base and y: a workgroup does both products of 32 tokens, and there is no workspace.
+//   2 x 20001 tokens (ragged), 1024 -> 4096, rank 32 (697 MB, 142 us at a large copy's
+//   rate): 149 us; 178 in the operands' order
+//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (49 MB): 8 + 12 us
 
 #include <type_traits>
 
@@ -28,7 +36,8 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr int kGroup = 64;  // outputs of a wave at a time
+constexpr int kSlab = 128;  // inputs that a wave takes at a time
+constexpr int kGroup = 64;  // outputs
 constexpr int kMaxRank = 128;
 constexpr int kFusedTiles = 2;  // tiles of 16 tokens of a workgroup that does both products
 
@@ -45,19 +54,20 @@ struct LowRankArgs {
   float* partial;          // [parts][tiles][tiles of rank][64][4]
   int64_t x_sb, x_ss, p_sb, p_ss, y_sb, y_ss;
   int64_t in, out, seq, adapters, rank;
-  int64_t tiles_of_seq;    // of 16 (fused: 16 TT) tokens
+  int64_t tiles_of_seq;    // of 16 (fused: 16 kFusedTiles) tokens
   int64_t tiles;
-  int parts, steps_of_part;
+  int parts, slabs_of_part, groups_of_wave;
 };
 
 // What a sequence's adapter asks for; used == 0: none.
 struct Adapter {
   int64_t index;
   int used;        // rows of down, a multiple of 8
+  float scale;
   int64_t count;   // tokens that it is added to
 };
 __device__ __forceinline__ Adapter adapter_of(const LowRankArgs& a, int64_t b) {
-  Adapter it{0, 0, 0};
+  Adapter it{0, 0, 1.0f, 0};
   const int64_t index = a.indices[b];
   if (index < 0 || index >= a.adapters) return it;
   int64_t rank = a.rank;
@@ -65,6 +75,7 @@ __device__ __forceinline__ Adapter adapter_of(const LowRankArgs& a, int64_t b) {
     const int64_t asked = ((int64_t)a.ranks[index] + 7) / 8 * 8;
     rank = asked < rank ? asked : rank;
   }
+  if (a.scales != nullptr) it.scale = a.scales[index];
   int64_t count = a.counts != nullptr ? (int64_t)a.counts[b] : a.seq;
   if (count > a.seq) count = a.seq;
   if (rank <= 0 || count <= 0) return it;
@@ -74,73 +85,111 @@ __device__ __forceinline__ Adapter adapter_of(const LowRankArgs& a, int64_t b) {
   return it;
 }
 
-// NP pairs of rank tiles; 0: a single tile.
-template <int NP>
-constexpr int kTiles = NP == 0 ? 1 : 2 * NP;
+// Lane l: quarter l / 16 of the operands' 16-byte parts, row (or column) l % 16; four by
+// four of these are corner l % 16 / 4 and side l % 4.
+__device__ __forceinline__ int quarter_of() { return (threadIdx.x & 63) >> 4; }
+__device__ __forceinline__ int corner_of() { return (threadIdx.x & 15) >> 2; }
+__device__ __forceinline__ int side_of() { return threadIdx.x & 3; }
 
-// Row of `down` at row m of tile t; rows from `used` on read row 0, and their h is
-// taken as 0.
-template <int NP>
-__device__ __forceinline__ int down_row(int t, int m, int used) {
-  const int row = NP == 0 ? m : 32 * (t / 2) + 8 * (m / 4) + 4 * (t & 1) + (m & 3);
-  return row < used ? row : 0;
+// Rows of `down` in tiles of 16, S pairs of them: row m of tile t is row 32 (t / 2) + 8 (m /
+// 4) + 4 (t % 2) + m % 4, so a lane's rows of a pair are 32 s + 8 quarter + 0..7.
+
+// lane ^ 1 (0xB1) or lane ^ 2 (0x4E), of every lane: not for a branch that some take.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
 }
-// h += down x over inputs [32 first, 32 last).  x: each tile's token row; w: each tile's
-// row of down.
-template <typename T, int NP, int TT, int UNROLL>
-__device__ __forceinline__ void shrink(const T* const (&x)[TT], const T* const (&w)[kTiles<NP>], int64_t in,
-                                       int64_t first, int64_t last, f32x4 (&h)[TT][kTiles<NP>]) {
+
+// Turns four registers' parts in four lanes: register j of lane i becomes register i of
+// lane j.
+template <typename V8>
+__device__ __forceinline__ void turn_in_four(V8 (&v)[4]) {
+  u32x4 r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = __builtin_bit_cast(u32x4, v[j]);
+  const bool odd = (threadIdx.x & 1) != 0, high = (threadIdx.x & 2) != 0;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const uint32_t a = r[j][d], b = r[j + 1][d], other_a = dpp<0xB1>(a), other_b = dpp<0xB1>(b);
+      r[j][d] = odd ? other_b : a;
+      r[j + 1][d] = odd ? b : other_a;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t a = r[j][d], b = r[j + 2][d], other_a = dpp<0x4E>(a), other_b = dpp<0x4E>(b);
+      r[j][d] = high ? other_b : a;
+      r[j + 2][d] = high ? b : other_a;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(V8, r[j]);
+}
+
+// h += down x over one slab of 128 inputs.  An access takes 256 bytes of four rows;
+// turned, register i of a lane holds its row's inputs 32 quarter + 8 i + 0..7 of the slab,
+// which is step i of the product.  x: the lane's rows 4 corner + 0..3 of each tile; w_first:
+// its first row of down in each pair.
+template <typename T, int S, int TT, bool WHOLE>
+__device__ __forceinline__ void shrink_slab(const T* const (&x)[TT][4], const T* down, const int64_t (&w_first)[S],
+                                            int64_t in, int64_t slab, f32x4 (&h)[TT][2 * S]) {
   typedef typename Vec8<T>::type V8;
-  constexpr int N = kTiles<NP>;
-  const int quarter = (threadIdx.x & 63) >> 4;
-  const int64_t whole = in / 32 < last ? in / 32 : last;  // steps without a ragged end
-  int64_t step = first;
-  for (; step + UNROLL <= whole; step += UNROLL) {
-    V8 xs[UNROLL][TT], ws[UNROLL][N];
+  const int64_t at = slab * kSlab + 32 * quarter_of() + 8 * side_of();
+  const bool there = WHOLE || at < in;
+  const int64_t k = there ? at : 0;
+  V8 xs[TT][4], ws[2 * S][4];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int64_t k = (step + u) * 32 + quarter * 8;
+  for (int i = 0; i < TT; ++i)
 #pragma unroll
-      for (int i = 0; i < TT; ++i) xs[u][i] = *reinterpret_cast<const V8*>(x[i] + k);
+    for (int j = 0; j < 4; ++j) xs[i][j] = *reinterpret_cast<const V8*>(x[i][j] + k);
 #pragma unroll
-      for (int t = 0; t < N; ++t) ws[u][t] = *reinterpret_cast<const V8*>(w[t] + k);
+  for (int t = 0; t < 2 * S; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      ws[t][j] = *reinterpret_cast<const V8*>(down + (4 * (t & 1) + j) * in + (w_first[t / 2] + k));
+  if constexpr (!WHOLE) {  // (both, as nothing times what is not there may be NaN)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) xs[i][j][e] = there ? xs[i][j][e] : (T)0.0f;
+#pragma unroll
+      for (int t = 0; t < 2 * S; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ws[t][j][e] = there ? ws[t][j][e] : (T)0.0f;
     }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws[u][t], xs[u][i], h[i][t]);
   }
-  for (; step < last; ++step) {
-    const int64_t k = step * 32 + quarter * 8;
-    const bool there = k < in;
-    V8 xs[TT];
 #pragma unroll
-    for (int i = 0; i < TT; ++i) {
+  for (int i = 0; i < TT; ++i) turn_in_four(xs[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) xs[i][e] = (T)0.0f;
-      if (there) xs[i] = *reinterpret_cast<const V8*>(x[i] + k);
-    }
+  for (int t = 0; t < 2 * S; ++t) {
+    turn_in_four(ws[t]);
 #pragma unroll
-    for (int t = 0; t < N; ++t) {
-      V8 ws;
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ws[e] = (T)0.0f;
-      if (there) ws = *reinterpret_cast<const V8*>(w[t] + k);
-#pragma unroll
-      for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws, xs[i], h[i][t]);
-    }
+      for (int i = 0; i < TT; ++i) h[i][t] = mfma16(ws[t][j], xs[i][j], h[i][t]);
   }
 }
 
-// A token's h, times 2^power, as the second product's operands.
-template <typename T, int NP>
+// Slabs [first, last), the one that the inputs end in by itself.
+template <typename T, int S, int TT>
+__device__ __forceinline__ void shrink(const T* const (&x)[TT][4], const T* down, const int64_t (&w_first)[S], int64_t in,
+                                       int64_t first, int64_t last, f32x4 (&h)[TT][2 * S]) {
+  const int64_t whole = in / kSlab < last ? in / kSlab : last;
+  int64_t slab = first;
+#pragma unroll 1
+  for (; slab < whole; ++slab) shrink_slab<T, S, TT, true>(x, down, w_first, in, slab, h);
+  if (slab < last) shrink_slab<T, S, TT, false>(x, down, w_first, in, slab, h);
+}
+
+// A token's h, times 2^power, as the second product's operands; factor: scale / 2^power.
+template <typename T, int S>
 struct Hidden {
   typedef typename Vec8<T>::type V8;
-  V8 high[NP == 0 ? 1 : NP];  // one tile: high and low in one operand
-  V8 low[NP == 0 ? 1 : NP];
-  int power;
+  V8 high[S], low[S];
+  float factor;
 };
 
 template <typename T>
@@ -150,235 +199,296 @@ __device__ __forceinline__ void split_number(float v, T& high, T& low) {
   low = from_f32<T>(fabsf(to_f32(high)) < INFINITY ? rest : 0.0f);
 }
 
-template <typename T, int NP>
-__device__ __forceinline__ Hidden<T, NP> make_hidden(const f32x4 (&h)[kTiles<NP>], int used) {
-  constexpr int N = kTiles<NP>;
-  const int quarter = (threadIdx.x & 63) >> 4;
-  float v[N][4];
+template <typename T, int S>
+__device__ __forceinline__ Hidden<T, S> make_hidden(const f32x4 (&h)[2 * S], int used, float scale) {
+  float v[2 * S][4];
   float largest = 0.0f;
 #pragma unroll
-  for (int t = 0; t < N; ++t)
+  for (int t = 0; t < 2 * S; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = NP == 0 ? 4 * quarter + i : 32 * (t / 2) + 8 * quarter + 4 * (t & 1) + i;
-      v[t][i] = row < used ? h[t][i] : 0.0f;
+      v[t][i] = 32 * (t / 2) + 8 * quarter_of() < used ? h[t][i] : 0.0f;
       largest = fmaxf(largest, fabsf(v[t][i]));
     }
   largest = fmaxf(largest, __shfl_xor(largest, 16));
   largest = fmaxf(largest, __shfl_xor(largest, 32));
-  int power = 0;  // the largest comes to lie in [2^14, 2^15)
+  // the largest comes to lie in [2^14, 2^15), where fp32 has room for scale / 2^power
+  int power = 0;
   if (largest > 0.0f && largest < INFINITY) power = 15 - __builtin_amdgcn_frexp_expf(largest);
-  Hidden<T, NP> out;
+  power = power < -100 ? -100 : power > 100 ? 100 : power;
+  Hidden<T, S> out;
 #pragma unroll
-  for (int t = 0; t < N; ++t)
+  for (int t = 0; t < 2 * S; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       T high, low;
       split_number<T>(ldexpf(v[t][i], power), high, low);
-      if constexpr (NP == 0) {
-        out.high[0][i] = high;
-        out.high[0][4 + i] = low;
-      } else {
-        out.high[t / 2][4 * (t & 1) + i] = high;
-        out.low[t / 2][4 * (t & 1) + i] = low;
-      }
+      out.high[t / 2][4 * (t & 1) + i] = high;
+      out.low[t / 2][4 * (t & 1) + i] = low;
     }
-  out.power = power;
+  out.factor = ldexpf(scale, -power);
   return out;
 }
 
-// What outputs [64 group, 64 group + 64) of a wave's tokens need: the rows of up, and
-// base.  A lane's token is column lane % 16; its outputs 8 (lane / 16) + 0..7 of either
-// half of the group, so that an access takes 64 bytes of a token.  Places outside the tensors read the nearest inside.
-template <typename T, int NP, int TT>
+// A wave's tokens as the outputs have them: a lane's are 4 quarter + 0..3 of each tile.
+template <typename T, int TT>
+struct Tokens {
+  const T* base[TT][4];
+  T* y[TT][4];
+  bool live[TT][4], added[TT][4];
+  __device__ Tokens(const LowRankArgs& a, int64_t b, int64_t first, int64_t count) {
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t token = first + 16 * i + 4 * quarter_of() + j;
+        const int64_t s = token < a.seq ? token : a.seq - 1;
+        live[i][j] = token < a.seq;
+        added[i][j] = token < count;
+        base[i][j] = static_cast<const T*>(a.base) + b * a.p_sb + s * a.p_ss;
+        y[i][j] = static_cast<T*>(a.y) + b * a.y_sb + s * a.y_ss;
+      }
+  }
+};
+// The lane's rows of x, tokens 4 corner + 0..3 of each tile.
+template <typename T, int TT>
+__device__ __forceinline__ void rows_of_x(const LowRankArgs& a, int64_t b, int64_t first, const T* (&x)[TT][4]) {
+#pragma unroll
+  for (int i = 0; i < TT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t token = first + 16 * i + 4 * corner_of() + j;
+      x[i][j] = static_cast<const T*>(a.x) + b * a.x_sb + (token < a.seq ? token : a.seq - 1) * a.x_ss;
+    }
+}
+// The lane's first row of down in each pair (rows from `used` on read the first ones, and
+// their h is taken as 0).
+template <int S>
+__device__ __forceinline__ void rows_of_down(int used, int64_t in, int64_t (&first)[S]) {
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int row = 32 * s + 8 * corner_of();
+    first[s] = (row < used ? row : 0) * in;
+  }
+}
+
+// The wave's part of LDS for a group's rows of up: an operand tile of 1 KiB for each
+// step s and t, the tiles 64 bytes apart from each other's banks.
+template <int S>
+struct UpStage {
+  static constexpr int TILE = 1024 + 64;
+  char bytes[4 * S * TILE];
+};
+
+// What a group's outputs of a wave's tokens need: the 64 rows of up, and base.  Places
+// behind `out` read the nearest inside.
+template <typename T, int S, int TT>
 struct Group {
   typedef typename Vec8<T>::type V8;
   typedef typename Vec8<T>::half_type V4;
-  static constexpr int S = NP == 0 ? 1 : NP;
-  V8 held[TT][2];
-  V8 w[4][S];
+  V4 held[TT][4];
+  V8 w[S][4];  // 64 bytes of 16 rows each, in memory's order
 
   __device__ __forceinline__ void load(const T* up, int64_t rank, int64_t out, int used, int64_t group,
-                                       const T* const (&base)[TT]) {
-    const int lane = threadIdx.x & 63, quarter = lane >> 4, m = lane & 15;
+                                       const Tokens<T, TT>& tokens) {
+    const int lane = threadIdx.x & 63;
+    const int64_t first = group * kGroup;
+    const int64_t asked = first + 4 * (lane & 15);
+    const int64_t column = asked < out ? asked : out - 4;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int64_t asked = group * kGroup + 32 * p + 8 * quarter;
-      const int64_t at = asked < out ? asked : out - 8;
+    for (int i = 0; i < TT; ++i)
 #pragma unroll
-      for (int i = 0; i < TT; ++i) held[i][p] = *reinterpret_cast<const V8*>(base[i] + at);
-    }
+      for (int j = 0; j < 4; ++j) held[i][j] = *reinterpret_cast<const V4*>(tokens.base[i][j] + column);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t asked = group * kGroup + 32 * (t / 2) + 8 * (m / 4) + 4 * (t & 1) + (m & 3);
-      const T* row = up + (asked < out ? asked : out - 1) * rank;
-      if constexpr (NP == 0) {
-        const V4 half = *reinterpret_cast<const V4*>(row + (4 * quarter < used ? 4 * quarter : 0));
-        w[t][0] = __builtin_shufflevector(half, half, 0, 1, 2, 3, 0, 1, 2, 3);
-      } else {
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = first + 16 * r + lane / 4;
+      const T* from = up + (row < out ? row : out - 1) * rank;
 #pragma unroll
-        for (int s = 0; s < NP; ++s) {
-          const int at = 32 * s + 8 * quarter;
-          w[t][s] = *reinterpret_cast<const V8*>(row + (at < used ? at : 0));
-        }
+      for (int s = 0; s < S; ++s) {
+        const int chunk = 32 * s + 8 * (lane & 3);
+        w[s][r] = *reinterpret_cast<const V8*>(from + (chunk < used ? chunk : 0));
       }
     }
   }
 
+  // Row 4 n + t of the group becomes row n of tile t.
+  __device__ __forceinline__ void stage(UpStage<S>& lds) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * r + lane / 4;
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        *reinterpret_cast<V8*>(lds.bytes + (s * 4 + row % 4) * UpStage<S>::TILE + (row / 4) * 64 + (lane & 3) * 16) = w[s][r];
+    }
+    // the wave's lanes read what the others wrote
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  static __device__ __forceinline__ void unstage() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
   // base + scale (up h).  Tokens that the adapter is not added to take base as it is,
   // tokens behind the sequence nothing.
-  __device__ __forceinline__ void finish(int64_t out, int64_t group, float scale, const Hidden<T, NP> (&h)[TT],
-                                         T* const (&y)[TT], const bool (&live)[TT], const bool (&added)[TT]) {
-    const int quarter = (threadIdx.x & 63) >> 4;
+  static __device__ __forceinline__ void finish(const UpStage<S>& lds, const V4 (&base)[TT][4], int64_t out, int64_t group,
+                                                const Hidden<T, S> (&h)[TT], const float (&factor)[TT][4],
+                                                const Tokens<T, TT>& tokens) {
+    const int lane = threadIdx.x & 63;
     f32x4 sums[TT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) sums[i][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int s = 0; s < S; ++s)
+      for (int s = 0; s < S; ++s) {
+        const V8 tile = *reinterpret_cast<const V8*>(lds.bytes + (s * 4 + t) * UpStage<S>::TILE + (lane & 15) * 64 +
+                                                     (lane >> 4) * 16);
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-          if constexpr (NP != 0) sums[i][t] = mfma16(w[t][s], h[i].low[s], sums[i][t]);
-          sums[i][t] = mfma16(w[t][s], h[i].high[s], sums[i][t]);
+          sums[i][t] = mfma16(h[i].low[s], tile, sums[i][t]);
+          sums[i][t] = mfma16(h[i].high[s], tile, sums[i][t]);
         }
+      }
     }
+    const int64_t column = group * kGroup + 4 * (lane & 15);
+    if (column >= out) return;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int64_t at = group * kGroup + 32 * p + 8 * quarter;
+    for (int i = 0; i < TT; ++i)
 #pragma unroll
-      for (int i = 0; i < TT; ++i)
-        if (live[i] && at < out) {
-          V8 sum = held[i][p];
-          if (added[i]) {
+      for (int j = 0; j < 4; ++j) {
+        V4 sum;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              sum[e] = from_f32<T>(fmaf(scale, ldexpf(sums[i][2 * p + e / 4][e % 4], -h[i].power), to_f32(held[i][p][e])));
-          }
-          *reinterpret_cast<V8*>(y[i] + at) = sum;
-        }
-    }
+        for (int t = 0; t < 4; ++t) sum[t] = from_f32<T>(fmaf(factor[i][j], sums[i][t][j], to_f32(base[i][j][t])));
+        if (tokens.live[i][j]) *reinterpret_cast<V4*>(tokens.y[i][j] + column) = tokens.added[i][j] ? sum : base[i][j];
+      }
   }
 };
+
+// Groups first, first + step, .. of a wave's tokens, whose first one's loads are under way:
+// a group's rows of up pass through LDS while the next one's loads begin.
+template <typename T, int S, int TT>
+__device__ __forceinline__ void expand(Group<T, S, TT>& data, UpStage<S>& lds, const T* up, int64_t rank, int64_t out,
+                                       int used, int64_t first, int64_t groups, int64_t step,
+                                       const Hidden<T, S> (&h)[TT], const Tokens<T, TT>& tokens) {
+  float factor[TT][4];
+#pragma unroll
+  for (int i = 0; i < TT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) factor[i][j] = __shfl(h[i].factor, 4 * quarter_of() + j);
+  for (int64_t g = first; g < groups; g += step) {
+    typename Vec8<T>::half_type base[TT][4];
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) base[i][j] = data.held[i][j];
+    data.stage(lds);
+    if (g + step >= groups) {
+      Group<T, S, TT>::finish(lds, base, out, g, h, factor, tokens);
+      break;
+    }
+    data.load(up, rank, out, used, g + step, tokens);
+    Group<T, S, TT>::finish(lds, base, out, g, h, factor, tokens);
+    Group<T, S, TT>::unstage();
+  }
+}
 
 // Tokens without an adapter, groups first, first + step, ..: base as it is.
 template <typename T, int TT, int DEEP>
 __device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t groups, int64_t step,
-                                            const T* const (&base)[TT], T* const (&y)[TT], const bool (&live)[TT]) {
-  const int quarter = (threadIdx.x & 63) >> 4;
+                                            const Tokens<T, TT>& tokens) {
+  typedef typename Vec8<T>::half_type V4;
   for (int64_t g = first; g < groups; g += DEEP * step) {
-    u32x4 held[DEEP][TT][2];
+    V4 held[DEEP][TT][4];
 #pragma unroll
     for (int d = 0; d < DEEP; ++d)
 #pragma unroll
       for (int i = 0; i < TT; ++i)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int64_t at = (g + d * step) * kGroup + 32 * p + 8 * quarter;
-          held[d][i][p] = load16(base[i] + (at < out ? at : out - 8));
+        for (int j = 0; j < 4; ++j) {
+          const int64_t at = (g + d * step) * kGroup + 4 * (threadIdx.x & 15);
+          held[d][i][j] = *reinterpret_cast<const V4*>(tokens.base[i][j] + (at < out ? at : out - 4));
         }
 #pragma unroll
     for (int d = 0; d < DEEP; ++d)
 #pragma unroll
       for (int i = 0; i < TT; ++i)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int64_t at = (g + d * step) * kGroup + 32 * p + 8 * quarter;
-          if (live[i] && at < out && y[i] != base[i]) store16(y[i] + at, held[d][i][p]);
+        for (int j = 0; j < 4; ++j) {
+          const int64_t at = (g + d * step) * kGroup + 4 * (threadIdx.x & 15);
+          if (tokens.live[i][j] && at < out && tokens.y[i][j] != tokens.base[i][j])
+            *reinterpret_cast<V4*>(tokens.y[i][j] + at) = held[d][i][j];
         }
   }
-}
-
-template <typename T, int TT>
-struct Tokens {
-  const T* x[TT];
-  const T* base[TT];
-  T* y[TT];
-  bool live[TT], added[TT];
-};
-// A lane's tokens `first` + 16 i + lane % 16 (behind the sequence: its last one, not live).
-template <typename T, int TT>
-__device__ __forceinline__ Tokens<T, TT> tokens_of(const LowRankArgs& a, int64_t b, int64_t first, int64_t count) {
-  Tokens<T, TT> out;
-#pragma unroll
-  for (int i = 0; i < TT; ++i) {
-    const int64_t token = first + 16 * i + (threadIdx.x & 15);
-    const int64_t s = token < a.seq ? token : a.seq - 1;
-    out.live[i] = token < a.seq;
-    out.added[i] = token < count;
-    out.x[i] = static_cast<const T*>(a.x) + b * a.x_sb + s * a.x_ss;
-    out.base[i] = static_cast<const T*>(a.base) + b * a.p_sb + s * a.p_ss;
-    out.y[i] = static_cast<T*>(a.y) + b * a.y_sb + s * a.y_ss;
-  }
-  return out;
 }
 
 // A workgroup takes 16 TT tokens.  Its waves share `in` for h, add their sums up in order
-// through LDS, and share `out`, the next group's loads under way while one is worked on.
-template <typename T, int NP, int TT>
+// through LDS, and share `out`.
+template <typename T, int S, int TT>
 __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankArgs a) {
-  constexpr int N = kTiles<NP>;
-  __shared__ f32x4 sums[kWaves][TT * N][64];
+  constexpr int N = 2 * S;
+  __shared__ __align__(16) union {
+    f32x4 sums[kWaves][TT * N][64];
+    UpStage<S> up[kWaves];
+  } lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tile = blockIdx.x;
   const int64_t b = tile / a.tiles_of_seq;
   const int64_t first = (tile - b * a.tiles_of_seq) * (16 * TT);
   const Adapter it = adapter_of(a, b);
-  const Tokens<T, TT> tokens = tokens_of<T, TT>(a, b, first, it.count);
   const int64_t groups = (a.out + kGroup - 1) / kGroup;
   if (it.used == 0 || first >= it.count) {
-    copy_groups<T, TT, 4>(a.out, wave, groups, kWaves, tokens.base, tokens.y, tokens.live);
+    const Tokens<T, TT> tokens(a, b, first, it.count);
+    copy_groups<T, TT, 2>(a.out, wave, groups, kWaves, tokens);
     return;
   }
-  const T* down = static_cast<const T*>(a.down) + it.index * a.rank * a.in;
-  const T* w[N];
-#pragma unroll
-  for (int t = 0; t < N; ++t) w[t] = down + (int64_t)down_row<NP>(t, lane & 15, it.used) * a.in;
   f32x4 h[TT][N];
 #pragma unroll
   for (int i = 0; i < TT; ++i)
 #pragma unroll
     for (int t = 0; t < N; ++t) h[i][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  const int64_t steps = (a.in + 31) / 32, share = (steps + kWaves - 1) / kWaves;
-  const int64_t to = (wave + 1) * share;
-  shrink<T, NP, TT, (N + TT > 6 ? 2 : 4)>(tokens.x, w, a.in, wave * share, to < steps ? to : steps, h);
+  {
+    const T* x[TT][4];
+    rows_of_x<T, TT>(a, b, first, x);
+    int64_t w_first[S];
+    rows_of_down<S>(it.used, a.in, w_first);
+    const int64_t slabs = (a.in + kSlab - 1) / kSlab, share = (slabs + kWaves - 1) / kWaves;
+    const int64_t to = (wave + 1) * share;
+    shrink<T, S, TT>(x, static_cast<const T*>(a.down) + it.index * a.rank * a.in, w_first, a.in, wave * share,
+                     to < slabs ? to : slabs, h);
+  }
 #pragma unroll
   for (int i = 0; i < TT; ++i)
 #pragma unroll
-    for (int t = 0; t < N; ++t) sums[wave][i * N + t][lane] = h[i][t];
+    for (int t = 0; t < N; ++t) lds.sums[wave][i * N + t][lane] = h[i][t];
+  // the first group's loads pass the waves' meeting
+  const Tokens<T, TT> tokens(a, b, first, it.count);
+  const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
+  Group<T, S, TT> data;
+  data.load(up, a.rank, a.out, it.used, wave < groups ? wave : 0, tokens);
   __syncthreads();
-  Hidden<T, NP> hidden[TT];
+  Hidden<T, S> hidden[TT];
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
 #pragma unroll
     for (int t = 0; t < N; ++t) {
-      h[i][t] = sums[0][i * N + t][lane];
+      h[i][t] = lds.sums[0][i * N + t][lane];
 #pragma unroll
-      for (int k = 1; k < kWaves; ++k) h[i][t] += sums[k][i * N + t][lane];
+      for (int k = 1; k < kWaves; ++k) h[i][t] += lds.sums[k][i * N + t][lane];
     }
-    hidden[i] = make_hidden<T, NP>(h[i], it.used);
+    hidden[i] = make_hidden<T, S>(h[i], it.used, it.scale);
   }
-  const float scale = a.scales != nullptr ? a.scales[it.index] : 1.0f;
-  const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
-  Group<T, NP, TT> buffer[2];
-  int64_t g = wave;
-  if (g < groups) buffer[0].load(up, a.rank, a.out, it.used, g, tokens.base);
-  while (g < groups) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (g >= groups) break;
-      if (g + kWaves < groups) buffer[1 - k].load(up, a.rank, a.out, it.used, g + kWaves, tokens.base);
-      buffer[k].finish(a.out, g, scale, hidden, tokens.y, tokens.live, tokens.added);
-      g += kWaves;
-    }
-  }
+  __syncthreads();
+  expand<T, S, TT>(data, lds.up[wave], up, a.rank, a.out, it.used, wave, groups, kWaves, hidden, tokens);
 }
 
-// Partial sums of h: workgroup (tile, part) takes the part's steps, its waves in turn.
-template <typename T, int NP>
+// Partial sums of h: workgroup (tile, part) takes the part's slabs, shared by its waves.
+template <typename T, int S>
 __global__ __launch_bounds__(kThreads) void low_rank_shrink_kernel(const LowRankArgs a) {
-  constexpr int N = kTiles<NP>;
+  constexpr int N = 2 * S;
   __shared__ f32x4 sums[kWaves - 1][N][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -388,70 +498,76 @@ __global__ __launch_bounds__(kThreads) void low_rank_shrink_kernel(const LowRank
   const int64_t first = (tile - b * a.tiles_of_seq) * 16;
   const Adapter it = adapter_of(a, b);
   if (it.used == 0 || first >= it.count) return;
-  const Tokens<T, 1> tokens = tokens_of<T, 1>(a, b, first, it.count);
-  const T* down = static_cast<const T*>(a.down) + it.index * a.rank * a.in;
-  const T* w[N];
-#pragma unroll
-  for (int t = 0; t < N; ++t) w[t] = down + (int64_t)down_row<NP>(t, lane & 15, it.used) * a.in;
+  const T* x[1][4];
+  rows_of_x<T, 1>(a, b, first, x);
+  int64_t w_first[S];
+  rows_of_down<S>(it.used, a.in, w_first);
   f32x4 h[1][N];
 #pragma unroll
   for (int t = 0; t < N; ++t) h[0][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  const int64_t steps = (a.in + 31) / 32;
-  const int64_t from = (int64_t)part * a.steps_of_part;
-  const int64_t to = from + a.steps_of_part < steps ? from + a.steps_of_part : steps;
+  const int64_t slabs = (a.in + kSlab - 1) / kSlab;
+  const int64_t from = (int64_t)part * a.slabs_of_part;
+  const int64_t to = from + a.slabs_of_part < slabs ? from + a.slabs_of_part : slabs;
   const int64_t share = (to - from + kWaves - 1) / kWaves;
   const int64_t mine = from + wave * share;
-  shrink<T, NP, 1, (N > 4 ? 2 : 4)>(tokens.x, w, a.in, mine, mine + share < to ? mine + share : to, h);
+  shrink<T, S, 1>(x, static_cast<const T*>(a.down) + it.index * a.rank * a.in, w_first, a.in, mine,
+                  mine + share < to ? mine + share : to, h);
   if (wave != 0) {
 #pragma unroll
     for (int t = 0; t < N; ++t) sums[wave - 1][t][lane] = h[0][t];
   }
   __syncthreads();
   if (wave != 0) return;
-  f32x4* partial = reinterpret_cast<f32x4*>(a.partial) + ((int64_t)part * a.tiles + tile) * N * 64;
+  f32x4* partial = reinterpret_cast<f32x4*>(a.partial) + ((int64_t)part * a.tiles + tile) * (N * 64) + lane;
 #pragma unroll
   for (int t = 0; t < N; ++t) {
     f32x4 sum = h[0][t];
 #pragma unroll
     for (int k = 0; k < kWaves - 1; ++k) sum += sums[k][t][lane];
-    partial[t * 64 + lane] = sum;
+    partial[t * 64] = sum;
   }
 }
 
-template <typename T, int NP>
+// The sums of h's parts, in order, and the outputs.  A wave's groups lie a workgroup's
+// waves apart.
+template <typename T, int S>
 __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRankArgs a) {
-  constexpr int N = kTiles<NP>;
+  constexpr int N = 2 * S;
+  __shared__ __align__(16) UpStage<S> lds[kWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t groups = (uint32_t)((a.out + kGroup - 1) / kGroup);
-  const uint32_t workgroups = (groups + kWaves - 1) / kWaves;  // of a tile
+  const uint32_t share = (uint32_t)a.groups_of_wave * kWaves;  // groups of a workgroup
+  const uint32_t workgroups = (groups + share - 1) / share;    // of a tile
   const int64_t tile = blockIdx.x / workgroups;
-  const int64_t group = (int64_t)(blockIdx.x % workgroups) * kWaves + wave;
-  if (group >= groups) return;
+  const int64_t from = (int64_t)(blockIdx.x % workgroups) * share, mine = from + wave;
+  const int64_t to = from + share < groups ? from + share : groups;
+  if (mine >= to) return;
   const int64_t b = tile / a.tiles_of_seq;
   const int64_t first = (tile - b * a.tiles_of_seq) * 16;
   const Adapter it = adapter_of(a, b);
-  const Tokens<T, 1> tokens = tokens_of<T, 1>(a, b, first, it.count);
+  const Tokens<T, 1> tokens(a, b, first, it.count);
   if (it.used == 0 || first >= it.count) {
-    copy_groups<T, 1, 1>(a.out, group, group + 1, 1, tokens.base, tokens.y, tokens.live);
+    copy_groups<T, 1, 1>(a.out, mine, to, kWaves, tokens);
     return;
   }
-  Group<T, NP, 1> data;
-  data.load(static_cast<const T*>(a.up) + it.index * a.out * a.rank, a.rank, a.out, it.used, group, tokens.base);
+  const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
+  // (the first group's loads before the parts', which they would wait for)
+  Group<T, S, 1> data;
+  data.load(up, a.rank, a.out, it.used, mine, tokens);
   f32x4 h[N];
 #pragma unroll
   for (int t = 0; t < N; ++t) h[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  if (tokens.added[0]) {
-    const f32x4* partial = reinterpret_cast<const f32x4*>(a.partial) + tile * N * 64 + lane;
-    // (of tiles that no row of down fills, what is read is not used)
+  if (first + (lane & 15) < it.count) {
+    const f32x4* partial = reinterpret_cast<const f32x4*>(a.partial) + tile * (N * 64) + lane;
+    // (of rows that no row of down fills, what is read is not used)
 #pragma unroll 4
     for (int p = 0; p < a.parts; ++p)
 #pragma unroll
-      for (int t = 0; t < N; ++t) h[t] += partial[(int64_t)p * a.tiles * N * 64 + t * 64];
+      for (int t = 0; t < N; ++t) h[t] += partial[(int64_t)p * a.tiles * (N * 64) + t * 64];
   }
-  const float scale = a.scales != nullptr ? a.scales[it.index] : 1.0f;
-  const Hidden<T, NP> hidden[1] = {make_hidden<T, NP>(h, it.used)};
-  data.finish(a.out, group, scale, hidden, tokens.y, tokens.live, tokens.added);
+  const Hidden<T, S> hidden[1] = {make_hidden<T, S>(h, it.used, it.scale)};
+  expand<T, S, 1>(data, lds[wave], up, a.rank, a.out, it.used, mine, to, kWaves, hidden, tokens);
 }
 
 // How a call is launched.
@@ -459,46 +575,56 @@ struct Plan {
   bool fused;
   int tokens;              // of a tile
   int64_t tiles_of_seq, tiles;
-  int parts, steps_of_part;
+  int parts, slabs_of_part, groups_of_wave;
   int rank_tiles;
   size_t bytes;
 };
-constexpr int64_t kManyTiles = 1024;  // of 16 tokens: from here on one launch does both products
+// Tiles of 16 tokens from which on one launch does both products.  4096 -> 4096, two
+// launches / one, us: 8704 tokens of rank 16 58 / 57, of rank 128 131 / 144; 17408 tokens
+// 108 / 109 and 228 / 231; 34816 tokens 195 / 188 and 434 / 405.  Requests of up to a
+// tile's tokens would leave the larger workgroups' places empty.
+constexpr int64_t kManyTiles = 1024;
 
-Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t rank) {
+Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t out, int64_t rank) {
   Plan p{};
-  p.rank_tiles = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
+  p.rank_tiles = rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
   p.tokens = 16;
   p.tiles_of_seq = ceil_div(seq, 16);
   p.tiles = batch * p.tiles_of_seq;
-  p.fused = p.tiles >= kManyTiles;
+  p.fused = p.tiles >= kManyTiles && seq > 16;
   if (p.fused) {
     p.tokens = 16 * kFusedTiles;
     p.tiles_of_seq = ceil_div(seq, p.tokens);
     p.tiles = batch * p.tiles_of_seq;
     return p;
   }
-  const int64_t steps = ceil_div(in, 32);
-  int64_t parts = ceil_div(1024, p.tiles);
-  const int64_t most = ceil_div(steps, 4 * kWaves);
+  // Parts for a workgroup a unit, a slab a wave at least: every wave of the second launch
+  // reads them all (64 tokens, 4096 -> 4096, rank 64: 18 us with 4, 20 with 8, 25 with 16).
+  const int64_t slabs = ceil_div(in, kSlab);
+  int64_t parts = ceil_div(256, p.tiles);
+  const int64_t most = ceil_div(slabs, kWaves);
   if (parts > most) parts = most;
-  p.steps_of_part = (int)ceil_div(steps, parts);
-  p.parts = (int)ceil_div(steps, p.steps_of_part);
+  p.slabs_of_part = (int)ceil_div(slabs, parts);
+  p.parts = (int)ceil_div(slabs, p.slabs_of_part);
+  // Several groups a wave, as long as that leaves waves for all units (16384 tokens, 4096
+  // outputs, rank 64: the second launch 130 us with one, 105 with eight).
+  const int64_t waves = p.tiles * ceil_div(out, kGroup);
+  p.groups_of_wave = waves >= 8 * 4096 ? 8 : waves >= 4 * 4096 ? 4 : waves >= 2 * 4096 ? 2 : 1;
   p.bytes = (size_t)(p.parts * p.tiles * p.rank_tiles) * 64 * sizeof(f32x4);
   return p;
 }
 
-template <typename T, int NP>
+template <typename T, int S>
 int launch(const LowRankArgs& a, const Plan& p, hipStream_t stream) {
   if (p.fused) {
-    hipLaunchKernelGGL((low_rank_fused_kernel<T, NP, kFusedTiles>), dim3((unsigned)p.tiles), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((low_rank_fused_kernel<T, S, kFusedTiles>), dim3((unsigned)p.tiles), dim3(kThreads), 0, stream, a);
     return check_hip(hipGetLastError(), "low-rank adapters launch");
   }
-  hipLaunchKernelGGL((low_rank_shrink_kernel<T, NP>), dim3((unsigned)(p.tiles * p.parts)), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((low_rank_shrink_kernel<T, S>), dim3((unsigned)(p.tiles * p.parts)), dim3(kThreads), 0, stream, a);
   const int status = check_hip(hipGetLastError(), "low-rank adapters launch");
   if (status != SAH_OK) return status;
-  const int64_t workgroups = ceil_div(ceil_div(a.out, kGroup), kWaves);
-  hipLaunchKernelGGL((low_rank_expand_kernel<T, NP>), dim3((unsigned)(p.tiles * workgroups)), dim3(kThreads), 0, stream,
+  const int64_t workgroups = ceil_div(ceil_div(a.out, kGroup), kWaves * p.groups_of_wave);
+  hipLaunchKernelGGL((low_rank_expand_kernel<T, S>), dim3((unsigned)(p.tiles * workgroups)), dim3(kThreads), 0, stream,
                      a);
   return check_hip(hipGetLastError(), "low-rank adapters launch");
 }
@@ -506,7 +632,6 @@ int launch(const LowRankArgs& a, const Plan& p, hipStream_t stream) {
 template <typename T>
 int launch_rank(const LowRankArgs& a, const Plan& p, hipStream_t stream) {
   switch (p.rank_tiles) {
-    case 1: return launch<T, 0>(a, p, stream);
     case 2: return launch<T, 1>(a, p, stream);
     case 4: return launch<T, 2>(a, p, stream);
     default: return launch<T, 4>(a, p, stream);
@@ -526,7 +651,7 @@ using namespace sah;
 extern "C" size_t sah_low_rank_adapters_workspace_bytes(int64_t batch, int64_t seq_len, int64_t in_features,
                                                         int64_t out_features, int64_t rank) {
   if (!sizes_ok(batch, seq_len, in_features, out_features, rank) || batch == 0 || seq_len == 0) return 0;
-  return plan_of(batch, seq_len, in_features, rank).bytes;
+  return plan_of(batch, seq_len, in_features, out_features, rank).bytes;
 }
 
 extern "C" int sah_low_rank_adapters(const void* x, const void* base, const void* down, const void* up,
@@ -568,7 +693,7 @@ extern "C" int sah_low_rank_adapters(const void* x, const void* base, const void
   const int64_t most = (int64_t)(UINT32_MAX / kThreads);
   if (tiles > most / ceil_div(out_features, kGroup))
     return fail(SAH_ERR_UNSUPPORTED, "%s: too many tokens for one launch", what);
-  const Plan plan = plan_of(batch, seq_len, in_features, rank);
+  const Plan plan = plan_of(batch, seq_len, in_features, out_features, rank);
   if (plan.bytes != 0 && (workspace == nullptr || workspace_bytes < plan.bytes))
     return fail(SAH_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", what, workspace == nullptr ? 0 : workspace_bytes,
                 plan.bytes);
@@ -599,7 +724,8 @@ extern "C" int sah_low_rank_adapters(const void* x, const void* base, const void
   a.tiles_of_seq = plan.tiles_of_seq;
   a.tiles = plan.tiles;
   a.parts = plan.parts;
-  a.steps_of_part = plan.steps_of_part;
+  a.slabs_of_part = plan.slabs_of_part;
+  a.groups_of_wave = plan.groups_of_wave;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == SAH_DTYPE_BF16 ? launch_rank<bf16>(a, plan, s) : launch_rank<f16>(a, plan, s);
 }
