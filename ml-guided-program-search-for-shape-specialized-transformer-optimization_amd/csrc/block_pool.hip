@@ -56,8 +56,12 @@ __device__ __forceinline__ int scan_threads(int value, int* sums, int& total) {
 // Bit i: place first + i is there and has holders.
 __device__ __forceinline__ uint32_t held_bits(const int32_t* holders, int64_t first, int64_t blocks) {
   int32_t count[kPerThread];
+  if (first + kPerThread <= blocks) {
+    __builtin_memcpy(count, holders + first, sizeof(count));
+  } else {
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) count[i] = first + i < blocks ? holders[first + i] : 0;
+    for (int i = 0; i < kPerThread; ++i) count[i] = first + i < blocks ? holders[first + i] : 0;
+  }
   uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) bits |= (count[i] > 0 ? 1u : 0u) << i;
@@ -213,6 +217,11 @@ __global__ __launch_bounds__(kThreads) void pool_fork_kernel(const Pool pool, co
   }
 }
 
+// Places and entries up to which one launch compacts a pool: 12.7 -> 8.4 us on the host,
+// which is what a small pool's compaction takes (4128 of either: 11 us on the GPU in one
+// launch, 8.6 + 4.6 in two).
+constexpr int64_t kSmallPool = 16384;
+
 struct CompactArgs {
   Pool pool;
   int32_t* origins;  // [blocks]
@@ -223,9 +232,29 @@ struct CompactArgs {
   int32_t* moves;    // workspace [1]
 };
 
+// The entries take their places' new names, and each hole its mover's holders, by threads
+// first, first + step, ...
+__device__ __forceinline__ void compact_apply(const CompactArgs& a, int used, int moves, int64_t first, int64_t step) {
+  for (int64_t i = first; i < moves; i += step) {
+    const int32_t hole = a.holes[i], mover = a.movers[i];
+    a.origins[hole] = mover;
+    a.pool.holders[hole] = a.pool.holders[mover];
+    a.pool.holders[mover] = 0;
+  }
+  const int64_t entries = (int64_t)a.pool.batch * a.pool.max_blocks;
+  for (int64_t i = first; i < entries; i += step) {
+    const int32_t place = a.pool.table[i];
+    if (place < used || place >= a.pool.blocks) continue;
+    // (ranks holds nothing for a place without holders, which nothing should name)
+    const int rank = a.ranks[place];
+    if (rank >= 0 && rank < moves && a.movers[rank] == place) a.pool.table[i] = a.holes[rank];
+  }
+}
+
 // `used` places have holders.  The free ones below `used` are as many as the held
 // ones from there on, and take their contents in order.  One workgroup counts, then
-// lists both.
+// lists both; of a small pool it does the rest too (APPLIES).
+template <bool APPLIES>
 __global__ __launch_bounds__(kScanThreads) void pool_compact_list_kernel(const CompactArgs a) {
   __shared__ int sums[2][kScanThreads / 64];
   const int64_t blocks = a.pool.blocks;
@@ -267,26 +296,14 @@ __global__ __launch_bounds__(kScanThreads) void pool_compact_list_kernel(const C
     *a.used = used;
     *a.moves = movers;
   }
+  if constexpr (APPLIES) {
+    __syncthreads();  // (after the last reads of holders, too)
+    compact_apply(a, used, movers, tid, kScanThreads);
+  }
 }
 
-// The entries take their places' new names, and each hole its mover's holders.
-__global__ __launch_bounds__(kThreads) void pool_compact_apply_kernel(const CompactArgs a, int64_t entries) {
-  const int64_t step = (int64_t)gridDim.x * kThreads;
-  const int64_t first = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int used = *a.used, moves = *a.moves;
-  for (int64_t i = first; i < moves; i += step) {
-    const int32_t hole = a.holes[i], mover = a.movers[i];
-    a.origins[hole] = mover;
-    a.pool.holders[hole] = a.pool.holders[mover];
-    a.pool.holders[mover] = 0;
-  }
-  for (int64_t i = first; i < entries; i += step) {
-    const int32_t place = a.pool.table[i];
-    if (place < used || place >= a.pool.blocks) continue;
-    // (ranks holds nothing for a place without holders, which nothing should name)
-    const int rank = a.ranks[place];
-    if (rank >= 0 && rank < moves && a.movers[rank] == place) a.pool.table[i] = a.holes[rank];
-  }
+__global__ __launch_bounds__(kThreads) void pool_compact_apply_kernel(const CompactArgs a) {
+  compact_apply(a, *a.used, *a.moves, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
 struct CopyArgs {
@@ -348,27 +365,51 @@ __global__ __launch_bounds__(kThreads) void cache_copy_kernel(const CopyArgs a) 
 
 // The tail of sequence sources[b] goes to sequence b.  A slice of the tails' bytes is a
 // problem of its own: a workgroup has read its slice of every tail that it copies
-// before it writes any.
+// before it writes any.  The sequences that change are listed first, so that a thread's
+// accesses are in flight together: 64 sequences, half of them copies, of 8 heads of 128 (17
+// MB) 4 us, 9.9 with each sequence's source looked up on its way (5.2 with slices of 1 KiB).
+constexpr int kForkLoads = 8;  // of a thread in flight
+
 __global__ __launch_bounds__(kThreads) void cache_fork_kernel(char* key_tail, char* value_tail, const int32_t* sources,
                                                               int batch, int64_t tail_bytes, int slice_bytes) {
-  extern __shared__ __align__(16) u32x4 held[];  // [batch][slice_bytes / 16]
-  const int lanes = slice_bytes / 16;            // a power of two
-  const int slot = threadIdx.x & (lanes - 1);
+  extern __shared__ __align__(16) u32x4 held[];  // [changed][slice_bytes / 16]
+  __shared__ int16_t targets[kMaxForked], origins[kMaxForked];
+  __shared__ int changed;
+  const int lanes = slice_bytes / 16;  // a power of two
   const uint32_t slices = (uint32_t)(tail_bytes / slice_bytes);
-  char* tail = blockIdx.x < slices ? key_tail : value_tail;
-  const int64_t at = (int64_t)(blockIdx.x % slices) * slice_bytes + slot * 16;
-  const int rows = kThreads / lanes;
-  for (int b = threadIdx.x / lanes; b < batch; b += rows) {
-    const int source = sources[b];
-    if (source < 0 || source >= batch || source == b) continue;
-    held[b * lanes + slot] = load16(tail + source * tail_bytes + at);
+  char* tail = (blockIdx.x < slices ? key_tail : value_tail) + (int64_t)(blockIdx.x % slices) * slice_bytes;
+  if (threadIdx.x < 64) {  // a wave lists them in order
+    int count = 0;
+    for (int at = 0; at < batch; at += 64) {
+      const int b = at + threadIdx.x;
+      const int source = b < batch ? sources[b] : -1;
+      const bool changes = source >= 0 && source < batch && source != b;
+      const uint64_t votes = __ballot(changes);
+      if (changes) {
+        const int place = count + __popcll(votes & ((1ull << threadIdx.x) - 1));
+        targets[place] = (int16_t)b;
+        origins[place] = (int16_t)source;
+      }
+      count += __popcll(votes);
+    }
+    if (threadIdx.x == 0) changed = count;
   }
   __syncthreads();
-  for (int b = threadIdx.x / lanes; b < batch; b += rows) {
-    const int source = sources[b];
-    if (source < 0 || source >= batch || source == b) continue;
-    store16(tail + b * tail_bytes + at, held[b * lanes + slot]);
+  const int parts = changed * lanes;
+  for (int at = threadIdx.x; at < parts; at += kForkLoads * kThreads) {
+    u32x4 data[kForkLoads];
+#pragma unroll
+    for (int i = 0; i < kForkLoads; ++i) {
+      const int part = at + i * kThreads;
+      if (part < parts) data[i] = load16(tail + origins[part / lanes] * tail_bytes + (part & (lanes - 1)) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < kForkLoads; ++i)
+      if (at + i * kThreads < parts) held[at + i * kThreads] = data[i];
   }
+  __syncthreads();
+  for (int part = threadIdx.x; part < parts; part += kThreads)
+    store16(tail + targets[part / lanes] * tail_bytes + (part & (lanes - 1)) * 16, held[part]);
 }
 
 struct TakeBackArgs {
@@ -559,14 +600,17 @@ extern "C" int sah_block_pool_compact(int32_t* block_table, int32_t* holders, in
   a.ranks = a.movers + num_blocks / 2 + 1;
   a.moves = a.ranks + num_blocks;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(pool_compact_list_kernel, dim3(1), dim3(kScanThreads), 0, s, a);
+  const int64_t entries = batch * max_blocks;
+  if (entries <= kSmallPool && num_blocks <= kSmallPool) {
+    hipLaunchKernelGGL(pool_compact_list_kernel<true>, dim3(1), dim3(kScanThreads), 0, s, a);
+    return check_hip(hipGetLastError(), "block pool compact launch");
+  }
+  hipLaunchKernelGGL(pool_compact_list_kernel<false>, dim3(1), dim3(kScanThreads), 0, s, a);
   status = check_hip(hipGetLastError(), "block pool compact launch");
   if (status != SAH_OK) return status;
-  const int64_t entries = batch * max_blocks;
   const int64_t most = entries > num_blocks / 2 ? entries : num_blocks / 2;
-  const int64_t grid = ceil_div(most > 0 ? most : 1, kThreads);
-  hipLaunchKernelGGL(pool_compact_apply_kernel, dim3((unsigned)(grid < 2048 ? grid : 2048)), dim3(kThreads), 0, s, a,
-                     entries);
+  const int64_t grid = ceil_div(most, kThreads);
+  hipLaunchKernelGGL(pool_compact_apply_kernel, dim3((unsigned)(grid < 2048 ? grid : 2048)), dim3(kThreads), 0, s, a);
   return check_hip(hipGetLastError(), "block pool compact launch");
 }
 
@@ -614,9 +658,9 @@ extern "C" int sah_block_cache_fork(void* key_tail, void* value_tail, const int3
     return fail(SAH_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
   if (!aligned16(key_tail) || !aligned16(value_tail))
     return fail(SAH_ERR_INVALID_ARGUMENT, "%s: tails must be 16-byte aligned", what);
-  // the widest slice whose part of every tail fits 64 KiB
-  int slice = 1024;
-  while (slice * batch > 65536) slice /= 2;
+  // the widest slice whose part of every tail fits 48 KiB
+  int slice = 512;
+  while (slice * batch > 49152) slice /= 2;
   const int64_t tail_bytes = kv_heads * kBlockTokens * head_dim * 2;
   hipLaunchKernelGGL(cache_fork_kernel, dim3((unsigned)(2 * (tail_bytes / slice))), dim3(kThreads),
                      (size_t)(slice * batch), reinterpret_cast<hipStream_t>(stream), static_cast<char*>(key_tail),

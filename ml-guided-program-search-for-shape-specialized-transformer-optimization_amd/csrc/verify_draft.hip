@@ -28,8 +28,8 @@
 // 56 us, decide 7, weigh 22, pick 6.  fp64's v_fma issues at fp32's rate here, but with
 // all rows in fp64 the vector units took 126 us for them.  The draw's two parts in one
 // launch, by the request's last workgroup, took 106 us instead of 27: each of the 4096
-// releases its L2's lines.  For one request (4 drafts, 32000 tokens) each part is a
-// launch's latency, 4 us.
+// releases its L2's lines.  For one request (4 drafts, 32000 tokens) the parts are
+// launches' latencies, 4 + 7.5 + 4 us.
 
 #include <type_traits>
 
@@ -46,6 +46,10 @@ constexpr int kDecideThreads = 1024;
 constexpr int kPickThreads = 256;
 constexpr int kPickChunk = kPickThreads * kVec;
 constexpr int kMaxDrafts = 1024;
+// Workgroups of the draw up to which each decides for itself, for a launch less: one request
+// of 32000 tokens and 4 drafts 7.5 us instead of 4.7 + 4.5, 8 of 131072 tokens and 3 drafts
+// 9.0 instead of 6.2 + 5.9; 16 with 7 drafts (1024 workgroups) 14.8 and 6.2 + 7.6.
+constexpr int64_t kFewWorkgroups = 512;
 constexpr double kLog2e = 1.4426950408889634074;
 // A row's sum in fp32, relative: an exponent |x| <= 64 (what lies below adds less than
 // 2^-33) is off by its difference's, its factor's and its product's rounding, 3 * 64 *
@@ -339,11 +343,23 @@ __device__ __forceinline__ RowSum merge_row(const RowPart* parts, int chunks, do
   return {wave_add(sum), top, wave_lowest(at)};
 }
 
+// What the threads of a workgroup that decides tell each other.
+struct Seen {
+  RowSum p, q;
+  int32_t stands;  // 1: the draft stands, 0: it does not, -1: too near to say
+  int32_t none;    // 1: no distribution to draw from
+};
+template <int THREADS>
+struct DecideShared {
+  Seen seen[THREADS / 64];
+  double sums[THREADS / 64];
+};
+
 // A row's sum of exponentials in fp64, by the workgroup.
-template <typename T>
-__device__ double exact_sum(const T* row, float top, double c, int64_t vocab, double* waves) {
+template <typename T, int THREADS>
+__device__ double exact_sum(const T* row, float top, double c, int64_t vocab, DecideShared<THREADS>& shared) {
   double sum = 0.0;
-  for (int64_t at = (int64_t)threadIdx.x * kVec; at < vocab; at += kDecideThreads * kVec) {
+  for (int64_t at = (int64_t)threadIdx.x * kVec; at < vocab; at += THREADS * kVec) {
     float l[kVec];
     load_logits<T>(row, at, vocab, l);
 #pragma unroll
@@ -351,36 +367,28 @@ __device__ double exact_sum(const T* row, float top, double c, int64_t vocab, do
   }
   sum = wave_add(sum);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+  if ((threadIdx.x & 63) == 0) shared.sums[threadIdx.x >> 6] = sum;
   __syncthreads();
   sum = 0.0;
-  for (int w = 0; w < kDecideThreads / 64; ++w) sum += waves[w];
+  for (int w = 0; w < THREADS / 64; ++w) sum += shared.sums[w];
   return sum;
 }
 
-// A workgroup a request; a wave a row of the target, with the draft's beside it.  16 rows
-// at a time, up to the first draft that does not stand.
-template <typename T>
-__global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(const VerifyArgs a) {
-  constexpr int WAVES = kDecideThreads / 64;
-  struct Seen {
-    RowSum p, q;
-    int32_t stands;   // 1: the draft stands, 0: it does not, -1: too near to say
-    int32_t none;     // 1: no distribution to draw from
-  };
-  __shared__ Seen seen[WAVES];
-  __shared__ double sums[WAVES];
-  const int64_t b = blockIdx.x;
+// Request b's decision by a workgroup, which leaves what it answers already where it
+// `writes`.  A wave takes a row of the target, with the draft's beside it; as many rows at
+// a time as there are waves, up to the first draft that does not stand.
+template <typename T, int THREADS>
+__device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShared<THREADS>& shared) {
+  constexpr int WAVES = THREADS / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int count = drafts_of(a, b);
   int64_t* answer = a.answer + b * (a.drafts + 1);
   if (count < 0) {
-    for (int i = tid; i <= a.drafts; i += kDecideThreads) answer[i] = -1;
-    if (tid == 0) {
-      a.accepted[b] = -1;
-      a.choices[b].mode = kDone;
+    if (writes) {
+      for (int i = tid; i <= a.drafts; i += THREADS) answer[i] = -1;
+      if (tid == 0) a.accepted[b] = -1;
     }
-    return;
+    return {0, kDone, 0.0f, 0.0f, 0.0, 0.0};
   }
   double c;
   const bool greedy = is_greedy(a, b, c);
@@ -417,46 +425,54 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(const Ver
           mine.stands = fabs(q - p) <= kFastError * p && p > 0.0 ? -1 : q < p ? 1 : 0;
         }
       }
-      if (lane == 0) seen[wave] = mine;
+      if (lane == 0) shared.seen[wave] = mine;
     }
     __syncthreads();
     for (int w = 0; w < WAVES && j < 0; ++w) {
       const int at = first + w;
-      int stands = seen[w].stands;
+      int stands = shared.seen[w].stands;
       if (stands < 0) {  // (the same for every thread)
         const int64_t token = tokens[at];
-        const Seen& it = seen[w];
+        const Seen& it = shared.seen[w];
         const T* p_row = target + at * a.t_ss;
-        const double p = weight_of(to_f32(p_row[token]), it.p.top, c) / exact_sum<T>(p_row, it.p.top, c, a.vocab, sums);
+        const double p =
+            weight_of(to_f32(p_row[token]), it.p.top, c) / exact_sum<T>(p_row, it.p.top, c, a.vocab, shared);
         double q = (double)uniforms[at];
         if (sampled) {
           const T* q_row = draft + at * a.d_ss;
-          q *= weight_of(to_f32(q_row[token]), it.q.top, c) / exact_sum<T>(q_row, it.q.top, c, a.vocab, sums);
+          q *= weight_of(to_f32(q_row[token]), it.q.top, c) / exact_sum<T>(q_row, it.q.top, c, a.vocab, shared);
         }
         stands = q < p ? 1 : 0;
       }
       if (stands == 0 || at == count) {
         j = at;
-        found = seen[w];
+        found = shared.seen[w];
       }
     }
     __syncthreads();
   }
 
   const bool done = greedy || found.none != 0;
-  for (int i = tid; i <= a.drafts; i += kDecideThreads) {
-    if (i < j)
-      answer[i] = tokens[i];
-    else if (i > j || done)  // answer[j] is the draw's otherwise
-      answer[i] = i == j && found.none == 0 ? found.p.at : -1;
+  if (writes) {
+    for (int i = tid; i <= a.drafts; i += THREADS) {
+      if (i < j)
+        answer[i] = tokens[i];
+      else if (i > j || done)  // answer[j] is the draw's otherwise
+        answer[i] = i == j && found.none == 0 ? found.p.at : -1;
+    }
+    if (tid == 0) a.accepted[b] = j;
   }
-  if (tid == 0) {
-    a.accepted[b] = j;
-    Choice choice{j, kDone, found.p.top, found.q.top, 0.0, c};
-    if (!done) choice.mode = j == count ? kFromTarget : sampled ? kResample : kWithout;
-    if (choice.mode == kResample) choice.ratio = found.p.sum / found.q.sum;
-    a.choices[b] = choice;
-  }
+  Choice choice{j, kDone, found.p.top, found.q.top, 0.0, c};
+  if (!done) choice.mode = j == count ? kFromTarget : sampled ? kResample : kWithout;
+  if (choice.mode == kResample) choice.ratio = found.p.sum / found.q.sum;
+  return choice;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(const VerifyArgs a) {
+  __shared__ DecideShared<kDecideThreads> shared;
+  const Choice it = decide<T>(a, blockIdx.x, true, shared);
+  if (threadIdx.x == 0) a.choices[blockIdx.x] = it;
 }
 
 // e_p and e_q of 8 tokens (e_q: 0 where it takes no part); zeros behind the row's end.
@@ -481,13 +497,21 @@ struct Rows {
   }
 };
 
-template <typename T>
+// DECIDES: every workgroup decides for itself, for one launch less.
+template <typename T, bool DECIDES>
 __global__ __launch_bounds__(kPickThreads) void verify_weigh_kernel(const VerifyArgs a) {
   constexpr int WAVES = kPickThreads / 64;
   __shared__ Weights waves[WAVES];
   const uint32_t chunk = blockIdx.x % (uint32_t)a.pick_chunks;
   const int64_t b = blockIdx.x / (uint32_t)a.pick_chunks;
-  const Choice it = a.choices[b];
+  Choice it;
+  if constexpr (DECIDES) {
+    __shared__ DecideShared<kPickThreads> shared;
+    it = decide<T>(a, b, chunk == 0, shared);
+    if (chunk == 0 && threadIdx.x == 0) a.choices[b] = it;
+  } else {
+    it = a.choices[b];
+  }
   if (it.mode == kDone) return;
   const Rows<T> rows(a, b, it);
   double p[kVec], q[kVec];
@@ -634,9 +658,13 @@ int launch(const VerifyArgs& a, const Layout& layout, hipStream_t stream) {
   const unsigned batch = (unsigned)a.batch;
   hipLaunchKernelGGL(verify_rows_kernel<T>, dim3((unsigned)(batch * layout.rows * layout.row_chunks)),
                      dim3(kRowThreads), 0, stream, a);
-  hipLaunchKernelGGL(verify_decide_kernel<T>, dim3(batch), dim3(kDecideThreads), 0, stream, a);
-  hipLaunchKernelGGL(verify_weigh_kernel<T>, dim3((unsigned)(batch * layout.pick_chunks)), dim3(kPickThreads), 0,
-                     stream, a);
+  const int64_t weighing = batch * layout.pick_chunks;
+  if (weighing <= kFewWorkgroups) {
+    hipLaunchKernelGGL((verify_weigh_kernel<T, true>), dim3((unsigned)weighing), dim3(kPickThreads), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(verify_decide_kernel<T>, dim3(batch), dim3(kDecideThreads), 0, stream, a);
+    hipLaunchKernelGGL((verify_weigh_kernel<T, false>), dim3((unsigned)weighing), dim3(kPickThreads), 0, stream, a);
+  }
   hipLaunchKernelGGL(verify_pick_kernel<T>, dim3(batch), dim3(kPickThreads), 0, stream, a);
   return check_hip(hipGetLastError(), "verify draft launch");
 }

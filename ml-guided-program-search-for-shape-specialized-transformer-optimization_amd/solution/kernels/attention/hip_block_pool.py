@@ -127,21 +127,24 @@ def _words_ok(words: torch.Tensor | None, size: int, index: int) -> bool:
     )
 
 
-def _pool_library(pool: BlockPool, *lengths: torch.Tensor | None):
-    """The library and the device where the kernels take a pool and whole numbers
-    [batch], else None."""
+def _pool_request(pool: BlockPool, words: torch.Tensor | None = None, more: torch.Tensor | None = None) -> tuple | None:
+    """The library, the device, batch, max_blocks and num_blocks where the kernels take a
+    pool and whole numbers [batch], else None."""
 
-    index = pool.block_table.get_device()
-    if not all(_words_ok(words, pool.batch, index) for words in lengths):
+    table = pool.block_table
+    index, (batch, max_blocks) = table.get_device(), table.shape
+    if words is not None and not _words_ok(words, batch, index):
+        return None
+    if more is not None and not _words_ok(more, batch, index):
         return None
     library = library_for(index)
-    return None if library is None else (library, index)
+    return None if library is None else (library, index, batch, max_blocks, pool.holders.shape[0])
 
 
 def _reserve_request(pool: BlockPool, starts: torch.Tensor, tokens: int, counts: torch.Tensor | None):
     if not isinstance(tokens, int) or isinstance(tokens, bool) or not 0 <= tokens <= _MAX_TOKENS:
         return None
-    return _pool_library(pool, starts, *(() if counts is None else (counts,)))
+    return None if starts is None else _pool_request(pool, starts, counts)
 
 
 def can_use_hip_block_pool_reserve(
@@ -165,12 +168,11 @@ def hip_block_pool_reserve(
     request = _reserve_request(pool, starts, tokens, counts)
     if request is None:
         raise RuntimeError("HIP block pool reserve is ineligible for the requested inputs")
-    library, index = request
-    sizes = (pool.batch, pool.max_blocks, pool.num_blocks, tokens)
+    library, index, *sizes = request
     missing = torch.empty_like(starts)
     try:
-        size = library.sah_block_pool_reserve_workspace_bytes(*sizes)
-        workspace = torch.empty(size, dtype=torch.uint8, device=starts.device) if size else None
+        size = library.sah_block_pool_reserve_workspace_bytes(*sizes, tokens)
+        workspace = starts.new_empty(size // 4)  # 0 bytes without sequences
         launch(
             index,
             library.sah_block_pool_reserve,
@@ -181,7 +183,8 @@ def hip_block_pool_reserve(
             None if counts is None else counts.data_ptr(),
             missing.data_ptr(),
             *sizes,
-            None if workspace is None else workspace.data_ptr(),
+            tokens,
+            workspace.data_ptr(),
             size,
         )
     except HipLibraryError as exc:
@@ -192,17 +195,17 @@ def hip_block_pool_reserve(
 def can_use_hip_block_pool_release(pool: BlockPool, lengths: torch.Tensor) -> bool:
     """Whether the release kernel takes these tensors."""
 
-    return _pool_library(pool, lengths) is not None
+    return lengths is not None and _pool_request(pool, lengths) is not None
 
 
 def hip_block_pool_release(pool: BlockPool, lengths: torch.Tensor) -> str:
     """Give up every block of a sequence but its first ``lengths[b] // 64`` (0 frees a
     sequence that has ended, a negative length leaves it)."""
 
-    request = _pool_library(pool, lengths)
+    request = None if lengths is None else _pool_request(pool, lengths)
     if request is None:
         raise RuntimeError("HIP block pool release is ineligible for the requested inputs")
-    library, index = request
+    library, index, *sizes = request
     try:
         launch(
             index,
@@ -211,19 +214,23 @@ def hip_block_pool_release(pool: BlockPool, lengths: torch.Tensor) -> str:
             pool.block_table.data_ptr(),
             pool.holders.data_ptr(),
             lengths.data_ptr(),
-            pool.batch,
-            pool.max_blocks,
-            pool.num_blocks,
+            *sizes,
         )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block pool release execution failed") from exc
     return HIP_BLOCK_POOL_RELEASE_BACKEND
 
 
+def _fork_request(pool: BlockPool, sources: torch.Tensor, lengths: torch.Tensor) -> tuple | None:
+    if sources is None or lengths is None or pool.block_table.shape[0] > MAX_FORKED_SEQUENCES:
+        return None
+    return _pool_request(pool, sources, lengths)
+
+
 def can_use_hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.Tensor) -> bool:
     """Whether the fork kernel takes these tensors."""
 
-    return pool.batch <= MAX_FORKED_SEQUENCES and _pool_library(pool, sources, lengths) is not None
+    return _fork_request(pool, sources, lengths) is not None
 
 
 def hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.Tensor) -> str:
@@ -235,9 +242,10 @@ def hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.T
     tails follow with :func:`hip_block_cache_fork`.  Up to 1024 sequences.
     """
 
-    if not can_use_hip_block_pool_fork(pool, sources, lengths):
+    request = _fork_request(pool, sources, lengths)
+    if request is None:
         raise RuntimeError("HIP block pool fork is ineligible for the requested inputs")
-    library, index = _pool_library(pool, sources, lengths)
+    library, index, *sizes = request
     try:
         launch(
             index,
@@ -247,9 +255,7 @@ def hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.T
             pool.holders.data_ptr(),
             sources.data_ptr(),
             lengths.data_ptr(),
-            pool.batch,
-            pool.max_blocks,
-            pool.num_blocks,
+            *sizes,
         )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block pool fork execution failed") from exc
@@ -259,7 +265,7 @@ def hip_block_pool_fork(pool: BlockPool, sources: torch.Tensor, lengths: torch.T
 def can_use_hip_block_pool_compact(pool: BlockPool) -> bool:
     """Whether the compaction kernels take this pool."""
 
-    return _pool_library(pool) is not None
+    return _pool_request(pool) is not None
 
 
 def hip_block_pool_compact(pool: BlockPool) -> tuple[torch.Tensor, torch.Tensor, str]:
@@ -270,15 +276,15 @@ def hip_block_pool_compact(pool: BlockPool) -> tuple[torch.Tensor, torch.Tensor,
     cache is read or appended to; ``used`` [1] (int32) counts the places in use.
     """
 
-    request = _pool_library(pool)
+    request = _pool_request(pool)
     if request is None:
         raise RuntimeError("HIP block pool compact is ineligible for the requested inputs")
-    library, index = request
+    library, index, *sizes = request
     origins = torch.empty_like(pool.holders)
     used = pool.holders.new_empty((1,))
     try:
-        size = library.sah_block_pool_compact_workspace_bytes(pool.num_blocks)
-        workspace = torch.empty(size, dtype=torch.uint8, device=origins.device)
+        size = library.sah_block_pool_compact_workspace_bytes(sizes[2])
+        workspace = origins.new_empty(size // 4)
         launch(
             index,
             library.sah_block_pool_compact,
@@ -287,9 +293,7 @@ def hip_block_pool_compact(pool: BlockPool) -> tuple[torch.Tensor, torch.Tensor,
             pool.holders.data_ptr(),
             origins.data_ptr(),
             used.data_ptr(),
-            pool.batch,
-            pool.max_blocks,
-            pool.num_blocks,
+            *sizes,
             workspace.data_ptr(),
             size,
         )
@@ -298,12 +302,12 @@ def hip_block_pool_compact(pool: BlockPool) -> tuple[torch.Tensor, torch.Tensor,
     return origins, used, HIP_BLOCK_POOL_COMPACT_BACKEND
 
 
-def _cache_library(cache: BlockCache, size: int, *words: torch.Tensor):
+def _cache_request(cache: BlockCache, size: int, words: torch.Tensor, more: torch.Tensor | None = None) -> tuple | None:
     """The library and the device where the kernels take a cache and whole numbers
     [size], else None."""
 
     index = cache.key_tail.get_device()
-    if not all(_words_ok(word, size, index) for word in words):
+    if not _words_ok(words, size, index) or (more is not None and not _words_ok(more, size, index)):
         return None
     library = library_for(index)
     return None if library is None else (library, index)
@@ -312,7 +316,7 @@ def _cache_library(cache: BlockCache, size: int, *words: torch.Tensor):
 def can_use_hip_block_cache_copy(cache: BlockCache, origins: torch.Tensor) -> bool:
     """Whether the copy kernel takes these tensors."""
 
-    return _cache_library(cache, cache.key_codes.shape[0], origins) is not None
+    return _cache_request(cache, cache.key_codes.shape[0], origins) is not None
 
 
 def hip_block_cache_copy(cache: BlockCache, origins: torch.Tensor) -> str:
@@ -323,10 +327,11 @@ def hip_block_cache_copy(cache: BlockCache, origins: torch.Tensor) -> str:
     the call keeps what it holds.
     """
 
-    request = _cache_library(cache, cache.key_codes.shape[0], origins)
+    request = _cache_request(cache, cache.key_codes.shape[0], origins)
     if request is None:
         raise RuntimeError("HIP block cache copy is ineligible for the requested inputs")
     library, index = request
+    blocks, heads, _, dim = cache.key_codes.shape
     try:
         launch(
             index,
@@ -334,28 +339,35 @@ def hip_block_cache_copy(cache: BlockCache, origins: torch.Tensor) -> str:
             "sah_block_cache_copy",
             *cache._pointers()[:4],
             origins.data_ptr(),
-            cache.kv_heads,
-            cache.head_dim,
-            cache.key_codes.shape[0],
+            heads,
+            dim,
+            blocks,
         )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block cache copy execution failed") from exc
     return HIP_BLOCK_CACHE_COPY_BACKEND
 
 
+def _cache_fork_request(cache: BlockCache, sources: torch.Tensor) -> tuple | None:
+    batch = cache.key_tail.shape[0]
+    return _cache_request(cache, batch, sources) if batch <= MAX_FORKED_SEQUENCES else None
+
+
 def can_use_hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> bool:
     """Whether the fork kernel takes these tensors."""
 
-    return cache.batch <= MAX_FORKED_SEQUENCES and _cache_library(cache, cache.batch, sources) is not None
+    return _cache_fork_request(cache, sources) is not None
 
 
 def hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> str:
     """Copy the incomplete block of sequence ``sources[b]``, as it was before the call, to
     sequence b, with the sources of :func:`hip_block_pool_fork`."""
 
-    if not can_use_hip_block_cache_fork(cache, sources):
+    request = _cache_fork_request(cache, sources)
+    if request is None:
         raise RuntimeError("HIP block cache fork is ineligible for the requested inputs")
-    library, index = _cache_library(cache, cache.batch, sources)
+    library, index = request
+    batch, heads, _, dim = cache.key_tail.shape
     try:
         launch(
             index,
@@ -364,9 +376,9 @@ def hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> str:
             cache.key_tail.data_ptr(),
             cache.value_tail.data_ptr(),
             sources.data_ptr(),
-            cache.batch,
-            cache.kv_heads,
-            cache.head_dim,
+            batch,
+            heads,
+            dim,
         )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block cache fork execution failed") from exc
@@ -376,7 +388,7 @@ def hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> str:
 def can_use_hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> bool:
     """Whether the take-back kernel takes these tensors."""
 
-    return _cache_library(cache, cache.batch, lengths, ends) is not None
+    return ends is not None and _cache_request(cache, cache.key_tail.shape[0], lengths, ends) is not None
 
 
 def hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> str:
@@ -389,7 +401,9 @@ def hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: to
     written; ``starts = ends`` from then on.
     """
 
-    request = _cache_library(cache, cache.batch, lengths, ends)
+    tail = cache.key_tail
+    batch, heads, _, dim = tail.shape
+    request = None if ends is None else _cache_request(cache, batch, lengths, ends)
     if request is None:
         raise RuntimeError("HIP block cache take back is ineligible for the requested inputs")
     library, index = request
@@ -401,12 +415,12 @@ def hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: to
             *cache._pointers(),
             lengths.data_ptr(),
             ends.data_ptr(),
-            cache.batch,
-            cache.kv_heads,
-            cache.head_dim,
+            batch,
+            heads,
+            dim,
             cache.key_codes.shape[0],
             cache.block_table.shape[1],
-            dtype_code(cache.key_tail.dtype),
+            dtype_code(tail.dtype),
         )
     except HipLibraryError as exc:
         raise RuntimeError("HIP block cache take back execution failed") from exc

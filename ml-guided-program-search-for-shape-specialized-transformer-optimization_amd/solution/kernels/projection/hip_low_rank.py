@@ -199,8 +199,8 @@ def _check_out(
     out: torch.Tensor | None, value: torch.Tensor, projected: torch.Tensor, adapters: LowRankAdapters
 ) -> tuple[torch.Tensor, tuple[int, int]]:
     if out is None:
-        out = projected.new_empty(projected.shape)
-        return out, _strides(out)
+        shape = projected.shape
+        return projected.new_empty(shape), ((shape[1] if len(shape) == 3 else 1) * shape[-1], shape[-1])
     strides = None
     if (
         out.dtype is projected.dtype
@@ -246,7 +246,7 @@ def hip_low_rank_adapters(
     scales, ranks = adapters.scales, adapters.ranks
     try:
         size = library.sah_low_rank_adapters_workspace_bytes(batch, seq_len, in_features, out_features, rank)
-        workspace = torch.empty(size, dtype=torch.uint8, device=value.device) if size else None
+        workspace = value.new_empty(size // 2) if size else None
         launch(
             index,
             library.sah_low_rank_adapters,

@@ -131,7 +131,7 @@ def hip_verify_draft(
     accepted = tokens.new_empty((batch,), dtype=torch.int32)
     try:
         size = library.sah_verify_draft_workspace_bytes(batch, drafts, vocab, 0 if draft is None else 1)
-        workspace = torch.empty(size, dtype=torch.uint8, device=target.device) if size else None
+        workspace = tokens.new_empty(-(-size // 8)) if size else None
         launch(
             index,
             library.sah_verify_draft,
