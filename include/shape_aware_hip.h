@@ -639,7 +639,7 @@ int sah_low_rank_adapters(
     int64_t y_stride_b, int64_t y_stride_s, int dtype,
     void* workspace, size_t workspace_bytes, sah_stream_t stream);
 
-/* Bytes of the partial sums of few tokens; 0 for many. */
+/* Bytes of the partial sums of few tokens; 0 where a call takes one launch. */
 size_t sah_low_rank_adapters_workspace_bytes(
     int64_t batch, int64_t seq_len, int64_t in_features, int64_t out_features, int64_t rank);
 

@@ -22,10 +22,12 @@
 // Few tokens are bound by the adapters' bytes and by latency, and a workgroup a token would
 // leave most of the chip idle: one launch shares `in` among workgroups and leaves partial
 // sums of h, another adds them up in order and shares `out`.  Many tokens are bound by x,
-// base and y: a workgroup does both products of 32 tokens, and there is no workspace.
+// base and y: a workgroup does both products of 32 tokens, and there is no workspace.  Nor
+// is there for few tokens of short inputs, where latency and launches are all there is.
 //   2 x 20001 tokens (ragged), 1024 -> 4096, rank 32 (697 MB, 142 us at a large copy's
 //   rate): 149 us; 178 in the operands' order
-//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (49 MB): 8 + 12 us
+//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (33 MB, 7 us): 7.2 + 8.9 us
+//   1 token, 1024 -> 1024, rank 16: 5.4 us
 
 #include <type_traits>
 
@@ -424,8 +426,9 @@ __device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t 
   }
 }
 
-// A workgroup takes 16 TT tokens.  Its waves share `in` for h, add their sums up in order
-// through LDS, and share `out`.
+// A workgroup takes 16 TT tokens and groups_of_wave groups of outputs a wave (all of them
+// where tokens are many).  Its waves share `in` for h, add their sums up in order through
+// LDS, and share the outputs.
 template <typename T, int S, int TT>
 __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankArgs a) {
   constexpr int N = 2 * S;
@@ -435,14 +438,18 @@ __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankA
   } lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tile = blockIdx.x;
+  const uint32_t groups = (uint32_t)((a.out + kGroup - 1) / kGroup);
+  const uint32_t portion = (uint32_t)a.groups_of_wave * kWaves;      // groups of a workgroup
+  const uint32_t workgroups = (groups + portion - 1) / portion;      // of a tile
+  const int64_t tile = blockIdx.x / workgroups;
+  const int64_t from = (int64_t)(blockIdx.x % workgroups) * portion;
+  const int64_t until = from + portion < groups ? from + portion : groups;
   const int64_t b = tile / a.tiles_of_seq;
   const int64_t first = (tile - b * a.tiles_of_seq) * (16 * TT);
   const Adapter it = adapter_of(a, b);
-  const int64_t groups = (a.out + kGroup - 1) / kGroup;
   if (it.used == 0 || first >= it.count) {
     const Tokens<T, TT> tokens(a, b, first, it.count);
-    copy_groups<T, TT, 2>(a.out, wave, groups, kWaves, tokens);
+    copy_groups<T, TT, 2>(a.out, from + wave, until, kWaves, tokens);
     return;
   }
   f32x4 h[TT][N];
@@ -468,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankA
   const Tokens<T, TT> tokens(a, b, first, it.count);
   const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
   Group<T, S, TT> data;
-  data.load(up, a.rank, a.out, it.used, wave < groups ? wave : 0, tokens);
+  data.load(up, a.rank, a.out, it.used, from + wave < until ? from + wave : from, tokens);
   __syncthreads();
   Hidden<T, S> hidden[TT];
 #pragma unroll
@@ -482,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankA
     hidden[i] = make_hidden<T, S>(h[i], it.used, it.scale);
   }
   __syncthreads();
-  expand<T, S, TT>(data, lds.up[wave], up, a.rank, a.out, it.used, wave, groups, kWaves, hidden, tokens);
+  expand<T, S, TT>(data, lds.up[wave], up, a.rank, a.out, it.used, from + wave, until, kWaves, hidden, tokens);
 }
 
 // Partial sums of h: workgroup (tile, part) takes the part's slabs, shared by its waves.
@@ -528,12 +535,16 @@ __global__ __launch_bounds__(kThreads) void low_rank_shrink_kernel(const LowRank
   }
 }
 
-// The sums of h's parts, in order, and the outputs.  A wave's groups lie a workgroup's
-// waves apart.
+// The sums of h's parts and the outputs.  A workgroup's waves share the parts and add
+// theirs up in order through LDS (each wave reading all of them: 64 tokens, 4096 -> 4096,
+// rank 64, 12.7 us instead of 8.9); a wave's groups lie a workgroup's waves apart.
 template <typename T, int S>
 __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRankArgs a) {
   constexpr int N = 2 * S;
-  __shared__ __align__(16) UpStage<S> lds[kWaves];
+  __shared__ __align__(16) union {
+    f32x4 sums[kWaves][N][64];
+    UpStage<S> up[kWaves];
+  } lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t groups = (uint32_t)((a.out + kGroup - 1) / kGroup);
@@ -542,32 +553,42 @@ __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRank
   const int64_t tile = blockIdx.x / workgroups;
   const int64_t from = (int64_t)(blockIdx.x % workgroups) * share, mine = from + wave;
   const int64_t to = from + share < groups ? from + share : groups;
-  if (mine >= to) return;
   const int64_t b = tile / a.tiles_of_seq;
   const int64_t first = (tile - b * a.tiles_of_seq) * 16;
   const Adapter it = adapter_of(a, b);
   const Tokens<T, 1> tokens(a, b, first, it.count);
-  if (it.used == 0 || first >= it.count) {
+  if (it.used == 0 || first >= it.count) {  // (the same for every wave)
     copy_groups<T, 1, 1>(a.out, mine, to, kWaves, tokens);
     return;
   }
   const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
   // (the first group's loads before the parts', which they would wait for)
   Group<T, S, 1> data;
-  data.load(up, a.rank, a.out, it.used, mine, tokens);
+  data.load(up, a.rank, a.out, it.used, mine < to ? mine : from, tokens);
   f32x4 h[N];
 #pragma unroll
   for (int t = 0; t < N; ++t) h[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   if (first + (lane & 15) < it.count) {
     const f32x4* partial = reinterpret_cast<const f32x4*>(a.partial) + tile * (N * 64) + lane;
     // (of rows that no row of down fills, what is read is not used)
-#pragma unroll 4
-    for (int p = 0; p < a.parts; ++p)
+    for (int p = a.parts > 1 ? wave : 0; p < a.parts; p += kWaves)
 #pragma unroll
       for (int t = 0; t < N; ++t) h[t] += partial[(int64_t)p * a.tiles * (N * 64) + t * 64];
   }
+  if (a.parts > 1) {  // the waves' shares of the parts, in order
+#pragma unroll
+    for (int t = 0; t < N; ++t) lds.sums[wave][t][lane] = h[t];
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      h[t] = lds.sums[0][t][lane];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) h[t] += lds.sums[k][t][lane];
+    }
+    __syncthreads();
+  }
   const Hidden<T, S> hidden[1] = {make_hidden<T, S>(h, it.used, it.scale)};
-  expand<T, S, 1>(data, lds[wave], up, a.rank, a.out, it.used, mine, to, kWaves, hidden, tokens);
+  expand<T, S, 1>(data, lds.up[wave], up, a.rank, a.out, it.used, mine, to, kWaves, hidden, tokens);
 }
 
 // How a call is launched.
@@ -584,6 +605,14 @@ struct Plan {
 // 108 / 109 and 228 / 231; 34816 tokens 195 / 188 and 434 / 405.  Requests of up to a
 // tile's tokens would leave the larger workgroups' places empty.
 constexpr int64_t kManyTiles = 1024;
+// Few tokens of short inputs take one launch as well: a workgroup a tile and four groups of
+// outputs, each with the first product to itself.  One / two launches, us: 1 and 8 tokens
+// of 1024 inputs, rank 16, 5.4 / 3.3 + 3.9 and 5.8 / 3.8 + 4.2, rank 64 6.9 / 4.0 + 4.4 and
+// 8.0 / 4.5 + 4.8; 7 tokens of 2048 inputs, rank 64, 10.0 / 5.0 + 4.8; and a launch is 3 us
+// of the host's.  4096 inputs, 1 token of rank 64: 13.2 / 4.6 + 5.1.  More workgroups read
+// `down` too often: 512 of rank 64 13.5 / 5.4 + 6.8, 4672 of rank 16 35 / 4.1 + 11.9.
+constexpr int64_t kShortIn = 2048;
+constexpr int64_t kFewWorkgroups = 256;
 
 Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t out, int64_t rank) {
   Plan p{};
@@ -596,10 +625,17 @@ Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t out, int64_t rank) 
     p.tokens = 16 * kFusedTiles;
     p.tiles_of_seq = ceil_div(seq, p.tokens);
     p.tiles = batch * p.tiles_of_seq;
+    p.groups_of_wave = (int)ceil_div(ceil_div(out, kGroup), kWaves);
     return p;
   }
-  // Parts for a workgroup a unit, a slab a wave at least: every wave of the second launch
-  // reads them all (64 tokens, 4096 -> 4096, rank 64: 18 us with 4, 20 with 8, 25 with 16).
+  if (in <= kShortIn && p.tiles * ceil_div(ceil_div(out, kGroup), kWaves) <= kFewWorkgroups) {
+    p.fused = true;
+    p.groups_of_wave = 1;
+    return p;
+  }
+  // Parts for a workgroup a unit, a slab a wave at least: every workgroup of the second
+  // launch reads them all (64 tokens, 4096 -> 4096, rank 64: 18 us with 4, 20 with 8, 25
+  // with 16, when every wave did).
   const int64_t slabs = ceil_div(in, kSlab);
   int64_t parts = ceil_div(256, p.tiles);
   const int64_t most = ceil_div(slabs, kWaves);
@@ -616,16 +652,19 @@ Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t out, int64_t rank) 
 
 template <typename T, int S>
 int launch(const LowRankArgs& a, const Plan& p, hipStream_t stream) {
+  const int64_t workgroups = ceil_div(ceil_div(a.out, kGroup), kWaves * p.groups_of_wave);
+  const dim3 grid((unsigned)(p.tiles * workgroups));
   if (p.fused) {
-    hipLaunchKernelGGL((low_rank_fused_kernel<T, S, kFusedTiles>), dim3((unsigned)p.tiles), dim3(kThreads), 0, stream, a);
+    if (p.tokens == 16)
+      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, 1>), grid, dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, kFusedTiles>), grid, dim3(kThreads), 0, stream, a);
     return check_hip(hipGetLastError(), "low-rank adapters launch");
   }
   hipLaunchKernelGGL((low_rank_shrink_kernel<T, S>), dim3((unsigned)(p.tiles * p.parts)), dim3(kThreads), 0, stream, a);
   const int status = check_hip(hipGetLastError(), "low-rank adapters launch");
   if (status != SAH_OK) return status;
-  const int64_t workgroups = ceil_div(ceil_div(a.out, kGroup), kWaves * p.groups_of_wave);
-  hipLaunchKernelGGL((low_rank_expand_kernel<T, S>), dim3((unsigned)(p.tiles * workgroups)), dim3(kThreads), 0, stream,
-                     a);
+  hipLaunchKernelGGL((low_rank_expand_kernel<T, S>), grid, dim3(kThreads), 0, stream, a);
   return check_hip(hipGetLastError(), "low-rank adapters launch");
 }
 

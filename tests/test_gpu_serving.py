@@ -354,6 +354,21 @@ def test_adapters_of_mixed_ranks_and_ragged_rows(gpu_device, dtype, seq):
     _check_adapters(gpu_device, value, projected, down, up, None, ranks, indices, counts, out="in place")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rank", [8, 32, 40, 64, 128])
+@pytest.mark.parametrize("seq,k,n", [(1, 2056, 200), (21, 4104, 72), (70, 520, 8200), (3, 16384, 16)])
+def test_adapters_of_few_tokens_and_long_rows(gpu_device, dtype, rank, seq, k, n):
+    """Inputs or outputs that two launches share, mixed ranks, ragged rows, strides, in place."""
+
+    ranks = [rank, rank - 7, 0, 200]
+    down, up, scales = _adapter_tensors(4, rank, k, n, dtype, 57, ranks=ranks)
+    indices, counts = [0, 1, 2, 3, -1, 1, 0], [seq, seq + 1, seq, seq - 1, seq, 0, 2]
+    value, projected = _rand((7, seq, k), 58, dtype), _rand((7, seq, n), 59, dtype)
+    _check_adapters(gpu_device, value, projected, down, up, scales, ranks, indices, counts)
+    turned = (lambda t: t.transpose(0, 1).contiguous().to(gpu_device).transpose(0, 1))  # noqa: E731
+    _check_adapters(gpu_device, value, projected, down, up, None, ranks, indices, counts, place=turned, out="in place")
+
+
 @pytest.mark.parametrize("batch", [1023, 1024, 1100])
 def test_adapters_of_one_token_of_many_requests(gpu_device, batch):
     down, up, scales = _adapter_tensors(50, 16, 64, 72, F16, 38)
@@ -403,12 +418,12 @@ def test_adapters_of_large_and_small_products(gpu_device, seq, dtype, size):
     _check_adapters(gpu_device, value, projected, down, up, scales, None, [0, 1])
 
 
-@pytest.mark.parametrize("seq", [20, 9000])
-def test_adapters_keep_bad_tokens_to_themselves(gpu_device, seq):
+@pytest.mark.parametrize("seq,features", [(20, 64), (9000, 64), (20, 4096)])
+def test_adapters_keep_bad_tokens_to_themselves(gpu_device, seq, features):
     from solution.kernels.projection import LowRankAdapters, hip_low_rank_adapters
 
-    down, up, scales = (t.to(gpu_device) for t in _adapter_tensors(2, 16, 64, 72, BF16, 48))
-    value, projected = _rand((2, seq, 64), 49, BF16).to(gpu_device), _rand((2, seq, 72), 50, BF16).to(gpu_device)
+    down, up, scales = (t.to(gpu_device) for t in _adapter_tensors(2, 16, features, 72, BF16, 48))
+    value, projected = _rand((2, seq, features), 49, BF16).to(gpu_device), _rand((2, seq, 72), 50, BF16).to(gpu_device)
     packed, indices = LowRankAdapters(down, up, scales), _words([0, 1], gpu_device)
     with torch.inference_mode():
         want = hip_low_rank_adapters(value, projected, packed, indices)[0]

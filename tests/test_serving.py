@@ -84,8 +84,8 @@ def test_verify_workspace_sizes():
 
 
 ADAPTERS = dict(
-    x=P, base=P, down=P, up=P, scales=None, ranks=None, indices=P, counts=None, y=P, batch=2, seq_len=3, in_features=64,
-    out_features=32, adapters=4, rank=16, x_sb=192, x_ss=64, p_sb=96, p_ss=32, y_sb=96, y_ss=32, dtype=BF16,
+    x=P, base=P, down=P, up=P, scales=None, ranks=None, indices=P, counts=None, y=P, batch=2, seq_len=3, in_features=4096,
+    out_features=32, adapters=4, rank=16, x_sb=12288, x_ss=4096, p_sb=96, p_ss=32, y_sb=96, y_ss=32, dtype=BF16,
     workspace=P, workspace_bytes=0, stream=None,
 )
 
@@ -137,7 +137,8 @@ def test_adapters_workspace_sizes():
     assert size(0, 1, 64, 64, 16) == size(1, 0, 64, 64, 16) == size(1, 1, 64, 64, 12) == size(1, 1, 60, 64, 16) == 0
     few = size(1, 1, 4096, 4096, 64)
     assert few > 0 and few % (64 * 16 * 4) == 0
-    assert size(64, 20000, 4096, 4096, 64) == 0
+    assert size(64, 20000, 4096, 4096, 64) == size(1, 1, 1024, 1024, 16) == 0
+    assert size(64, 1, 1024, 4096, 16) > 0
 
 
 POOL = dict(table=P, holders=P)
