@@ -654,7 +654,7 @@ size_t sah_low_rank_adapters_workspace_bytes(
  * and u_i q_i(x_i) < p_i(x_i), u_i = uniforms[b][i] in [0, 1).  The token after the ones
  * that stand is drawn by u = uniforms[b][drafts] from max(p - q, 0) at the first that
  * does not stand, from p where all do: the lowest v for which the sum of the weights up
- * to v is above u times the sum of all.  In fp64 throughout.
+ * to v is above u times the sum of all, as fp64 decides it.
  *   accepted[b]  the drafts that stand
  *   answer[b]    [drafts + 1]: these, the token drawn, -1 behind
  * temperatures[b] (NULL: 1) not above 0 (or NaN) asks for the likeliest token: a draft

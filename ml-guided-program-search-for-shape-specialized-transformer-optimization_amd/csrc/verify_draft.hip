@@ -18,18 +18,18 @@
 //   3. weigh: of row j alone, in fp64.  With e_p, e_q the exponentials and r = sum e_p /
 //      sum e_q, the weights are in proportion to max(e_p - r e_q, 0).  r is known to
 //      fp32's precision; a chunk adds up e_p, e_q, and both over the tokens S where
-//      e_p > r e_q.  Its weight is then sum_S e_p - r sum_S e_q for the r that the
-//      sums of all chunks give: a token that changes sides between one r and the other
-//      has a weight of their distance at most, and so many do, which leaves the
-//      distance's square;
-//   4. pick: r, the chunk in which the sum passes the border, the token.
+//      e_p > r e_q, and keeps how near e_p / e_q comes to r.  Its weight is then sum_S e_p
+//      - r sum_S e_q for the r that the sums of all chunks give, unless a token changes
+//      sides between the two;
+//   4. pick: r, such chunks again (one in some thousand draws, or many where draft and
+//      target are all but the same), the chunk in which the sum passes the border, the token.
 //
 // 64 requests, 7 drafts, 131072 tokens, bf16 (252 MB, 51 us at a large copy's rate): rows
-// 56 us, decide 7, weigh 22, pick 6.  fp64's v_fma issues at fp32's rate here, but with
+// 57 us, decide 7, weigh 25, pick 6.  fp64's v_fma issues at fp32's rate here, but with
 // all rows in fp64 the vector units took 126 us for them.  The draw's two parts in one
-// launch, by the request's last workgroup, took 106 us instead of 27: each of the 4096
+// launch, by the request's last workgroup, took 106 us instead of 30: each of the 4096
 // releases its L2's lines.  For one request (4 drafts, 32000 tokens) the parts are
-// launches' latencies, 4 + 7.5 + 4 us.
+// launches' latencies, 4 + 8 + 5 us.
 
 #include <type_traits>
 
@@ -67,7 +67,7 @@ struct Choice {
   int32_t row;      // the first draft that does not stand, or the number of drafts
   int32_t mode;     // how the next token is drawn
   float p_top, q_top;
-  double ratio;     // sum e_p / sum e_q, about
+  double ratio_log2;  // of sum e_p / sum e_q, about
   double c;         // log2(e) / temperature
 };
 enum { kDone = 0, kFromTarget = 1, kWithout = 2, kResample = 3 };
@@ -75,6 +75,7 @@ enum { kDone = 0, kFromTarget = 1, kWithout = 2, kResample = 3 };
 struct Weights {
   double p, q;          // sums of e_p, e_q
   double p_over, q_over;  // where e_p > ratio e_q
+  double near;            // the least distance of a token's e_p / e_q from ratio, in log2
 };
 
 struct VerifyArgs {
@@ -113,8 +114,11 @@ __device__ __forceinline__ double exp2_upto0(double x) {
   y = fma(y, f, 1.0);
   return ldexp(y, (int)n);
 }
+__device__ __forceinline__ double exponent_of(float logit, float top, double c) {
+  return ((double)logit - (double)top) * c;
+}
 __device__ __forceinline__ double weight_of(float logit, float top, double c) {
-  return exp2_upto0(((double)logit - (double)top) * c);
+  return exp2_upto0(exponent_of(logit, top, c));
 }
 
 // log2(e) / temperature, and whether the request answers greedily instead (a temperature
@@ -464,7 +468,7 @@ __device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShar
   }
   Choice choice{j, kDone, found.p.top, found.q.top, 0.0, c};
   if (!done) choice.mode = j == count ? kFromTarget : sampled ? kResample : kWithout;
-  if (choice.mode == kResample) choice.ratio = found.p.sum / found.q.sum;
+  if (choice.mode == kResample) choice.ratio_log2 = log2(found.p.sum / found.q.sum);
   return choice;
 }
 
@@ -486,14 +490,24 @@ struct Rows {
     q_row = static_cast<const T*>(a.draft) + b * a.d_sb + it.row * a.d_ss;
     drafted = it.mode == kWithout ? a.tokens[b * a.drafts + it.row] : -1;
   }
-  __device__ __forceinline__ void weigh(const VerifyArgs& a, const Choice& it, int64_t first, double* p, double* q) const {
+  // apart: log2 of e_p / e_q over ratio, +inf without a draft's row (NaN where both are 0)
+  __device__ __forceinline__ void weigh(const VerifyArgs& a, const Choice& it, int64_t first, double* p, double* q,
+                                        double* apart) const {
     float pl[kVec], ql[kVec];
     load_logits<T>(p_row, first, a.vocab, pl);
     if (it.mode == kResample) load_logits<T>(q_row, first, a.vocab, ql);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) p[e] = first + e == drafted ? 0.0 : weight_of(pl[e], it.p_top, it.c);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) q[e] = it.mode == kResample ? weight_of(ql[e], it.q_top, it.c) : 0.0;
+    for (int e = 0; e < kVec; ++e) {
+      const double x = exponent_of(pl[e], it.p_top, it.c);
+      p[e] = first + e == drafted ? 0.0 : exp2_upto0(x);
+      q[e] = 0.0;
+      apart[e] = INFINITY;
+      if (it.mode == kResample) {
+        const double y = exponent_of(ql[e], it.q_top, it.c);
+        q[e] = exp2_upto0(y);
+        apart[e] = x - y - it.ratio_log2;
+      }
+    }
   }
 };
 
@@ -514,22 +528,24 @@ __global__ __launch_bounds__(kPickThreads) void verify_weigh_kernel(const Verify
   }
   if (it.mode == kDone) return;
   const Rows<T> rows(a, b, it);
-  double p[kVec], q[kVec];
-  rows.weigh(a, it, (int64_t)chunk * kPickChunk + threadIdx.x * kVec, p, q);
-  Weights sum{0.0, 0.0, 0.0, 0.0};
+  double p[kVec], q[kVec], apart[kVec];
+  rows.weigh(a, it, (int64_t)chunk * kPickChunk + threadIdx.x * kVec, p, q, apart);
+  Weights sum{0.0, 0.0, 0.0, 0.0, INFINITY};
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
     sum.p += p[e];
     sum.q += q[e];
-    const bool over = p[e] > it.ratio * q[e];
+    const bool over = apart[e] > 0.0;
     sum.p_over += over ? p[e] : 0.0;
     sum.q_over += over ? q[e] : 0.0;
+    sum.near = fmin(sum.near, fabs(apart[e]));
   }
   sum.p_over = wave_add(sum.p_over);
   if (it.mode == kResample) {
     sum.p = wave_add(sum.p);
     sum.q = wave_add(sum.q);
     sum.q_over = wave_add(sum.q_over);
+    sum.near = wave_reduce(sum.near, [](double a, double b) { return fmin(a, b); });
   }
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -539,8 +555,24 @@ __global__ __launch_bounds__(kPickThreads) void verify_weigh_kernel(const Verify
     sum.q += waves[w].q;
     sum.p_over += waves[w].p_over;
     sum.q_over += waves[w].q_over;
+    sum.near = fmin(sum.near, waves[w].near);
   }
   a.weights[b * a.pick_chunks + chunk] = sum;
+}
+
+// The weights of 8 tokens with the ratio as it is, and their sum.
+template <typename T>
+__device__ __forceinline__ double weigh_exactly(const Rows<T>& rows, const VerifyArgs& a, const Choice& it, int64_t first,
+                                                double ratio, double* p) {
+  double q[kVec], apart[kVec], sum = 0.0;
+  rows.weigh(a, it, first, p, q, apart);
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    p[e] -= ratio * q[e];
+    p[e] = p[e] > 0.0 ? p[e] : 0.0;
+    sum += p[e];
+  }
+  return sum;
 }
 
 template <typename T>
@@ -552,7 +584,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Choice it = a.choices[b];
   if (it.mode == kDone) return;
-  const Weights* weights = a.weights + b * a.pick_chunks;
+  Weights* weights = a.weights + b * a.pick_chunks;
+  const Rows<T> rows(a, b, it);
 
   // Every wave for itself: the ratio, the whole, and the chunk in which the sum passes
   // u times the whole.
@@ -564,6 +597,27 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
       q += weights[i].q;
     }
     ratio = wave_add(p) / wave_add(q);
+    // Chunks where a token may have changed sides, again (exponents are off by 2^-53 of
+    // at most 1100 each, as far as they matter).
+    const double moved = fabs(log2(ratio) - it.ratio_log2) + 1e-12;
+    for (int at = 0; at < a.pick_chunks; at += 64) {
+      uint64_t again = __ballot(at + lane < a.pick_chunks && weights[at + lane].near <= moved);
+      while (again != 0) {  // (the same for every wave)
+        const int i = at + __ffsll((unsigned long long)again) - 1;
+        again &= again - 1;
+        double p[kVec];
+        const double up_to = wave_add(weigh_exactly<T>(rows, a, it, (int64_t)i * kPickChunk + tid * kVec, ratio, p));
+        if (lane == 0) sums[wave] = up_to;
+        __syncthreads();
+        if (tid == 0) {
+          double sum = 0.0;
+          for (int w = 0; w < WAVES; ++w) sum += sums[w];
+          weights[i].p_over = sum;
+          weights[i].q_over = 0.0;
+        }
+        __syncthreads();
+      }
+    }
   }
   auto weight = [&](int i) {
     if (i >= a.pick_chunks) return 0.0;
@@ -596,16 +650,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   }
 
   const int64_t first = (int64_t)chosen * kPickChunk + tid * kVec;
-  const Rows<T> rows(a, b, it);
-  double p[kVec], q[kVec];
-  rows.weigh(a, it, first, p, q);
-  double own = 0.0;
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    p[e] -= ratio * q[e];
-    p[e] = p[e] > 0.0 ? p[e] : 0.0;
-    own += p[e];
-  }
+  double p[kVec];
+  const double own = weigh_exactly<T>(rows, a, it, first, ratio, p);
   const double up_to = wave_up_to(own);
   if (lane == 63) sums[wave] = up_to;
   __syncthreads();

@@ -197,6 +197,26 @@ def test_verify_random_numbers_at_the_border(gpu_device, dtype, sampled, vocab):
     assert min(want[1]) >= drafts // 2 - 1 and min(want[1]) < drafts
 
 
+@pytest.mark.parametrize("batch,vocab", [(5, 777), (5, 50_021), (16, 131_073)])
+@pytest.mark.parametrize("near", [1e-6, 1e-5, 1e-4, "one token"])
+def test_verify_distributions_that_lie_close(gpu_device, batch, vocab, near):
+    """p / q lies within 1e-6 .. 1e-4 of 1 for all tokens, or for all but a rare one, and
+    max(p - q, 0) is as small: its tokens are those that the exact ratio of the two sums names."""
+
+    generator = _generator(18)
+    target = torch.randn((batch, 2, vocab), generator=generator) * 0.5
+    if near == "one token":
+        draft = target[:, :1].clone()
+        tokens = torch.randint(0, vocab, (batch, 1), generator=generator)
+        draft[torch.arange(batch), 0, tokens[:, 0]] += 1.0
+    else:
+        draft = target[:, :1] + near * torch.randn((batch, 1, vocab), generator=generator)
+        tokens = (draft - target[:, :1]).argmax(-1)
+    uniforms = torch.stack((torch.full((batch,), 1 - 2.0**-24), torch.rand((batch,), generator=generator)), dim=1)
+    want = _verify(gpu_device, target, tokens, uniforms, draft)
+    assert want[1] == [0] * batch and len({row[0] for row in want[0]}) > 1
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_verify_logits_of_any_strides(gpu_device, dtype):
     target, draft, tokens, uniforms = _drafted(3, 2, 1001, dtype, 17)
