@@ -59,6 +59,7 @@ HIP_BLOCK_CACHE_TAKE_BACK_BACKEND = "hip_block_cache_take_back"
 
 MAX_FORKED_SEQUENCES = 1024
 _MAX_TOKENS = 2**31 - 1
+_MAX_ENTRIES = 2**31 - 1
 
 
 @dataclass(frozen=True, eq=False)
@@ -133,6 +134,8 @@ def _pool_request(pool: BlockPool, words: torch.Tensor | None = None, more: torc
 
     table = pool.block_table
     index, (batch, max_blocks) = table.get_device(), table.shape
+    if batch * max_blocks > _MAX_ENTRIES:
+        return None
     if words is not None and not _words_ok(words, batch, index):
         return None
     if more is not None and not _words_ok(more, batch, index):

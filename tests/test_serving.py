@@ -78,9 +78,9 @@ def test_verify_entry_refuses_before_launch(changes, status):
 def test_verify_workspace_sizes():
     size = _library.load_library().sah_verify_draft_workspace_bytes
     assert size(0, 3, 1000, 1) == size(2, 1025, 1000, 1) == size(2, 3, 0, 1) == size(-1, 3, 1000, 1) == 0
-    # 16 bytes a row and 8192 logits of it, 32 bytes a request and 2048 logits, 32 a request
-    assert size(2, 3, 1000, 1) == 2 * (7 * 16 + 32 + 32)
-    assert size(2, 3, 8193, 0) == 2 * (4 * 2 * 16 + 5 * 32 + 32)
+    # 16 bytes a row and 8192 logits of it, 40 bytes a request and 2048 logits, 32 a request
+    assert size(2, 3, 1000, 1) == 2 * (7 * 16 + 40 + 32)
+    assert size(2, 3, 8193, 0) == 2 * (4 * 2 * 16 + 5 * 40 + 32)
 
 
 ADAPTERS = dict(
@@ -154,6 +154,7 @@ OF_POOL = [
     ({"max_blocks": 1 << 26}, INVALID),
     ({"num_blocks": -1}, INVALID),
     ({"num_blocks": 2**31 - 1}, INVALID),
+    ({"batch": 1 << 16, "max_blocks": 1 << 15}, UNSUPPORTED),
     ({"table": None}, INVALID),
     ({"holders": None}, INVALID),
     ({"table": P + 2}, INVALID),
@@ -187,7 +188,6 @@ def test_reserve_entry_refuses_before_launch(changes, status):
         ({"max_blocks": 0}, OK),
         ({"lengths": None}, INVALID),
         ({"lengths": P + 2}, INVALID),
-        ({"batch": 1 << 20, "max_blocks": 1 << 20}, UNSUPPORTED),
     ],
 )
 def test_release_entry_refuses_before_launch(changes, status):
