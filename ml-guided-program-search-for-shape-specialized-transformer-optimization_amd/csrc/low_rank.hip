@@ -26,7 +26,7 @@
 // is there for few tokens of short inputs, where latency and launches are all there is.
 //   2 x 20001 tokens (ragged), 1024 -> 4096, rank 32 (697 MB, 142 us at a large copy's
 //   rate): 149 us; 178 in the operands' order
-//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (33 MB, 7 us): 7.2 + 8.9 us
+//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (33 MB, 7 us): 7.2 + 7.6 us
 //   1 token, 1024 -> 1024, rank 16: 5.4 us
 
 #include <type_traits>
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_shrink_kernel(const LowRank
 
 // The sums of h's parts and the outputs.  A workgroup's waves share the parts and add
 // theirs up in order through LDS (each wave reading all of them: 64 tokens, 4096 -> 4096,
-// rank 64, 12.7 us instead of 8.9); a wave's groups lie a workgroup's waves apart.
+// rank 64, 12.7 us instead of 8.9, with a group a wave); a wave's groups lie a workgroup's waves apart.
 template <typename T, int S>
 __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRankArgs a) {
   constexpr int N = 2 * S;
@@ -642,10 +642,11 @@ Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t out, int64_t rank) 
   if (parts > most) parts = most;
   p.slabs_of_part = (int)ceil_div(slabs, parts);
   p.parts = (int)ceil_div(slabs, p.slabs_of_part);
-  // Several groups a wave, as long as that leaves waves for all units (16384 tokens, 4096
-  // outputs, rank 64: the second launch 130 us with one, 105 with eight).
+  // Several groups a wave, as long as that leaves waves for all units (64 tokens, 4096 ->
+  // 4096, rank 64: the second launch 8.9 us with one, 7.6 with two, 8.8 with four; 16384
+  // tokens, 4096 outputs, rank 64: 130 us with one, 105 with eight).
   const int64_t waves = p.tiles * ceil_div(out, kGroup);
-  p.groups_of_wave = waves >= 8 * 4096 ? 8 : waves >= 4 * 4096 ? 4 : waves >= 2 * 4096 ? 2 : 1;
+  p.groups_of_wave = waves >= 8 * 4096 ? 8 : waves >= 4 * 4096 ? 4 : waves >= 4096 ? 2 : 1;
   p.bytes = (size_t)(p.parts * p.tiles * p.rank_tiles) * 64 * sizeof(f32x4);
   return p;
 }

@@ -29,7 +29,7 @@
 // all rows in fp64 the vector units took 126 us for them.  The draw's two parts in one
 // launch, by the request's last workgroup, took 106 us instead of 30: each of the 4096
 // releases its L2's lines.  For one request (4 drafts, 32000 tokens) the parts are
-// launches' latencies, 4 + 8 + 5 us.
+// latencies, 4 + 13 us.
 
 #include <type_traits>
 
@@ -50,6 +50,12 @@ constexpr int kMaxDrafts = 1024;
 // of 32000 tokens and 4 drafts 7.5 us instead of 4.7 + 4.5, 8 of 131072 tokens and 3 drafts
 // 9.0 instead of 6.2 + 5.9; 16 with 7 drafts (1024 workgroups) 14.8 and 6.2 + 7.6.
 constexpr int64_t kFewWorkgroups = 512;
+// And up to which a request's last one also draws, for another: 16 13.3 us instead of 8.6 +
+// 4.8, 125 9.9 instead of 6.0 + 4.2, 128 15.4 instead of 8.1 + 5.0, where a launch is 3 us
+// of the host's; 256 16.5 instead of 8.4 + 5.0, 512 22 instead of 10.4 + 5.6, as each
+// releases its L2's lines.
+constexpr int64_t kFewestWorkgroups = 128;
+enum { kDecided = 0, kDecides = 1, kDraws = 2 };
 constexpr double kLog2e = 1.4426950408889634074;
 // A row's sum in fp32, relative: an exponent |x| <= 64 (what lies below adds less than
 // 2^-33) is off by its difference's, its factor's and its product's rounding, 3 * 64 *
@@ -69,13 +75,14 @@ struct Choice {
   float p_top, q_top;
   double ratio_log2;  // of sum e_p / sum e_q, about
   double c;         // log2(e) / temperature
+  int32_t parted;   // workgroups of the request's draw that have left their sums
 };
 enum { kDone = 0, kFromTarget = 1, kWithout = 2, kResample = 3 };
 
 struct Weights {
   double p, q;          // sums of e_p, e_q
   double p_over, q_over;  // where e_p > ratio e_q
-  double near;            // the least distance of a token's e_p / e_q from ratio, in log2
+  float near;             // the least distance of a token's e_p / e_q from ratio, in log2
 };
 
 struct VerifyArgs {
@@ -264,6 +271,7 @@ __global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(const VerifyAr
   const int r = (int)(request_row % (uint32_t)rows);
   const int tid = threadIdx.x, wave = tid >> 6;
   const int count = drafts_of(a, b);
+  if (r == 0 && chunk == 0 && tid == 0) a.choices[b].parted = 0;
   const bool is_draft = r > a.drafts;
   if (is_draft ? r - a.drafts - 1 >= count : r > count) return;
   double factor;
@@ -392,7 +400,7 @@ __device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShar
       for (int i = tid; i <= a.drafts; i += THREADS) answer[i] = -1;
       if (tid == 0) a.accepted[b] = -1;
     }
-    return {0, kDone, 0.0f, 0.0f, 0.0, 0.0};
+    return {0, kDone, 0.0f, 0.0f, 0.0, 0.0, 0};
   }
   double c;
   const bool greedy = is_greedy(a, b, c);
@@ -466,7 +474,7 @@ __device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShar
     }
     if (tid == 0) a.accepted[b] = j;
   }
-  Choice choice{j, kDone, found.p.top, found.q.top, 0.0, c};
+  Choice choice{j, kDone, found.p.top, found.q.top, 0.0, c, 0};
   if (!done) choice.mode = j == count ? kFromTarget : sampled ? kResample : kWithout;
   if (choice.mode == kResample) choice.ratio_log2 = log2(found.p.sum / found.q.sum);
   return choice;
@@ -511,55 +519,6 @@ struct Rows {
   }
 };
 
-// DECIDES: every workgroup decides for itself, for one launch less.
-template <typename T, bool DECIDES>
-__global__ __launch_bounds__(kPickThreads) void verify_weigh_kernel(const VerifyArgs a) {
-  constexpr int WAVES = kPickThreads / 64;
-  __shared__ Weights waves[WAVES];
-  const uint32_t chunk = blockIdx.x % (uint32_t)a.pick_chunks;
-  const int64_t b = blockIdx.x / (uint32_t)a.pick_chunks;
-  Choice it;
-  if constexpr (DECIDES) {
-    __shared__ DecideShared<kPickThreads> shared;
-    it = decide<T>(a, b, chunk == 0, shared);
-    if (chunk == 0 && threadIdx.x == 0) a.choices[b] = it;
-  } else {
-    it = a.choices[b];
-  }
-  if (it.mode == kDone) return;
-  const Rows<T> rows(a, b, it);
-  double p[kVec], q[kVec], apart[kVec];
-  rows.weigh(a, it, (int64_t)chunk * kPickChunk + threadIdx.x * kVec, p, q, apart);
-  Weights sum{0.0, 0.0, 0.0, 0.0, INFINITY};
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    sum.p += p[e];
-    sum.q += q[e];
-    const bool over = apart[e] > 0.0;
-    sum.p_over += over ? p[e] : 0.0;
-    sum.q_over += over ? q[e] : 0.0;
-    sum.near = fmin(sum.near, fabs(apart[e]));
-  }
-  sum.p_over = wave_add(sum.p_over);
-  if (it.mode == kResample) {
-    sum.p = wave_add(sum.p);
-    sum.q = wave_add(sum.q);
-    sum.q_over = wave_add(sum.q_over);
-    sum.near = wave_reduce(sum.near, [](double a, double b) { return fmin(a, b); });
-  }
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < WAVES; ++w) {
-    sum.p += waves[w].p;
-    sum.q += waves[w].q;
-    sum.p_over += waves[w].p_over;
-    sum.q_over += waves[w].q_over;
-    sum.near = fmin(sum.near, waves[w].near);
-  }
-  a.weights[b * a.pick_chunks + chunk] = sum;
-}
-
 // The weights of 8 tokens with the ratio as it is, and their sum.
 template <typename T>
 __device__ __forceinline__ double weigh_exactly(const Rows<T>& rows, const VerifyArgs& a, const Choice& it, int64_t first,
@@ -575,15 +534,13 @@ __device__ __forceinline__ double weigh_exactly(const Rows<T>& rows, const Verif
   return sum;
 }
 
+// Request b's draw from its chunks' sums, by a workgroup.
 template <typename T>
-__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
+__device__ void pick(const VerifyArgs& a, int64_t b, const Choice& it) {
   constexpr int WAVES = kPickThreads / 64;
   __shared__ double sums[WAVES];
   __shared__ int32_t picks[WAVES], lasts[WAVES];
-  const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Choice it = a.choices[b];
-  if (it.mode == kDone) return;
   Weights* weights = a.weights + b * a.pick_chunks;
   const Rows<T> rows(a, b, it);
 
@@ -598,8 +555,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     }
     ratio = wave_add(p) / wave_add(q);
     // Chunks where a token may have changed sides, again (exponents are off by 2^-53 of
-    // at most 1100 each, as far as they matter).
-    const double moved = fabs(log2(ratio) - it.ratio_log2) + 1e-12;
+    // at most 1100 each, as far as they matter, and near by 2^-24 of itself).
+    const double moved = fabs(log2(ratio) - it.ratio_log2) * 1.000001 + 1e-12;
     for (int at = 0; at < a.pick_chunks; at += 64) {
       uint64_t again = __ballot(at + lane < a.pick_chunks && weights[at + lane].near <= moved);
       while (again != 0) {  // (the same for every wave)
@@ -657,28 +614,96 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   __syncthreads();
   double run = start + (up_to - own);
   for (int w = 0; w < wave; ++w) run += sums[w];
-  int32_t pick = INT32_MAX, last = -1;
+  int32_t found = INT32_MAX, last = -1;
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
     run += p[e];
     if (p[e] > 0.0) {
       last = (int32_t)(first + e);
-      if (run > bound && pick == INT32_MAX) pick = last;
+      if (run > bound && found == INT32_MAX) found = last;
     }
   }
-  pick = wave_lowest(pick);
+  found = wave_lowest(found);
   last = -wave_lowest(-last);
   if (lane == 0) {
-    picks[wave] = pick;
+    picks[wave] = found;
     lasts[wave] = last;
   }
   __syncthreads();
   if (tid != 0) return;
   for (int w = 1; w < WAVES; ++w) {
-    pick = picks[w] < pick ? picks[w] : pick;
+    found = picks[w] < found ? picks[w] : found;
     last = lasts[w] > last ? lasts[w] : last;
   }
-  *answer = pick != INT32_MAX ? pick : last;
+  *answer = found != INT32_MAX ? found : last;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
+  const Choice it = a.choices[blockIdx.x];
+  if (it.mode != kDone) pick<T>(a, blockIdx.x, it);
+}
+
+// HOW: from kDecides on every workgroup decides for itself, and with kDraws a request's last
+// one draws.
+template <typename T, int HOW>
+__global__ __launch_bounds__(kPickThreads) void verify_weigh_kernel(const VerifyArgs a) {
+  constexpr int WAVES = kPickThreads / 64;
+  __shared__ Weights waves[WAVES];
+  const uint32_t chunk = blockIdx.x % (uint32_t)a.pick_chunks;
+  const int64_t b = blockIdx.x / (uint32_t)a.pick_chunks;
+  Choice it;
+  if constexpr (HOW >= kDecides) {
+    __shared__ DecideShared<kPickThreads> shared;
+    it = decide<T>(a, b, chunk == 0, shared);
+    if (HOW == kDecides && chunk == 0 && threadIdx.x == 0) a.choices[b] = it;
+  } else {
+    it = a.choices[b];
+  }
+  if (it.mode == kDone) return;
+  const Rows<T> rows(a, b, it);
+  double p[kVec], q[kVec], apart[kVec];
+  rows.weigh(a, it, (int64_t)chunk * kPickChunk + threadIdx.x * kVec, p, q, apart);
+  Weights sum{0.0, 0.0, 0.0, 0.0, INFINITY};
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    sum.p += p[e];
+    sum.q += q[e];
+    const bool over = apart[e] > 0.0;
+    sum.p_over += over ? p[e] : 0.0;
+    sum.q_over += over ? q[e] : 0.0;
+    sum.near = fminf(sum.near, fabsf((float)apart[e]));
+  }
+  sum.p_over = wave_add(sum.p_over);
+  if (it.mode == kResample) {
+    sum.p = wave_add(sum.p);
+    sum.q = wave_add(sum.q);
+    sum.q_over = wave_add(sum.q_over);
+    sum.near = wave_reduce(sum.near, [](float a, float b) { return fminf(a, b); });
+  }
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < WAVES; ++w) {
+      sum.p += waves[w].p;
+      sum.q += waves[w].q;
+      sum.p_over += waves[w].p_over;
+      sum.q_over += waves[w].q_over;
+      sum.near = fminf(sum.near, waves[w].near);
+    }
+    a.weights[b * a.pick_chunks + chunk] = sum;
+  }
+  if constexpr (HOW == kDraws) {
+    __shared__ bool is_last;
+    if (threadIdx.x == 0) {
+      __threadfence();
+      is_last = atomicAdd(&a.choices[b].parted, 1) == a.pick_chunks - 1;
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    pick<T>(a, b, it);
+  }
 }
 
 struct Layout {
@@ -705,13 +730,18 @@ int launch(const VerifyArgs& a, const Layout& layout, hipStream_t stream) {
   hipLaunchKernelGGL(verify_rows_kernel<T>, dim3((unsigned)(batch * layout.rows * layout.row_chunks)),
                      dim3(kRowThreads), 0, stream, a);
   const int64_t weighing = batch * layout.pick_chunks;
+  const dim3 grid((unsigned)weighing), threads(kPickThreads);
+  if (weighing <= kFewestWorkgroups) {
+    hipLaunchKernelGGL((verify_weigh_kernel<T, kDraws>), grid, threads, 0, stream, a);
+    return check_hip(hipGetLastError(), "verify draft launch");
+  }
   if (weighing <= kFewWorkgroups) {
-    hipLaunchKernelGGL((verify_weigh_kernel<T, true>), dim3((unsigned)weighing), dim3(kPickThreads), 0, stream, a);
+    hipLaunchKernelGGL((verify_weigh_kernel<T, kDecides>), grid, threads, 0, stream, a);
   } else {
     hipLaunchKernelGGL(verify_decide_kernel<T>, dim3(batch), dim3(kDecideThreads), 0, stream, a);
-    hipLaunchKernelGGL((verify_weigh_kernel<T, false>), dim3((unsigned)weighing), dim3(kPickThreads), 0, stream, a);
+    hipLaunchKernelGGL((verify_weigh_kernel<T, kDecided>), grid, threads, 0, stream, a);
   }
-  hipLaunchKernelGGL(verify_pick_kernel<T>, dim3(batch), dim3(kPickThreads), 0, stream, a);
+  hipLaunchKernelGGL(verify_pick_kernel<T>, dim3(batch), threads, 0, stream, a);
   return check_hip(hipGetLastError(), "verify draft launch");
 }
 

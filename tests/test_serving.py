@@ -78,9 +78,9 @@ def test_verify_entry_refuses_before_launch(changes, status):
 def test_verify_workspace_sizes():
     size = _library.load_library().sah_verify_draft_workspace_bytes
     assert size(0, 3, 1000, 1) == size(2, 1025, 1000, 1) == size(2, 3, 0, 1) == size(-1, 3, 1000, 1) == 0
-    # 16 bytes a row and 8192 logits of it, 40 bytes a request and 2048 logits, 32 a request
-    assert size(2, 3, 1000, 1) == 2 * (7 * 16 + 40 + 32)
-    assert size(2, 3, 8193, 0) == 2 * (4 * 2 * 16 + 5 * 40 + 32)
+    # 16 bytes a row and 8192 logits of it, 40 bytes a request and 2048 logits, 40 a request
+    assert size(2, 3, 1000, 1) == 2 * (7 * 16 + 40 + 40)
+    assert size(2, 3, 8193, 0) == 2 * (4 * 2 * 16 + 5 * 40 + 40)
 
 
 ADAPTERS = dict(
