@@ -25,11 +25,11 @@
 //      target are all but the same), the chunk in which the sum passes the border, the token.
 //
 // 64 requests, 7 drafts, 131072 tokens, bf16 (252 MB, 51 us at a large copy's rate): rows
-// 57 us, decide 7, weigh 25, pick 6.  fp64's v_fma issues at fp32's rate here, but with
-// all rows in fp64 the vector units took 126 us for them.  The draw's two parts in one
-// launch, by the request's last workgroup, took 106 us instead of 30: each of the 4096
-// releases its L2's lines.  For one request (4 drafts, 32000 tokens) the parts are
-// latencies, 4 + 13 us.
+// 57 us, decide 7, weigh 19.6, pick 5.6.  The draw's two parts in one launch, by the
+// request's last workgroup, took 106 us instead of 30, as each of the 4096 releases its
+// L2's lines.  All rows in fp64 took 126 us (some 80 with the exponential as it is now, 24
+// instructions of four cycles a logit).  For one request (4 drafts, 32000 tokens) the parts
+// are latencies, 4 + 11 us.
 
 #include <type_traits>
 
@@ -47,12 +47,12 @@ constexpr int kPickThreads = 256;
 constexpr int kPickChunk = kPickThreads * kVec;
 constexpr int kMaxDrafts = 1024;
 // Workgroups of the draw up to which each decides for itself, for a launch less: one request
-// of 32000 tokens and 4 drafts 7.5 us instead of 4.7 + 4.5, 8 of 131072 tokens and 3 drafts
-// 9.0 instead of 6.2 + 5.9; 16 with 7 drafts (1024 workgroups) 14.8 and 6.2 + 7.6.
+// of 32000 tokens and 4 drafts 7.1 us instead of 4.6 + 4.0, 8 of 131072 tokens and 3 drafts
+// (512) 8.9 instead of 6.0 + 5.2; 16 with 7 drafts (1024) 14.4 and 6.4 + 7.0.
 constexpr int64_t kFewWorkgroups = 512;
-// And up to which a request's last one also draws, for another: 16 13.3 us instead of 8.6 +
-// 4.8, 125 9.9 instead of 6.0 + 4.2, 128 15.4 instead of 8.1 + 5.0, where a launch is 3 us
-// of the host's; 256 16.5 instead of 8.4 + 5.0, 512 22 instead of 10.4 + 5.6, as each
+// And up to which a request's last one also draws, for another: 16 11.4 us instead of 7.1 +
+// 4.1, 125 9.4 instead of 5.5 + 3.7, 128 12.9 instead of 7.0 + 4.4, where a launch is 3 us
+// of the host's; 256 15.6 instead of 7.2 + 4.5, 512 21 instead of 8.9 + 5.1, as each
 // releases its L2's lines.
 constexpr int64_t kFewestWorkgroups = 128;
 enum { kDecided = 0, kDecides = 1, kDraws = 2 };
@@ -103,29 +103,30 @@ struct VerifyArgs {
 
 // 2^x for x <= 0, 0 from below the smallest number on (and for NaN, which no row that is
 // drawn from has): x = n + f with |f| <= 1/2, and for 2^f the polynomial that meets it at
-// the 11 Chebyshev points of that interval, off by 2^-51 of it.
-__device__ __forceinline__ double exp2_upto0(double x) {
-  x = fmax(x, -1100.0);
-  const double n = __builtin_rint(x);
-  const double f = x - n;
-  double y = 0x1.e6063f7217bc6p-28;
-  y = fma(y, f, 0x1.b675bca4eeebbp-24);
-  y = fma(y, f, 0x1.62bfd47773353p-20);
-  y = fma(y, f, 0x1.ffcb54062e698p-17);
-  y = fma(y, f, 0x1.430913096fd9fp-13);
-  y = fma(y, f, 0x1.5d87fe9d7a584p-10);
-  y = fma(y, f, 0x1.3b2ab6fba1ddap-7);
-  y = fma(y, f, 0x1.c6b08d703ce49p-5);
-  y = fma(y, f, 0x1.ebfbdff82c598p-3);
-  y = fma(y, f, 0x1.62e42fefa3a19p-1);
-  y = fma(y, f, 1.0);
-  return ldexp(y, (int)n);
-}
+// the 11 Chebyshev points of that interval, off by 2^-51 of it.  Its coefficients stay in
+// scalar registers, out of the compiler's sight: as literals each takes two moves beside
+// the fma that adds it (weigh of 64 requests of 131072 tokens 25 us instead of 19.6).
+struct Exp2 {
+  double k[10];
+  __device__ __forceinline__ Exp2()
+      : k{0x1.e6063f7217bc6p-28, 0x1.b675bca4eeebbp-24, 0x1.62bfd47773353p-20, 0x1.ffcb54062e698p-17,
+          0x1.430913096fd9fp-13, 0x1.5d87fe9d7a584p-10, 0x1.3b2ab6fba1ddap-7,  0x1.c6b08d703ce49p-5,
+          0x1.ebfbdff82c598p-3,  0x1.62e42fefa3a19p-1} {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) asm("" : "+s"(k[i]));
+  }
+  __device__ __forceinline__ double operator()(double x) const {
+    x = fmax(x, -1100.0);
+    const double n = __builtin_rint(x);
+    const double f = x - n;
+    double y = k[0];
+#pragma unroll
+    for (int i = 1; i < 10; ++i) y = fma(y, f, k[i]);
+    return ldexp(fma(y, f, 1.0), (int)n);
+  }
+};
 __device__ __forceinline__ double exponent_of(float logit, float top, double c) {
   return ((double)logit - (double)top) * c;
-}
-__device__ __forceinline__ double weight_of(float logit, float top, double c) {
-  return exp2_upto0(exponent_of(logit, top, c));
 }
 
 // log2(e) / temperature, and whether the request answers greedily instead (a temperature
@@ -337,7 +338,7 @@ struct RowSum {
   int32_t at;
   __device__ bool there() const { return top > -INFINITY && top < INFINITY && sum == sum; }
 };
-__device__ __forceinline__ RowSum merge_row(const RowPart* parts, int chunks, double c) {
+__device__ __forceinline__ RowSum merge_row(const RowPart* parts, int chunks, double c, const Exp2& power) {
   const int lane = threadIdx.x & 63;
   RowPart part{0.0, -INFINITY, INT32_MAX};
   if (lane < chunks) part = parts[lane];
@@ -349,7 +350,7 @@ __device__ __forceinline__ RowSum merge_row(const RowPart* parts, int chunks, do
   for (int i = lane; i < chunks; i += 64) {
     if (i != lane) part = parts[i];
     // (a sum that is NaN stays it)
-    if (part.sum != 0.0) sum += part.sum * weight_of(part.top, top, c);
+    if (part.sum != 0.0) sum += part.sum * power(exponent_of(part.top, top, c));
     if (part.top == top && part.at < at) at = part.at;
   }
   return {wave_add(sum), top, wave_lowest(at)};
@@ -369,13 +370,14 @@ struct DecideShared {
 
 // A row's sum of exponentials in fp64, by the workgroup.
 template <typename T, int THREADS>
-__device__ double exact_sum(const T* row, float top, double c, int64_t vocab, DecideShared<THREADS>& shared) {
+__device__ double exact_sum(const T* row, float top, double c, int64_t vocab, const Exp2& power,
+                            DecideShared<THREADS>& shared) {
   double sum = 0.0;
   for (int64_t at = (int64_t)threadIdx.x * kVec; at < vocab; at += THREADS * kVec) {
     float l[kVec];
     load_logits<T>(row, at, vocab, l);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) sum += weight_of(l[e], top, c);
+    for (int e = 0; e < kVec; ++e) sum += power(exponent_of(l[e], top, c));
   }
   sum = wave_add(sum);
   __syncthreads();
@@ -412,6 +414,7 @@ __device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShar
   const int64_t* tokens = a.tokens + b * a.drafts;
   const float* uniforms = a.uniforms + b * (a.drafts + 1);
 
+  const Exp2 power;
   int j = -1;
   Seen found{};
   for (int first = 0; j < 0; first += WAVES) {
@@ -423,17 +426,17 @@ __device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShar
       if (known) p_logit = to_f32(target[i * a.t_ss + token]);
       if (known && sampled) q_logit = to_f32(draft[i * a.d_ss + token]);
       Seen mine{};
-      mine.p = merge_row(parts + (int64_t)i * a.row_chunks, a.row_chunks, c);
+      mine.p = merge_row(parts + (int64_t)i * a.row_chunks, a.row_chunks, c, power);
       mine.q = {1.0, 0.0f, 0};
-      if (sampled && i < count) mine.q = merge_row(parts + (int64_t)(a.drafts + 1 + i) * a.row_chunks, a.row_chunks, c);
+      if (sampled && i < count) mine.q = merge_row(parts + (int64_t)(a.drafts + 1 + i) * a.row_chunks, a.row_chunks, c, power);
       mine.none = mine.p.there() && mine.q.there() ? 0 : 1;
       if (mine.none == 0 && known) {
         if (greedy) {
           mine.stands = mine.p.at == token ? 1 : 0;
         } else {
-          const double p = weight_of(p_logit, mine.p.top, c) / mine.p.sum;
+          const double p = power(exponent_of(p_logit, mine.p.top, c)) / mine.p.sum;
           double q = (double)uniforms[i];
-          if (sampled) q *= weight_of(q_logit, mine.q.top, c) / mine.q.sum;
+          if (sampled) q *= power(exponent_of(q_logit, mine.q.top, c)) / mine.q.sum;
           mine.stands = fabs(q - p) <= kFastError * p && p > 0.0 ? -1 : q < p ? 1 : 0;
         }
       }
@@ -448,11 +451,11 @@ __device__ Choice decide(const VerifyArgs& a, int64_t b, bool writes, DecideShar
         const Seen& it = shared.seen[w];
         const T* p_row = target + at * a.t_ss;
         const double p =
-            weight_of(to_f32(p_row[token]), it.p.top, c) / exact_sum<T>(p_row, it.p.top, c, a.vocab, shared);
+            power(exponent_of(to_f32(p_row[token]), it.p.top, c)) / exact_sum<T>(p_row, it.p.top, c, a.vocab, power, shared);
         double q = (double)uniforms[at];
         if (sampled) {
           const T* q_row = draft + at * a.d_ss;
-          q *= weight_of(to_f32(q_row[token]), it.q.top, c) / exact_sum<T>(q_row, it.q.top, c, a.vocab, shared);
+          q *= power(exponent_of(to_f32(q_row[token]), it.q.top, c)) / exact_sum<T>(q_row, it.q.top, c, a.vocab, power, shared);
         }
         stands = q < p ? 1 : 0;
       }
@@ -493,6 +496,7 @@ struct Rows {
   const T* p_row;
   const T* q_row;
   int64_t drafted;  // the token that a certain draft takes out
+  Exp2 power;
   __device__ Rows(const VerifyArgs& a, int64_t b, const Choice& it) {
     p_row = static_cast<const T*>(a.target) + b * a.t_sb + it.row * a.t_ss;
     q_row = static_cast<const T*>(a.draft) + b * a.d_sb + it.row * a.d_ss;
@@ -504,16 +508,20 @@ struct Rows {
     float pl[kVec], ql[kVec];
     load_logits<T>(p_row, first, a.vocab, pl);
     if (it.mode == kResample) load_logits<T>(q_row, first, a.vocab, ql);
+    if (it.mode == kResample) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const double x = exponent_of(pl[e], it.p_top, it.c);
-      p[e] = first + e == drafted ? 0.0 : exp2_upto0(x);
-      q[e] = 0.0;
-      apart[e] = INFINITY;
-      if (it.mode == kResample) {
-        const double y = exponent_of(ql[e], it.q_top, it.c);
-        q[e] = exp2_upto0(y);
+      for (int e = 0; e < kVec; ++e) {
+        const double x = exponent_of(pl[e], it.p_top, it.c), y = exponent_of(ql[e], it.q_top, it.c);
+        p[e] = power(x);
+        q[e] = power(y);
         apart[e] = x - y - it.ratio_log2;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        p[e] = power(exponent_of(first + e == drafted ? -INFINITY : pl[e], it.p_top, it.c));
+        q[e] = 0.0;
+        apart[e] = INFINITY;
       }
     }
   }
