@@ -685,7 +685,7 @@ size_t sah_verify_draft_workspace_bytes(int64_t batch, int64_t drafts, int64_t v
  * counts the entries of block_table [batch, max_blocks] that name a place; a place
  * without holders is free, an entry of -1 names none.  Layers of the same sequences
  * share one table and one book.  Results do not depend on the schedule.  All tensors
- * contiguous, 4-byte aligned.
+ * contiguous, 4-byte aligned; a table has at most 2^31 - 1 entries.
  */
 
 /*

@@ -252,9 +252,9 @@ def hip_block_cache_append(
 
     Tokens are taken back by lowering ``starts``: within the sequence's incomplete
     block, or to a multiple of 64.  Not elsewhere below that block, whose tokens stand
-    where the earlier block's stood before it was coded (to go back there, read the
-    block's first tokens with :func:`hip_block_cache_read` and append them anew, from
-    the multiple of 64 on).
+    where the earlier block's stood before it was coded: to go back there, call
+    :func:`hip_block_cache_take_back` first (or read the block's first tokens with
+    :func:`hip_block_cache_read` and append them anew, from the multiple of 64 on).
     """
 
     request = _append_request(cache, key, value, starts, counts)
