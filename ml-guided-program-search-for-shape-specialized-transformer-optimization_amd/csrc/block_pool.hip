@@ -346,6 +346,7 @@ struct CopyArgs {
 
 constexpr int kCopyLoads = 4;                          // 16-byte loads of a thread in flight
 constexpr int kCopyPart = kThreads * 16 * kCopyLoads;  // bytes of a unit
+constexpr int64_t kPastBytes = (int64_t)256 << 20;     // of a layer's codes: the last-level cache
 
 __device__ __forceinline__ bool is_written(const CopyArgs& a, int64_t place) {
   const int64_t origin = a.origins[place];
@@ -355,7 +356,10 @@ __device__ __forceinline__ bool is_written(const CopyArgs& a, int64_t place) {
 // Place t takes what place origins[t] holds.  No place that is read is written: where
 // an origin is itself written, the pair is left out.  Units of 16 KiB; a workgroup
 // takes every gridDim-th, and looks 64 of them up at a time.  Bound by its bytes: 1000
-// places of 16 heads of 64 (262 MB with the writes, 53 us at a large copy's rate) 60 us.
+// places of 16 heads of 64 (262 MB with the writes, 53 us at a large copy's rate) 57 us
+// past the caches (PAST), 60.5 through them, where the cache's codes fill the last-level
+// one.
+template <bool PAST>
 __global__ __launch_bounds__(kThreads) void cache_copy_kernel(const CopyArgs a) {
   const int lane = threadIdx.x & 63;
   const int units_of_place = 2 * a.parts;
@@ -380,10 +384,16 @@ __global__ __launch_bounds__(kThreads) void cache_copy_kernel(const CopyArgs a) 
       u32x4 data[kCopyLoads];
 #pragma unroll
       for (int i = 0; i < kCopyLoads; ++i)
-        if (first + i * kThreads * 16 < a.place_bytes) data[i] = load16(from + first + i * kThreads * 16);
+        if (first + i * kThreads * 16 < a.place_bytes) data[i] = PAST ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + first + i * kThreads * 16))
+                         : load16(from + first + i * kThreads * 16);
 #pragma unroll
       for (int i = 0; i < kCopyLoads; ++i)
-        if (first + i * kThreads * 16 < a.place_bytes) store16(to + first + i * kThreads * 16, data[i]);
+        if (first + i * kThreads * 16 < a.place_bytes) {
+          if (PAST)
+            __builtin_nontemporal_store(data[i], reinterpret_cast<u32x4*>(to + first + i * kThreads * 16));
+          else
+            store16(to + first + i * kThreads * 16, data[i]);
+        }
       if (part == 0)
         for (int h = threadIdx.x; h < a.heads; h += kThreads)
           a.scales[which][target * a.heads + h] = a.scales[which][origin * a.heads + h];
@@ -670,7 +680,11 @@ extern "C" int sah_block_cache_copy(void* key_codes, void* value_codes, float* k
   a.units = num_blocks * 2 * a.parts;
   a.heads = (int)kv_heads;
   const unsigned grid = (unsigned)(a.units < 2048 ? a.units : 2048);
-  hipLaunchKernelGGL(cache_copy_kernel, dim3(grid), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), a);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (2 * num_blocks * a.place_bytes > kPastBytes)
+    hipLaunchKernelGGL(cache_copy_kernel<true>, dim3(grid), dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(cache_copy_kernel<false>, dim3(grid), dim3(kThreads), 0, s, a);
   return check_hip(hipGetLastError(), "block cache copy launch");
 }
 

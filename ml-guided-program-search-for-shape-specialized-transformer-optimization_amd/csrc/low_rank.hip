@@ -282,9 +282,22 @@ struct UpStage {
   char bytes[4 * S * TILE];
 };
 
+// Four outputs of base or y, past the caches where PAST.
+template <bool PAST, typename V4, typename T>
+__device__ __forceinline__ V4 fetch(const T* p) {
+  return PAST ? __builtin_nontemporal_load(reinterpret_cast<const V4*>(p)) : *reinterpret_cast<const V4*>(p);
+}
+template <bool PAST, typename V4, typename T>
+__device__ __forceinline__ void put(T* p, V4 v) {
+  if (PAST)
+    __builtin_nontemporal_store(v, reinterpret_cast<V4*>(p));
+  else
+    *reinterpret_cast<V4*>(p) = v;
+}
+
 // What a group's outputs of a wave's tokens need: the 64 rows of up, and base.  Places
 // behind `out` read the nearest inside.
-template <typename T, int S, int TT>
+template <typename T, int S, int TT, bool PAST = false>
 struct Group {
   typedef typename Vec8<T>::type V8;
   typedef typename Vec8<T>::half_type V4;
@@ -300,7 +313,7 @@ struct Group {
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) held[i][j] = *reinterpret_cast<const V4*>(tokens.base[i][j] + column);
+      for (int j = 0; j < 4; ++j) held[i][j] = fetch<PAST, V4>(tokens.base[i][j] + column);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int64_t row = first + 16 * r + lane / 4;
@@ -364,15 +377,15 @@ struct Group {
         V4 sum;
 #pragma unroll
         for (int t = 0; t < 4; ++t) sum[t] = from_f32<T>(fmaf(factor[i][j], sums[i][t][j], to_f32(base[i][j][t])));
-        if (tokens.live[i][j]) *reinterpret_cast<V4*>(tokens.y[i][j] + column) = tokens.added[i][j] ? sum : base[i][j];
+        if (tokens.live[i][j]) put<PAST>(tokens.y[i][j] + column, tokens.added[i][j] ? sum : base[i][j]);
       }
   }
 };
 
 // Groups first, first + step, .. of a wave's tokens, whose first one's loads are under way:
 // a group's rows of up pass through LDS while the next one's loads begin.
-template <typename T, int S, int TT>
-__device__ __forceinline__ void expand(Group<T, S, TT>& data, UpStage<S>& lds, const T* up, int64_t rank, int64_t out,
+template <typename T, int S, int TT, bool PAST>
+__device__ __forceinline__ void expand(Group<T, S, TT, PAST>& data, UpStage<S>& lds, const T* up, int64_t rank, int64_t out,
                                        int used, int64_t first, int64_t groups, int64_t step,
                                        const Hidden<T, S> (&h)[TT], const Tokens<T, TT>& tokens) {
   float factor[TT][4];
@@ -388,17 +401,17 @@ __device__ __forceinline__ void expand(Group<T, S, TT>& data, UpStage<S>& lds, c
       for (int j = 0; j < 4; ++j) base[i][j] = data.held[i][j];
     data.stage(lds);
     if (g + step >= groups) {
-      Group<T, S, TT>::finish(lds, base, out, g, h, factor, tokens);
+      Group<T, S, TT, PAST>::finish(lds, base, out, g, h, factor, tokens);
       break;
     }
     data.load(up, rank, out, used, g + step, tokens);
-    Group<T, S, TT>::finish(lds, base, out, g, h, factor, tokens);
-    Group<T, S, TT>::unstage();
+    Group<T, S, TT, PAST>::finish(lds, base, out, g, h, factor, tokens);
+    Group<T, S, TT, PAST>::unstage();
   }
 }
 
 // Tokens without an adapter, groups first, first + step, ..: base as it is.
-template <typename T, int TT, int DEEP>
+template <typename T, int TT, int DEEP, bool PAST>
 __device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t groups, int64_t step,
                                             const Tokens<T, TT>& tokens) {
   typedef typename Vec8<T>::half_type V4;
@@ -411,7 +424,7 @@ __device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int64_t at = (g + d * step) * kGroup + 4 * (threadIdx.x & 15);
-          held[d][i][j] = *reinterpret_cast<const V4*>(tokens.base[i][j] + (at < out ? at : out - 4));
+          held[d][i][j] = fetch<PAST, V4>(tokens.base[i][j] + (at < out ? at : out - 4));
         }
 #pragma unroll
     for (int d = 0; d < DEEP; ++d)
@@ -420,8 +433,8 @@ __device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int64_t at = (g + d * step) * kGroup + 4 * (threadIdx.x & 15);
-          if (tokens.live[i][j] && at < out && tokens.y[i][j] != tokens.base[i][j])
-            *reinterpret_cast<V4*>(tokens.y[i][j] + at) = held[d][i][j];
+          if (tokens.live[i][j] && g + d * step < groups && at < out && tokens.y[i][j] != tokens.base[i][j])
+            put<PAST>(tokens.y[i][j] + at, held[d][i][j]);
         }
   }
 }
@@ -429,7 +442,7 @@ __device__ __forceinline__ void copy_groups(int64_t out, int64_t first, int64_t 
 // A workgroup takes 16 TT tokens and groups_of_wave groups of outputs a wave (all of them
 // where tokens are many).  Its waves share `in` for h, add their sums up in order through
 // LDS, and share the outputs.
-template <typename T, int S, int TT>
+template <typename T, int S, int TT, bool PAST>
 __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankArgs a) {
   constexpr int N = 2 * S;
   __shared__ __align__(16) union {
@@ -449,7 +462,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankA
   const Adapter it = adapter_of(a, b);
   if (it.used == 0 || first >= it.count) {
     const Tokens<T, TT> tokens(a, b, first, it.count);
-    copy_groups<T, TT, 2>(a.out, from + wave, until, kWaves, tokens);
+    copy_groups<T, TT, 2, PAST>(a.out, from + wave, until, kWaves, tokens);
     return;
   }
   f32x4 h[TT][N];
@@ -474,7 +487,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankA
   // the first group's loads pass the waves' meeting
   const Tokens<T, TT> tokens(a, b, first, it.count);
   const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
-  Group<T, S, TT> data;
+  Group<T, S, TT, PAST> data;
   data.load(up, a.rank, a.out, it.used, from + wave < until ? from + wave : from, tokens);
   __syncthreads();
   Hidden<T, S> hidden[TT];
@@ -489,7 +502,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_fused_kernel(const LowRankA
     hidden[i] = make_hidden<T, S>(h[i], it.used, it.scale);
   }
   __syncthreads();
-  expand<T, S, TT>(data, lds.up[wave], up, a.rank, a.out, it.used, from + wave, until, kWaves, hidden, tokens);
+  expand<T, S, TT, PAST>(data, lds.up[wave], up, a.rank, a.out, it.used, from + wave, until, kWaves, hidden, tokens);
 }
 
 // Partial sums of h: workgroup (tile, part) takes the part's slabs, shared by its waves.
@@ -558,7 +571,7 @@ __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRank
   const Adapter it = adapter_of(a, b);
   const Tokens<T, 1> tokens(a, b, first, it.count);
   if (it.used == 0 || first >= it.count) {  // (the same for every wave)
-    copy_groups<T, 1, 1>(a.out, mine, to, kWaves, tokens);
+    copy_groups<T, 1, 1, false>(a.out, mine, to, kWaves, tokens);
     return;
   }
   const T* up = static_cast<const T*>(a.up) + it.index * a.out * a.rank;
@@ -588,12 +601,13 @@ __global__ __launch_bounds__(kThreads) void low_rank_expand_kernel(const LowRank
     __syncthreads();
   }
   const Hidden<T, S> hidden[1] = {make_hidden<T, S>(h, it.used, it.scale)};
-  expand<T, S, 1>(data, lds.up[wave], up, a.rank, a.out, it.used, mine, to, kWaves, hidden, tokens);
+  expand<T, S, 1, false>(data, lds.up[wave], up, a.rank, a.out, it.used, mine, to, kWaves, hidden, tokens);
 }
 
 // How a call is launched.
 struct Plan {
   bool fused;
+  bool past;               // base and y past the caches
   int tokens;              // of a tile
   int64_t tiles_of_seq, tiles;
   int parts, slabs_of_part, groups_of_wave;
@@ -605,6 +619,10 @@ struct Plan {
 // 108 / 109 and 228 / 231; 34816 tokens 195 / 188 and 434 / 405.  Requests of up to a
 // tile's tokens would leave the larger workgroups' places empty.
 constexpr int64_t kManyTiles = 1024;
+// Outputs (of 2 bytes) from which on base and y pass the caches: more than half of the 256 MB
+// last-level cache, which the next operator could not find there anyway (2 x 20001
+// tokens, 4096 outputs: 138 us instead of 149).
+constexpr int64_t kPastOutputs = (int64_t)64 << 20;
 // Few tokens of short inputs take one launch as well: a workgroup a tile and four groups of
 // outputs, each with the first product to itself.  One / two launches, us: 1 and 8 tokens
 // of 1024 inputs, rank 16, 5.4 / 3.3 + 3.9 and 5.8 / 3.8 + 4.2, rank 64 6.9 / 4.0 + 4.4 and
@@ -626,6 +644,7 @@ Plan plan_of(int64_t batch, int64_t seq, int64_t in, int64_t out, int64_t rank) 
     p.tiles_of_seq = ceil_div(seq, p.tokens);
     p.tiles = batch * p.tiles_of_seq;
     p.groups_of_wave = (int)ceil_div(ceil_div(out, kGroup), kWaves);
+    p.past = batch * seq * out > kPastOutputs;
     return p;
   }
   if (in <= kShortIn && p.tiles * ceil_div(ceil_div(out, kGroup), kWaves) <= kFewWorkgroups) {
@@ -657,9 +676,11 @@ int launch(const LowRankArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned)(p.tiles * workgroups));
   if (p.fused) {
     if (p.tokens == 16)
-      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, 1>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, 1, false>), grid, dim3(kThreads), 0, stream, a);
+    else if (p.past)
+      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, kFusedTiles, true>), grid, dim3(kThreads), 0, stream, a);
     else
-      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, kFusedTiles>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((low_rank_fused_kernel<T, S, kFusedTiles, false>), grid, dim3(kThreads), 0, stream, a);
     return check_hip(hipGetLastError(), "low-rank adapters launch");
   }
   hipLaunchKernelGGL((low_rank_shrink_kernel<T, S>), dim3((unsigned)(p.tiles * p.parts)), dim3(kThreads), 0, stream, a);

@@ -389,6 +389,15 @@ def test_adapters_of_few_tokens_and_long_rows(gpu_device, dtype, rank, seq, k, n
     _check_adapters(gpu_device, value, projected, down, up, None, ranks, indices, counts, place=turned, out="in place")
 
 
+@pytest.mark.parametrize("dtype,rank", [(BF16, 16), (F16, 72)])
+def test_adapters_of_outputs_larger_than_the_caches(gpu_device, dtype, rank):
+    ranks = [rank, rank - 9, 0]
+    down, up, scales = _adapter_tensors(3, rank, 40, 4096, dtype, 60, ranks=ranks)
+    value, projected = _rand((4, 4500, 40), 61, dtype), _rand((4, 4500, 4096), 62, dtype)
+    for out in (None, "in place"):
+        _check_adapters(gpu_device, value, projected, down, up, scales, ranks, [1, 2, 0, -1], [4500, 4500, 33, 7], out=out)
+
+
 @pytest.mark.parametrize("batch", [1023, 1024, 1100])
 def test_adapters_of_one_token_of_many_requests(gpu_device, batch):
     down, up, scales = _adapter_tensors(50, 16, 64, 72, F16, 38)
