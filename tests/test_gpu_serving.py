@@ -197,6 +197,25 @@ def test_verify_random_numbers_at_the_border(gpu_device, dtype, sampled, vocab):
     assert min(want[1]) >= drafts // 2 - 1 and min(want[1]) < drafts
 
 
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("batch", [128, 129, 512, 513, 1500])
+def test_verify_of_many_requests_of_every_kind(gpu_device, batch, sampled):
+    """Batches on both sides of where decision and draw become launches of their own."""
+
+    generator = _generator(19)
+    target, draft, tokens, uniforms = _drafted(batch, 3, 203, BF16, 20, near=0.1)
+    if not sampled:
+        tokens = target[:, :3].float().argmax(-1)
+    counts = torch.randint(-1, 5, (batch,), generator=generator).tolist()
+    temperatures = torch.tensor([1.0, 0.0, 0.4, math.inf, 1.0])[torch.randint(0, 5, (batch,), generator=generator)].tolist()
+    target[::11, 1] = math.nan
+    target[5::17, 0, 3:] = -math.inf
+    draft[7::13, 0, 9] = math.inf
+    tokens[9::19, 0] = 203
+    want = _verify(gpu_device, target, tokens, uniforms, draft if sampled else None, counts, temperatures)
+    assert set(want[1]) == {-1, 0, 1, 2, 3}
+
+
 @pytest.mark.parametrize("batch,vocab", [(5, 777), (5, 50_021), (16, 131_073)])
 @pytest.mark.parametrize("near", [1e-6, 1e-5, 1e-4, "one token"])
 def test_verify_distributions_that_lie_close(gpu_device, batch, vocab, near):
