@@ -153,7 +153,10 @@ typedef uint32_t LooseWords __attribute__((ext_vector_type(4), aligned(2)));
 
 // Logits [at, at + 8) of a row as fp32; -inf from the row's end on.  Rows start at any
 // element.  ONCE: past the caches, which the pass over all rows would fill with what nothing
-// reads again (rows 53 us instead of 56, weigh 20.1 instead of 19.5).
+// reads again.  Rows of 64 requests in turn with other inputs 53 us instead of 56, weigh
+// 20.1 instead of 19.5; of logits just written, 32 requests 25.4 instead of 26.2, 64 51 and
+// 51, 128 97 instead of 115; of the same logits again and again 28.7 instead of 26.7, 52 instead
+// of 47, 93 instead of 96.
 template <typename T, bool ONCE = false>
 __device__ __forceinline__ void load_logits(const T* row, int64_t at, int64_t vocab, float* out) {
   if (at + kVec <= vocab) {
