@@ -614,7 +614,7 @@ int sah_linear_w4(
  * Low-rank adapters of many requests beside a shared projection:
  *   y[b][s] = round_to(dtype, base[b][s] + scale_a (x[b][s] down_a^T) up_a^T),
  * a = indices[b], with fp32 accumulation in both products.  The middle factor enters the
- * second product as two 16-bit numbers (off by 2^-16 of itself in bf16, 2^-22 in fp16).
+ * second product as three bf16 numbers (off by 2^-24 of itself) or two fp16 ones (2^-22).
  * A sequence whose index is outside [0, adapters), and rows from counts[b] on (counts
  * NULL: none), take base as it is.
  *

@@ -14,10 +14,12 @@
 // four lanes in registers, rows of `up` through the wave's own part of LDS, and the second
 // product's columns are outputs 4 n + t, so that 16 lanes take 128 bytes of base and y.
 //
-// h is fp32.  It enters the second product as the sum of two 16-bit numbers, off by
-// 2^-16 (bf16) or 2^-22 (fp16) of itself: one number's 2^-9 would be as much as the
-// output's own rounding.  A token's h is taken in a power of two of its own, its largest
-// below 2^15, so that fp16 reaches.
+// h is fp32.  It enters the second product as the sum of three bf16 numbers, off by 2^-24
+// of itself as fp32 is, or of two fp16 numbers, off by 2^-22: with one number its 2^-8 would
+// be as much as the output's own rounding, and with two bf16 numbers some 0.2% of the
+// outputs are rounded another way (2 x 20001 tokens below 139.4 us with three, 138.5 with
+// two; 34816 tokens 4096 -> 4096, rank 64, 208 and 204, rank 128, 339 and 320).  A token's h is taken in a power of two of its own, its
+// largest below 2^15, so that fp16 reaches.
 //
 // Few tokens are bound by the adapters' bytes and by latency, and a workgroup a token would
 // leave most of the chip idle: one launch shares `in` among workgroups and leaves partial
@@ -186,19 +188,25 @@ __device__ __forceinline__ void shrink(const T* const (&x)[TT][4], const T* down
   if (slab < last) shrink_slab<T, S, TT, false>(x, down, w_first, in, slab, h);
 }
 
-// A token's h, times 2^power, as the second product's operands; factor: scale / 2^power.
+// A token's h, times 2^power, as the second product's operands, the largest part first;
+// factor: scale / 2^power.
 template <typename T, int S>
 struct Hidden {
+  static constexpr int PARTS = std::is_same<T, bf16>::value ? 3 : 2;
   typedef typename Vec8<T>::type V8;
-  V8 high[S], low[S];
+  V8 part[PARTS][S];
   float factor;
 };
 
-template <typename T>
-__device__ __forceinline__ void split_number(float v, T& high, T& low) {
-  high = from_f32<T>(v);
-  const float rest = v - to_f32(high);
-  low = from_f32<T>(fabsf(to_f32(high)) < INFINITY ? rest : 0.0f);
+template <int PARTS, typename T>
+__device__ __forceinline__ void split_number(float v, T (&part)[PARTS]) {
+  part[0] = from_f32<T>(v);
+  float rest = fabsf(to_f32(part[0])) < INFINITY ? v - to_f32(part[0]) : 0.0f;
+#pragma unroll
+  for (int i = 1; i < PARTS; ++i) {
+    part[i] = from_f32<T>(rest);
+    rest -= to_f32(part[i]);
+  }
 }
 
 template <typename T, int S>
@@ -223,10 +231,10 @@ __device__ __forceinline__ Hidden<T, S> make_hidden(const f32x4 (&h)[2 * S], int
   for (int t = 0; t < 2 * S; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      T high, low;
-      split_number<T>(ldexpf(v[t][i], power), high, low);
-      out.high[t / 2][4 * (t & 1) + i] = high;
-      out.low[t / 2][4 * (t & 1) + i] = low;
+      T part[Hidden<T, S>::PARTS];
+      split_number(ldexpf(v[t][i], power), part);
+#pragma unroll
+      for (int k = 0; k < Hidden<T, S>::PARTS; ++k) out.part[k][t / 2][4 * (t & 1) + i] = part[k];
     }
   out.factor = ldexpf(scale, -power);
   return out;
@@ -362,10 +370,9 @@ struct Group {
         const V8 tile = *reinterpret_cast<const V8*>(lds.bytes + (s * 4 + t) * UpStage<S>::TILE + (lane & 15) * 64 +
                                                      (lane >> 4) * 16);
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          sums[i][t] = mfma16(h[i].low[s], tile, sums[i][t]);
-          sums[i][t] = mfma16(h[i].high[s], tile, sums[i][t]);
-        }
+        for (int i = 0; i < TT; ++i)
+#pragma unroll
+          for (int k = Hidden<T, S>::PARTS - 1; k >= 0; --k) sums[i][t] = mfma16(h[i].part[k][s], tile, sums[i][t]);
       }
     }
     const int64_t column = group * kGroup + 4 * (lane & 15);

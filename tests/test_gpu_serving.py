@@ -466,6 +466,35 @@ def test_adapters_of_large_and_small_products(gpu_device, seq, dtype, size):
     _check_adapters(gpu_device, value, projected, down, up, scales, None, [0, 1])
 
 
+@pytest.mark.parametrize("dtype,bits", [(BF16, 24), (F16, 22)])
+@pytest.mark.parametrize("rank", [16, 64, 128])
+@pytest.mark.parametrize("seq,k,n", [(1, 24, 72), (20, 4104, 136), (9000, 24, 72), (17_000, 24, 4096)])
+def test_adapters_whose_middle_factors_differ_in_the_last_bits(gpu_device, dtype, bits, rank, seq, k, n):
+    """Directions in pairs with h = a + b + c and a + b, of which an output takes the
+    difference c: whole numbers (times 2^-12) of up to ``bits`` bits whose every sum fp32
+    holds, so the answer is exact where h reaches the second product with all its bits."""
+
+    from solution.kernels.projection import LowRankAdapters, hip_low_rank_adapters
+
+    last = bits - 16
+    down, up = torch.zeros((1, rank, k)), torch.zeros((1, n, rank))
+    pairs = rank // 2
+    draw = lambda low, high: torch.randint(low, high, (pairs,), generator=_generator(48 + rank)).float()  # noqa: E731
+    first, middle, least = draw(128, 256) * 2.0 ** (8 + last), draw(128, 256) * 2.0**last, draw(2 ** (last - 1), 2**last)
+    for place, part in ((0, first), (k // 2, middle), (k - 1, least)):
+        down[0, 0::2, place] = down[0, 1::2, place] = part * 2.0**-12
+    down[0, 1::2, k - 1] = 0
+    taken = torch.arange(n) % pairs
+    up[0, torch.arange(n), 2 * taken], up[0, torch.arange(n), 2 * taken + 1] = 1.0, -1.0
+    given = [t.to(dtype) for t in (torch.ones(1, seq, k), torch.zeros(1, seq, n), down, up)]
+    assert torch.equal(given[2].float(), down)
+    value, projected, down, up = (t.to(gpu_device) for t in given)
+    with torch.inference_mode():
+        got = hip_low_rank_adapters(value, projected, LowRankAdapters(down, up), _words([0], gpu_device))[0]
+    want = (least[taken] * 2.0**-12).to(dtype).to(gpu_device)
+    assert torch.equal(got, want.expand(1, seq, n))
+
+
 @pytest.mark.parametrize("seq,features", [(20, 64), (9000, 64), (20, 4096)])
 def test_adapters_keep_bad_tokens_to_themselves(gpu_device, seq, features):
     from solution.kernels.projection import LowRankAdapters, hip_low_rank_adapters
