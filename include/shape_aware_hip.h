@@ -693,8 +693,10 @@ size_t sah_verify_draft_workspace_bytes(int64_t batch, int64_t drafts, int64_t v
  * count as tokens) behind starts[b] completes and whose entry names none: the lowest free
  * places in order, sequence by sequence and block by block.  A sequence with a
  * negative start takes none.  missing[b]: its blocks that found no free place, or
- * lie behind max_blocks; the append drops them, and they may be reserved later only if
- * nothing was appended to them.  workspace of
+ * lie behind max_blocks; the append drops them with all that they held, and they may be
+ * reserved later only if nothing was appended to them.  Of n tokens, those up to the first of
+ * them are min(n, 64 ((starts[b] + n) / 64 + 1 - missing[b]) - 1 - starts[b]), where a
+ * sequence's entries are named from the front, as these calls do.  workspace of
  * sah_block_pool_reserve_workspace_bytes(), 4-byte aligned, not shared by calls that overlap.
  */
 int sah_block_pool_reserve(

@@ -7,16 +7,24 @@ nothing here waits for the host, so a captured step may hold any of it.  Sequenc
 go on from the same tokens share the places of their complete blocks, which are never
 written again.
 
-A step with drafts, of ``drafts + 1`` new tokens a sequence, for every layer::
+A step with drafts, of ``wanted`` [batch] new tokens (int32, at most ``drafts + 1``), for
+every layer::
 
-    hip_block_pool_reserve(pool, starts, drafts + 1)
+    missing, _ = hip_block_pool_reserve(pool, starts, drafts + 1, wanted)
+    counts = torch.minimum(wanted, 64 * ((starts + wanted) // 64 + 1 - missing) - 1 - starts)
     ...                                            # append, attention, the model's logits
-    answer, accepted, _ = hip_verify_draft(logits, tokens, uniforms, draft_logits)
-    lengths, ends = starts + drafts + 1, starts + 1 + accepted
+    answer, accepted, _ = hip_verify_draft(logits, tokens, uniforms, draft_logits, counts=counts - 1)
+    lengths, ends = starts + counts, starts + 1 + accepted
     for cache in caches:
         hip_block_cache_take_back(cache, lengths, ends)
     hip_block_pool_release(pool, ends)
     starts = ends
+
+``counts`` are the tokens up to the first block that found no place: appended beyond them,
+a block is dropped, and with it what the tail held before.  The append and the attention
+get them too.  A sequence that can take none (``counts`` 0) takes no part in the
+verification (``accepted`` -1), stays where it was and has the same tokens to append in a
+later step.
 
 Beams and parallel samples go on from ``sources`` [batch]::
 
@@ -165,7 +173,10 @@ def hip_block_pool_reserve(
     behind ``starts`` completes: the lowest free ones, sequence by sequence.
 
     Before the append.  Returns ``missing`` [batch] (int32), the blocks that found no free
-    place or lie behind the table: the append drops those.
+    place or lie behind the table.  The append drops those with all that they held; of ``n``
+    tokens, ``min(n, 64 * ((starts + n) // 64 + 1 - missing) - 1 - starts)`` stay before
+    the first of them (where a sequence's entries are named from the front, as these
+    calls do).
     """
 
     request = _reserve_request(pool, starts, tokens, counts)

@@ -169,3 +169,51 @@ class Book:
             self.holders[hole], self.holders[mover] = self.holders[mover], 0
         self.table = [[moves.get(p, p) for p in row] for row in self.table]
         return origins, len(used)
+
+
+class TokenCache:
+    """Token numbers where a layer's cache holds keys and values: a tail of 64 a sequence, the
+    places' blocks, and the book's table.  LOST is what nobody can read back."""
+
+    LOST = -1
+
+    def __init__(self, book):
+        self.book = book
+        self.tails = [[self.LOST] * BLOCK for _ in book.table]
+        self.places = [[self.LOST] * BLOCK for _ in book.holders]
+
+    def _place(self, b, block):
+        row = self.book.table[b]
+        place = row[block] if block < len(row) else -1
+        return place if self.book.is_place(place) else None
+
+    def append(self, starts, counts, tokens):
+        for b, (start, count) in enumerate(zip(starts, counts)):
+            for i in range(count):
+                self.tails[b][(start + i) % BLOCK] = tokens[b][i]
+                place = self._place(b, (start + i) // BLOCK)
+                if (start + i) % BLOCK == BLOCK - 1 and place is not None:
+                    self.places[place] = list(self.tails[b])
+
+    def read(self, b, length):
+        held = []
+        for block in range(length // BLOCK):
+            place = self._place(b, block)
+            held += [self.LOST] * BLOCK if place is None else self.places[place]
+        return held + self.tails[b][: length % BLOCK]
+
+    def take_back(self, lengths, ends):
+        for b, (length, end) in enumerate(zip(lengths, ends)):
+            if end >= 0 and end % BLOCK and end // BLOCK < length // BLOCK:
+                place = self._place(b, end // BLOCK)
+                self.tails[b] = [self.LOST] * BLOCK if place is None else list(self.places[place])
+
+    def fork(self, sources):
+        before = self.tails
+        self.tails = [list(before[s if 0 <= s < len(before) else b]) for b, s in enumerate(sources)]
+
+    def copy(self, origins):
+        before = [list(place) for place in self.places]
+        for target, origin in enumerate(origins):
+            if origin >= 0:
+                self.places[target] = before[origin]

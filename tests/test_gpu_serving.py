@@ -1051,6 +1051,63 @@ def test_steps_with_drafts_across_blocks(gpu_device):
             assert ((a - w).abs() <= bound).all(), b
 
 
+@pytest.mark.parametrize("places", [1, 2, 3, 6])
+def test_steps_of_a_pool_that_runs_out(gpu_device, places):
+    """Steps that ask for more places than there are, with the tokens that each appends cut
+    to those before the first block without one: what stood stays, finite and as the
+    tokens' own keys and values, and sequences go on as long as no block must be complete."""
+
+    from solution.kernels.attention import hip_block_pool_reserve
+    from solution.kernels.sampling import hip_verify_draft
+
+    batch, vocab, drafts = 5, 101, 7
+    model = _Serving(gpu_device, batch, vocab=vocab, num_blocks=places, max_tokens=192, seed=94)
+    generator = _generator(95)
+    with torch.inference_mode():
+        first = [60, 57, 63, 30, 100]
+        prompt = torch.randint(0, vocab, (batch, 100), generator=generator).to(gpu_device)
+        starts = _words(first, gpu_device)
+        model.logits(prompt, torch.zeros_like(starts), starts)
+        assert model.pool.block_table[4].tolist() == [0, -1, -1]
+        history = [prompt[b, :n].tolist() for b, n in enumerate(first)]
+        wanted = _words([8, 8, 8, 3, 8], gpu_device)
+        short = 0
+        for step in range(16):
+            tokens = torch.randint(0, vocab, (batch, drafts + 1), generator=generator).to(gpu_device)
+            missing, _ = hip_block_pool_reserve(model.pool, starts, drafts + 1, wanted)
+            counts = torch.minimum(wanted, 64 * ((starts + wanted) // 64 + 1 - missing) - 1 - starts)
+            logits = model.logits(tokens, starts, counts)
+            same = logits[:, :drafts].float().argmax(-1)  # the first of them stand
+            cut = torch.randint(0, drafts + 1, (batch, 1), generator=generator).to(gpu_device)
+            same = torch.where(torch.arange(drafts, device=gpu_device) < cut, same, (same + 1) % vocab)
+            zero = torch.zeros(batch, device=gpu_device)
+            uniforms = torch.rand((batch, drafts + 1), device=gpu_device)
+            answer, accepted, _ = hip_verify_draft(logits, same, uniforms, counts=counts - 1, temperatures=zero)
+            assert torch.equal(accepted, torch.minimum(cut[:, 0], counts - 1).int())
+            lengths, ends = starts + counts, starts + 1 + accepted
+            model.settle(lengths, ends)
+            for b, (start, end) in enumerate(zip(starts.tolist(), ends.tolist())):
+                history[b] += tokens[b, : end - start].tolist()
+                # a sequence waits only where its next token would complete a block without a place
+                assert end > start or (start % 64 == 63 and int(missing[b]) > 0), (step, b)
+            short += int((missing > 0).sum())
+            starts = ends
+            assert model.pool.block_table.ge(0).sum(1).tolist() == [n // 64 for n in starts.tolist()]
+        assert short > 0
+        whole = _Serving(gpu_device, batch, vocab=vocab, max_tokens=192, seed=94)
+        most = int(starts.max())
+        tokens = torch.tensor([h + [0] * (most - len(h)) for h in history], device=gpu_device)
+        whole.logits(tokens, torch.zeros_like(starts), starts)
+        got, want = _held(model.cache, starts), _held(whole.cache, starts)
+    for mine, other in zip(got, want):
+        for b, n in enumerate(starts.tolist()):
+            a, w = mine[b, :, :n].double().cpu(), other[b, :, :n].double().cpu()
+            # as in test_steps_with_drafts_across_blocks: two codings on either side
+            largest = torch.stack([t.abs().amax(dim=(1, 2)) for t in (a, w)]).amax(0)[:, None, None]
+            bound = 4 * (2.0**-4 * torch.maximum(a.abs(), w.abs()) + 2.0**-10 * largest / 224)
+            assert a.isfinite().all() and ((a - w).abs() <= bound).all(), b
+
+
 def test_beams_share_blocks_and_part(gpu_device):
     """Forked sequences hold what their sources held, then their own tokens; the
     sources' stay as they were; after compaction all of it stands at lower places."""

@@ -4,9 +4,15 @@ pool's and the adapters' own tensors."""
 
 from __future__ import annotations
 
+import re
+import textwrap
+from pathlib import Path
+
 import pytest
 import torch
 
+from serving_reference import Book, TokenCache
+from solution.kernels.attention import hip_block_pool as pool_module
 from solution.kernels.attention import (
     BlockCache,
     BlockPool,
@@ -452,3 +458,89 @@ def test_operators_refuse_cpu_tensors():
         with pytest.raises(RuntimeError, match="ineligible"):
             call()
     assert pool.block_table.eq(-1).all()
+
+
+# ---------------------------------------------------------------------------
+# the documented recipes, run on whole numbers
+
+
+def _recipes(where):
+    """The documented calls for the block pool, as texts: a step's before and after the
+    model's own part, and what follows them."""
+
+    if where == "docstring":
+        blocks = re.findall(r"::\n\n((?:    .*\n|\n)+)", pool_module.__doc__)
+        text = "\n".join(textwrap.dedent(block) for block in blocks)
+    else:
+        document = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
+        (text,) = [block for block in re.findall(r"```python\n(.*?)```", document, re.S) if "hip_block_pool_reserve(pool" in block]
+        text = text[re.search(r"^.*hip_block_pool_reserve\(pool", text, re.M).start() :]
+    before, rest = text.split("\n...", 1)
+    after, others = rest[rest.index("answer, accepted") :].split("starts = ends\n", 1)
+    return before, after + "starts = ends\n", others
+
+
+def _words(values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def _stand_ins(book, caches, accepts):
+    """The calls that the recipes make, on a book and caches of whole numbers; ``accepts``
+    says how many drafts of a request stand at most."""
+
+    def reserve(pool, starts, tokens, counts=None):
+        return _words(book.reserve(starts.tolist(), tokens, None if counts is None else counts.tolist())), "marker"
+
+    def verify(logits, tokens, uniforms, draft=None, *, counts=None, temperatures=None):
+        count = [tokens.shape[1]] * tokens.shape[0] if counts is None else counts.tolist()
+        return tokens, _words([-1 if c < 0 else min(c, a) for c, a in zip(count, accepts)]), "marker"
+
+    def compact(pool):
+        origins, used = book.compact()
+        return _words(origins), _words([used]), "marker"
+
+    return dict(
+        torch=torch, pool=book, caches=caches, logits=None, uniforms=None, draft_logits=None, temperatures=None,
+        hip_block_pool_reserve=reserve,
+        hip_verify_draft=verify,
+        hip_block_cache_take_back=lambda cache, lengths, ends: cache.take_back(lengths.tolist(), ends.tolist()),
+        hip_block_pool_release=lambda pool, lengths: book.release(lengths.tolist()),
+        hip_block_pool_fork=lambda pool, sources, lengths: book.fork(sources.tolist(), lengths.tolist()),
+        hip_block_cache_fork=lambda cache, sources: cache.fork(sources.tolist()),
+        hip_block_pool_compact=compact,
+        hip_block_cache_copy=lambda cache, origins: cache.copy(origins.tolist()),
+    )
+
+
+@pytest.mark.parametrize("where", ["docstring", "integration"])
+@pytest.mark.parametrize("blocks", [0, 1, 2, 3, 5, 30])
+def test_documented_step_keeps_its_tokens_where_places_run_out(where, blocks):
+    """Steps of sequences that ask for fewer and for more places than there are: whatever
+    was kept is held, and a sequence goes on wherever its next token needs no block."""
+
+    before, after, _ = _recipes(where)
+    drafts, starts = 7, [60, 57, 63, 0, 126, 10]
+    width = 4
+    book = Book([[-1] * width for _ in starts], [0] * (blocks + 2))
+    cache = TokenCache(book)
+    book.table[4][0], book.holders[0] = 0, 1  # one sequence has a block
+    book.holders[1] = 1  # and one place is someone else's
+    kept = [[1000 * b + i for i in range(n)] for b, n in enumerate(starts)]
+    cache.append([0] * len(starts), starts, kept)
+    wants = [8, 8, 8, 8, 8, 3]
+    accepts = [7, 2, 0, 7, 5, 1]
+    names = _stand_ins(book, [cache], accepts) | dict(drafts=drafts, starts=_words(starts))
+    for step in range(40):
+        names |= dict(wanted=_words(wants), tokens=torch.zeros((len(starts), drafts), dtype=torch.int64))
+        now = names["starts"].tolist()
+        fresh = [[100_000 * (step + 1) + 1000 * b + i for i in range(drafts + 1)] for b in range(len(starts))]
+        exec(before, names)
+        counts = names["counts"].tolist() if "counts" in names else [drafts + 1] * len(starts)
+        cache.append(now, counts, fresh)
+        exec(after, names)
+        for b, (start, end) in enumerate(zip(now, names["starts"].tolist())):
+            assert start <= end <= start + wants[b]
+            if start % 64 < 63:  # its next token fits the tail
+                assert end > start or start >= 64 * width + 63
+            kept[b] = kept[b] + fresh[b][: end - start]
+            assert cache.read(b, end) == kept[b], (step, b)
