@@ -26,12 +26,14 @@ get them too.  A sequence that can take none (``counts`` 0) takes no part in the
 verification (``accepted`` -1), stays where it was and has the same tokens to append in a
 later step.
 
-Beams and parallel samples go on from ``sources`` [batch]::
+Beams and parallel samples go on from ``sources`` [batch] (int32; a sequence whose source is
+outside [0, batch) stays as it is)::
 
-    hip_block_pool_fork(pool, sources, lengths)
+    hip_block_pool_fork(pool, sources, starts)
     for cache in caches:
         hip_block_cache_fork(cache, sources)
-    lengths = lengths[sources]
+    itself = torch.arange(len(sources), device=sources.device)
+    starts = starts[torch.where((sources >= 0) & (sources < len(sources)), sources, itself)]
 
 and a pool is compacted, for a smaller one or a copy elsewhere, by::
 

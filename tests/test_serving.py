@@ -544,3 +544,36 @@ def test_documented_step_keeps_its_tokens_where_places_run_out(where, blocks):
                 assert end > start or start >= 64 * width + 63
             kept[b] = kept[b] + fresh[b][: end - start]
             assert cache.read(b, end) == kept[b], (step, b)
+
+
+@pytest.mark.parametrize("where", ["docstring", "integration"])
+@pytest.mark.parametrize("sources", [[1, 0, -1, 3, 7, 0], [-1] * 6, [6, 6, 6, 0, 0, 0], [5, 4, 3, 2, 1, 0]])
+def test_documented_beams_go_on_where_their_sources_were(where, sources):
+    """Behind a step whose drafts stood in part: every sequence holds what its source
+    held, as long as that was, and goes on from there; so it does after the compaction."""
+
+    before, after, others = _recipes(where)
+    drafts, first = 7, [60, 130, 64, 5, 200, 127]
+    batch, width = len(first), 5
+    book = Book([[-1] * width for _ in first], [0] * 40)
+    cache = TokenCache(book)
+    kept = [[1000 * b + i for i in range(n)] for b, n in enumerate(first)]
+    names = _stand_ins(book, [cache], [7, 2, 0, 7, 5, 1]) | dict(drafts=drafts)
+    book.reserve([0] * batch, max(first), first)
+    cache.append([0] * batch, first, kept)
+    names |= dict(starts=_words(first), wanted=_words([8] * batch), tokens=torch.zeros((batch, drafts), dtype=torch.int64))
+    fresh = [[100_000 + 1000 * b + i for i in range(drafts + 1)] for b in range(batch)]
+    exec(before, names)
+    cache.append(first, [drafts + 1] * batch, fresh)
+    exec(after, names)
+    kept = [kept[b] + fresh[b][: n - first[b]] for b, n in enumerate(names["starts"].tolist())]
+    names["sources"] = _words(sources)
+    names["lengths"] = names["lengths"].clone()
+    exec(others, names)
+    want = [kept[s if 0 <= s < batch else b] for b, s in enumerate(sources)]
+    assert names["starts"].tolist() == [len(tokens) for tokens in want]
+    for b, tokens in enumerate(want):
+        assert cache.read(b, len(tokens)) == tokens
+        # nothing is named behind what is held
+        assert [block for block, place in enumerate(book.table[b]) if place >= 0] == list(range(len(tokens) // 64))
+    assert sorted({p for row in book.table for p in row if p >= 0}) == list(range(int(names["used"])))
