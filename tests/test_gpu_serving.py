@@ -513,6 +513,41 @@ def test_adapters_keep_bad_tokens_to_themselves(gpu_device, seq, features):
     assert torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0))
 
 
+def _run_adapters(device, value, projected, down, up, ranks=None):
+    """One adapter's outputs on the CPU."""
+
+    from solution.kernels.projection import LowRankAdapters, hip_low_rank_adapters
+
+    packed = LowRankAdapters(down.to(device), up.to(device), None, None if ranks is None else _words(ranks, device))
+    indices = _words([0] * value.shape[0], device)
+    with torch.inference_mode():
+        return hip_low_rank_adapters(value.to(device), projected.to(device), packed, indices)[0].cpu()
+
+
+def _same_with_infinities(got, want):
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(0.5, 1e30, -1e30), want.nan_to_num(0.5, 1e30, -1e30))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("seq,k,n", [(1, 24, 72), (20, 4104, 136), (9000, 24, 72), (17_000, 24, 4096)])
+def test_adapters_with_an_infinite_middle_factor(gpu_device, dtype, seq, k, n):
+    """A weight of `down` is infinite, and with it one direction's h, beside others of 2^24,
+    beyond fp16's range: infinite outputs of its sign, NaN where its input is 0."""
+
+    down, up, value = torch.zeros((1, 16, k)), torch.zeros((1, n, 16)), torch.zeros((1, seq, k))
+    down[0, 0, 0], down[0, 1:, k - 1] = math.inf, 512.0
+    up[0, :, 0] = torch.where(torch.arange(n) % 3 == 0, -0.25, 2.0)
+    up[0, :, 1] = torch.where(torch.arange(n) % 2 == 0, -1.0, 1.0)
+    value[0, :, 0] = torch.tensor([1.0, -1.0, 0.5, 0.0])[torch.arange(seq) % 4]
+    value[0, :, k - 1] = 2.0**15
+    projected = _rand((1, seq, n), 96, dtype)
+    got = _run_adapters(gpu_device, value.to(dtype), projected, down.to(dtype), up.to(dtype))
+    want = (value[0, :, :1] * math.inf) * up[0, :, 0]
+    assert float(want[0, 0]) == -math.inf and float(want[0, 1]) == math.inf
+    _same_with_infinities(got[0].float(), want)
+
+
 def test_adapters_of_more_than_four_gigabytes(gpu_device):
     """Offsets beyond 32 bits in the weights, the inputs and the outputs."""
 
