@@ -324,17 +324,17 @@ struct Group {
   __device__ __forceinline__ void load(const T* up, int64_t rank, int64_t out, int used, int64_t group,
                                        const Tokens<T, TT>& tokens) {
     const int lane = threadIdx.x & 63;
-    const int64_t first = group * kGroup;
-    const int64_t asked = first + 4 * (lane & 15);
-    const int64_t column = asked < out ? asked : out - 4;
+    const int first = (int)group * kGroup, last = (int)out;
+    const int asked = first + 4 * (lane & 15);
+    const int column = asked < last ? asked : last - 4;
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) held[i][j] = fetch<PAST, V4>(tokens.base[i][j] + column);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t row = first + 16 * r + lane / 4;
-      const T* from = up + (row < out ? row : out - 1) * rank;
+      const int row = first + 16 * r + lane / 4;
+      const T* from = up + (row < last ? row : last - 1) * rank;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int chunk = 32 * s + 8 * (lane & 3);
@@ -343,16 +343,30 @@ struct Group {
     }
   }
 
+  static __device__ __forceinline__ char* place_of(UpStage<S>& lds, int s, int r) {
+    const int lane = threadIdx.x & 63, row = 16 * r + lane / 4;
+    return lds.bytes + (s * 4 + row % 4) * UpStage<S>::TILE + (row / 4) * 64 + (lane & 3) * 16;
+  }
+
+  // Zeros for the directions from `used` on, which no group's rows replace: h is 0 there, and
+  // 0 times what load() reads in their place may be NaN.
+  static __device__ __forceinline__ void clear(UpStage<S>& lds, int used) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (32 * s + 8 * side_of() >= used) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) store16(place_of(lds, s, r), (u32x4){0u, 0u, 0u, 0u});
+      }
+  }
+
   // Row 4 n + t of the group becomes row n of tile t.
-  __device__ __forceinline__ void stage(UpStage<S>& lds) const {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ void stage(UpStage<S>& lds, int used) const {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * r + lane / 4;
+    for (int s = 0; s < S; ++s)
+      if (32 * s + 8 * side_of() < used) {
 #pragma unroll
-      for (int s = 0; s < S; ++s)
-        *reinterpret_cast<V8*>(lds.bytes + (s * 4 + row % 4) * UpStage<S>::TILE + (row / 4) * 64 + (lane & 3) * 16) = w[s][r];
-    }
+        for (int r = 0; r < 4; ++r) *reinterpret_cast<V8*>(place_of(lds, s, r)) = w[s][r];
+      }
     // the wave's lanes read what the others wrote
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -364,28 +378,39 @@ struct Group {
   }
 
   // base + scale (up h).  Tokens that the adapter is not added to take base as it is,
-  // tokens behind the sequence nothing.
+  // tokens behind the sequence nothing.  The products with h's smaller parts come first: they
+  // are NaN or infinite only with an infinite (or NaN) row of up, and then any number
+  // will do beside those with the largest, whose infinity or NaN it is.
   static __device__ __forceinline__ void finish(const UpStage<S>& lds, const V4 (&base)[TT][4], int64_t out, int64_t group,
                                                 const Hidden<T, S> (&h)[TT], const float (&factor)[TT][4],
                                                 const Tokens<T, TT>& tokens) {
     const int lane = threadIdx.x & 63;
     f32x4 sums[TT][4];
+    constexpr float kMost = 3.40282347e38f;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
+      V8 tile[S];
 #pragma unroll
       for (int i = 0; i < TT; ++i) sums[i][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const V8 tile = *reinterpret_cast<const V8*>(lds.bytes + (s * 4 + t) * UpStage<S>::TILE + (lane & 15) * 64 +
-                                                     (lane >> 4) * 16);
+        tile[s] = *reinterpret_cast<const V8*>(lds.bytes + (s * 4 + t) * UpStage<S>::TILE + (lane & 15) * 64 +
+                                               (lane >> 4) * 16);
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
-          for (int k = Hidden<T, S>::PARTS - 1; k >= 0; --k) sums[i][t] = mfma16(h[i].part[k][s], tile, sums[i][t]);
+          for (int k = Hidden<T, S>::PARTS - 1; k > 0; --k) sums[i][t] = mfma16(h[i].part[k][s], tile[s], sums[i][t]);
+      }
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[i][t][j] = __builtin_amdgcn_fmed3f(sums[i][t][j], -kMost, kMost);
+#pragma unroll
+        for (int s = 0; s < S; ++s) sums[i][t] = mfma16(h[i].part[0][s], tile[s], sums[i][t]);
       }
     }
-    const int64_t column = group * kGroup + 4 * (lane & 15);
-    if (column >= out) return;
+    const int column = (int)group * kGroup + 4 * (lane & 15);
+    if (column >= (int)out) return;
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll
@@ -409,13 +434,14 @@ __device__ __forceinline__ void expand(Group<T, S, TT, PAST>& data, UpStage<S>& 
   for (int i = 0; i < TT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) factor[i][j] = __shfl(h[i].factor, 4 * quarter_of() + j);
+  Group<T, S, TT, PAST>::clear(lds, used);
   for (int64_t g = first; g < groups; g += step) {
     typename Vec8<T>::half_type base[TT][4];
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) base[i][j] = data.held[i][j];
-    data.stage(lds);
+    data.stage(lds, used);
     if (g + step >= groups) {
       Group<T, S, TT, PAST>::finish(lds, base, out, g, h, factor, tokens);
       break;

@@ -548,6 +548,37 @@ def test_adapters_with_an_infinite_middle_factor(gpu_device, dtype, seq, k, n):
     _same_with_infinities(got[0].float(), want)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rank,own", [(16, None), (16, 7), (64, 24), (128, None), (128, 100)])
+@pytest.mark.parametrize("seq,k,n", [(1, 24, 72), (3, 24, 72), (20, 4104, 136), (9000, 24, 72), (17_000, 24, 4096)])
+def test_adapters_with_infinite_weights_of_the_outputs(gpu_device, dtype, rank, own, seq, k, n):
+    """Weights of `up` are infinite: outputs of the sign of their direction's h, NaN where two
+    of different signs meet and for an h of 0, and all others as they are without these."""
+
+    own = own or rank
+    down, up = torch.zeros((1, rank, k)), _rand((1, n, rank), 97, F32, own**-0.5)
+    down[0, :own] = _rand((own, k), 98, F32, k**-0.5)
+    up[0, :, own : -(-own // 8) * 8] = 0
+    value, projected = _rand((1, seq, k), 99, dtype), _rand((1, seq, n), 100, dtype)
+    value[0, 3 * seq // 4] = 0  # an h of 0
+    down, up = down.to(dtype), up.to(dtype)
+    ranks = None if own == rank else [own]
+    want = _run_adapters(gpu_device, value, projected, down, up, ranks)
+    bad = up.clone()
+    bad[0, 1, 0], bad[0, 5, own - 1], bad[0, 8, [0, 2]] = math.inf, -math.inf, math.inf
+    h = value[0].double() @ down[0].double().t()
+    sign = h[:, [0, 2, own - 1]].sign()
+    # (an h so near 0 that fp32's sums may miss its sign stays out)
+    sure = (h[:, [0, 2, own - 1]].abs() > (k + 8) * 2.0**-24 * (value[0].double().abs() @ down[0].double().abs().t())[:, [0, 2, own - 1]]).all(1)
+    sure[3 * seq // 4] = True
+    assert sure.sum() > 0.5 * seq
+    want = want[0].float()
+    want[:, 1], want[:, 5] = (sign[:, 0] * math.inf).float(), (-sign[:, 2] * math.inf).float()
+    want[:, 8] = (sign[:, 0] * math.inf + sign[:, 1] * math.inf).float()
+    got = _run_adapters(gpu_device, value, projected, down, bad, ranks)[0].float()
+    _same_with_infinities(got[sure], want[sure])
+
+
 def test_adapters_of_more_than_four_gigabytes(gpu_device):
     """Offsets beyond 32 bits in the weights, the inputs and the outputs."""
 
