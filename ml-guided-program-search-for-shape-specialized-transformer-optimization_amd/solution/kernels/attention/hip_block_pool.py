@@ -70,6 +70,11 @@ HIP_BLOCK_CACHE_TAKE_BACK_BACKEND = "hip_block_cache_take_back"
 MAX_FORKED_SEQUENCES = 1024
 _MAX_TOKENS = 2**31 - 1
 _MAX_ENTRIES = 2**31 - 1
+_MAX_SEQUENCES = (2**31 - 1) // 1024
+_MAX_BLOCKS = (2**31 - 1) // BLOCK_TOKENS  # of a sequence
+_MAX_PLACES = 2**31 - 1 - 16384
+_MAX_KV_HEADS = 65536
+_MAX_WORKGROUPS = (2**32 - 1) // 256
 
 
 @dataclass(frozen=True, eq=False)
@@ -144,7 +149,9 @@ def _pool_request(pool: BlockPool, words: torch.Tensor | None = None, more: torc
 
     table = pool.block_table
     index, (batch, max_blocks) = table.get_device(), table.shape
-    if batch * max_blocks > _MAX_ENTRIES:
+    if batch > _MAX_SEQUENCES or max_blocks > _MAX_BLOCKS or batch * max_blocks > _MAX_ENTRIES:
+        return None
+    if pool.holders.shape[0] > _MAX_PLACES:
         return None
     if words is not None and not _words_ok(words, batch, index):
         return None
@@ -325,6 +332,8 @@ def _cache_request(cache: BlockCache, size: int, words: torch.Tensor, more: torc
     index = cache.key_tail.get_device()
     if not _words_ok(words, size, index) or (more is not None and not _words_ok(more, size, index)):
         return None
+    if cache.key_tail.shape[1] > _MAX_KV_HEADS or cache.key_codes.shape[0] > _MAX_TOKENS:
+        return None
     library = library_for(index)
     return None if library is None else (library, index)
 
@@ -401,10 +410,17 @@ def hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> str:
     return HIP_BLOCK_CACHE_FORK_BACKEND
 
 
+def _take_back_request(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> tuple | None:
+    batch, heads = cache.key_tail.shape[:2]
+    if ends is None or cache.block_table.shape[1] > _MAX_BLOCKS or batch > _MAX_WORKGROUPS // (2 * heads):
+        return None
+    return _cache_request(cache, batch, lengths, ends)
+
+
 def can_use_hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> bool:
     """Whether the take-back kernel takes these tensors."""
 
-    return ends is not None and _cache_request(cache, cache.key_tail.shape[0], lengths, ends) is not None
+    return _take_back_request(cache, lengths, ends) is not None
 
 
 def hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> str:
@@ -419,7 +435,7 @@ def hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: to
 
     tail = cache.key_tail
     batch, heads, _, dim = tail.shape
-    request = None if ends is None else _cache_request(cache, batch, lengths, ends)
+    request = _take_back_request(cache, lengths, ends)
     if request is None:
         raise RuntimeError("HIP block cache take back is ineligible for the requested inputs")
     library, index = request

@@ -28,6 +28,9 @@ from ..hip._library import (
 HIP_LOW_RANK_ADAPTERS_BACKEND = "hip_low_rank_adapters"
 SUPPORTED_DTYPES = frozenset({torch.bfloat16, torch.float16})
 MAX_RANK = 128
+_MAX_FEATURES = 2**24
+_MAX_INT32 = 2**31 - 1
+_MAX_WORKGROUPS = (2**32 - 1) // 256  # of 16 tokens and 64 outputs each
 
 
 @dataclass(frozen=True, eq=False)
@@ -164,7 +167,11 @@ def _request(
     if shape[-1] != down.shape[2] or projected.shape != (*shape[:-1], adapters.up.shape[1]):
         return None
     batch, seq_len = shape[0], shape[1] if len(shape) == 3 else 1
-    if indices is None:
+    if indices is None or max(batch, seq_len, down.shape[0]) > _MAX_INT32:
+        return None
+    if max(shape[-1], projected.shape[-1]) > _MAX_FEATURES:
+        return None
+    if batch * -(-seq_len // 16) > _MAX_WORKGROUPS // -(-projected.shape[-1] // 64):
         return None
     for words in (indices, counts):
         if words is not None and (

@@ -51,7 +51,8 @@ def _request(
     counts: torch.Tensor | None,
     temperatures: torch.Tensor | None,
 ) -> tuple | None:
-    """The library, the device and the sizes of a request that the kernels take, else None."""
+    """The library, the device, the sizes and the workspace's bytes of a request that the
+    kernels take, else None."""
 
     dtype, index, shape = target.dtype, target.get_device(), target.shape
     if dtype not in SUPPORTED_DTYPES or len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
@@ -79,7 +80,12 @@ def _request(
     ):
         return None
     library = library_for(index)
-    return None if library is None else (library, index, batch, drafts, vocab)
+    if library is None:
+        return None
+    size = library.sah_verify_draft_workspace_bytes(batch, drafts, vocab, 0 if draft is None else 1)
+    if batch and not size:  # more rows than a launch has workgroups for
+        return None
+    return library, index, batch, drafts, vocab, size
 
 
 def can_use_hip_verify_draft(
@@ -126,11 +132,10 @@ def hip_verify_draft(
     request = _request(target, tokens, uniforms, draft, counts, temperatures)
     if request is None:
         raise RuntimeError("HIP draft verification is ineligible for the requested inputs")
-    library, index, batch, drafts, vocab = request
+    library, index, batch, drafts, vocab, size = request
     answer = tokens.new_empty((batch, drafts + 1))
     accepted = tokens.new_empty((batch,), dtype=torch.int32)
     try:
-        size = library.sah_verify_draft_workspace_bytes(batch, drafts, vocab, 0 if draft is None else 1)
         workspace = tokens.new_empty(-(-size // 8)) if size else None
         launch(
             index,

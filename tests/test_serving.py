@@ -5,6 +5,7 @@ pool's and the adapters' own tensors."""
 from __future__ import annotations
 
 import re
+import sys
 import textwrap
 from pathlib import Path
 
@@ -430,6 +431,127 @@ def test_adapter_outputs_apart_from_inputs():
     assert not low_rank_module._apart(store[:, 0], store[:, 1])  # rows of one lie between the other's
     assert not low_rank_module._apart(store, store[1])
     assert low_rank_module._apart(store[:0], store)
+
+
+@pytest.fixture
+def any_device(monkeypatch):
+    """The library for tensors without storage, whose sizes alone are looked at: on the
+    device "meta", no call beyond the predicates."""
+
+    verify_module = sys.modules[hip_verify_draft.__module__]
+    for module in (verify_module, low_rank_module, pool_module):
+        monkeypatch.setattr(module, "library_for", lambda index: _library.load_library())
+
+
+def _meta(*shape, dtype=torch.int32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize(
+    "batch,drafts,vocab,sampled,taken",
+    [
+        ((2**32 - 1) // 1024, 0, 2, False, True),
+        ((2**32 - 1) // 1024 + 1, 0, 2, False, False),
+        ((2**32 - 1) // 1024 // 2049, 1024, 100, True, True),
+        ((2**32 - 1) // 1024 // 2049 + 1, 1024, 100, True, False),
+        (1, 0, 2**31 - 1 - 8192, False, True),
+        (1, 0, 2**31 - 8192, False, False),
+        (1, 1025, 100, False, False),
+        (0, 3, 100, True, True),
+    ],
+)
+def test_verify_predicate_at_the_entry_s_limits(any_device, batch, drafts, vocab, sampled, taken):
+    target, draft = (_meta(batch, n, vocab, dtype=torch.bfloat16) for n in (drafts + 1, drafts))
+    tokens, uniforms = _meta(batch, drafts, dtype=torch.int64), _meta(batch, drafts + 1, dtype=torch.float32)
+    assert can_use_hip_verify_draft(target, tokens, uniforms, draft if sampled else None) == taken
+    if not taken:
+        sizes = dict(batch=batch, drafts=drafts, vocab=vocab, draft=P if sampled else None)
+        assert _call("sah_verify_draft", VERIFY, **sizes, workspace_bytes=1 << 40) == UNSUPPORTED
+
+
+@pytest.mark.parametrize(
+    "batch,seq,k,n,taken",
+    [
+        (1, 1, 2**24, 8, True),
+        (1, 1, 2**24 + 8, 8, False),
+        (1, 1, 8, 2**24, True),
+        (1, 1, 8, 2**24 + 8, False),
+        ((2**32 - 1) // 256, 1, 8, 8, True),
+        ((2**32 - 1) // 256 + 1, 1, 8, 8, False),
+        (1, 16 * ((2**32 - 1) // 256 // 3), 8, 136, True),
+        (1, 16 * ((2**32 - 1) // 256 // 3) + 1, 8, 136, False),
+    ],
+)
+def test_adapters_predicate_at_the_entry_s_limits(any_device, batch, seq, k, n, taken):
+    down, up = _meta(1, 8, k, dtype=torch.bfloat16), _meta(1, n, 8, dtype=torch.bfloat16)
+    value, projected = _meta(batch, seq, k, dtype=torch.bfloat16), _meta(batch, seq, n, dtype=torch.bfloat16)
+    assert can_use_hip_low_rank_adapters(value, projected, LowRankAdapters(down, up), _meta(batch)) == taken
+    if not taken:
+        sizes = dict(batch=batch, seq_len=seq, in_features=k, out_features=n, adapters=1, rank=8)
+        rows = dict(x_sb=seq * k, x_ss=k, p_sb=seq * n, p_ss=n, y_sb=seq * n, y_ss=n)
+        assert _call("sah_low_rank_adapters", ADAPTERS, **sizes, **rows, workspace_bytes=1 << 40) == UNSUPPORTED
+
+
+@pytest.mark.parametrize(
+    "batch,max_blocks,num_blocks,taken",
+    [
+        (2097151, 1, 5, True),
+        (2097152, 1, 5, False),
+        (1, 2**25 - 1, 5, True),
+        (1, 2**25, 5, False),
+        (65536, 32767, 5, True),
+        (65536, 32768, 5, False),
+        (2, 3, 2**31 - 1 - 16384, True),
+        (2, 3, 2**31 - 16384, False),
+    ],
+)
+def test_pool_predicates_at_the_entries_limits(any_device, batch, max_blocks, num_blocks, taken):
+    pool, words = BlockPool(_meta(batch, max_blocks), _meta(num_blocks)), _meta(batch)
+    assert can_use_hip_block_pool_reserve(pool, words, 3) == taken
+    assert pool_module.can_use_hip_block_pool_release(pool, words) == taken
+    assert pool_module.can_use_hip_block_pool_compact(pool) == taken
+    assert pool_module.can_use_hip_block_pool_fork(pool, words, words) == (taken and batch <= 1024)
+    if not taken:
+        sizes = dict(batch=batch, max_blocks=max_blocks, num_blocks=num_blocks)
+        for name, defaults in (("reserve", RESERVE), ("release", RELEASE), ("fork", FORK), ("compact", COMPACT)):
+            more = {"workspace_bytes": 1 << 40} if "workspace" in defaults else {}
+            assert _call("sah_block_pool_" + name, defaults, **sizes, **more) in (INVALID, UNSUPPORTED)
+
+
+@pytest.mark.parametrize(
+    "batch,heads,blocks,width,taken",
+    [
+        (2, 65536, 5, 3, (True, True, True)),
+        (2, 65537, 5, 3, (False, False, False)),
+        (1025, 2, 5, 3, (True, False, True)),
+        ((2**32 - 1) // 256 // 4, 2, 5, 3, (True, False, True)),
+        ((2**32 - 1) // 256 // 4 + 1, 2, 5, 3, (True, False, False)),
+        (1, 1, 2**31 - 1, 3, (True, True, True)),
+        (1, 1, 2**31, 3, (False, False, False)),
+        (1, 1, 5, 2**25 - 1, (True, True, True)),
+        (1, 1, 5, 2**25, (True, True, False)),
+    ],
+)
+def test_cache_predicates_at_the_entries_limits(any_device, batch, heads, blocks, width, taken):
+    """Of the copy, the tails' fork and the take-back."""
+
+    codes, scales = _meta(blocks, heads, 64, 64, dtype=torch.uint8), _meta(blocks, heads, dtype=torch.float32)
+    tail = _meta(batch, heads, 64, 64, dtype=torch.bfloat16)
+    cache, words = BlockCache(codes, codes, scales, scales, tail, tail, _meta(batch, width)), _meta(batch)
+    got = (
+        can_use_hip_block_cache_copy(cache, _meta(blocks)),
+        pool_module.can_use_hip_block_cache_fork(cache, words),
+        pool_module.can_use_hip_block_cache_take_back(cache, words, words),
+    )
+    assert got == taken
+    refused = (INVALID, UNSUPPORTED)
+    if not taken[0]:
+        assert _call("sah_block_cache_copy", COPY, kv_heads=heads, num_blocks=blocks) in refused
+    if not taken[1] and blocks <= 2**31 - 1:
+        assert _call("sah_block_cache_fork", TAILS, batch=batch, kv_heads=heads) in refused
+    if not taken[2]:
+        sizes = dict(batch=batch, kv_heads=heads, num_blocks=blocks, max_blocks=width)
+        assert _call("sah_block_cache_take_back", TAKE, **sizes) in refused
 
 
 def test_operators_refuse_cpu_tensors():
