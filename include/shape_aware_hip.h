@@ -658,7 +658,8 @@ size_t sah_low_rank_adapters_workspace_bytes(
  *   accepted[b]  the drafts that stand
  *   answer[b]    [drafts + 1]: these, the token drawn, -1 behind
  * temperatures[b] (NULL: 1) not above 0 (or NaN) asks for the likeliest token: a draft
- * stands where it is the target's (ties: the lowest), which also is the token drawn.
+ * stands where it is the target's (ties: the lowest), which also is the token drawn.  Those
+ * above 1.2e38 count as that.
  * counts[b] (NULL: drafts) is the number of the request's drafts, at most drafts; below 0
  * the request takes no part: accepted and answer are -1.  A draft outside [0, vocab)
  * does not stand.  Logits of -inf have no weight.  A row that is asked for, of target

@@ -130,7 +130,9 @@ __device__ __forceinline__ double exponent_of(float logit, float top, double c) 
 }
 
 // log2(e) / temperature, and whether the request answers greedily instead (a temperature
-// that is not above 0).  An infinite one keeps masked logits at weight 0.
+// that is not above 0).  At least fp32's smallest normal number, for the rows' exponents:
+// an infinite temperature keeps masked logits at weight 0, and only logits that lie 1e36 and
+// more apart tell it, or one above 1.2e38, from 1.2e38.
 __device__ __forceinline__ bool is_greedy(const VerifyArgs& a, int64_t b, double& c) {
   const float t = a.temperatures != nullptr ? a.temperatures[b] : 1.0f;
   if (!(t > 0.0f)) {
@@ -138,7 +140,7 @@ __device__ __forceinline__ bool is_greedy(const VerifyArgs& a, int64_t b, double
     return true;
   }
   c = kLog2e / (double)t;
-  if (c < 1e-30) c = 1e-30;
+  if (c < 0x1p-126) c = 0x1p-126;
   return false;
 }
 

@@ -112,6 +112,18 @@ def test_verify_temperatures(gpu_device, dtype):
         _verify(gpu_device, target, tokens, uniforms, given, None, temperatures)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("size", [1e25, 1e31, 1e36])
+def test_verify_large_logits_at_large_temperatures(gpu_device, dtype, sampled, size):
+    target, draft, tokens, uniforms = _drafted(6, 3, 9001, F32, 22, near=0.1)
+    target, draft = (target * size).to(dtype), (draft * size).to(dtype)
+    target[2, :, 17:4000] = -math.inf
+    temperatures = [size * t for t in (1.0, 0.5, 3.0, 1.0, 8.0, 1.5)]
+    want = _verify(gpu_device, target, tokens, uniforms, draft if sampled else None, None, temperatures)
+    assert len({row[0] for row in want[0]}) > 1
+
+
 def test_verify_greedy_ties_take_the_lowest_token(gpu_device):
     target = torch.zeros((4, 3, 20_000), dtype=BF16)
     target[0, 0, [9000, 19_999]] = 3.0
