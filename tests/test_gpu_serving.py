@@ -209,6 +209,28 @@ def test_verify_random_numbers_at_the_border(gpu_device, dtype, sampled, vocab):
     assert min(want[1]) >= drafts // 2 - 1 and min(want[1]) < drafts
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("batch,vocab", [(130, 50), (600, 50), (110, 9001)])
+def test_verify_random_numbers_at_the_border_of_many_requests(gpu_device, dtype, sampled, batch, vocab):
+    """As above, where the decision is the draw's launch's and where it has one of its own:
+    numbers below p / q for the first drafts, on either side of it for the others."""
+
+    drafts = 18
+    target, draft, tokens, uniforms = _drafted(batch, drafts, vocab, dtype, 23 + vocab)
+    if not sampled:
+        tokens = target[:, :drafts].float().argmax(-1)
+    p = torch.softmax(target[:, :drafts].double(), -1).gather(-1, tokens[..., None])[..., 0]
+    q = torch.softmax(draft.double(), -1).gather(-1, tokens[..., None])[..., 0] if sampled else torch.ones_like(p)
+    border = (p / q).clamp(max=0.999).float()
+    step = torch.randint(-1, 2, border.shape, generator=_generator(24))
+    step[:, : drafts // 2] = -1
+    border = torch.where(step < 0, torch.nextafter(border, torch.zeros(())), border)
+    uniforms[:, :drafts] = torch.where(step > 0, torch.nextafter(border, torch.ones(())), border)
+    want = _verify(gpu_device, target, tokens, uniforms, draft if sampled else None)
+    assert min(want[1]) >= drafts // 2 - 1 and min(want[1]) < drafts
+
+
 @pytest.mark.parametrize("sampled", [True, False])
 @pytest.mark.parametrize("batch", [128, 129, 512, 513, 1500])
 def test_verify_of_many_requests_of_every_kind(gpu_device, batch, sampled):
@@ -744,6 +766,21 @@ def test_reserve_takes_the_lowest_of_many_places(gpu_device):
         assert int(pool.holders.sum()) == 99_998 + min(want, 5)
 
 
+@pytest.mark.parametrize("blocks", [5, 6, 7])
+def test_reserve_that_runs_out_part_way(gpu_device, blocks):
+    from solution.kernels.attention import hip_block_pool_reserve
+
+    free = [16_383, 16_384, 70_000, 99_999, 100_002]
+    holders = torch.ones(100_003, dtype=torch.int32)
+    holders[free] = 0
+    pool = _pool(gpu_device, [[-1] * 7, [-1] * 7, [5] * 7], holders.tolist())
+    missing, _ = hip_block_pool_reserve(pool, _words([0, 0, 0], gpu_device), blocks * 64, _words([blocks * 64, 64, 9], gpu_device))
+    assert pool.block_table.tolist() == [free + [-1] * 2, [-1] * 7, [5] * 7]
+    assert missing.tolist() == [blocks - 5, 1, 0]
+    holders[free] = 1
+    assert torch.equal(pool.holders.cpu(), holders)
+
+
 def test_reserve_of_far_positions(gpu_device):
     from solution.kernels.attention import hip_block_pool_reserve
 
@@ -900,6 +937,29 @@ def test_copy_of_more_than_four_gigabytes(gpu_device):
     for name, parts in held.items():
         for (target, _), part in zip(want, parts):
             assert torch.equal(getattr(cache, name)[target], part), (name, target)
+
+
+@pytest.mark.parametrize("heads,dim,blocks", [(16, 64, 4200), (3, 128, 6000), (1, 64, 40_000)])
+def test_copy_of_blocks_of_a_cache_larger_than_the_caches(gpu_device, heads, dim, blocks):
+    """Any plan over more than 256 MB of codes: some places from others, some from places of
+    no cache, some from themselves, some left out as their origin is written."""
+
+    from solution.kernels.attention import hip_block_cache_copy
+
+    cache = _filled_cache(gpu_device, 1, heads, dim, F16, blocks, [[0]], 77)
+    assert cache.key_codes.numel() + cache.value_codes.numel() > 256 << 20
+    before = {name: getattr(cache, name).clone() for name in _CODES}
+    generator = _generator(78)
+    origins = torch.where(torch.rand(blocks, generator=generator) < 0.4,
+                          torch.randint(-2, blocks + 2, (blocks,), generator=generator), -1)
+    place = torch.arange(blocks)
+    written = (origins >= 0) & (origins < blocks) & (origins != place)
+    takes = written & ~written[origins.clamp(0, blocks - 1)]
+    assert 0.1 * blocks < int(takes.sum()) < int(written.sum())
+    want = torch.where(takes, origins, place).to(gpu_device)
+    hip_block_cache_copy(cache, _words(origins.tolist(), gpu_device))
+    for name, held in before.items():
+        assert torch.equal(getattr(cache, name), held[want]), name
 
 
 @pytest.mark.parametrize("batch", [1, 2, 5, 64, 65, 300, 1024])
@@ -1280,6 +1340,99 @@ def test_captured_steps_replay_as_eager_ones(gpu_device):
     assert torch.equal(models[0].pool.holders, models[1].pool.holders)
     for name in _CODES + ("key_tail", "value_tail"):
         assert torch.equal(getattr(models[0].cache, name), getattr(models[1].cache, name)), name
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("batch,vocab", [(4, 9001), (70, 4097), (600, 203)])
+def test_captured_verification_of_few_and_many_requests(gpu_device, batch, vocab, sampled):
+    """Two, three and four launches of a graph, replayed on other inputs beside eager calls."""
+
+    from solution.kernels.sampling import hip_verify_draft
+
+    drafts = 3
+    generator = _generator(101)
+
+    def inputs(seed):
+        made = [t.to(gpu_device) for t in _drafted(batch, drafts, vocab, BF16, seed, near=0.2)]
+        made.append(torch.randint(-1, drafts + 2, (batch,), generator=generator).int().to(gpu_device))
+        heat = torch.tensor([1.0, 0.0, 0.5])[torch.randint(0, 3, (batch,), generator=generator)]
+        return made + [heat.to(gpu_device)]
+
+    def call(target, draft, tokens, uniforms, counts, temperatures):
+        return hip_verify_draft(target, tokens, uniforms, draft if sampled else None, counts=counts, temperatures=temperatures)[:2]
+
+    with torch.inference_mode():
+        held = inputs(102)
+        call(*held)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = call(*held)
+        answers = set()
+        for i in range(5):
+            fresh = inputs(103 + i)
+            want = call(*fresh)
+            for mine, other in zip(held, fresh):
+                mine.copy_(other)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(captured[0], want[0]) and torch.equal(captured[1], want[1]), i
+            answers |= set(captured[1].tolist())
+        assert len(answers) > (2 if sampled else 1)  # (a certain draft of many tokens seldom stands)
+
+
+@pytest.mark.parametrize("batch,width,blocks", [(6, 9, 60), (40, 30, 20_000)])
+def test_captured_forks_and_compactions_replay_as_eager_ones(gpu_device, batch, width, blocks):
+    """Reserve, fork, release, compaction and copy in one graph, on sources and lengths that
+    change; pools compacted in one launch and in two."""
+
+    from solution.kernels.attention import (
+        BlockPool, hip_block_cache_copy, hip_block_cache_fork, hip_block_pool_compact, hip_block_pool_fork,
+        hip_block_pool_release, hip_block_pool_reserve,
+    )
+
+    tokens = 130
+    caches = [_filled_cache(gpu_device, batch, 2, 64, BF16, blocks, [[-1] * width] * batch, 104) for _ in range(2)]
+    pools = [BlockPool(c.block_table, torch.zeros(blocks, dtype=torch.int32, device=gpu_device)) for c in caches]
+    for pool in pools:  # some places are someone else's, so that there is something to move
+        pool.holders[::3] = 1
+    generator = _generator(105)
+
+    def step(pool, cache, starts, sources, lengths, ends):
+        missing = hip_block_pool_reserve(pool, starts, tokens)[0]
+        hip_block_pool_fork(pool, sources, lengths)
+        hip_block_cache_fork(cache, sources)
+        hip_block_pool_release(pool, ends)
+        origins, used, _ = hip_block_pool_compact(pool)
+        hip_block_cache_copy(cache, origins)
+        return missing, origins, used
+
+    with torch.inference_mode():
+        static = [torch.zeros(batch, dtype=torch.int32, device=gpu_device) for _ in range(4)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step(pools[0], caches[0], *static)
+        starts, moved = torch.zeros(batch, dtype=torch.int64), 0
+        for i in range(8):
+            sources = torch.randint(-1, batch + 1, (batch,), generator=generator)
+            lengths = starts + tokens
+            origin = torch.where((sources >= 0) & (sources < batch), sources, torch.arange(batch))
+            ends = (lengths[origin] - torch.randint(0, 150, (batch,), generator=generator)).clamp(min=0)
+            ends[torch.rand(batch, generator=generator) < 0.1] = 0
+            given = [_words(t.tolist(), gpu_device) for t in (starts, sources, lengths, ends)]
+            want = step(pools[1], caches[1], *given)
+            for mine, other in zip(static, given):
+                mine.copy_(other)
+            graph.replay()
+            torch.cuda.synchronize()
+            for mine, other in zip(captured, want):
+                assert torch.equal(mine, other), i
+            assert torch.equal(pools[0].block_table, pools[1].block_table), i
+            assert torch.equal(pools[0].holders, pools[1].holders), i
+            for name in _CODES + ("key_tail", "value_tail"):
+                assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), (i, name)
+            moved += int((want[1] >= 0).sum())
+            starts = ends
+        assert moved > 0
 
 
 def test_two_streams_at_once(gpu_device):
