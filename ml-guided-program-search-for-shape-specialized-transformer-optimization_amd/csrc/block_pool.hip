@@ -95,7 +95,8 @@ struct ReserveArgs {
 // its sums over the sequences before, that many free places, the entries.  The search
 // ends with the last free place that is wanted; a thread reads 16 places in four accesses.
 // 64 sequences of 8 tokens in a pool of 4032 places, or 32 of 777 in 6016: 6 us, four
-// steps of accesses and barriers (a copy's time of what it reads would be 0.01).
+// steps of accesses and barriers (a copy's time of what it reads would be 0.01); a pool
+// without free places, which is searched whole, of 65536 11 us, of 262144 31.
 __global__ __launch_bounds__(kScanThreads) void pool_reserve_kernel(const ReserveArgs a) {
   __shared__ int sums[2][kScanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -230,8 +231,8 @@ __global__ __launch_bounds__(kThreads) void pool_fork_kernel(const Pool pool, co
 }
 
 // Places and entries up to which one launch compacts a pool: 12.7 -> 8.4 us on the host,
-// which is what a small pool's compaction takes (4128 of either: 10 us on the GPU in one
-// launch, 8.6 + 4.6 in two).
+// which is what a small pool's compaction takes (4128 of either: 9.3 us on the GPU in one
+// launch, 8.6 + 4.6 in two; 16384 21 us).
 constexpr int64_t kSmallPool = 16384;
 
 struct CompactArgs {
@@ -256,7 +257,7 @@ __device__ __forceinline__ void compact_apply(const CompactArgs& a, int used, in
     a.pool.holders[mover] = 0;
   }
   // (four entries' accesses in flight together: 32 sequences of 129 blocks, by one
-  // workgroup, 9.9 us instead of 11)
+  // workgroup, the whole call a ninth less)
   const int64_t entries = (int64_t)a.pool.batch * a.pool.max_blocks;
   for (int64_t i = first; i < entries; i += kApplyEntries * step) {
     int32_t place[kApplyEntries], rank[kApplyEntries], hole[kApplyEntries];
@@ -277,7 +278,8 @@ __device__ __forceinline__ void compact_apply(const CompactArgs& a, int used, in
 
 // `used` places have holders.  The free ones below `used` are as many as the held
 // ones from there on, and take their contents in order.  One workgroup counts, then
-// lists both; of a small pool it does the rest too (APPLIES).
+// lists both; of a small pool it does the rest too (APPLIES).  It reads the counts twice,
+// 16384 places a pass: 65536 places 54 us with the second launch, 262144 202.
 template <bool APPLIES>
 __global__ __launch_bounds__(kScanThreads) void pool_compact_list_kernel(const CompactArgs a) {
   __shared__ int sums[2][kScanThreads / 64];

@@ -27,9 +27,9 @@
 // base and y: a workgroup does both products of 32 tokens, and there is no workspace.  Nor
 // is there for few tokens of short inputs, where latency and launches are all there is.
 //   2 x 20001 tokens (ragged), 1024 -> 4096, rank 32 (697 MB, 142 us at a large copy's
-//   rate): 138 us; 149 through the caches, 178 in the operands' order as well
-//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (33 MB, 7 us): 7.2 + 7.6 us
-//   1 token, 1024 -> 1024, rank 16: 5.4 us
+//   rate): 139 us; some 10 more through the caches, 40 in the operands' order as well
+//   64 tokens, 4096 -> 4096, an adapter each of rank 64 (33 MB, 7 us): 7.3 + 7.9 us
+//   1 token, 1024 -> 4096, rank 16: 5.7 us
 
 #include <type_traits>
 
@@ -658,10 +658,11 @@ struct Plan {
   int rank_tiles;
   size_t bytes;
 };
-// Tiles of 16 tokens from which on one launch does both products.  4096 -> 4096, two
-// launches / one, us: 8704 tokens of rank 16 58 / 57, of rank 128 131 / 144; 17408 tokens
-// 108 / 109 and 228 / 231; 34816 tokens 195 / 188 and 434 / 405.  Requests of up to a
-// tile's tokens would leave the larger workgroups' places empty.
+// Tiles of 16 tokens from which on one launch does both products.  4096 -> 4096, bf16, two
+// launches / one, us: 8704 tokens of rank 16 63 / 63, of rank 64 84 / 80, of rank 128 121 /
+// 134; 17408 tokens 103 / 94, 139 / 126 and 202 / 200; 34816 tokens 185 / 168, 255 / 207
+// and 368 / 336.  Requests of up to a tile's tokens would leave the larger workgroups'
+// places empty.
 constexpr int64_t kManyTiles = 1024;
 // Outputs (of 2 bytes) from which on base and y pass the caches: more than half of the 256 MB
 // last-level cache, which the next operator could not find there anyway (2 x 20001

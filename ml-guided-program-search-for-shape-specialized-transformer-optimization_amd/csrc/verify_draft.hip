@@ -10,7 +10,9 @@
 // A token is chosen at a border between two, of which there are as many as tokens: sums
 // wrong by 1e-7, as fp32 leaves them, choose another token once in 10^7 / vocabulary
 // requests.  The choice here is that of exact arithmetic, but for borders closer than some
-// 1e-14 of the whole:
+// 1e-14 of p's mass (an exponential of fp64 is off by 2^-51 and its exponent's rounding, some
+// 1e-15; of the whole that max(p - q, 0) has, 1e-14 over how far p and q lie apart: 1e-8
+// where they differ by 1e-6):
 //   1. rows: a chunk of a row's largest logit and sum of exponentials, in fp32 (a row's
 //      sum comes out right to kFastError).  The one pass over all logits, bound by them;
 //   2. decide: p_i(x_i), q_i(x_i) from these; where the test's two sides lie within
@@ -26,7 +28,7 @@
 //
 // 64 requests, 7 drafts, 131072 tokens, bf16 (252 MB, 51 us at a large copy's rate): rows
 // 53 us, decide 7, weigh 20, pick 5.4.  The draw's two parts in one launch, by the
-// request's last workgroup, took 106 us instead of 30, as each of the 4096 releases its
+// request's last workgroup, took 106 us instead of 27, as each of the 4096 releases its
 // L2's lines.  All rows in fp64 took 126 us (some 80 with the exponential as it is now, 24
 // instructions of four cycles a logit).  For one request (4 drafts, 32000 tokens) the parts
 // are latencies, 4 + 11 us.
@@ -53,7 +55,8 @@ constexpr int64_t kFewWorkgroups = 512;
 // And up to which a request's last one also draws, for another: 16 11.4 us instead of 7.1 +
 // 4.1, 125 9.4 instead of 5.5 + 3.7, 128 12.9 instead of 7.0 + 4.4, where a launch is 3 us
 // of the host's; 256 15.6 instead of 7.2 + 4.5, 512 21 instead of 8.9 + 5.1, as each
-// releases its L2's lines.
+// releases its L2's lines.  (A captured step has no such launch to save: it gains nothing
+// and pays 1.5 us at 128.)
 constexpr int64_t kFewestWorkgroups = 128;
 enum { kDecided = 0, kDecides = 1, kDraws = 2 };
 constexpr double kLog2e = 1.4426950408889634074;
@@ -158,7 +161,9 @@ typedef uint32_t LooseWords __attribute__((ext_vector_type(4), aligned(2)));
 // reads again.  Rows of 64 requests in turn with other inputs 53 us instead of 56, weigh
 // 20.1 instead of 19.5; of logits just written, 32 requests 25.4 instead of 26.2, 64 51 and
 // 51, 128 97 instead of 115; of the same logits again and again 28.7 instead of 26.7, 52 instead
-// of 47, 93 instead of 96.
+// of 47, 93 instead of 96.  At every size, without a border: logits that come from memory, or
+// that the model has just written, are a program's case and gain or lose nothing, and
+// smaller batches than these are bound by latency.
 template <typename T, bool ONCE = false>
 __device__ __forceinline__ void load_logits(const T* row, int64_t at, int64_t vocab, float* out) {
   if (at + kVec <= vocab) {
