@@ -92,6 +92,12 @@ class BlockCache:
         for tensor in (self.key_codes, self.value_codes, self.key_tail, self.value_tail):
             if tensor.data_ptr() % 16:
                 raise ValueError("the cache's codes and tails must be 16-byte aligned")
+        # whether csrc/block_pool.hip's kernels take its sizes (looked at on every call):
+        # copies and forks of blocks, and tokens taken back
+        moves = heads <= 65536 and blocks <= _MAX_LENGTH
+        goes_back = self.block_table.shape[1] <= _MAX_LENGTH // BLOCK_TOKENS and batch <= (2**32 - 1) // 256 // (2 * heads)
+        object.__setattr__(self, "_moves", moves)
+        object.__setattr__(self, "_goes_back", moves and goes_back)
 
     @classmethod
     def allocate(

@@ -73,8 +73,6 @@ _MAX_ENTRIES = 2**31 - 1
 _MAX_SEQUENCES = (2**31 - 1) // 1024
 _MAX_BLOCKS = (2**31 - 1) // BLOCK_TOKENS  # of a sequence
 _MAX_PLACES = 2**31 - 1 - 16384
-_MAX_KV_HEADS = 65536
-_MAX_WORKGROUPS = (2**32 - 1) // 256
 
 
 @dataclass(frozen=True, eq=False)
@@ -95,6 +93,10 @@ class BlockPool:
             raise ValueError("a pool is block_table [batch, max_blocks] and holders [num_blocks], both int32")
         if not table.is_contiguous() or not holders.is_contiguous() or holders.device != table.device:
             raise ValueError("the pool's tensors must be contiguous and on one device")
+        batch, max_blocks = table.shape
+        fits = batch <= _MAX_SEQUENCES and max_blocks <= _MAX_BLOCKS and batch * max_blocks <= _MAX_ENTRIES
+        # whether the kernels take its sizes (looked at on every call)
+        object.__setattr__(self, "_fits", fits and holders.shape[0] <= _MAX_PLACES)
 
     @classmethod
     def allocate(
@@ -149,9 +151,7 @@ def _pool_request(pool: BlockPool, words: torch.Tensor | None = None, more: torc
 
     table = pool.block_table
     index, (batch, max_blocks) = table.get_device(), table.shape
-    if batch > _MAX_SEQUENCES or max_blocks > _MAX_BLOCKS or batch * max_blocks > _MAX_ENTRIES:
-        return None
-    if pool.holders.shape[0] > _MAX_PLACES:
+    if not pool._fits:
         return None
     if words is not None and not _words_ok(words, batch, index):
         return None
@@ -332,7 +332,7 @@ def _cache_request(cache: BlockCache, size: int, words: torch.Tensor, more: torc
     index = cache.key_tail.get_device()
     if not _words_ok(words, size, index) or (more is not None and not _words_ok(more, size, index)):
         return None
-    if cache.key_tail.shape[1] > _MAX_KV_HEADS or cache.key_codes.shape[0] > _MAX_TOKENS:
+    if not cache._moves:
         return None
     library = library_for(index)
     return None if library is None else (library, index)
@@ -411,10 +411,9 @@ def hip_block_cache_fork(cache: BlockCache, sources: torch.Tensor) -> str:
 
 
 def _take_back_request(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> tuple | None:
-    batch, heads = cache.key_tail.shape[:2]
-    if ends is None or cache.block_table.shape[1] > _MAX_BLOCKS or batch > _MAX_WORKGROUPS // (2 * heads):
+    if ends is None or not cache._goes_back:
         return None
-    return _cache_request(cache, batch, lengths, ends)
+    return _cache_request(cache, cache.key_tail.shape[0], lengths, ends)
 
 
 def can_use_hip_block_cache_take_back(cache: BlockCache, lengths: torch.Tensor, ends: torch.Tensor) -> bool:

@@ -29,7 +29,6 @@ HIP_LOW_RANK_ADAPTERS_BACKEND = "hip_low_rank_adapters"
 SUPPORTED_DTYPES = frozenset({torch.bfloat16, torch.float16})
 MAX_RANK = 128
 _MAX_FEATURES = 2**24
-_MAX_INT32 = 2**31 - 1
 _MAX_WORKGROUPS = (2**32 - 1) // 256  # of 16 tokens and 64 outputs each
 
 
@@ -39,7 +38,7 @@ class LowRankAdapters:
     weight.
 
     ``down`` [adapters, rank, in_features] and ``up`` [adapters, out_features, rank] in
-    bfloat16 or float16, rank a multiple of 8 up to 128, features multiples of 8.
+    bfloat16 or float16, rank a multiple of 8 up to 128, features multiples of 8 up to 2^24.
     ``scales`` [adapters] (float32, 1 without).  ``ranks`` [adapters] (int32) names each
     adapter's own rank where they differ; its directions from there to the next multiple
     of 8 are zeros, and those behind are not read.
@@ -60,6 +59,8 @@ class LowRankAdapters:
             raise ValueError("the rank must be a multiple of 8 up to 128")
         if not self.in_features or not self.out_features or self.in_features % 8 or self.out_features % 8:
             raise ValueError("in_features and out_features must be multiples of 8")
+        if max(self.in_features, self.out_features) > _MAX_FEATURES:
+            raise ValueError("in_features and out_features must be at most 2^24")
         for tensor, dtype in ((self.scales, torch.float32), (self.ranks, torch.int32)):
             if tensor is not None and (tensor.shape != (down.shape[0],) or tensor.dtype != dtype):
                 raise ValueError("scales must be [adapters] in float32 and ranks [adapters] in int32")
@@ -70,6 +71,8 @@ class LowRankAdapters:
                 raise ValueError("the adapters' tensors must be contiguous, on one device and need no gradient")
         if down.data_ptr() % 16 or up.data_ptr() % 16:
             raise ValueError("down and up must be 16-byte aligned")
+        # tiles of 16 tokens that a launch takes (looked at on every call)
+        object.__setattr__(self, "_most_tiles", _MAX_WORKGROUPS // -(-self.out_features // 64))
 
     @classmethod
     def pack(
@@ -167,11 +170,7 @@ def _request(
     if shape[-1] != down.shape[2] or projected.shape != (*shape[:-1], adapters.up.shape[1]):
         return None
     batch, seq_len = shape[0], shape[1] if len(shape) == 3 else 1
-    if indices is None or max(batch, seq_len, down.shape[0]) > _MAX_INT32:
-        return None
-    if max(shape[-1], projected.shape[-1]) > _MAX_FEATURES:
-        return None
-    if batch * -(-seq_len // 16) > _MAX_WORKGROUPS // -(-projected.shape[-1] // 64):
+    if indices is None or batch * -(-seq_len // 16) > adapters._most_tiles:
         return None
     for words in (indices, counts):
         if words is not None and (

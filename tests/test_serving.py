@@ -485,7 +485,11 @@ def test_verify_predicate_at_the_entry_s_limits(any_device, batch, drafts, vocab
 def test_adapters_predicate_at_the_entry_s_limits(any_device, batch, seq, k, n, taken):
     down, up = _meta(1, 8, k, dtype=torch.bfloat16), _meta(1, n, 8, dtype=torch.bfloat16)
     value, projected = _meta(batch, seq, k, dtype=torch.bfloat16), _meta(batch, seq, n, dtype=torch.bfloat16)
-    assert can_use_hip_low_rank_adapters(value, projected, LowRankAdapters(down, up), _meta(batch)) == taken
+    if max(k, n) > 2**24:
+        with pytest.raises(ValueError, match="at most"):
+            LowRankAdapters(down, up)
+    else:
+        assert can_use_hip_low_rank_adapters(value, projected, LowRankAdapters(down, up), _meta(batch)) == taken
     if not taken:
         sizes = dict(batch=batch, seq_len=seq, in_features=k, out_features=n, adapters=1, rank=8)
         rows = dict(x_sb=seq * k, x_ss=k, p_sb=seq * n, p_ss=n, y_sb=seq * n, y_ss=n)
