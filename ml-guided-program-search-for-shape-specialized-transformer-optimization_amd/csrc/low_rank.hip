@@ -17,9 +17,9 @@
 // h is fp32.  It enters the second product as the sum of three bf16 numbers, off by 2^-24
 // of itself as fp32 is, or of two fp16 numbers, off by 2^-22: with one number its 2^-8 would
 // be as much as the output's own rounding, and with two bf16 numbers some 0.2% of the
-// outputs are rounded another way (2 x 20001 tokens below 139.4 us with three, 138.5 with
-// two; 34816 tokens 4096 -> 4096, rank 64, 208 and 204, rank 128, 339 and 320).  A token's h is taken in a power of two of its own, its
-// largest below 2^15, so that fp16 reaches.
+// outputs are rounded another way (34816 tokens 4096 -> 4096, rank 64, 208 us with three
+// numbers, 204 with two, rank 128, 339 and 320).  A token's h is taken in a power of two of
+// its own, its largest below 2^15, so that fp16 reaches.
 //
 // Few tokens are bound by the adapters' bytes and by latency, and a workgroup a token would
 // leave most of the chip idle: one launch shares `in` among workgroups and leaves partial

@@ -598,8 +598,9 @@ def _recipes(where):
         blocks = re.findall(r"::\n\n((?:    .*\n|\n)+)", pool_module.__doc__)
         text = "\n".join(textwrap.dedent(block) for block in blocks)
     else:
-        document = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
-        (text,) = [block for block in re.findall(r"```python\n(.*?)```", document, re.S) if "hip_block_pool_reserve(pool" in block]
+        documents = [path.read_text() for path in Path(__file__).resolve().parents[1].glob("*.md")]
+        blocks = [block for document in documents for block in re.findall(r"```python\n(.*?)```", document, re.S)]
+        (text,) = [block for block in blocks if "hip_block_pool_reserve(pool" in block]
         text = text[re.search(r"^.*hip_block_pool_reserve\(pool", text, re.M).start() :]
     before, rest = text.split("\n...", 1)
     after, others = rest[rest.index("answer, accepted") :].split("starts = ends\n", 1)
@@ -638,7 +639,7 @@ def _stand_ins(book, caches, accepts):
     )
 
 
-@pytest.mark.parametrize("where", ["docstring", "integration"])
+@pytest.mark.parametrize("where", ["docstring", "guide"])
 @pytest.mark.parametrize("blocks", [0, 1, 2, 3, 5, 30])
 def test_documented_step_keeps_its_tokens_where_places_run_out(where, blocks):
     """Steps of sequences that ask for fewer and for more places than there are: whatever
@@ -672,7 +673,7 @@ def test_documented_step_keeps_its_tokens_where_places_run_out(where, blocks):
             assert cache.read(b, end) == kept[b], (step, b)
 
 
-@pytest.mark.parametrize("where", ["docstring", "integration"])
+@pytest.mark.parametrize("where", ["docstring", "guide"])
 @pytest.mark.parametrize("sources", [[1, 0, -1, 3, 7, 0], [-1] * 6, [6, 6, 6, 0, 0, 0], [5, 4, 3, 2, 1, 0]])
 def test_documented_beams_go_on_where_their_sources_were(where, sources):
     """Behind a step whose drafts stood in part: every sequence holds what its source
